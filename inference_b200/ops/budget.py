@@ -1,0 +1,226 @@
+"""Long paged caches on a budget (csrc/kernels/page_select.cu, attention_budget.cu, cache_evict.cu).
+
+Two ways to spend less than the whole cache on a new token, both beside `paged_attention`:
+
+  read less    `summarize_pages` keeps an 8-bit summary of every full page, `select_pages` picks the pages that promise a token the most,
+               `selected_attention` reads these alone
+  keep less    `tracked_attention` reads the whole cache and adds up the weight that each entry receives, `evict_tokens` lets the entries of least
+               weight go and closes their holes
+
+Caches are one layer's pages [blocks, kv heads, block_size, width] with the block tables of `PagedSequence`. bf16, or fp32 in the 32-bit mode; widths up to 256.
+Calls run on the current stream, take no host reads and can be captured into graphs; buffers that a call fills (summaries, weights, positions, the cache) belong
+to the caller. Steps are described as in `paged_attention`: kv_lens int32 [num_seqs] counts a sequence's tokens with the new ones, cu_q int32 [num_seqs + 1]
+are the new tokens' ranges, or None where every sequence has max_q_len of them; rows behind the last range are left as they were."""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from .._native import kernels
+from .runtime import KernelError, check, ptr, require_cuda, stream_ptr
+
+MAX_WIDTH, MAX_GROUP, MAX_SPLITS = 256, 128, 64
+SELECT_SMEM = 200 * 1024
+
+
+@dataclass
+class PageSummaries:
+    """codes int8 [blocks, kv heads, D] and scales fp32 [blocks, kv heads]: codes * scale is a full page's mean key to within half a step, the
+    largest code is 127. A page with a key that is not finite has the scale NaN and is selected before all others. Pages not summarised yet hold whatever the buffers held."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @classmethod
+    def empty(cls, kcache: torch.Tensor) -> "PageSummaries":
+        blocks, heads, _, width = kcache.shape
+        return cls(torch.zeros((blocks, heads, width), dtype=torch.int8, device=kcache.device),
+                   torch.zeros((blocks, heads), dtype=torch.float32, device=kcache.device))
+
+    def values(self) -> torch.Tensor:
+        """The mean keys that the summaries stand for, fp32 [blocks, kv heads, D]."""
+        return self.codes * self.scales[..., None]
+
+
+@dataclass
+class PageSelection:
+    """pages int32 [T, kv heads, N]: places in the sequence (page p holds tokens p * block_size and on), -1 behind the first counts int32 [T, kv heads]."""
+    pages: torch.Tensor
+    counts: torch.Tensor
+
+
+def _require(ok: bool, what: str) -> None:
+    if not ok:
+        raise KernelError(what)
+
+
+def _place(first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    """All operands on the current device: launches go to its current stream."""
+    require_cuda(first, *others)
+    dev = torch.cuda.current_device()
+    for t in (first, *others):
+        if t is not None and t.device.index != dev:
+            raise KernelError(f"operands lie on {t.device}, the current device is cuda:{dev}")
+
+
+def _check_cache(kcache: torch.Tensor, vcache: torch.Tensor | None = None) -> None:
+    _require(kcache.dim() == 4 and kcache.dtype in (torch.bfloat16, torch.float32) and kcache.is_contiguous() and kcache.shape[3] <= MAX_WIDTH,
+             "pages are contiguous [blocks, kv heads, block_size, width] in bf16 or fp32, at most 256 wide")
+    _require(vcache is None or (vcache.dim() == 4 and vcache.dtype == kcache.dtype and vcache.is_contiguous() and vcache.shape[:3] == kcache.shape[:3]
+                                and vcache.shape[3] <= MAX_WIDTH), "value pages match the key pages in type, number, heads and block_size")
+
+
+def _check_step(table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor | None, max_q_len: int, tokens: int | None) -> int:
+    n = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
+    _require(table.dtype == kv_lens.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == n and table.stride(1) == 1 and kv_lens.is_contiguous(),
+             "block_table is int32 [num_seqs, pages] with rows of unit stride, kv_lens int32 [num_seqs]")
+    _require(cu_q is None or (cu_q.dtype == torch.int32 and cu_q.shape == (n + 1,) and cu_q.is_contiguous()), "cu_q is int32 [num_seqs + 1]")
+    _require(max_q_len >= 1 and (cu_q is not None or tokens is None or tokens == n * max_q_len), "without cu_q every sequence has max_q_len tokens")
+    _require(n < 65536 and table.shape[1] >= 1, "at most 65535 sequences, of a page at least")
+    return n
+
+
+def _check_rows(q: torch.Tensor, kv_heads: int, width: int) -> int:
+    _require(q.dim() == 3 and q.stride(2) == 1 and q.shape[2] == width and q.shape[1] % kv_heads == 0 and 1 <= q.shape[1] // kv_heads <= MAX_GROUP,
+             "q is [T, heads, width], unit inner stride, up to 128 heads to a key/value head")
+    return q.shape[1] // kv_heads
+
+
+def summarize_pages(kcache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, summaries: PageSummaries, *, cu_q: torch.Tensor | None,
+                    max_q_len: int) -> None:
+    """Fills the summaries of the pages that the step's new tokens complete: the last tokens of each sequence, already in the cache (max_q_len bounds their
+    number). s = sum of a page's keys, a = max |s|: codes rint(127 s / a), scale a / (127 block_size); sums and quotient in 64 bits."""
+    codes, scales = summaries.codes, summaries.scales
+    _place(kcache, block_table, kv_lens, codes, scales, cu_q)
+    _check_cache(kcache)
+    n = _check_step(block_table, kv_lens, cu_q, max_q_len, None)
+    blocks, heads, bs, D = kcache.shape
+    _require(codes.dtype == torch.int8 and codes.shape == (blocks, heads, D) and codes.is_contiguous() and scales.dtype == torch.float32
+             and scales.shape == (blocks, heads) and scales.is_contiguous(), "summaries belong to these pages: int8 [blocks, kv heads, D], fp32 [blocks, kv heads]")
+    dims = (ctypes.c_int * 9)(n, max_q_len, block_table.shape[1], blocks, bs, heads, D, kcache.dtype == torch.float32, 0)
+    check(kernels().swb_page_summaries(dims, kcache.data_ptr(), codes.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), ptr(cu_q),
+                                       kv_lens.data_ptr(), stream_ptr()), "swb_page_summaries")
+
+
+def select_pages(q: torch.Tensor, summaries: PageSummaries, block_table: torch.Tensor, kv_lens: torch.Tensor, *, cu_q: torch.Tensor | None, max_q_len: int,
+                 block_size: int, top: int, first: int = 1, last: int = 4) -> PageSelection:
+    """The pages that each new token reads, per key/value head: its first `first`, its last `last` (its own page among them, at least one) and between these the
+    `top` of largest score, ties to the lowest page; all of them where that is no fewer. In ascending order.
+
+    q [T, Hq, D] bf16 or fp32 (token and head strides free). The group's queries are rounded to 8-bit codes of one step, max |q| / 127; score = the page's scale * max over the
+    group of the codes' dot product. A token whose queries are not all finite, or all zero, finds every page alike."""
+    codes, scales = summaries.codes, summaries.scales
+    _place(q, codes, scales, block_table, kv_lens, cu_q)
+    T = q.shape[0]
+    n = _check_step(block_table, kv_lens, cu_q, max_q_len, T)
+    _require(codes.dim() == 3 and codes.dtype == torch.int8 and codes.is_contiguous() and scales.dtype == torch.float32 and scales.shape == codes.shape[:2]
+             and scales.is_contiguous() and codes.shape[2] <= MAX_WIDTH, "summaries are int8 [blocks, kv heads, D] and fp32 [blocks, kv heads]")
+    blocks, heads, D = codes.shape
+    _require(q.dtype in (torch.bfloat16, torch.float32), "q is bf16 or fp32")
+    G = _check_rows(q, heads, D)
+    _require(block_size >= 1 and top >= 0 and first >= 0 and last >= 1, "block_size >= 1, top >= 0, first >= 0, last >= 1")
+    lib = kernels()
+    _require(lib.swb_page_select_smem(block_table.shape[1], G, D) <= SELECT_SMEM, "a selection is made over at most 200 KB of scores (4 bytes a page)")
+    pages = torch.empty((T, heads, first + top + last), dtype=torch.int32, device=q.device)
+    counts = torch.empty((T, heads), dtype=torch.int32, device=q.device)
+    dims = (ctypes.c_int * 14)(T, n, max_q_len, block_table.shape[1], blocks, block_size, heads, G, D, first, top, last, q.dtype == torch.float32, 0)
+    check(lib.swb_page_select(dims, q.data_ptr(), q.stride(0), q.stride(1), codes.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), ptr(cu_q),
+                              kv_lens.data_ptr(), pages.data_ptr(), counts.data_ptr(), stream_ptr()), "swb_page_select")
+    return PageSelection(pages, counts)
+
+
+def budget_splits(problems: int, keys: int, sms: int = 148) -> int:
+    """Blocks that share a problem's keys: two to an SM where problems (tokens * kv heads) are fewer, none of less than 64 keys."""
+    return max(1, min(2 * sms // max(1, problems), (keys + 63) // 64, MAX_SPLITS))
+
+
+def _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, softcap, num_splits, out, keys, selection=None, weights=None) -> torch.Tensor:
+    _place(q, kcache, vcache, block_table, kv_lens, cu_q, out, weights)
+    _check_cache(kcache, vcache)
+    T, Hq, D = q.shape
+    n = _check_step(block_table, kv_lens, cu_q, max_q_len, T)
+    blocks, heads, bs, _ = kcache.shape
+    Dv = vcache.shape[3]
+    G = _check_rows(q, heads, kcache.shape[3])
+    _require(q.dtype == kcache.dtype, "queries and cache have one type")
+    if out is None:
+        out = torch.empty((T, Hq * Dv), dtype=q.dtype, device=q.device)
+    _require(out.shape == (T, Hq * Dv) and out.dtype == q.dtype and out.stride(1) == 1, "out is [T, heads * value width] in the type of q, unit inner stride")
+    splits = budget_splits(T * heads, keys) if num_splits is None else num_splits
+    _require(1 <= splits <= MAX_SPLITS, "1 to 64 splits")
+    lib, capacity = kernels(), block_table.shape[1] * bs
+    nbytes = lib.swb_attn_budget_workspace(T, heads, G, Dv, splits, capacity, weights is not None)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None     # the call's own: two streams or graphs share none
+    width = selection.pages.shape[2] if selection is not None else 0
+    dims = (ctypes.c_int * 16)(T, n, max_q_len, block_table.shape[1], blocks, bs, heads, G, D, Dv, width, splits, q.dtype == torch.float32, 0, 0, 0)
+    w_seq, w_head = (weights.stride(0), weights.stride(1)) if weights is not None else (0, 0)
+    strides = (ctypes.c_longlong * 8)(q.stride(0), q.stride(1), out.stride(0), block_table.stride(0), w_seq, w_head, 0, 0)
+    check(lib.swb_attn_budget(dims, strides, q.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), block_table.data_ptr(), ptr(cu_q), kv_lens.data_ptr(),
+                              ptr(selection.pages) if selection is not None else None, ptr(selection.counts) if selection is not None else None, ptr(weights), scale,
+                              softcap, ptr(ws), nbytes, stream_ptr()), "swb_attn_budget")
+    return out
+
+
+def selected_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, selection: PageSelection, *,
+                       cu_q: torch.Tensor | None, max_q_len: int, scale: float, softcap: float = 0.0, num_splits: int | None = None,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of every new token over the pages selected for it, causal within them -> [T, Hq * Dv] in the type of q.
+
+    q [T, Hq, D] and the caches of one type. softcap > 0: scores s become softcap tanh(s / softcap). Lists may come from elsewhere than `select_pages`: in any order; pages that
+    a token does not see, or that are not in the table, add nothing; a page listed twice counts twice. A token without keys gets zeros."""
+    pages, counts = selection.pages, selection.counts
+    require_cuda(pages, counts)
+    _require(pages.dtype == counts.dtype == torch.int32 and pages.dim() == 3 and pages.shape[:2] == (q.shape[0], kcache.shape[1]) and counts.shape == pages.shape[:2]
+             and pages.shape[2] >= 1 and pages.is_contiguous() and counts.is_contiguous() and pages.device == counts.device == q.device,
+             "the selection is int32 [T, kv heads, N >= 1] and [T, kv heads], contiguous, beside q")
+    return _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, softcap, num_splits, out, min(pages.shape[2], block_table.shape[1]) * kcache.shape[2],
+                      selection=selection)
+
+
+def tracked_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, weights: torch.Tensor, *,
+                      cu_q: torch.Tensor | None, max_q_len: int, scale: float, softcap: float = 0.0, num_splits: int | None = None,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of every new token over all keys that it sees -> [T, Hq * Dv], which also adds the softmax weights of the step, summed over its tokens and the query heads of
+    a group, to weights fp32 [num_seqs, kv heads, >= table pages * block_size] (unit inner stride; entry j of a row belongs to cache entry j).
+
+    For decode steps, and for the last tokens of a prompt. Each token reads its keys on its own, and scores are kept until the sums are
+    known: 4 bytes a token, query head and key of the table's width."""
+    _require(weights.dim() == 3 and weights.dtype == torch.float32 and weights.stride(2) == 1 and weights.shape[:2] == (kv_lens.shape[0], kcache.shape[1])
+             and weights.shape[2] >= block_table.shape[1] * kcache.shape[2] and not _overlaps(weights), "weights are fp32 [num_seqs, kv heads, an entry for each the table has room for]")
+    return _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, softcap, num_splits, out, block_table.shape[1] * kcache.shape[2], weights=weights)
+
+
+def _overlaps(x: torch.Tensor) -> bool:
+    """Whether two rows of x [A, B, N] share memory (expanded or overlapping views), which calls that write them refuse."""
+    (a, sa), (b, sb) = sorted(((x.shape[i], x.stride(i)) for i in (0, 1)), key=lambda e: e[1])
+    return (a > 1 and sa < x.shape[2]) or (b > 1 and sb < (a - 1) * sa + x.shape[2])
+
+
+def evict_tokens(kcache: torch.Tensor, vcache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, weights: torch.Tensor, positions: torch.Tensor,
+                 next_positions: torch.Tensor, *, keep: int, recent: int, first: int = 0) -> torch.Tensor:
+    """Shrinks every sequence of more than `keep` cached tokens to `keep`, per key/value head, and returns the new lengths int32 [num_seqs].
+
+    A head keeps the entries whose position is below `first` or among the last `recent` in front of next_positions int32 [num_seqs] (the position of the
+    sequence's next token), and of the others those of largest weight (fp32 [num_seqs, kv heads, N], as `tracked_attention` adds them up; ties: the lowest index). Entries that stay
+    and lie behind `keep` move in order into the holes in front of it: their rows of both caches, weight and position. positions int32 [num_seqs, kv heads, N]: -1 for
+    entries without a record, which stand in order in front of the next position (all of them before the first call); the call records those it keeps. Weights behind `keep` become 0, positions -1.
+    Everything is done in place. Pages must not be shared with a sequence that is not to lose tokens, nor between sequences of the call (`PagedSequence.unshare`)."""
+    _place(kcache, vcache, block_table, kv_lens, weights, positions, next_positions)
+    _check_cache(kcache, vcache)
+    n = _check_step(block_table, kv_lens, None, 1, None)
+    blocks, heads, bs, D = kcache.shape
+    for name, t, kind in (("weights", weights, torch.float32), ("positions", positions, torch.int32)):
+        _require(t.dim() == 3 and t.dtype == kind and t.stride(2) == 1 and t.shape[:2] == (n, heads) and t.shape[2] >= block_table.shape[1] * bs and not _overlaps(t),
+                 f"{name} are {kind} [num_seqs, kv heads, an entry for each the table has room for]")
+    _require(next_positions.dtype == torch.int32 and next_positions.shape == (n,) and next_positions.is_contiguous(), "next_positions are int32 [num_seqs]")
+    _require(keep >= 1 and recent >= 0 and first >= 0 and recent + first <= keep, "0 <= first, recent; first + recent <= keep")
+    capacity, size = block_table.shape[1] * bs, kcache.element_size()
+    lib = kernels()
+    moves = torch.empty(lib.swb_evict_moves(n, heads, capacity, keep), dtype=torch.int32, device=kcache.device)
+    lens = torch.empty(n, dtype=torch.int32, device=kcache.device)
+    dims = (ctypes.c_int * 12)(n, heads, block_table.shape[1], blocks, bs, D * size, vcache.shape[3] * size, capacity, keep, recent, first, 0)
+    strides = (ctypes.c_longlong * 4)(weights.stride(0), weights.stride(1), positions.stride(0), positions.stride(1))
+    check(lib.swb_evict(dims, strides, kcache.data_ptr(), vcache.data_ptr(), block_table.data_ptr(), block_table.stride(0), kv_lens.data_ptr(), lens.data_ptr(),
+                        next_positions.data_ptr(), weights.data_ptr(), positions.data_ptr(), moves.data_ptr(), stream_ptr()), "swb_evict")
+    return lens
