@@ -10,11 +10,14 @@
 // Masked keys (behind what a token sees, on pages that are not there) take no part: their scores are -inf whatever the products were, and
 // their values are not multiplied at all, so that what the memory holds there does not matter.
 #include "attention_common.cuh"
+#include "gemm_tcgen05.cuh"
 
 #include <climits>
 
 namespace swb {
 using namespace attn;
+
+SWB_REGISTER_STATUS_UNIT(attn_budget);
 
 namespace {
 
@@ -44,6 +47,7 @@ struct BudgetParams {
   long long capacity;
   float* weights;            // [num_seqs, Hkv, .], inner stride 1
   long long w_seq, w_head;
+  int q_vec;                 // rows of q are 16-byte aligned
 };
 
 // What a query token is: its sequence and the keys it sees.
@@ -172,6 +176,277 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_budget_plain_kernel(const 
   }
 }
 
+// ---- bf16, widths up to 128, pages of 16-key groups: matrix instructions fed by TMA ------------------------------------------------------------------------
+//
+// Every warp runs on its own: it has a ring of groups of 16 keys (K and V, at most 4 KB each) that it fills with TMA boxes and empties itself, so that no
+// warp waits for another before the end. Group i of a block goes to warp i % 4. With queries as rows of 16, S = Q K^T leaves the weights of a head and pairs of
+// neighbouring keys in a thread, which is what the second operand of O^T = V^T P^T wants: nothing is moved in between, and heads
+// are the 8 columns of that product, so a group of up to 8 query heads wastes none of it.
+constexpr int FW = 4, FS = 3;                       // warps; groups in a warp's ring
+constexpr int HALF_BYTES = 2048, GROUP_BYTES = 4 * HALF_BYTES;      // 16 rows of 64 columns; K low, K high, V low, V high
+constexpr int SQ_BYTES = ROWS * 256, LDO = 132;
+constexpr int FAST_SMEM = 1024 + FW * FS * GROUP_BYTES + SQ_BYTES + 256;
+static_assert(FW * ROWS * LDO * 4 + FW * ROWS * 8 <= FW * FS * GROUP_BYTES, "the warps' results fit where the ring was");
+
+// 16-byte chunk c (0..15) of row r (0..15) of a K or V group: two boxes of 64 columns with the 128-byte swizzle
+__device__ __forceinline__ uint32_t group_off(int r, int c) { return (uint32_t)(((c >> 3) << 11) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
+__device__ __forceinline__ uint32_t q_off(int r, int c) { return (uint32_t)(r * 256 + ((c ^ (r & 7)) << 4)); }
+
+template <int NT>         // eights of query heads: 1 or 2
+__global__ void __launch_bounds__(FW * 32, 2) attn_budget_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const BudgetParams p) {
+  pdl_launch_dependents();
+  extern __shared__ uint8_t fast_smem[];
+  uint8_t* smem = fast_smem + ((1024u - (smem_u32(fast_smem) & 1023u)) & 1023u);
+  uint8_t* sQ = smem + FW * FS * GROUP_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sQ + SQ_BYTES);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(bars + FW * FS);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint8_t* ring = smem + warp * FS * GROUP_BYTES;
+  uint64_t* full = bars + warp * FS;
+  if (tid == 0) {
+    for (int i = 0; i < FW * FS; ++i) mbar_init(&bars[i], 1);
+    *s_abort = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  __syncthreads();
+  pdl_wait(TL_ATTN_DECODE);
+  const int S = p.num_splits, split = blockIdx.x % S, y = blockIdx.x / S, hy = y % (p.Hkv * p.head_tiles), t = y / (p.Hkv * p.head_tiles);
+  const int h = hy / p.head_tiles, ht = hy % p.head_tiles, g0 = ht * ROWS, rows = min(ROWS, p.G - g0);
+  if (p.cu_q && t >= p.cu_q[p.num_seqs]) return;
+  const Token tok = token_of(p, t);
+  const int sub = p.bs >> 4;                        // groups of a page
+  const size_t list = (size_t)t * p.Hkv + h;
+  const int* pages = p.pages ? p.pages + list * p.width : nullptr;
+  const int groups = p.pages ? min(max(p.counts[list], 0), p.width) * sub : (tok.seen + 15) >> 4;
+  const int per = (groups + S - 1) / S, lo = min(split * per, groups), n = min(groups, lo + per) - lo;
+  const int mine = n > warp ? (n - warp + FW - 1) / FW : 0;
+  const int k_halves = (p.D + 63) >> 6, v_halves = (p.Dv + 63) >> 6, boxes = k_halves + v_halves;
+  const int* table = p.table + tok.seq * p.table_stride;
+
+  // Rows and live keys of this warp's groups i0..i0 + 31, one to a lane.
+  int row_l = 0, live_l = 0;
+  const auto locate = [&](int i0) {
+    const int i = i0 + lane;
+    live_l = 0;
+    if (i < mine) {
+      const int g = lo + warp + i * FW, page = pages ? pages[g / sub] : g / sub, off = (g % sub) * 16;
+      if (page >= 0 && page < p.max_blocks) {
+        const int block = table[page];
+        live_l = (unsigned)block < (unsigned)p.num_blocks ? max(0, min(16, tok.seen - (page * p.bs + off))) : 0;
+        row_l = (block * p.Hkv + h) * p.bs + off;
+      }
+    }
+  };
+  int live_st = 0;                                  // lane s: live keys of the group in stage s
+  const auto issue = [&](int i, int stage) {
+    if (i >= mine) return;
+    if ((i & 31) == 0) locate(i);
+    const int row = __shfl_sync(0xffffffffu, row_l, i & 31), live = __shfl_sync(0xffffffffu, live_l, i & 31);
+    if (lane == stage) live_st = live;
+    if (live == 0) return;                          // nothing is read of a group without live keys
+    if (lane == 0) mbar_arrive_expect_tx(&full[stage], (uint32_t)boxes * HALF_BYTES);
+    __syncwarp();
+    if (lane < boxes) {
+      const bool is_k = lane < k_halves;
+      const int half = is_k ? lane : lane - k_halves;
+      tma_load_2d(ring + stage * GROUP_BYTES + (is_k ? 0 : 2 * HALF_BYTES) + half * HALF_BYTES, is_k ? &tmap_k : &tmap_v, &full[stage], half * 64, row);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < FS; ++i) issue(i, i);
+
+  const bf16* q = reinterpret_cast<const bf16*>(p.q) + t * p.q_stride_tok + (size_t)(h * p.G + g0) * p.q_stride_head;
+  for (int i = tid; i < ROWS * 16; i += FW * 32) {
+    const int r = i >> 4, c = i & 15;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (r < rows && c * 8 < p.D) {
+      const bf16* from = q + r * p.q_stride_head + c * 8;
+      if (p.q_vec) {
+        x = *reinterpret_cast<const uint4*>(from);
+      } else {
+        const uint16_t* w = reinterpret_cast<const uint16_t*>(from);
+        x = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+      }
+    }
+    *reinterpret_cast<uint4*>(sQ + q_off(r, c)) = x;
+  }
+  __syncthreads();
+  const int gr = lane >> 2, t4 = lane & 3, mi = lane >> 3;
+  uint32_t qf[8][4];
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) {
+    ldsm_x4(smem_u32(sQ) + q_off((mi & 1) * 8 + (lane & 7), kk * 2 + (mi >> 1)), qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3]);
+    if (NT == 1) qf[kk][1] = qf[kk][3] = 0u;        // rows 8..15 are no heads
+  }
+  const int k_steps = (p.D + 15) >> 4, v_steps = (p.Dv + 15) >> 4;
+
+  float o[NT][8][4], m[NT], l[NT];
+#pragma unroll
+  for (int x = 0; x < NT; ++x) {
+    m[x] = -INFINITY, l[x] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[x][i][0] = o[x][i][1] = o[x][i][2] = o[x][i][3] = 0.f;
+  }
+  float* score[NT];                                 // of this lane's heads, at the block's first key
+#pragma unroll
+  for (int x = 0; x < NT; ++x) {
+    const int r = gr + 8 * x;
+    score[x] = p.scores && r < rows ? p.scores + ((size_t)t * p.Hkv * p.G + h * p.G + g0 + r) * p.capacity + (size_t)lo * 16 : nullptr;
+  }
+  uint32_t phases = 0;
+  int stage = 0;
+  bool ok = true;
+  for (int i = 0; i < mine; ++i) {
+    const int live = __shfl_sync(0xffffffffu, live_st, stage);
+    if (live > 0) {
+      if (!mbar_wait(&full[stage], (phases >> stage) & 1u, s_abort, 700 + stage)) {
+        ok = false;
+        break;
+      }
+      phases ^= 1u << stage;
+      if (lane == stage) live_st = 0;               // nothing in flight there
+      const uint32_t sK = smem_u32(ring + stage * GROUP_BYTES), sV = sK + 2 * HALF_BYTES;
+      if (live < 16) {                              // what lies behind the last live key is not multiplied
+        for (int j = lane; j < (16 - live) * 8 * v_halves; j += 32) {
+          const int half = j / ((16 - live) * 8), at = j % ((16 - live) * 8);
+          *reinterpret_cast<uint4*>(ring + stage * GROUP_BYTES + (2 + half) * HALF_BYTES + live * 128 + at * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      float s[2][4];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        if (kk >= k_steps) break;
+        uint32_t b0, b1, b2, b3;
+        ldsm_x4(sK + group_off((mi >> 1) * 8 + (lane & 7), kk * 2 + (mi & 1)), b0, b1, b2, b3);
+        mma_16816(s[0], qf[kk], b0, b1);
+        mma_16816(s[1], qf[kk], b2, b3);
+      }
+      uint32_t pf[NT][2];
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+        float v[4];                                 // keys 2 t4, 2 t4 + 1, 8 + 2 t4, 9 + 2 t4 of head gr + 8 x
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = (e >> 1) * 8 + t4 * 2 + (e & 1);
+          const float raw = score_transform(s[e >> 1][2 * x + (e & 1)], p.scale, p.softcap);
+          v[e] = key < live ? raw : -INFINITY;
+        }
+        if (score[x]) {
+          float* to = score[x] + (size_t)(warp + i * FW) * 16 + t4 * 2;
+          *reinterpret_cast<float2*>(to) = make_float2(v[0], v[1]);
+          *reinterpret_cast<float2*>(to + 8) = make_float2(v[2], v[3]);
+        }
+        float top = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float now = fmaxf(m[x], top), base = now == -INFINITY ? 0.f : now;
+        if (__any_sync(0xffffffffu, now > m[x])) {  // otherwise every factor is one
+          const float alpha = exp2f(m[x] - base);
+          l[x] *= alpha;
+          const float a0 = __shfl_sync(0xffffffffu, alpha, t4 * 8), a1 = __shfl_sync(0xffffffffu, alpha, t4 * 8 + 4);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[x][j][0] *= a0, o[x][j][1] *= a1, o[x][j][2] *= a0, o[x][j][3] *= a1;
+          m[x] = now;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = exp2f(v[e] - base);
+        l[x] += (v[0] + v[1]) + (v[2] + v[3]);
+        pf[x][0] = pack_bf16(v[0], v[1]), pf[x][1] = pack_bf16(v[2], v[3]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j >= v_steps) break;
+        uint32_t a[4];
+        ldsm_x4_trans(sV + group_off((mi >> 1) * 8 + (lane & 7), j * 2 + (mi & 1)), a[0], a[1], a[2], a[3]);
+#pragma unroll
+        for (int x = 0; x < NT; ++x) mma_16816(o[x][j], a, pf[x][0], pf[x][1]);
+      }
+      __syncwarp();                                 // every lane has read the stage
+    } else {
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+        if (score[x]) {                             // a page that is not there: its keys weigh nothing
+          float* to = score[x] + (size_t)(warp + i * FW) * 16 + t4 * 2;
+          *reinterpret_cast<float2*>(to) = *reinterpret_cast<float2*>(to + 8) = make_float2(-INFINITY, -INFINITY);
+        }
+    }
+    issue(i + FS, stage);
+    if (++stage == FS) stage = 0;
+  }
+  if (!ok) {                                        // a wait ran out: let the copies in flight land before the memory goes away
+    for (int s = 0; s < FS; ++s)
+      for (int it = 0; __shfl_sync(0xffffffffu, live_st, s) > 0 && it < (1 << 20); ++it)
+        if (mbar_try_wait(&full[s], (phases >> s) & 1u)) break;
+  }
+  __syncthreads();                                  // the rings are free
+  float* sO = reinterpret_cast<float*>(smem);       // [FW][ROWS][LDO]
+  float* sM = sO + FW * ROWS * LDO;                 // [FW][ROWS][2]
+#pragma unroll
+  for (int x = 0; x < NT; ++x) {
+    float sum = l[x];
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    if (t4 == 0) *reinterpret_cast<float2*>(sM + (warp * ROWS + gr + 8 * x) * 2) = make_float2(m[x], sum);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sO[(warp * ROWS + 8 * x + t4 * 2 + (e & 1)) * LDO + j * 16 + gr + (e >> 1) * 8] = o[x][j][e];
+  }
+  __syncthreads();
+  const size_t problem = ((size_t)t * p.Hkv + h) * p.head_tiles + ht;
+  for (int i = tid; i < rows * p.Dv; i += FW * 32) {
+    const int r = i / p.Dv, d = i % p.Dv;
+    float M = -INFINITY, L = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < FW; ++w) M = fmaxf(M, sM[(w * ROWS + r) * 2]);
+    const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int w = 0; w < FW; ++w) {
+      const float e = exp2f(sM[(w * ROWS + r) * 2] - base);
+      L = fmaf(e, sM[(w * ROWS + r) * 2 + 1], L);
+      x = fmaf(e, sO[(w * ROWS + r) * LDO + d], x);
+    }
+    if (p.part_o) {
+      const size_t at = (problem * S + split) * ROWS + r;
+      p.part_o[at * p.Dv + d] = x;
+      if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(M, L);
+    } else {
+      reinterpret_cast<bf16*>(p.out)[t * p.out_stride_tok + (size_t)(h * p.G + g0 + r) * p.Dv + d] = __float2bfloat16(L == 0.f ? 0.f : x / L);
+    }
+  }
+}
+
+bool fast_fits(const BudgetParams& p, int fp32) {
+  return !fp32 && p.D % 8 == 0 && p.Dv % 8 == 0 && p.D <= 128 && p.Dv <= 128 && p.bs % 16 == 0 && (long long)p.num_blocks * p.Hkv * p.bs <= INT_MAX &&
+         ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) & 15) == 0;
+}
+
+int launch_fast(BudgetParams p, cudaStream_t s) {
+  p.q_vec = (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 && p.q_stride_tok % 8 == 0 && p.q_stride_head % 8 == 0;
+  CUtensorMap tk, tv;
+  const int rows = p.num_blocks * p.Hkv * p.bs;
+  int rc = make_tmap_bf16_2d(&tk, p.k, rows, p.D, p.D, 16);
+  if (rc) return rc;
+  rc = make_tmap_bf16_2d(&tv, p.v, rows, p.Dv, p.Dv, 16);
+  if (rc) return rc;
+  auto kernel = p.G <= 8 ? attn_budget_kernel<1> : attn_budget_kernel<2>;
+  static bool configured[2][64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[p.G <= 8][dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FAST_SMEM);
+    if (e != cudaSuccess) return -(int)e;
+    if (dev >= 0 && dev < 64) configured[p.G <= 8][dev] = true;
+  }
+  return launch_kernel(kernel, dim3(p.num_splits * p.Hkv * p.head_tiles * p.tokens), dim3(FW * 32), FAST_SMEM, s, tk, tv, p);
+}
+
 // ---- joining ------------------------------------------------------------------------------------------------------------------------------------------
 constexpr int JOIN_THREADS = 128, MAX_SPLITS = 64;
 
@@ -280,7 +555,7 @@ int swb_attn_budget(const int* dims, const long long* strides, const void* q, vo
       !k || !v || !table || !kv_lens)
     return -3;
   p.head_tiles = heads_in_tiles(p.G);
-  if ((long long)p.tokens * p.Hkv * p.head_tiles * p.num_splits > INT_MAX) return -3;
+  if ((long long)p.tokens * p.Hkv * p.head_tiles * p.num_splits > INT_MAX || (long long)p.max_blocks * p.bs > INT_MAX || (long long)p.width * p.bs > INT_MAX) return -3;
   p.q = q, p.out = out, p.k = k, p.v = v, p.table = table, p.cu_q = cu_q, p.kv_lens = kv_lens, p.pages = pages, p.counts = counts, p.weights = weights;
   p.q_stride_tok = strides[0], p.q_stride_head = strides[1], p.out_stride_tok = strides[2], p.table_stride = strides[3], p.w_seq = strides[4], p.w_head = strides[5];
   p.scale = scale, p.softcap = softcap, p.capacity = (long long)p.max_blocks * p.bs;
@@ -292,7 +567,7 @@ int swb_attn_budget(const int* dims, const long long* strides, const void* q, vo
     if (weights) p.scores = p.part_ml + rows * 2;
   }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  int rc = fp32 ? launch_plain<float>(p, s) : launch_plain<bf16>(p, s);
+  int rc = fast_fits(p, fp32) ? launch_fast(p, s) : fp32 ? launch_plain<float>(p, s) : launch_plain<bf16>(p, s);
   if (rc || !p.part_o) return rc;
   const dim3 grid(p.Hkv * p.head_tiles * p.tokens);
   rc = fp32 ? launch_kernel(attn_budget_join_kernel<float>, grid, dim3(JOIN_THREADS), 0, s, p)
