@@ -41,7 +41,8 @@ __device__ __forceinline__ int entry_position(const int* pos, int i, int len, in
 __global__ void __launch_bounds__(EVICT_THREADS, 1) evict_plan_kernel(const EvictParams p) {
   pdl_launch_dependents();
   extern __shared__ uint32_t evict_keys[];
-  __shared__ int hist[SELECT_BINS + 64];
+  __shared__ __align__(16) int hist[SELECT_INTS];
+  const Team<EVICT_THREADS> team(threadIdx.x);
   const int h = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait();
   const int len = min(p.kv_lens[seq], min(p.max_blocks * p.bs, p.capacity)), keep = p.keep;
@@ -63,32 +64,27 @@ __global__ void __launch_bounds__(EVICT_THREADS, 1) evict_plan_kernel(const Evic
     for (int i = tid; i < len; i += EVICT_THREADS) evict_keys[i] = fresh_key(i);
   const auto key = [&](int i) -> uint32_t { return cached ? evict_keys[i] : fresh_key(i); };
   __syncthreads();
-  const Threshold th = select_threshold<EVICT_THREADS>(key, len, keep, hist);
+  const Threshold th = select_threshold(team, key, len, keep, hist);
   const int seg = ((len + EVICT_THREADS - 1) / EVICT_THREADS) * 32;
   const int lo = min(warp * seg, len), hi = min(lo + seg, len);
   int eq = 0;
   for (int i = lo + lane; i < hi; i += 32) eq += key(i) == th.key;
-  const int eq_before = warps_before<EVICT_THREADS>(__reduce_add_sync(0xffffffffu, eq), hist);
-  int holes = 0, sources = 0;                  // of this lane
-  for_each_choice(key, th, lo, hi, eq_before, [&](int i, bool in, int) {
-    holes += i < keep && !in;
-    sources += i >= keep && in;
+  const int eq_before = warps_before(team, __reduce_add_sync(0xffffffffu, eq), hist);
+  int holes = 0, sources = 0;                  // of this warp's run
+  for_each_choice(key, th, lo, hi, eq_before, [&](int i, bool in, uint32_t) {
+    holes += __popc(__ballot_sync(0xffffffffu, i < keep && i < hi && !in));
+    sources += __popc(__ballot_sync(0xffffffffu, i >= keep && in));
   });
   int total = 0;
-  int hole_at = warps_before<EVICT_THREADS>(__reduce_add_sync(0xffffffffu, holes), hist, &total);
-  int source_at = warps_before<EVICT_THREADS>(__reduce_add_sync(0xffffffffu, sources), hist);
-  // whole warps visit 32 neighbours: their order within the warp is a population count away
-  for (int i0 = lo, eqb = eq_before; i0 < hi; i0 += 32) {
-    const int i = i0 + lane;
-    const uint32_t k = i < hi ? key(i) : 0u, below = (1u << lane) - 1u;
-    const uint32_t eqs = __ballot_sync(0xffffffffu, i < hi && k == th.key);
-    const bool in = i < hi && (k > th.key || (k == th.key && eqb + __popc(eqs & below) < th.ties));
-    const bool hole = i < hi && i < keep && !in, source = i >= keep && in;
-    const uint32_t hs = __ballot_sync(0xffffffffu, hole), ss = __ballot_sync(0xffffffffu, source);
+  int hole_at = warps_before(team, holes, hist, &total);
+  int source_at = warps_before(team, sources, hist);
+  for_each_choice(key, th, lo, hi, eq_before, [&](int i, bool in, uint32_t) {
+    const bool hole = i < keep && i < hi && !in, source = i >= keep && in;
+    const uint32_t hs = __ballot_sync(0xffffffffu, hole), ss = __ballot_sync(0xffffffffu, source), below = (1u << lane) - 1u;
     if (hole) moves[1 + hole_at + __popc(hs & below)] = i;
     if (source) moves[1 + p.max_moves + source_at + __popc(ss & below)] = i;
-    hole_at += __popc(hs), source_at += __popc(ss), eqb += __popc(eqs);
-  }
+    hole_at += __popc(hs), source_at += __popc(ss);
+  });
   if (tid == 0) moves[0] = total;
   __syncthreads();
   // weights and positions: records for what stays, then the moves, then the tail is cleared

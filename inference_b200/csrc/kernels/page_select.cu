@@ -89,92 +89,204 @@ struct SelectParams {
   int* counts;               // [tokens, Hkv]
 };
 
-constexpr int SELECT_THREADS = 256;
+constexpr int SELECT_THREADS = 256, SELECT_WARPS = SELECT_THREADS / 32;
 
-// A block per (token, head). Shared memory: keys [pages], codes of the group's queries [G, D rounded up to 16].
-template <typename E>
-__global__ void __launch_bounds__(SELECT_THREADS) page_select_kernel(const SelectParams p) {
+__device__ __forceinline__ void mma_s8(int* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Eight codes of a row from column d on, zeros behind its end.
+__device__ __forceinline__ uint2 load_codes(const int8_t* row, int d, int D, bool vec) {
+  uint2 x = make_uint2(0, 0);
+  if (d >= D) return x;
+  if (vec) return __ldg(reinterpret_cast<const uint2*>(row + d));
+  for (int i = 0; i < 8 && d + i < D; ++i) {
+    const uint32_t b = (uint32_t)(uint8_t)row[d + i];
+    if (i < 4) x.x |= b << (8 * i);
+    else x.y |= b << (8 * i - 32);
+  }
+  return x;
+}
+
+// A block per (run of TT tokens of a sequence, head). The dot products are 8-bit matrix products: 16 rows are the tokens' query heads (a token's heads are
+// filled up to a power of two, Gp, with copies of its first, which change no maximum), 8 columns are pages. A page's row is fetched in one piece: the lane of page g
+// and quarter t holds columns 32 s + 8 t and on of step s, and the queries' codes are read in the same order, so the order of the columns within a
+// step is another than the instruction's and the sum the same. A warp has 32 pages on their way at a time.
+// Then the tokens are shared out among teams of warps, each of which chooses among its token's scores.
+// Shared memory: the teams' histograms, codes of the queries [TT, G, 32 KS], keys [TT, pages].
+template <typename E, int TT, int KS>
+__global__ void __launch_bounds__(SELECT_THREADS, KS == 4 ? 3 : 2) page_select_kernel(const SelectParams p) {
+  constexpr int TEAM = SELECT_THREADS / TT, LD = 32 * KS;
   pdl_launch_dependents();
-  extern __shared__ uint4 select_smem[];
-  __shared__ int hist[SELECT_BINS + 64];
-  __shared__ float s_amax[SELECT_THREADS / 32];
-  __shared__ int s_bad;
+  extern __shared__ __align__(16) uint8_t select_smem[];
+  __shared__ float s_amax[SELECT_WARPS];
+  __shared__ int s_bad[TT];
+  const Team<TEAM> team(threadIdx.x);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int h = blockIdx.x % p.Hkv, t = blockIdx.x / p.Hkv;
-  const int Dp = (p.D + 15) & ~15;
-  int8_t* qc = reinterpret_cast<int8_t*>(select_smem);
-  uint32_t* keys = reinterpret_cast<uint32_t*>(qc + p.G * Dp);
-  if (tid == 0) s_bad = 0;
+  int* hist = reinterpret_cast<int*>(select_smem) + team.id * SELECT_INTS;
+  int8_t* qc = reinterpret_cast<int8_t*>(select_smem + TT * SELECT_INTS * 4);
+  uint32_t* keys = reinterpret_cast<uint32_t*>(qc + TT * p.G * LD);
+  const int h = blockIdx.x % p.Hkv, run = blockIdx.x / p.Hkv, runs = (p.uniform_q + TT - 1) / TT, seq = run / runs;
+  if (tid < TT) s_bad[tid] = 0;
   pdl_wait();
-  if (p.cu_q && t >= p.cu_q[p.num_seqs]) return;          // behind the last sequence
-  const int seq = seq_of_token(p.cu_q, p.num_seqs, p.uniform_q, t);
-  const int q0 = p.cu_q ? p.cu_q[seq] : seq * p.uniform_q, q_len = p.cu_q ? p.cu_q[seq + 1] - q0 : p.uniform_q;
-  const int seen = min(p.kv_lens[seq] - (q_len - 1 - (t - q0)), p.max_blocks * p.bs);
-  const int n = seen > 0 ? (seen + p.bs - 1) / p.bs : 0;
-  const int width = p.first + p.top + p.last;
+  const int q0 = p.cu_q ? p.cu_q[seq] : seq * p.uniform_q, q1 = p.cu_q ? p.cu_q[seq + 1] : q0 + p.uniform_q;
+  const int t0 = q0 + (run % runs) * TT;
+  if (t0 >= min(q1, p.tokens)) return;
+  const int len = p.kv_lens[seq], width = p.first + p.top + p.last;
+  const auto pages_of = [&](int t) {               // pages that token t sees
+    const int seen = min(len - (q1 - 1 - t), p.max_blocks * p.bs);
+    return seen > 0 ? (seen + p.bs - 1) / p.bs : 0;
+  };
+  // this team's token: what needs no scores
+  const int t = t0 + team.id, n = t < min(q1, p.tokens) ? pages_of(t) : 0;
   int* out = p.pages + ((size_t)t * p.Hkv + h) * width;
-  if (tid == 0) p.counts[(size_t)t * p.Hkv + h] = min(n, width);
-  if (n <= width) {
-    for (int i = tid; i < width; i += SELECT_THREADS) out[i] = i < n ? i : -1;
-    return;
-  }
-  for (int i = tid; i < p.first; i += SELECT_THREADS) out[i] = i;
-  for (int i = tid; i < p.last; i += SELECT_THREADS) out[p.first + p.top + i] = n - p.last + i;
-  if (p.top == 0) return;
-  __syncthreads();                                         // s_bad is set
-  // the group's queries as codes of one step
-  const E* q = reinterpret_cast<const E*>(p.q) + t * p.q_stride_tok + (size_t)h * p.G * p.q_stride_head;
-  float a = 0.f;
-  bool bad = false;
-  for (int i = tid; i < p.G * p.D; i += SELECT_THREADS) {
-    const float x = fabsf(to_f(q[(i / p.D) * p.q_stride_head + i % p.D]));
-    a = fmaxf(a, x);
-    bad |= !(x < INFINITY);
-  }
-  a = warp_max(a);
-  if (lane == 0) s_amax[warp] = a;
-  if (bad) s_bad = 1;
-  __syncthreads();
-  a = 0.f;
-#pragma unroll
-  for (int w = 0; w < SELECT_THREADS / 32; ++w) a = fmaxf(a, s_amax[w]);
-  bad = s_bad != 0;
-  for (int i = tid; i < p.G * Dp; i += SELECT_THREADS) {
-    const int g = i / Dp, d = i % Dp;
-    const float x = d < p.D ? to_f(q[g * p.q_stride_head + d]) : 0.f;
-    qc[i] = bad || a == 0.f ? (int8_t)0 : (int8_t)(int)rint(127.0 * (double)x / (double)a);
-  }
-  __syncthreads();
-  const int cand = n - p.first - p.last;
-  for (int i = tid; i < cand; i += SELECT_THREADS) {
-    const int block = p.table[seq * p.table_stride + p.first + i];
-    float score = -INFINITY;                               // a page that is not there ranks last
-    if ((unsigned)block < (unsigned)p.num_blocks) {
-      const size_t at = (size_t)block * p.Hkv + h;
-      const int8_t* c = p.codes + at * p.D;
-      int best = INT_MIN;
-      for (int g = 0; g < p.G; ++g) {
-        int dot = 0;
-        for (int d = 0; d < p.D; ++d) dot += (int)c[d] * (int)qc[g * Dp + d];
-        best = max(best, dot);
-      }
-      score = __fmul_rn((float)best, p.scales[at]);
+  if (t < min(q1, p.tokens)) {
+    if (team.rank == 0) p.counts[(size_t)t * p.Hkv + h] = min(n, width);
+    if (n <= width) {
+      for (int i = team.rank; i < width; i += TEAM) out[i] = i < n ? i : -1;
+    } else {
+      for (int i = team.rank; i < p.first; i += TEAM) out[i] = i;
+      for (int i = team.rank; i < p.last; i += TEAM) out[p.first + p.top + i] = n - p.last + i;
     }
-    keys[i] = float_key(score);
   }
-  const auto key = [&](int i) { return keys[i]; };
+  const int most = pages_of(min(min(t0 + TT, q1), p.tokens) - 1), cand = most - p.first - p.last;      // the last token sees most
+  if (p.top == 0 || most <= width) return;
+  __syncthreads();                                 // s_bad is set
+  // the token's queries as codes of one step
+  if (n > width) {
+    const E* q = reinterpret_cast<const E*>(p.q) + t * p.q_stride_tok + (size_t)h * p.G * p.q_stride_head;
+    float a = 0.f;
+    bool bad = false;
+    for (int g = 0; g < p.G; ++g)
+      for (int d = team.rank; d < p.D; d += TEAM) {
+        const float x = fabsf(to_f(q[g * p.q_stride_head + d]));
+        a = fmaxf(a, x);
+        bad |= !(x < INFINITY);
+      }
+    a = warp_max(a);
+    if (lane == 0) s_amax[warp] = a;
+    if (bad) s_bad[team.id] = 1;
+    team.sync();
+    a = 0.f;
+    for (int w = 0; w < Team<TEAM>::WARPS; ++w) a = fmaxf(a, s_amax[team.id * Team<TEAM>::WARPS + w]);
+    bad = s_bad[team.id] != 0;
+    int8_t* to = qc + team.id * p.G * LD;
+    for (int g = 0; g < p.G; ++g)
+      for (int d = team.rank; d < LD; d += TEAM) {
+        const float x = d < p.D ? to_f(q[g * p.q_stride_head + d]) : 0.f;
+        to[g * LD + d] = bad || a == 0.f ? (int8_t)0 : (int8_t)(int)rint(127.0 * (double)x / (double)a);
+      }
+  }
   __syncthreads();
-  const Threshold th = select_threshold<SELECT_THREADS>(key, cand, p.top, hist);
-  const int seg = ((cand + SELECT_THREADS - 1) / SELECT_THREADS) * 32;
-  const int lo = min(warp * seg, cand), hi = min(lo + seg, cand);
+
+  const int gr = lane >> 2, t4 = lane & 3;
+  int Gp = 1;
+  while (Gp < p.G && Gp < 16) Gp <<= 1;
+  const int row_tiles = (p.G + 15) / 16;           // more than one for one token only (TT Gp <= 16)
+  uint32_t a[KS][4];
+  const auto load_rows = [&](int tile) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = gr + 8 * half, tok = min(r / Gp, TT - 1), g = tile * 16 + r % Gp;
+      const uint2* from = reinterpret_cast<const uint2*>(qc + (tok * p.G + (g < p.G ? g : 0)) * LD);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const uint2 x = from[s * 4 + t4];
+        a[s][half] = x.x, a[s][2 + half] = x.y;
+      }
+    }
+  };
+  if (row_tiles == 1) load_rows(0);
+  const bool vec = (p.D & 7) == 0 && (reinterpret_cast<uintptr_t>(p.codes) & 7) == 0;
+  const int* table = p.table + seq * p.table_stride + p.first;
+  const auto locate = [&](int i) {
+    const int block = i < cand ? table[i] : -1;
+    return (unsigned)block < (unsigned)p.num_blocks ? block : -1;
+  };
+  int next = locate(warp * 32 + lane);
+  for (int i0 = warp * 32; i0 < cand; i0 += SELECT_THREADS) {
+    const int block = next;
+    const float scale = block >= 0 ? p.scales[(size_t)block * p.Hkv + h] : 0.f;
+    uint2 b[4][KS];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int mine = __shfl_sync(0xffffffffu, block, u * 8 + gr);
+      const int8_t* row = p.codes + ((size_t)max(mine, 0) * p.Hkv + h) * p.D;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) b[u][s] = mine >= 0 ? load_codes(row, s * 32 + t4 * 8, p.D, vec) : make_uint2(0, 0);
+    }
+    next = locate(i0 + SELECT_THREADS + lane);
+    const uint32_t there = __ballot_sync(0xffffffffu, block >= 0);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      int best[4] = {INT_MIN, INT_MIN, INT_MIN, INT_MIN};        // of the pages 2 t4 and 2 t4 + 1 for rows gr and gr + 8
+      for (int tile = 0; tile < row_tiles; ++tile) {
+        if (row_tiles > 1) load_rows(tile);
+        int c[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) mma_s8(c, a[s], b[u][s].x, b[u][s].y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) best[e] = max(best[e], c[e]);
+      }
+      // the maximum over a token's rows: lanes that differ in the low bits of gr, and both halves where it has 16
+      for (int o = 4; o < 4 * Gp && o < 32; o <<= 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) best[e] = max(best[e], __shfl_xor_sync(0xffffffffu, best[e], o));
+      }
+      if (Gp == 16) best[0] = max(best[0], best[2]), best[1] = max(best[1], best[3]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int page = u * 8 + t4 * 2 + (e & 1), r = gr + (e >> 1) * 8, tok = r / Gp;
+        const float sc = __shfl_sync(0xffffffffu, scale, page);
+        if (r % Gp == 0 && tok < TT && i0 + page < cand)
+          keys[tok * p.max_blocks + i0 + page] = float_key((there >> page) & 1u ? __fmul_rn((float)best[e], sc) : -INFINITY);
+      }
+    }
+  }
+  __syncthreads();
+  if (n <= width) return;                          // whole teams leave
+  const int want = n - p.first - p.last;           // this token's candidates
+  const uint32_t* own = keys + team.id * p.max_blocks;
+  const auto key = [&](int i) { return own[i]; };
+  const Threshold th = select_threshold(team, key, want, p.top, hist);
+  const int seg = ((want + TEAM - 1) / TEAM) * 32;
+  const int lo = min(team.warp() * seg, want), hi = min(lo + seg, want);
   int gt = 0, eq = 0;
-  for (int i = lo + lane; i < hi; i += 32) gt += keys[i] > th.key, eq += keys[i] == th.key;
+  for (int i = lo + lane; i < hi; i += 32) gt += own[i] > th.key, eq += own[i] == th.key;
   gt = __reduce_add_sync(0xffffffffu, gt), eq = __reduce_add_sync(0xffffffffu, eq);
-  const int eq_before = warps_before<SELECT_THREADS>(eq, hist), gt_before = warps_before<SELECT_THREADS>(gt, hist);
-  int* to = out + p.first + gt_before + min(eq_before, th.ties);
-  for_each_choice(key, th, lo, hi, eq_before, [&](int i, bool in, int before) {
-    if (in) to[before] = p.first + i;
+  const int eq_before = warps_before(team, eq, hist), gt_before = warps_before(team, gt, hist);
+  int at = p.first + gt_before + min(eq_before, th.ties);
+  for_each_choice(key, th, lo, hi, eq_before, [&](int i, bool in, uint32_t ins) {
+    if (in) out[at + __popc(ins & ((1u << lane) - 1u))] = p.first + i;
+    at += __popc(ins);
   });
+}
+
+// Tokens of a block: as many as the 16 rows of a product hold (4 at most), where sequences have them, as long as two blocks of an SM have room for the scores.
+int select_tokens(int uniform, int G, int pages) {
+  int TT = 1;
+  while (TT < 4 && TT * 2 * G <= 16 && TT < uniform && (long long)TT * 2 * pages * 4 <= 64 * 1024) TT *= 2;
+  return TT;
+}
+
+template <typename E, int TT, int KS>
+int launch_select(const SelectParams& p, cudaStream_t s) {
+  const size_t smem = TT * ((size_t)SELECT_INTS * 4 + (size_t)p.G * 32 * KS + 4 * (size_t)p.max_blocks);
+  auto kernel = page_select_kernel<E, TT, KS>;
+  if (smem > 47 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return -(int)e;
+  }
+  return launch_kernel(kernel, dim3((unsigned)(p.num_seqs * ((p.uniform_q + TT - 1) / TT) * p.Hkv)), dim3(SELECT_THREADS), smem, s, p);
+}
+
+template <typename E>
+int launch_select(const SelectParams& p, cudaStream_t s) {
+  const int TT = select_tokens(p.uniform_q, p.G, p.max_blocks);
+  if (p.D <= 128) return TT == 4 ? launch_select<E, 4, 4>(p, s) : TT == 2 ? launch_select<E, 2, 4>(p, s) : launch_select<E, 1, 4>(p, s);
+  return TT == 4 ? launch_select<E, 4, 8>(p, s) : TT == 2 ? launch_select<E, 2, 8>(p, s) : launch_select<E, 1, 8>(p, s);
 }
 
 }  // namespace
@@ -199,9 +311,9 @@ int swb_page_summaries(const int* dims, const void* k, void* codes, void* scales
 }
 
 // Bytes of shared memory that a selection over `pages` pages needs; above the limit of a block it is refused.
-long long swb_page_select_smem(int pages, int G, int D) { return (long long)G * ((D + 15) & ~15) + 4ll * pages; }
+long long swb_page_select_smem(int pages, int G, int D) { return 4ll * swb::SELECT_INTS + (long long)G * (D <= 128 ? 128 : 256) + 4ll * pages; }
 
-// See SelectParams. dims: host int[14] = tokens, num_seqs, tokens of each sequence (without cu_q), table width, blocks, block_size, Hkv, G, D, first,
+// See SelectParams. dims: host int[14] = tokens, num_seqs, tokens of each sequence (with cu_q: at most), table width, blocks, block_size, Hkv, G, D, first,
 // top, last, fp32, 0.
 int swb_page_select(const int* dims, const void* q, long long q_stride_tok, long long q_stride_head, const void* codes, const void* scales, const int* table,
                     long long table_stride, const int* cu_q, const int* kv_lens, int* pages, int* counts, void* stream) {
@@ -209,7 +321,7 @@ int swb_page_select(const int* dims, const void* q, long long q_stride_tok, long
   const int T = dims[0], seqs = dims[1], uniform = dims[2], max_blocks = dims[3], blocks = dims[4], bs = dims[5], Hkv = dims[6], G = dims[7], D = dims[8];
   const int first = dims[9], top = dims[10], last = dims[11], fp32 = dims[12];
   if (T <= 0 || seqs <= 0) return 0;
-  if ((long long)T * Hkv > INT_MAX || bs < 1 || Hkv < 1 || G < 1 || D < 1 || blocks < 1 || max_blocks < 1 || first < 0 || top < 0 || last < 1 || (!cu_q && uniform < 1) || !q || !codes ||
+  if ((long long)seqs * uniform * Hkv > INT_MAX || bs < 1 || Hkv < 1 || G < 1 || D < 1 || blocks < 1 || max_blocks < 1 || first < 0 || top < 0 || last < 1 || uniform < 1 || D > 256 || (long long)max_blocks * bs > INT_MAX || !q || !codes ||
       !scales || !table || !kv_lens || !pages || !counts)
     return -3;
   const long long smem = swb_page_select_smem(max_blocks, G, D);
@@ -217,12 +329,7 @@ int swb_page_select(const int* dims, const void* q, long long q_stride_tok, long
   const SelectParams p{q, q_stride_tok, q_stride_head, reinterpret_cast<const int8_t*>(codes), reinterpret_cast<const float*>(scales), table, table_stride,
                        max_blocks, blocks, bs, Hkv, G, D, cu_q, kv_lens, seqs, uniform, T, first, top, last, pages, counts};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  auto kernel = fp32 ? page_select_kernel<float> : page_select_kernel<bf16>;
-  if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return -(int)e;
-  }
-  return launch_kernel(kernel, dim3(Hkv * T), dim3(SELECT_THREADS), (size_t)smem, s, p);
+  return fp32 ? launch_select<float>(p, s) : launch_select<bf16>(p, s);
 }
 
 }  // extern "C"
