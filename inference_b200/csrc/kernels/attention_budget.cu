@@ -450,6 +450,25 @@ int launch_fast(BudgetParams p, cudaStream_t s) {
 // ---- joining ------------------------------------------------------------------------------------------------------------------------------------------
 constexpr int JOIN_THREADS = 128, MAX_SPLITS = 64;
 
+// {maximum, sum} of row r in each split of a problem -> factors of the splits' values, exp2(max - common) / sum: one warp, S <= 64.
+__device__ __forceinline__ void split_factors(const float* ml, int S, int lane, float* factor, float* common, float* inv_sum) {
+  float m[2], l[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int s = lane + 32 * i;
+    const float2 x = s < S ? __ldcg(reinterpret_cast<const float2*>(ml + (size_t)s * ROWS * 2)) : make_float2(-INFINITY, 0.f);
+    m[i] = x.x, l[i] = x.y;
+  }
+  const float M = warp_max(fmaxf(m[0], m[1])), base = M == -INFINITY ? 0.f : M;
+  const float e0 = exp2f(m[0] - base), e1 = exp2f(m[1] - base);
+  const float L = warp_sum(fmaf(e0, l[0], e1 * l[1])), inv = L == 0.f ? 0.f : 1.f / L;
+  if (factor) {
+    if (lane < S) factor[lane] = e0 * inv;
+    if (lane + 32 < S) factor[lane + 32] = e1 * inv;
+  }
+  if (common && lane == 0) *common = base, *inv_sum = inv;
+}
+
 // A block per problem: the parts of each row, weighed by their distance to the common maximum.
 template <typename E>
 __global__ void __launch_bounds__(JOIN_THREADS) attn_budget_join_kernel(const BudgetParams p) {
@@ -460,22 +479,14 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_budget_join_kernel(const Bu
   pdl_wait();
   if (p.cu_q && t >= p.cu_q[p.num_seqs]) return;
   const size_t problem = ((size_t)t * p.Hkv + h) * p.head_tiles + ht;
-  if (tid < rows) {
-    const float* ml = p.part_ml + (problem * S * ROWS + tid) * 2;
-    float M = -INFINITY, L = 0.f;
-    for (int s = 0; s < S; ++s) M = fmaxf(M, ml[(size_t)s * ROWS * 2]);
-    const float base = M == -INFINITY ? 0.f : M;
-    for (int s = 0; s < S; ++s) L += (s_w[tid][s] = exp2f(ml[(size_t)s * ROWS * 2] - base)) * ml[(size_t)s * ROWS * 2 + 1];
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    for (int s = 0; s < S; ++s) s_w[tid][s] *= inv;
-  }
+  for (int r = tid >> 5; r < rows; r += JOIN_THREADS / 32) split_factors(p.part_ml + (problem * S * ROWS + r) * 2, S, tid & 31, s_w[r], nullptr, nullptr);
   __syncthreads();
   for (int i = tid; i < rows * p.Dv; i += JOIN_THREADS) {
     const int r = i / p.Dv, d = i % p.Dv;
     const float* o = p.part_o + (problem * S * ROWS + r) * p.Dv + d;
     float x = 0.f;
-    for (int s = 0; s < S; ++s)
-      if (s_w[r][s] != 0.f) x = fmaf(s_w[r][s], o[(size_t)s * ROWS * p.Dv], x);
+#pragma unroll 8
+    for (int s = 0; s < S; ++s) x = fmaf(s_w[r][s], __ldcg(o + (size_t)s * ROWS * p.Dv), x);
     store_out(reinterpret_cast<E*>(p.out) + t * p.out_stride_tok + (size_t)(h * p.G + g0 + r) * p.Dv + d, x);
   }
 }
@@ -496,19 +507,15 @@ __global__ void __launch_bounds__(WEIGH_THREADS) attn_budget_weigh_kernel(const 
   for (int t = q0; t < q1; ++t) {
     const int seen = p.kv_lens[seq] - (q1 - 1 - t);
     __syncthreads();
-    for (int g = tid; g < p.G; g += WEIGH_THREADS) {
+    for (int g = tid >> 5; g < p.G; g += WEIGH_THREADS / 32) {
       const size_t problem = ((size_t)t * p.Hkv + h) * p.head_tiles + g / ROWS;
-      const float* ml = p.part_ml + (problem * S * ROWS + g % ROWS) * 2;
-      float M = -INFINITY, L = 0.f;
-      for (int s = 0; s < S; ++s) M = fmaxf(M, ml[(size_t)s * ROWS * 2]);
-      const float base = M == -INFINITY ? 0.f : M;
-      for (int s = 0; s < S; ++s) L += exp2f(ml[(size_t)s * ROWS * 2] - base) * ml[(size_t)s * ROWS * 2 + 1];
-      s_m[g] = base, s_inv[g] = L == 0.f ? 0.f : 1.f / L;
+      split_factors(p.part_ml + (problem * S * ROWS + g % ROWS) * 2, S, tid & 31, nullptr, &s_m[g], &s_inv[g]);
     }
     __syncthreads();
     if (j < seen && j < len) {
       const float* s = p.scores + ((size_t)t * p.Hkv + h) * p.G * p.capacity + j;
-      for (int g = 0; g < p.G; ++g) sum = fmaf(exp2f(s[g * p.capacity] - s_m[g]), s_inv[g], sum);
+#pragma unroll 4
+      for (int g = 0; g < p.G; ++g) sum = fmaf(exp2f(__ldcg(s + g * p.capacity) - s_m[g]), s_inv[g], sum);
     }
   }
   if (j < len) p.weights[seq * p.w_seq + h * p.w_head + j] += sum;

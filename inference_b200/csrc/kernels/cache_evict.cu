@@ -30,7 +30,7 @@ struct EvictParams {
   int max_moves;
 };
 
-constexpr int EVICT_THREADS = 1024;
+constexpr int EVICT_THREADS = 512;
 constexpr int EVICT_CACHED = 40960;            // keys held in shared memory; longer rows are read again in every pass
 
 __device__ __forceinline__ int entry_position(const int* pos, int i, int len, int next) {
@@ -38,7 +38,7 @@ __device__ __forceinline__ int entry_position(const int* pos, int i, int len, in
   return x >= 0 ? x : next - (len - i);
 }
 
-__global__ void __launch_bounds__(EVICT_THREADS, 1) evict_plan_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(EVICT_THREADS, 2) evict_plan_kernel(const EvictParams p) {
   pdl_launch_dependents();
   extern __shared__ uint32_t evict_keys[];
   __shared__ __align__(16) int hist[SELECT_INTS];
@@ -60,30 +60,35 @@ __global__ void __launch_bounds__(EVICT_THREADS, 1) evict_plan_kernel(const Evic
     return at < p.first || at >= next - p.recent ? 0xffffffffu : float_key(w[i]);
   };
   const bool cached = len <= EVICT_CACHED;
-  if (cached)
-    for (int i = tid; i < len; i += EVICT_THREADS) evict_keys[i] = fresh_key(i);
+  clear_bins(team, hist);
+  __syncthreads();
+  for (int i = tid; i < len; i += EVICT_THREADS) {
+    const uint32_t k = fresh_key(i);
+    if (cached) evict_keys[i] = k;
+    count_key(hist, k);
+  }
   const auto key = [&](int i) -> uint32_t { return cached ? evict_keys[i] : fresh_key(i); };
   __syncthreads();
   const Threshold th = select_threshold(team, key, len, keep, hist);
-  const int seg = ((len + EVICT_THREADS - 1) / EVICT_THREADS) * 32;
-  const int lo = min(warp * seg, len), hi = min(lo + seg, len);
-  int eq = 0;
-  for (int i = lo + lane; i < hi; i += 32) eq += key(i) == th.key;
-  const int eq_before = warps_before(team, __reduce_add_sync(0xffffffffu, eq), hist);
-  int holes = 0, sources = 0;                  // of this warp's run
-  for_each_choice(key, th, lo, hi, eq_before, [&](int i, bool in, uint32_t) {
-    holes += __popc(__ballot_sync(0xffffffffu, i < keep && i < hi && !in));
-    sources += __popc(__ballot_sync(0xffffffffu, i >= keep && in));
+  // Every warp has a run of the entries in front of `keep` and one of those behind. What is kept in front of a run follows from the keys above and equal
+  // to the threshold there, and holes are what is not kept in front of `keep`, sources what is kept behind.
+  const auto run = [&](int n) { return ((n + EVICT_THREADS - 1) / EVICT_THREADS) * 32; };
+  const int lo_a = min(warp * run(keep), keep), hi_a = min(lo_a + run(keep), keep);
+  const int lo_b = min(keep + warp * run(len - keep), len), hi_b = min(lo_b + run(len - keep), len);
+  const PairSums a = sum_over_warps(team, count_run(key, th, lo_a, hi_a), reinterpret_cast<int2*>(hist));
+  const PairSums b = sum_over_warps(team, count_run(key, th, lo_b, hi_b), reinterpret_cast<int2*>(hist) + 32);
+  const int kept_a = a.all.x + min(a.all.y, th.ties), total = keep - kept_a;
+  int hole_at = lo_a - (a.before.x + min(a.before.y, th.ties));
+  for_each_choice(key, th, lo_a, hi_a, a.before.y, [&](int i, bool in, uint32_t) {
+    const bool hole = i < hi_a && !in;
+    const uint32_t holes = __ballot_sync(0xffffffffu, hole);
+    if (hole) moves[1 + hole_at + __popc(holes & ((1u << lane) - 1u))] = i;
+    hole_at += __popc(holes);
   });
-  int total = 0;
-  int hole_at = warps_before(team, holes, hist, &total);
-  int source_at = warps_before(team, sources, hist);
-  for_each_choice(key, th, lo, hi, eq_before, [&](int i, bool in, uint32_t) {
-    const bool hole = i < keep && i < hi && !in, source = i >= keep && in;
-    const uint32_t hs = __ballot_sync(0xffffffffu, hole), ss = __ballot_sync(0xffffffffu, source), below = (1u << lane) - 1u;
-    if (hole) moves[1 + hole_at + __popc(hs & below)] = i;
-    if (source) moves[1 + p.max_moves + source_at + __popc(ss & below)] = i;
-    hole_at += __popc(hs), source_at += __popc(ss);
+  int source_at = a.all.x + b.before.x + min(a.all.y + b.before.y, th.ties) - kept_a;
+  for_each_choice(key, th, lo_b, hi_b, a.all.y + b.before.y, [&](int i, bool in, uint32_t ins) {
+    if (in) moves[1 + p.max_moves + source_at + __popc(ins & ((1u << lane) - 1u))] = i;
+    source_at += __popc(ins);
   });
   if (tid == 0) moves[0] = total;
   __syncthreads();

@@ -110,19 +110,27 @@ __device__ __forceinline__ uint2 load_codes(const int8_t* row, int d, int D, boo
   return x;
 }
 
+// rint(127 x / a), |x| <= a. Where both are bf16, 127 x has 15 bits and the quotient, a fraction over a's 8 bits and powers of two, is either a
+// half exactly or further from one than 2^-16 of itself: its rounding to 32 bits moves nothing across. Other numbers are divided in 64 bits.
+template <typename E>
+__device__ __forceinline__ int8_t query_code(float x, float a) {
+  if constexpr (sizeof(E) == 2) return (int8_t)(int)rintf(__fdiv_rn(127.f * x, a));
+  else return (int8_t)(int)rint(127.0 * (double)x / (double)a);
+}
+
 // A block per (run of TT tokens of a sequence, head). The dot products are 8-bit matrix products: 16 rows are the tokens' query heads (a token's heads are
 // filled up to a power of two, Gp, with copies of its first, which change no maximum), 8 columns are pages. A page's row is fetched in one piece: the lane of page g
 // and quarter t holds columns 32 s + 8 t and on of step s, and the queries' codes are read in the same order, so the order of the columns within a
-// step is another than the instruction's and the sum the same. A warp has 32 pages on their way at a time.
+// step is another than the instruction's and the sum the same. A warp looks 32 pages up at a time and has 16 of them on their way.
 // Then the tokens are shared out among teams of warps, each of which chooses among its token's scores.
 // Shared memory: the teams' histograms, codes of the queries [TT, G, 32 KS], keys [TT, pages].
 template <typename E, int TT, int KS>
-__global__ void __launch_bounds__(SELECT_THREADS, KS == 4 ? 3 : 2) page_select_kernel(const SelectParams p) {
+__global__ void __launch_bounds__(SELECT_THREADS, KS == 4 ? 4 : 2) page_select_kernel(const SelectParams p) {
   constexpr int TEAM = SELECT_THREADS / TT, LD = 32 * KS;
   pdl_launch_dependents();
   extern __shared__ __align__(16) uint8_t select_smem[];
   __shared__ float s_amax[SELECT_WARPS];
-  __shared__ int s_bad[TT];
+  __shared__ int s_bad[TT], s_cand[TT];           // s_cand: pages to choose among
   const Team<TEAM> team(threadIdx.x);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int* hist = reinterpret_cast<int*>(select_smem) + team.id * SELECT_INTS;
@@ -142,6 +150,7 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 4 ? 3 : 2) page_select_k
   // this team's token: what needs no scores
   const int t = t0 + team.id, n = t < min(q1, p.tokens) ? pages_of(t) : 0;
   int* out = p.pages + ((size_t)t * p.Hkv + h) * width;
+  if (team.rank == 0) s_cand[team.id] = n > width ? n - p.first - p.last : 0;
   if (t < min(q1, p.tokens)) {
     if (team.rank == 0) p.counts[(size_t)t * p.Hkv + h] = min(n, width);
     if (n <= width) {
@@ -153,7 +162,8 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 4 ? 3 : 2) page_select_k
   }
   const int most = pages_of(min(min(t0 + TT, q1), p.tokens) - 1), cand = most - p.first - p.last;      // the last token sees most
   if (p.top == 0 || most <= width) return;
-  __syncthreads();                                 // s_bad is set
+  clear_bins(team, hist);
+  __syncthreads();                                 // s_bad is set, the bins are clear
   // the token's queries as codes of one step
   if (n > width) {
     const E* q = reinterpret_cast<const E*>(p.q) + t * p.q_stride_tok + (size_t)h * p.G * p.q_stride_head;
@@ -176,7 +186,7 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 4 ? 3 : 2) page_select_k
     for (int g = 0; g < p.G; ++g)
       for (int d = team.rank; d < LD; d += TEAM) {
         const float x = d < p.D ? to_f(q[g * p.q_stride_head + d]) : 0.f;
-        to[g * LD + d] = bad || a == 0.f ? (int8_t)0 : (int8_t)(int)rint(127.0 * (double)x / (double)a);
+        to[g * LD + d] = bad || a == 0.f ? (int8_t)0 : query_code<E>(x, a);
       }
   }
   __syncthreads();
@@ -209,39 +219,45 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 4 ? 3 : 2) page_select_k
   for (int i0 = warp * 32; i0 < cand; i0 += SELECT_THREADS) {
     const int block = next;
     const float scale = block >= 0 ? p.scales[(size_t)block * p.Hkv + h] : 0.f;
-    uint2 b[4][KS];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int mine = __shfl_sync(0xffffffffu, block, u * 8 + gr);
-      const int8_t* row = p.codes + ((size_t)max(mine, 0) * p.Hkv + h) * p.D;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) b[u][s] = mine >= 0 ? load_codes(row, s * 32 + t4 * 8, p.D, vec) : make_uint2(0, 0);
-    }
-    next = locate(i0 + SELECT_THREADS + lane);
     const uint32_t there = __ballot_sync(0xffffffffu, block >= 0);
+    next = locate(i0 + SELECT_THREADS + lane);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      int best[4] = {INT_MIN, INT_MIN, INT_MIN, INT_MIN};        // of the pages 2 t4 and 2 t4 + 1 for rows gr and gr + 8
-      for (int tile = 0; tile < row_tiles; ++tile) {
-        if (row_tiles > 1) load_rows(tile);
-        int c[4] = {0, 0, 0, 0};
+    for (int u0 = 0; u0 < 4; u0 += 2) {
+      uint2 b[2][KS];
 #pragma unroll
-        for (int s = 0; s < KS; ++s) mma_s8(c, a[s], b[u][s].x, b[u][s].y);
+      for (int u = 0; u < 2; ++u) {
+        const int mine = __shfl_sync(0xffffffffu, block, (u0 + u) * 8 + gr);
+        const int8_t* row = p.codes + ((size_t)max(mine, 0) * p.Hkv + h) * p.D;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) best[e] = max(best[e], c[e]);
+        for (int s = 0; s < KS; ++s) b[u][s] = mine >= 0 ? load_codes(row, s * 32 + t4 * 8, p.D, vec) : make_uint2(0, 0);
       }
-      // the maximum over a token's rows: lanes that differ in the low bits of gr, and both halves where it has 16
-      for (int o = 4; o < 4 * Gp && o < 32; o <<= 1) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) best[e] = max(best[e], __shfl_xor_sync(0xffffffffu, best[e], o));
-      }
-      if (Gp == 16) best[0] = max(best[0], best[2]), best[1] = max(best[1], best[3]);
+      for (int u = 0; u < 2; ++u) {
+        int best[4] = {INT_MIN, INT_MIN, INT_MIN, INT_MIN};      // of the pages 2 t4 and 2 t4 + 1 for rows gr and gr + 8
+        for (int tile = 0; tile < row_tiles; ++tile) {
+          if (row_tiles > 1) load_rows(tile);
+          int c[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int page = u * 8 + t4 * 2 + (e & 1), r = gr + (e >> 1) * 8, tok = r / Gp;
-        const float sc = __shfl_sync(0xffffffffu, scale, page);
-        if (r % Gp == 0 && tok < TT && i0 + page < cand)
-          keys[tok * p.max_blocks + i0 + page] = float_key((there >> page) & 1u ? __fmul_rn((float)best[e], sc) : -INFINITY);
+          for (int s = 0; s < KS; ++s) mma_s8(c, a[s], b[u][s].x, b[u][s].y);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) best[e] = max(best[e], c[e]);
+        }
+        // the maximum over a token's rows: lanes that differ in the low bits of gr, and both halves where it has 16
+        for (int o = 4; o < 4 * Gp && o < 32; o <<= 1) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) best[e] = max(best[e], __shfl_xor_sync(0xffffffffu, best[e], o));
+        }
+        if (Gp == 16) best[0] = max(best[0], best[2]), best[1] = max(best[1], best[3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int page = (u0 + u) * 8 + t4 * 2 + (e & 1), r = gr + (e >> 1) * 8, tok = r / Gp;
+          const float sc = __shfl_sync(0xffffffffu, scale, page);
+          if (r % Gp == 0 && tok < TT && i0 + page < s_cand[tok]) {
+            const uint32_t k = float_key((there >> page) & 1u ? __fmul_rn((float)best[e], sc) : -INFINITY);
+            keys[tok * p.max_blocks + i0 + page] = k;
+            count_key(reinterpret_cast<int*>(select_smem) + tok * SELECT_INTS, k);
+          }
+        }
       }
     }
   }
@@ -253,12 +269,9 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 4 ? 3 : 2) page_select_k
   const Threshold th = select_threshold(team, key, want, p.top, hist);
   const int seg = ((want + TEAM - 1) / TEAM) * 32;
   const int lo = min(team.warp() * seg, want), hi = min(lo + seg, want);
-  int gt = 0, eq = 0;
-  for (int i = lo + lane; i < hi; i += 32) gt += own[i] > th.key, eq += own[i] == th.key;
-  gt = __reduce_add_sync(0xffffffffu, gt), eq = __reduce_add_sync(0xffffffffu, eq);
-  const int eq_before = warps_before(team, eq, hist), gt_before = warps_before(team, gt, hist);
-  int at = p.first + gt_before + min(eq_before, th.ties);
-  for_each_choice(key, th, lo, hi, eq_before, [&](int i, bool in, uint32_t ins) {
+  const PairSums sums = sum_over_warps(team, count_run(key, th, lo, hi), reinterpret_cast<int2*>(hist));
+  int at = p.first + sums.before.x + min(sums.before.y, th.ties);
+  for_each_choice(key, th, lo, hi, sums.before.y, [&](int i, bool in, uint32_t ins) {
     if (in) out[at + __popc(ins & ((1u << lane) - 1u))] = p.first + i;
     at += __popc(ins);
   });

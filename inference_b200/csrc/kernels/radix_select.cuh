@@ -28,70 +28,101 @@ struct Team {
   }
 };
 
-// The `want`-th largest of the n keys (1 <= want <= n): keys above `key` are in, and of those equal to it the first `ties`.
+// The `want`-th largest of n keys (1 <= want <= n): keys above `key` are in, and of those equal to it the first `ties`.
 struct Threshold {
   uint32_t key;
   int ties;
 };
 
-// Three rounds over the keys (11, 11 and 10 bits from the top): a histogram of the keys that agree with the digits found so far, then the bin
-// in which the count from above reaches `want`. Counts are whole numbers, so the result does not depend on the order of the atomics. The first digit is
-// a sign, an exponent and two bits more: numbers of one spread fall into some twenty bins, so that few lanes of a warp meet in one. `hist` holds SELECT_INTS ints
-// of shared memory of 16-byte alignment; the whole team calls it (it begins with a barrier, behind which the keys are read).
-template <int SIZE, typename Key>
-__device__ Threshold select_threshold(const Team<SIZE>& team, const Key& key, int n, int want, int* hist) {
+// Histogram of the first digit, 11 bits from the top: a sign, an exponent and two bits more, so numbers of one spread fall into some twenty bins and few lanes
+// of a warp meet in one. The caller clears the bins, adds every key once, and puts the team's barrier behind each of both. `hist`: SELECT_INTS ints of shared
+// memory with 16-byte alignment.
+template <int SIZE>
+__device__ __forceinline__ void clear_bins(const Team<SIZE>& team, int* hist) {
+  for (int i = team.rank; i < SELECT_BINS / 4; i += SIZE) reinterpret_cast<int4*>(hist)[i] = make_int4(0, 0, 0, 0);
+}
+__device__ __forceinline__ void count_key(int* hist, uint32_t key) { atomicAdd(&hist[key >> 21], 1); }
+
+// The bin in which the count from the top reaches `want`, in totals: {bin, what is left to find in it, its count, 0}. Ends with a barrier.
+template <int SIZE>
+__device__ __forceinline__ void find_bin(const Team<SIZE>& team, const int* hist, int want, int* totals) {
   constexpr int PER = SELECT_BINS / SIZE;
   static_assert(SELECT_BINS % SIZE == 0 && PER >= 2 && SIZE <= 1024, "bins are shared out evenly");
-  int* totals = hist + SELECT_BINS;            // [32] of the warps, then {bin, left}
-  const int lane = team.lane();
-  uint32_t prefix = 0, mask = 0;
+  // the thread of rank r holds the r-th run of PER bins from the top
+  const int* run = hist + SELECT_BINS - (team.rank + 1) * PER;
+  int mine[PER], sum = 0;
+  if constexpr (PER % 4 == 0) {
+#pragma unroll
+    for (int j = 0; j < PER; j += 4) *reinterpret_cast<int4*>(mine + j) = *reinterpret_cast<const int4*>(run + j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) mine[j] = run[j];
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) sum += mine[j];
+  int incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (team.lane() >= o) incl += v;
+  }
+  if (team.lane() == 31) totals[team.warp()] = incl;
+  team.sync();
+  int before = incl - sum;
+  for (int w = 0; w < team.warp(); ++w) before += totals[w];
+  if (before < want && want <= before + sum) {
+#pragma unroll
+    for (int j = PER - 1; j >= 0; --j) {
+      if (before < want && want <= before + mine[j])
+        totals[32] = SELECT_BINS - (team.rank + 1) * PER + j, totals[33] = want - before, totals[34] = mine[j], totals[35] = 0;
+      before += mine[j];
+    }
+  }
+  team.sync();
+}
+
+// From the first digit's histogram on. A bin with no more keys than the team has threads is gathered and every thread counts what lies above its key; a fuller
+// one is taken apart by its other 21 bits. Counts are whole numbers, so the result does not depend on the order of the atomics. The bins' memory is
+// free afterwards (behind a barrier of the team).
+template <int SIZE, typename Key>
+__device__ Threshold select_threshold(const Team<SIZE>& team, const Key& key, int n, int want, int* hist) {
+  int* totals = hist + SELECT_BINS;            // [32] of the warps, then find_bin's, then {key, ties}
+  find_bin(team, hist, want, totals);
+  const uint32_t bin = (uint32_t)totals[32];
+  const int left = totals[33], m = totals[34];
+  if (m <= SIZE) {
+    uint32_t* list = reinterpret_cast<uint32_t*>(hist);
+    for (int i = team.rank; i < n; i += SIZE) {
+      const uint32_t k = key(i);
+      if ((k >> 21) == bin) list[atomicAdd(&totals[35], 1)] = k;
+    }
+    team.sync();
+    if (team.rank < m) {
+      const uint32_t mine = list[team.rank];
+      int above = 0, same = 0;
+      for (int j = 0; j < m; ++j) above += list[j] > mine, same += list[j] == mine;
+      if (above < left && left <= above + same) totals[36] = (int)mine, totals[37] = left - above;      // one key fits: its owners write the same
+    }
+    team.sync();
+    return Threshold{(uint32_t)totals[36], totals[37]};
+  }
+  uint32_t prefix = bin << 21, mask = 0x7ffu << 21;
+  want = left;
 #pragma unroll 1
-  for (int round = 0; round < 3; ++round) {
-    const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, width = round == 2 ? 10 : 11;
-    for (int i = team.rank; i < SELECT_BINS / 4; i += SIZE) reinterpret_cast<int4*>(hist)[i] = make_int4(0, 0, 0, 0);
+  for (int round = 0; round < 2; ++round) {
+    const int shift = round == 0 ? 10 : 0;
+    const uint32_t digit = round == 0 ? 0x7ffu : 0x3ffu;
+    clear_bins(team, hist);                    // every thread is past its reads of the bins: find_bin ended with a barrier
     team.sync();
     for (int i = team.rank; i < n; i += SIZE) {
       const uint32_t k = key(i);
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << width) - 1u)], 1);
+      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digit], 1);
     }
     team.sync();
-    // the thread of rank r holds the r-th run of PER bins from the top
-    const int* run = hist + SELECT_BINS - (team.rank + 1) * PER;
-    int mine[PER], sum = 0;
-    if constexpr (PER % 4 == 0) {
-#pragma unroll
-      for (int j = 0; j < PER; j += 4) *reinterpret_cast<int4*>(mine + j) = *reinterpret_cast<const int4*>(run + j);
-    } else {
-#pragma unroll
-      for (int j = 0; j < PER; ++j) mine[j] = run[j];
-    }
-#pragma unroll
-    for (int j = 0; j < PER; ++j) sum += mine[j];
-    int incl = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    if (lane == 31) totals[team.warp()] = incl;
-    team.sync();
-    int before = incl - sum;
-    for (int w = 0; w < team.warp(); ++w) before += totals[w];
-    if (before < want && want <= before + sum) {
-#pragma unroll
-      for (int j = PER - 1; j >= 0; --j) {
-        if (before < want && want <= before + mine[j]) {
-          totals[32] = SELECT_BINS - (team.rank + 1) * PER + j;
-          totals[33] = want - before;
-        }
-        before += mine[j];
-      }
-    }
-    team.sync();
+    find_bin(team, hist, want, totals);
     prefix |= (uint32_t)totals[32] << shift;
-    mask |= ((1u << width) - 1u) << shift;
+    mask |= digit << shift;
     want = totals[33];
-    // the next round's first barrier stands between these reads and the next writes of `totals`
   }
   return Threshold{prefix, want};
 }
@@ -112,20 +143,33 @@ __device__ __forceinline__ void for_each_choice(const Key& key, const Threshold&
   }
 }
 
-// Exclusive sum of `v` (one value of each warp, given by all its lanes) over the team's warps in front; `slot` holds 32 ints. Begins and ends with a barrier.
+// Exclusive sums of `v` (one pair of each warp, given by all its lanes) over the team's warps in front, and those of all. `slot` holds 32 pairs that nobody reads or
+// writes around the call; a barrier stands within.
+struct PairSums {
+  int2 before, all;
+};
 template <int SIZE>
-__device__ __forceinline__ int warps_before(const Team<SIZE>& team, int v, int* slot, int* total = nullptr) {
-  team.sync();
+__device__ __forceinline__ PairSums sum_over_warps(const Team<SIZE>& team, int2 v, int2* slot) {
   if (team.lane() == 0) slot[team.warp()] = v;
   team.sync();
-  int before = 0, all = 0;
+  PairSums s{make_int2(0, 0), make_int2(0, 0)};
   for (int w = 0; w < Team<SIZE>::WARPS; ++w) {
-    if (w == team.warp()) before = all;
-    all += slot[w];
+    if (w == team.warp()) s.before = s.all;
+    const int2 x = slot[w];
+    s.all.x += x.x, s.all.y += x.y;
   }
-  if (total) *total = all;
-  team.sync();
-  return before;
+  return s;
+}
+
+// How many keys of a warp's run lie above the threshold, and how many are equal to it.
+template <typename Key>
+__device__ __forceinline__ int2 count_run(const Key& key, const Threshold& t, int first, int last) {
+  int above = 0, same = 0;
+  for (int i = first + (int)(threadIdx.x & 31); i < last; i += 32) {
+    const uint32_t k = key(i);
+    above += k > t.key, same += k == t.key;
+  }
+  return make_int2(__reduce_add_sync(0xffffffffu, above), __reduce_add_sync(0xffffffffu, same));
 }
 
 }  // namespace swb
