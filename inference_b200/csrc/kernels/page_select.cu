@@ -87,6 +87,7 @@ struct SelectParams {
   int first, top, last;
   int* pages;                // [tokens, Hkv, first + top + last]
   int* counts;               // [tokens, Hkv]
+  int fp32;                  // type of q
 };
 
 constexpr int SELECT_THREADS = 256, SELECT_WARPS = SELECT_THREADS / 32;
@@ -97,8 +98,10 @@ __device__ __forceinline__ void mma_s8(int* c, const uint32_t* a, uint32_t b0, u
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Eight codes of a row from column d on, zeros behind its end.
+// Eight codes of a row from column d on, zeros behind its end. FULL: rows are 32 KS codes, 8-byte aligned.
+template <bool FULL>
 __device__ __forceinline__ uint2 load_codes(const int8_t* row, int d, int D, bool vec) {
+  if (FULL) return __ldg(reinterpret_cast<const uint2*>(row + d));
   uint2 x = make_uint2(0, 0);
   if (d >= D) return x;
   if (vec) return __ldg(reinterpret_cast<const uint2*>(row + d));
@@ -110,21 +113,24 @@ __device__ __forceinline__ uint2 load_codes(const int8_t* row, int d, int D, boo
   return x;
 }
 
-// rint(127 x / a), |x| <= a. Where both are bf16, 127 x has 15 bits and the quotient, a fraction over a's 8 bits and powers of two, is either a
-// half exactly or further from one than 2^-16 of itself: its rounding to 32 bits moves nothing across. Other numbers are divided in 64 bits.
-template <typename E>
-__device__ __forceinline__ int8_t query_code(float x, float a) {
-  if constexpr (sizeof(E) == 2) return (int8_t)(int)rintf(__fdiv_rn(127.f * x, a));
-  else return (int8_t)(int)rint(127.0 * (double)x / (double)a);
+__device__ __forceinline__ float load_query(const SelectParams& p, long long at) {
+  return p.fp32 ? reinterpret_cast<const float*>(p.q)[at] : __bfloat162float(reinterpret_cast<const bf16*>(p.q)[at]);
 }
 
-// A block per (run of TT tokens of a sequence, head). The dot products are 8-bit matrix products: 16 rows are the tokens' query heads (a token's heads are
-// filled up to a power of two, Gp, with copies of its first, which change no maximum), 8 columns are pages. A page's row is fetched in one piece: the lane of page g
-// and quarter t holds columns 32 s + 8 t and on of step s, and the queries' codes are read in the same order, so the order of the columns within a
-// step is another than the instruction's and the sum the same. A warp looks 32 pages up at a time and has 16 of them on their way.
+// rint(127 x / a), |x| <= a. Where both are bf16, 127 x has 15 bits and the quotient, a fraction over a's 8 bits and powers of two, is either a
+// half exactly or further from one than 2^-16 of itself: its rounding to 32 bits moves nothing across. Other numbers are divided in 64 bits.
+__device__ __forceinline__ int8_t query_code(float x, float a, bool fp32) {
+  return fp32 ? (int8_t)(int)rint(127.0 * (double)x / (double)a) : (int8_t)(int)rintf(__fdiv_rn(127.f * x, a));
+}
+
+// A block per (run of TT tokens of a sequence, head). The dot products are 8-bit matrix products: 16 rows are pages, 8 columns the tokens' query heads (a token's heads
+// are filled up to a power of two, Gp, with copies of its first, which change no maximum), so that a head's neighbours are a thread's own or a shuffle away and
+// every thread ends with one page's score for one token. A page's row is fetched in one piece: the lane of page g and quarter t holds columns 32 s + 8 t and on of
+// step s, and the queries' codes are read in the same order, so the order of the columns within a step is another than the instruction's and the
+// sum the same. A warp looks 32 pages up at a time and has 16 of them on their way.
 // Then the tokens are shared out among teams of warps, each of which chooses among its token's scores.
 // Shared memory: the teams' histograms, codes of the queries [TT, G, 32 KS], keys [TT, pages].
-template <typename E, int TT, int KS>
+template <int TT, int KS, bool FULL>
 __global__ void __launch_bounds__(SELECT_THREADS, KS == 4 ? 4 : 2) page_select_kernel(const SelectParams p) {
   constexpr int TEAM = SELECT_THREADS / TT, LD = 32 * KS;
   pdl_launch_dependents();
@@ -166,12 +172,12 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 4 ? 4 : 2) page_select_k
   __syncthreads();                                 // s_bad is set, the bins are clear
   // the token's queries as codes of one step
   if (n > width) {
-    const E* q = reinterpret_cast<const E*>(p.q) + t * p.q_stride_tok + (size_t)h * p.G * p.q_stride_head;
+    const long long q = t * p.q_stride_tok + (long long)h * p.G * p.q_stride_head;
     float a = 0.f;
     bool bad = false;
     for (int g = 0; g < p.G; ++g)
       for (int d = team.rank; d < p.D; d += TEAM) {
-        const float x = fabsf(to_f(q[g * p.q_stride_head + d]));
+        const float x = fabsf(load_query(p, q + g * p.q_stride_head + d));
         a = fmaxf(a, x);
         bad |= !(x < INFINITY);
       }
@@ -185,35 +191,40 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 4 ? 4 : 2) page_select_k
     int8_t* to = qc + team.id * p.G * LD;
     for (int g = 0; g < p.G; ++g)
       for (int d = team.rank; d < LD; d += TEAM) {
-        const float x = d < p.D ? to_f(q[g * p.q_stride_head + d]) : 0.f;
-        to[g * LD + d] = bad || a == 0.f ? (int8_t)0 : query_code<E>(x, a);
+        const float x = d < p.D ? load_query(p, q + g * p.q_stride_head + d) : 0.f;
+        to[g * LD + d] = bad || a == 0.f ? (int8_t)0 : query_code(x, a, p.fp32);
       }
   }
   __syncthreads();
 
+  constexpr int NT = TT == 4 ? 2 : 1;              // products beside each other: TT Gp <= 8 NT, or one token in turns of 8 heads
   const int gr = lane >> 2, t4 = lane & 3;
   int Gp = 1;
-  while (Gp < p.G && Gp < 16) Gp <<= 1;
-  const int row_tiles = (p.G + 15) / 16;           // more than one for one token only (TT Gp <= 16)
-  uint32_t a[KS][4];
-  const auto load_rows = [&](int tile) {
+  while (Gp < p.G && Gp < 8) Gp <<= 1;
+  const int turns = TT == 1 ? (p.G + 7) / 8 : 1;
+  uint2 b[NT][KS];
+  const auto load_heads = [&](int turn) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int r = gr + 8 * half, tok = min(r / Gp, TT - 1), g = tile * 16 + r % Gp;
+    for (int x = 0; x < NT; ++x) {
+      const int c = x * 8 + gr, tok = min(c / Gp, TT - 1), g = turn * 8 + c % Gp;
       const uint2* from = reinterpret_cast<const uint2*>(qc + (tok * p.G + (g < p.G ? g : 0)) * LD);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const uint2 x = from[s * 4 + t4];
-        a[s][half] = x.x, a[s][2 + half] = x.y;
-      }
+      for (int s = 0; s < KS; ++s) b[x][s] = from[s * 4 + t4];
     }
   };
-  if (row_tiles == 1) load_rows(0);
+  if (turns == 1) load_heads(0);
   const bool vec = (p.D & 7) == 0 && (reinterpret_cast<uintptr_t>(p.codes) & 7) == 0;
   const int* table = p.table + seq * p.table_stride + p.first;
   const auto locate = [&](int i) {
     const int block = i < cand ? table[i] : -1;
     return (unsigned)block < (unsigned)p.num_blocks ? block : -1;
+  };
+  // keeps the score of page i (in bounds: less than the token's own number) for a token
+  const auto keep = [&](int tok, int i, int best, float scale, bool there) {
+    if (tok >= TT || i >= s_cand[tok]) return;
+    const uint32_t k = float_key(there ? __fmul_rn((float)best, scale) : -INFINITY);
+    keys[tok * p.max_blocks + i] = k;
+    count_key(reinterpret_cast<int*>(select_smem) + tok * SELECT_INTS, k);
   };
   int next = locate(warp * 32 + lane);
   for (int i0 = warp * 32; i0 < cand; i0 += SELECT_THREADS) {
@@ -222,40 +233,64 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 4 ? 4 : 2) page_select_k
     const uint32_t there = __ballot_sync(0xffffffffu, block >= 0);
     next = locate(i0 + SELECT_THREADS + lane);
 #pragma unroll
-    for (int u0 = 0; u0 < 4; u0 += 2) {
-      uint2 b[2][KS];
+    for (int u = 0; u < 2; ++u) {
+      uint32_t a[KS][4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int mine = __shfl_sync(0xffffffffu, block, (u0 + u) * 8 + gr);
-        const int8_t* row = p.codes + ((size_t)max(mine, 0) * p.Hkv + h) * p.D;
+      for (int half = 0; half < 2; ++half) {
+        const int mine = __shfl_sync(0xffffffffu, block, u * 16 + half * 8 + gr);
+        const int8_t* row = p.codes + ((size_t)max(mine, 0) * p.Hkv + h) * p.D;      // a page that is not there: any row, its score is not used
 #pragma unroll
-        for (int s = 0; s < KS; ++s) b[u][s] = mine >= 0 ? load_codes(row, s * 32 + t4 * 8, p.D, vec) : make_uint2(0, 0);
+        for (int s = 0; s < KS; ++s) {
+          const uint2 x = load_codes<FULL>(row, s * 32 + t4 * 8, p.D, vec);
+          a[s][half] = x.x, a[s][2 + half] = x.y;
+        }
       }
+      int c[NT][4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        int best[4] = {INT_MIN, INT_MIN, INT_MIN, INT_MIN};      // of the pages 2 t4 and 2 t4 + 1 for rows gr and gr + 8
-        for (int tile = 0; tile < row_tiles; ++tile) {
-          if (row_tiles > 1) load_rows(tile);
-          int c[4] = {0, 0, 0, 0};
+      for (int x = 0; x < NT; ++x) {
+        c[x][0] = c[x][1] = c[x][2] = c[x][3] = 0;
+        if (turns == 1) {
 #pragma unroll
-          for (int s = 0; s < KS; ++s) mma_s8(c, a[s], b[u][s].x, b[u][s].y);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) best[e] = max(best[e], c[e]);
+          for (int s = 0; s < KS; ++s) mma_s8(c[x], a[s], b[x][s].x, b[x][s].y);
         }
-        // the maximum over a token's rows: lanes that differ in the low bits of gr, and both halves where it has 16
-        for (int o = 4; o < 4 * Gp && o < 32; o <<= 1) {
+      }
+      if (turns > 1) {
+        int best[4] = {INT_MIN, INT_MIN, INT_MIN, INT_MIN};
+        for (int turn = 0; turn < turns; ++turn) {
+          load_heads(turn);
+          int d[4] = {0, 0, 0, 0};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) best[e] = max(best[e], __shfl_xor_sync(0xffffffffu, best[e], o));
+          for (int s = 0; s < KS; ++s) mma_s8(d, a[s], b[0][s].x, b[0][s].y);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) best[e] = max(best[e], d[e]);
         }
-        if (Gp == 16) best[0] = max(best[0], best[2]), best[1] = max(best[1], best[3]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int page = (u0 + u) * 8 + t4 * 2 + (e & 1), r = gr + (e >> 1) * 8, tok = r / Gp;
-          const float sc = __shfl_sync(0xffffffffu, scale, page);
-          if (r % Gp == 0 && tok < TT && i0 + page < s_cand[tok]) {
-            const uint32_t k = float_key((there >> page) & 1u ? __fmul_rn((float)best[e], sc) : -INFINITY);
-            keys[tok * p.max_blocks + i0 + page] = k;
-            count_key(reinterpret_cast<int*>(select_smem) + tok * SELECT_INTS, k);
+        for (int e = 0; e < 4; ++e) c[0][e] = best[e];
+      }
+      // c: pages gr and gr + 8, columns 2 t4 and 2 t4 + 1
+      const int odd = t4 & 1, mine = u * 16 + gr + 8 * odd;
+      const float sc = __shfl_sync(0xffffffffu, scale, mine), other = __shfl_sync(0xffffffffu, scale, mine ^ 8);
+      const bool here = (there >> mine) & 1u;
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+        if (Gp >= 4) {
+          int lo = max(c[x][0], c[x][1]), hi = max(c[x][2], c[x][3]);
+          lo = max(lo, __shfl_xor_sync(0xffffffffu, lo, 1)), hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
+          if (Gp == 8) lo = max(lo, __shfl_xor_sync(0xffffffffu, lo, 2)), hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, 2));
+          if (Gp == 4 || t4 < 2) keep(x * (8 / Gp) + (Gp == 4 ? t4 >> 1 : 0), i0 + mine, odd ? hi : lo, sc, here);
+        } else {
+          const float sc_lo = odd ? other : sc, sc_hi = odd ? sc : other;
+          const int lo_page = u * 16 + gr, hi_page = lo_page + 8;
+          const bool lo_here = (there >> lo_page) & 1u, hi_here = (there >> hi_page) & 1u;
+          if (Gp == 2) {
+            keep(x * 4 + t4, i0 + lo_page, max(c[x][0], c[x][1]), sc_lo, lo_here);
+            keep(x * 4 + t4, i0 + hi_page, max(c[x][2], c[x][3]), sc_hi, hi_here);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              keep(x * 8 + t4 * 2 + e, i0 + lo_page, c[x][e], sc_lo, lo_here);
+              keep(x * 8 + t4 * 2 + e, i0 + hi_page, c[x][2 + e], sc_hi, hi_here);
+            }
           }
         }
       }
@@ -277,17 +312,18 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 4 ? 4 : 2) page_select_k
   });
 }
 
-// Tokens of a block: as many as the 16 rows of a product hold (4 at most), where sequences have them, as long as two blocks of an SM have room for the scores.
+// Tokens of a block: as many as the 16 columns of two products hold (4 at most), where sequences have them, as long as the scores leave room for two blocks on an SM.
 int select_tokens(int uniform, int G, int pages) {
-  int TT = 1;
-  while (TT < 4 && TT * 2 * G <= 16 && TT < uniform && (long long)TT * 2 * pages * 4 <= 64 * 1024) TT *= 2;
+  int Gp = 1, TT = 1;
+  while (Gp < G) Gp <<= 1;
+  while (TT < 4 && TT * 2 * Gp <= (TT == 1 ? 8 : 16) && TT < uniform && (long long)TT * 2 * pages * 4 <= 64 * 1024) TT *= 2;
   return TT;
 }
 
-template <typename E, int TT, int KS>
+template <int TT, int KS, bool FULL>
 int launch_select(const SelectParams& p, cudaStream_t s) {
   const size_t smem = TT * ((size_t)SELECT_INTS * 4 + (size_t)p.G * 32 * KS + 4 * (size_t)p.max_blocks);
-  auto kernel = page_select_kernel<E, TT, KS>;
+  auto kernel = page_select_kernel<TT, KS, FULL>;
   if (smem > 47 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return -(int)e;
@@ -295,11 +331,10 @@ int launch_select(const SelectParams& p, cudaStream_t s) {
   return launch_kernel(kernel, dim3((unsigned)(p.num_seqs * ((p.uniform_q + TT - 1) / TT) * p.Hkv)), dim3(SELECT_THREADS), smem, s, p);
 }
 
-template <typename E>
+template <int KS, bool FULL>
 int launch_select(const SelectParams& p, cudaStream_t s) {
   const int TT = select_tokens(p.uniform_q, p.G, p.max_blocks);
-  if (p.D <= 128) return TT == 4 ? launch_select<E, 4, 4>(p, s) : TT == 2 ? launch_select<E, 2, 4>(p, s) : launch_select<E, 1, 4>(p, s);
-  return TT == 4 ? launch_select<E, 4, 8>(p, s) : TT == 2 ? launch_select<E, 2, 8>(p, s) : launch_select<E, 1, 8>(p, s);
+  return TT == 4 ? launch_select<4, KS, FULL>(p, s) : TT == 2 ? launch_select<2, KS, FULL>(p, s) : launch_select<1, KS, FULL>(p, s);
 }
 
 }  // namespace
@@ -340,9 +375,10 @@ int swb_page_select(const int* dims, const void* q, long long q_stride_tok, long
   const long long smem = swb_page_select_smem(max_blocks, G, D);
   if (smem > 200 * 1024) return -3;
   const SelectParams p{q, q_stride_tok, q_stride_head, reinterpret_cast<const int8_t*>(codes), reinterpret_cast<const float*>(scales), table, table_stride,
-                       max_blocks, blocks, bs, Hkv, G, D, cu_q, kv_lens, seqs, uniform, T, first, top, last, pages, counts};
+                       max_blocks, blocks, bs, Hkv, G, D, cu_q, kv_lens, seqs, uniform, T, first, top, last, pages, counts, fp32};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return fp32 ? launch_select<float>(p, s) : launch_select<bf16>(p, s);
+  if (D == 128 && (reinterpret_cast<uintptr_t>(codes) & 7) == 0) return launch_select<4, true>(p, s);
+  return D <= 128 ? launch_select<4, false>(p, s) : launch_select<8, false>(p, s);
 }
 
 }  // extern "C"
