@@ -88,6 +88,7 @@ struct SelectParams {
   int* pages;                // [tokens, Hkv, first + top + last]
   int* counts;               // [tokens, Hkv]
   int fp32;                  // type of q
+  int q_vec;                 // bf16 rows of 16-byte alignment
 };
 
 constexpr int SELECT_THREADS = 256, SELECT_WARPS = SELECT_THREADS / 32;
@@ -98,19 +99,17 @@ __device__ __forceinline__ void mma_s8(int* c, const uint32_t* a, uint32_t b0, u
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Eight codes of a row from column d on, zeros behind its end. FULL: rows are 32 KS codes, 8-byte aligned.
+// Sixteen codes of a row from column d on, zeros behind its end. FULL: rows are 32 KS codes, 16-byte aligned.
 template <bool FULL>
-__device__ __forceinline__ uint2 load_codes(const int8_t* row, int d, int D, bool vec) {
-  if (FULL) return __ldg(reinterpret_cast<const uint2*>(row + d));
-  uint2 x = make_uint2(0, 0);
-  if (d >= D) return x;
-  if (vec) return __ldg(reinterpret_cast<const uint2*>(row + d));
-  for (int i = 0; i < 8 && d + i < D; ++i) {
-    const uint32_t b = (uint32_t)(uint8_t)row[d + i];
-    if (i < 4) x.x |= b << (8 * i);
-    else x.y |= b << (8 * i - 32);
-  }
-  return x;
+__device__ __forceinline__ uint4 load_codes(const int8_t* row, int d, int D, bool vec) {
+  if (FULL) return __ldg(reinterpret_cast<const uint4*>(row + d));
+  if (d >= D) return make_uint4(0, 0, 0, 0);
+  if (vec) return __ldg(reinterpret_cast<const uint4*>(row + d));
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (d + i < D) w[i >> 2] |= (uint32_t)(uint8_t)row[d + i] << (8 * (i & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 __device__ __forceinline__ float load_query(const SelectParams& p, long long at) {
@@ -124,26 +123,29 @@ __device__ __forceinline__ int8_t query_code(float x, float a, bool fp32) {
 }
 
 // A block per (run of TT tokens of a sequence, head). The dot products are 8-bit matrix products: 16 rows are pages, 8 columns the tokens' query heads (a token's heads
-// are filled up to a power of two, Gp, with copies of its first, which change no maximum), so that a head's neighbours are a thread's own or a shuffle away and
-// every thread ends with one page's score for one token. A page's row is fetched in one piece: the lane of page g and quarter t holds columns 32 s + 8 t and on of
-// step s, and the queries' codes are read in the same order, so the order of the columns within a step is another than the instruction's and the
-// sum the same. A warp looks 32 pages up at a time and has 16 of them on their way.
+// are filled up to a power of two, with copies of its first, which change no maximum; GP is that power where it is known), so that a head's neighbours are a thread's own or a shuffle away and
+// every thread ends with one page's score for one token. A page's row is fetched 16 codes at a time (a load of a warp then touches eight lines; with 8
+// codes sixteen loads touched each line four times, and the look-ups in the cache's tags bound the kernel): the lane of page g and quarter t holds columns 64 j + 16 t and on,
+// for two steps, and the queries' codes are read in the same order, so the order of the columns within a step is another than the instruction's and the sum the same.
 // Then the tokens are shared out among teams of warps, each of which chooses among its token's scores.
 // Shared memory: the teams' histograms, codes of the queries [TT, G, 32 KS], keys [TT, pages].
-template <int TT, int KS, bool FULL>
-__global__ void __launch_bounds__(SELECT_THREADS, KS == 4 ? 4 : 2) page_select_kernel(const SelectParams p) {
+template <int TT, int KS, bool FULL, int GP>
+__global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 ? 4 : 3) page_select_kernel(const SelectParams p) {
   constexpr int TEAM = SELECT_THREADS / TT, LD = 32 * KS;
   pdl_launch_dependents();
   extern __shared__ __align__(16) uint8_t select_smem[];
   __shared__ float s_amax[SELECT_WARPS];
+  __shared__ uint32_t s_largest[TT];
   __shared__ int s_bad[TT], s_cand[TT];           // s_cand: pages to choose among
   const Team<TEAM> team(threadIdx.x);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int* hist = reinterpret_cast<int*>(select_smem) + team.id * SELECT_INTS;
   int8_t* qc = reinterpret_cast<int8_t*>(select_smem + TT * SELECT_INTS * 4);
   uint32_t* keys = reinterpret_cast<uint32_t*>(qc + TT * p.G * LD);
-  const int h = blockIdx.x % p.Hkv, run = blockIdx.x / p.Hkv, runs = (p.uniform_q + TT - 1) / TT, seq = run / runs;
-  if (tid < TT) s_bad[tid] = 0;
+  // blocks that run together share what they read: the tokens of a prompt a head's codes, the heads of a decode step a page's memory
+  const int runs = (p.uniform_q + TT - 1) / TT, all_runs = runs * p.num_seqs;
+  const int h = TT > 1 ? blockIdx.x / all_runs : blockIdx.x % p.Hkv, run = TT > 1 ? blockIdx.x % all_runs : blockIdx.x / p.Hkv, seq = run / runs;
+  if (tid < TT) s_bad[tid] = 0, s_largest[tid] = 0u;
   pdl_wait();
   const int q0 = p.cu_q ? p.cu_q[seq] : seq * p.uniform_q, q1 = p.cu_q ? p.cu_q[seq + 1] : q0 + p.uniform_q;
   const int t0 = q0 + (run % runs) * TT;
@@ -173,143 +175,194 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 4 ? 4 : 2) page_select_k
   // the token's queries as codes of one step
   if (n > width) {
     const long long q = t * p.q_stride_tok + (long long)h * p.G * p.q_stride_head;
+    int8_t* to = qc + team.id * p.G * LD;
     float a = 0.f;
     bool bad = false;
-    for (int g = 0; g < p.G; ++g)
-      for (int d = team.rank; d < p.D; d += TEAM) {
-        const float x = fabsf(load_query(p, q + g * p.q_stride_head + d));
-        a = fmaxf(a, x);
-        bad |= !(x < INFINITY);
+    const auto look = [&](float x) {
+      a = fmaxf(a, fabsf(x));
+      bad |= !(fabsf(x) < INFINITY);
+    };
+    const auto known = [&]() {                       // the largest size of all, and whether every number is finite
+      a = warp_max(a);
+      if (lane == 0) s_amax[warp] = a;
+      if (bad) s_bad[team.id] = 1;
+      team.sync();
+      a = 0.f;
+      for (int w = 0; w < Team<TEAM>::WARPS; ++w) a = fmaxf(a, s_amax[team.id * Team<TEAM>::WARPS + w]);
+      bad = s_bad[team.id] != 0 || a == 0.f;
+    };
+    if (FULL && p.q_vec) {                           // eight bf16 numbers at a time
+      const bf16* from = reinterpret_cast<const bf16*>(p.q) + q;
+      float x[8];
+      for (int i = team.rank; i < p.G * 16; i += TEAM) {
+        load_row8(from + (i >> 4) * p.q_stride_head + (i & 15) * 8, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) look(x[e]);
       }
-    a = warp_max(a);
-    if (lane == 0) s_amax[warp] = a;
-    if (bad) s_bad[team.id] = 1;
-    team.sync();
-    a = 0.f;
-    for (int w = 0; w < Team<TEAM>::WARPS; ++w) a = fmaxf(a, s_amax[team.id * Team<TEAM>::WARPS + w]);
-    bad = s_bad[team.id] != 0;
-    int8_t* to = qc + team.id * p.G * LD;
-    for (int g = 0; g < p.G; ++g)
-      for (int d = team.rank; d < LD; d += TEAM) {
+      known();
+      for (int i = team.rank; i < p.G * 16; i += TEAM) {
+        load_row8(from + (i >> 4) * p.q_stride_head + (i & 15) * 8, x);
+        uint32_t w[2] = {0u, 0u};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!bad) w[e >> 2] |= (uint32_t)(uint8_t)query_code(x[e], a, 0) << (8 * (e & 3));
+        *reinterpret_cast<uint2*>(to + i * 8) = make_uint2(w[0], w[1]);
+      }
+    } else {
+#pragma unroll 4
+      for (int i = team.rank; i < p.G * p.D; i += TEAM) look(load_query(p, q + (i / p.D) * p.q_stride_head + i % p.D));
+      known();
+#pragma unroll 4
+      for (int i = team.rank; i < p.G * LD; i += TEAM) {
+        const int g = i / LD, d = i % LD;
         const float x = d < p.D ? load_query(p, q + g * p.q_stride_head + d) : 0.f;
-        to[g * LD + d] = bad || a == 0.f ? (int8_t)0 : query_code(x, a, p.fp32);
+        to[i] = bad ? (int8_t)0 : query_code(x, a, p.fp32);
       }
+    }
   }
   __syncthreads();
 
   constexpr int NT = TT == 4 ? 2 : 1;              // products beside each other: TT Gp <= 8 NT, or one token in turns of 8 heads
   const int gr = lane >> 2, t4 = lane & 3;
-  int Gp = 1;
-  while (Gp < p.G && Gp < 8) Gp <<= 1;
-  const int turns = TT == 1 ? (p.G + 7) / 8 : 1;
+  int Gp = GP ? GP : 1;
+  while (!GP && Gp < p.G && Gp < 8) Gp <<= 1;
+  const int turns = TT == 1 && !GP ? (p.G + 7) / 8 : 1;
   uint2 b[NT][KS];
   const auto load_heads = [&](int turn) {
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
       const int c = x * 8 + gr, tok = min(c / Gp, TT - 1), g = turn * 8 + c % Gp;
-      const uint2* from = reinterpret_cast<const uint2*>(qc + (tok * p.G + (g < p.G ? g : 0)) * LD);
+      const uint4* from = reinterpret_cast<const uint4*>(qc + (tok * p.G + (g < p.G ? g : 0)) * LD);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) b[x][s] = from[s * 4 + t4];
+      for (int s = 0; s < KS; s += 2) {
+        const uint4 y = from[s * 2 + t4];
+        b[x][s] = make_uint2(y.x, y.y), b[x][s + 1] = make_uint2(y.z, y.w);
+      }
     }
   };
   if (turns == 1) load_heads(0);
-  const bool vec = (p.D & 7) == 0 && (reinterpret_cast<uintptr_t>(p.codes) & 7) == 0;
+  const bool vec = (p.D & 15) == 0 && (reinterpret_cast<uintptr_t>(p.codes) & 15) == 0;
   const int* table = p.table + seq * p.table_stride + p.first;
   const auto locate = [&](int i) {
     const int block = i < cand ? table[i] : -1;
     return (unsigned)block < (unsigned)p.num_blocks ? block : -1;
   };
-  // keeps the score of page i (in bounds: less than the token's own number) for a token
-  const auto keep = [&](int tok, int i, int best, float scale, bool there) {
-    if (tok >= TT || i >= s_cand[tok]) return;
+  // keeps the score of candidate i for a token, which has `most` of them
+  const auto keep = [&](int tok, int most, int i, int best, float scale, bool there) -> uint32_t {
+    if (i >= most) return 0u;
     const uint32_t k = float_key(there ? __fmul_rn((float)best, scale) : -INFINITY);
     keys[tok * p.max_blocks + i] = k;
-    count_key(reinterpret_cast<int*>(select_smem) + tok * SELECT_INTS, k);
+    return k;
   };
-  int next = locate(warp * 32 + lane);
-  for (int i0 = warp * 32; i0 < cand; i0 += SELECT_THREADS) {
-    const int block = next;
-    const float scale = block >= 0 ? p.scales[(size_t)block * p.Hkv + h] : 0.f;
-    const uint32_t there = __ballot_sync(0xffffffffu, block >= 0);
-    next = locate(i0 + SELECT_THREADS + lane);
+  // the largest key of each token, where a thread keeps keys of several
+  const auto note = [&](int tok, uint32_t k) {
+    if (k) atomicMax(&s_largest[tok], k);
+  };
+  // with four heads and more a thread ends with one score in each product: page gr or gr + 8, and this token
+  const int odd_quarter = t4 & 1, tok0 = Gp == 4 ? t4 >> 1 : 0;
+  int most_of[NT];
+  uint32_t largest[NT];                            // of the keys that this thread keeps for that token
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      uint32_t a[KS][4];
+  for (int x = 0; x < NT; ++x) {
+    largest[x] = 0u;
+    const int tok = x * (8 / Gp) + tok0;
+    most_of[x] = tok < TT && (Gp == 4 || t4 < 2) ? s_cand[tok] : 0;
+  }
+  // rows gr and gr + 8 of the u-th 16 of a warp's 32 pages
+  const auto fetch = [&](uint32_t (*a)[4], int blocks, int u) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int mine = __shfl_sync(0xffffffffu, block, u * 16 + half * 8 + gr);
-        const int8_t* row = p.codes + ((size_t)max(mine, 0) * p.Hkv + h) * p.D;      // a page that is not there: any row, its score is not used
+    for (int half = 0; half < 2; ++half) {
+      const int mine = __shfl_sync(0xffffffffu, blocks, u * 16 + half * 8 + gr);
+      const int8_t* row = p.codes + ((size_t)max(mine, 0) * p.Hkv + h) * p.D;        // a page that is not there: any row, its score is not used
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const uint2 x = load_codes<FULL>(row, s * 32 + t4 * 8, p.D, vec);
-          a[s][half] = x.x, a[s][2 + half] = x.y;
-        }
+      for (int s = 0; s < KS; s += 2) {
+        const uint4 x = load_codes<FULL>(row, s * 32 + t4 * 16, p.D, vec);
+        a[s][half] = x.x, a[s][2 + half] = x.y, a[s + 1][half] = x.z, a[s + 1][2 + half] = x.w;
       }
-      int c[NT][4];
+    }
+  };
+  const auto score = [&](const uint32_t (*a)[4], int i0, int u, float scale, uint32_t there) {
+    int c[NT][4];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      c[x][0] = c[x][1] = c[x][2] = c[x][3] = 0;
+      if (turns == 1) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) mma_s8(c[x], a[s], b[x][s].x, b[x][s].y);
+      }
+    }
+    if (turns > 1) {
+      int best[4] = {INT_MIN, INT_MIN, INT_MIN, INT_MIN};
+      for (int turn = 0; turn < turns; ++turn) {
+        load_heads(turn);
+        int d[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) mma_s8(d, a[s], b[0][s].x, b[0][s].y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) best[e] = max(best[e], d[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[0][e] = best[e];
+    }
+    // c: pages gr and gr + 8, columns 2 t4 and 2 t4 + 1
+    const int mine = u * 16 + gr + 8 * odd_quarter;
+    const float sc = __shfl_sync(0xffffffffu, scale, mine);
+    const bool here = (there >> mine) & 1u;
+    if (GP || Gp >= 4) {
 #pragma unroll
       for (int x = 0; x < NT; ++x) {
-        c[x][0] = c[x][1] = c[x][2] = c[x][3] = 0;
-        if (turns == 1) {
-#pragma unroll
-          for (int s = 0; s < KS; ++s) mma_s8(c[x], a[s], b[x][s].x, b[x][s].y);
-        }
+        int lo = max(c[x][0], c[x][1]), hi = max(c[x][2], c[x][3]);
+        lo = max(lo, __shfl_xor_sync(0xffffffffu, lo, 1)), hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
+        if (Gp == 8) lo = max(lo, __shfl_xor_sync(0xffffffffu, lo, 2)), hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, 2));
+        largest[x] = max(largest[x], keep(x * (8 / Gp) + tok0, most_of[x], i0 + mine, odd_quarter ? hi : lo, sc, here));
       }
-      if (turns > 1) {
-        int best[4] = {INT_MIN, INT_MIN, INT_MIN, INT_MIN};
-        for (int turn = 0; turn < turns; ++turn) {
-          load_heads(turn);
-          int d[4] = {0, 0, 0, 0};
-#pragma unroll
-          for (int s = 0; s < KS; ++s) mma_s8(d, a[s], b[0][s].x, b[0][s].y);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) best[e] = max(best[e], d[e]);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c[0][e] = best[e];
-      }
-      // c: pages gr and gr + 8, columns 2 t4 and 2 t4 + 1
-      const int odd = t4 & 1, mine = u * 16 + gr + 8 * odd;
-      const float sc = __shfl_sync(0xffffffffu, scale, mine), other = __shfl_sync(0xffffffffu, scale, mine ^ 8);
-      const bool here = (there >> mine) & 1u;
+    } else {
+      const float other = __shfl_sync(0xffffffffu, scale, mine ^ 8), sc_lo = odd_quarter ? other : sc, sc_hi = odd_quarter ? sc : other;
+      const int lo_page = u * 16 + gr, hi_page = lo_page + 8;
+      const bool lo_here = (there >> lo_page) & 1u, hi_here = (there >> hi_page) & 1u;
 #pragma unroll
       for (int x = 0; x < NT; ++x) {
-        if (Gp >= 4) {
-          int lo = max(c[x][0], c[x][1]), hi = max(c[x][2], c[x][3]);
-          lo = max(lo, __shfl_xor_sync(0xffffffffu, lo, 1)), hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
-          if (Gp == 8) lo = max(lo, __shfl_xor_sync(0xffffffffu, lo, 2)), hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, 2));
-          if (Gp == 4 || t4 < 2) keep(x * (8 / Gp) + (Gp == 4 ? t4 >> 1 : 0), i0 + mine, odd ? hi : lo, sc, here);
+        if (Gp == 2) {
+          const int tok = x * 4 + t4, most = tok < TT ? s_cand[tok] : 0;
+          note(tok, keep(tok, most, i0 + lo_page, max(c[x][0], c[x][1]), sc_lo, lo_here));
+          note(tok, keep(tok, most, i0 + hi_page, max(c[x][2], c[x][3]), sc_hi, hi_here));
         } else {
-          const float sc_lo = odd ? other : sc, sc_hi = odd ? sc : other;
-          const int lo_page = u * 16 + gr, hi_page = lo_page + 8;
-          const bool lo_here = (there >> lo_page) & 1u, hi_here = (there >> hi_page) & 1u;
-          if (Gp == 2) {
-            keep(x * 4 + t4, i0 + lo_page, max(c[x][0], c[x][1]), sc_lo, lo_here);
-            keep(x * 4 + t4, i0 + hi_page, max(c[x][2], c[x][3]), sc_hi, hi_here);
-          } else {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              keep(x * 8 + t4 * 2 + e, i0 + lo_page, c[x][e], sc_lo, lo_here);
-              keep(x * 8 + t4 * 2 + e, i0 + hi_page, c[x][2 + e], sc_hi, hi_here);
-            }
+          for (int e = 0; e < 2; ++e) {
+            const int tok = x * 8 + t4 * 2 + e, most = tok < TT ? s_cand[tok] : 0;
+            note(tok, keep(tok, most, i0 + lo_page, c[x][e], sc_lo, lo_here));
+            note(tok, keep(tok, most, i0 + hi_page, c[x][2 + e], sc_hi, hi_here));
           }
         }
       }
     }
+  };
+  // while 16 pages are scored the next 16 are on their way, and the blocks of the 32 behind them
+  uint32_t even[KS][4], odd[KS][4];
+  const auto scales_of = [&](int block) { return block >= 0 ? p.scales[(size_t)block * p.Hkv + h] : 0.f; };
+  int i0 = warp * 32, block = locate(i0 + lane), next = locate(i0 + SELECT_THREADS + lane);
+  float scale = scales_of(block);
+  if (i0 < cand) fetch(even, block, 0);
+  for (; i0 < cand; i0 += SELECT_THREADS) {
+    const uint32_t there = __ballot_sync(0xffffffffu, block >= 0);
+    fetch(odd, block, 1);
+    score(even, i0, 0, scale, there);
+    const float here = scale;
+    block = next;
+    next = locate(i0 + 2 * SELECT_THREADS + lane);
+    scale = scales_of(block);
+    if (i0 + SELECT_THREADS < cand) fetch(even, block, 0);
+    score(odd, i0, 1, here, there);
   }
+#pragma unroll
+  for (int x = 0; x < NT; ++x)
+    if (most_of[x] > 0 && largest[x]) atomicMax(&s_largest[x * (8 / Gp) + tok0], largest[x]);
   __syncthreads();
   if (n <= width) return;                          // whole teams leave
   const int want = n - p.first - p.last;           // this token's candidates
   const uint32_t* own = keys + team.id * p.max_blocks;
   const auto key = [&](int i) { return own[i]; };
-  const Threshold th = select_threshold(team, key, want, p.top, hist);
-  const int seg = ((want + TEAM - 1) / TEAM) * 32;
-  const int lo = min(team.warp() * seg, want), hi = min(lo + seg, want);
-  const PairSums sums = sum_over_warps(team, count_run(key, th, lo, hi), reinterpret_cast<int2*>(hist));
-  int at = p.first + sums.before.x + min(sums.before.y, th.ties);
-  for_each_choice(key, th, lo, hi, sums.before.y, [&](int i, bool in, uint32_t ins) {
-    if (in) out[at + __popc(ins & ((1u << lane) - 1u))] = p.first + i;
-    at += __popc(ins);
-  });
+  choose_in_order(team, key, want, p.top, s_largest[team.id], hist, [&](int place, int i) { out[p.first + place] = p.first + i; });
 }
 
 // Tokens of a block: as many as the 16 columns of two products hold (4 at most), where sequences have them, as long as the scores leave room for two blocks on an SM.
@@ -320,10 +373,10 @@ int select_tokens(int uniform, int G, int pages) {
   return TT;
 }
 
-template <int TT, int KS, bool FULL>
+template <int TT, int KS, bool FULL, int GP>
 int launch_select(const SelectParams& p, cudaStream_t s) {
   const size_t smem = TT * ((size_t)SELECT_INTS * 4 + (size_t)p.G * 32 * KS + 4 * (size_t)p.max_blocks);
-  auto kernel = page_select_kernel<TT, KS, FULL>;
+  auto kernel = page_select_kernel<TT, KS, FULL, GP>;
   if (smem > 47 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return -(int)e;
@@ -331,10 +384,19 @@ int launch_select(const SelectParams& p, cudaStream_t s) {
   return launch_kernel(kernel, dim3((unsigned)(p.num_seqs * ((p.uniform_q + TT - 1) / TT) * p.Hkv)), dim3(SELECT_THREADS), smem, s, p);
 }
 
-template <int KS, bool FULL>
+template <int KS, bool FULL, int GP>
 int launch_select(const SelectParams& p, cudaStream_t s) {
   const int TT = select_tokens(p.uniform_q, p.G, p.max_blocks);
-  return TT == 4 ? launch_select<4, KS, FULL>(p, s) : TT == 2 ? launch_select<2, KS, FULL>(p, s) : launch_select<1, KS, FULL>(p, s);
+  if constexpr (GP != 8)
+    if (TT == 4) return launch_select<4, KS, FULL, GP>(p, s);
+  return TT == 2 ? launch_select<2, KS, FULL, GP>(p, s) : launch_select<1, KS, FULL, GP>(p, s);
+}
+
+// Groups of 3 or 4 and of 5 to 8 heads of 128 columns have kernels of their own: without the choice of the reduction and the ends of rows in the loop they
+// issue half the instructions, which bound them.
+int launch_select(const SelectParams& p, cudaStream_t s) {
+  if (p.D == 128 && (reinterpret_cast<uintptr_t>(p.codes) & 15) == 0 && p.G > 2 && p.G <= 8) return p.G <= 4 ? launch_select<4, true, 4>(p, s) : launch_select<4, true, 8>(p, s);
+  return p.D <= 128 ? launch_select<4, false, 0>(p, s) : launch_select<8, false, 0>(p, s);
 }
 
 }  // namespace
@@ -375,10 +437,10 @@ int swb_page_select(const int* dims, const void* q, long long q_stride_tok, long
   const long long smem = swb_page_select_smem(max_blocks, G, D);
   if (smem > 200 * 1024) return -3;
   const SelectParams p{q, q_stride_tok, q_stride_head, reinterpret_cast<const int8_t*>(codes), reinterpret_cast<const float*>(scales), table, table_stride,
-                       max_blocks, blocks, bs, Hkv, G, D, cu_q, kv_lens, seqs, uniform, T, first, top, last, pages, counts, fp32};
+                       max_blocks, blocks, bs, Hkv, G, D, cu_q, kv_lens, seqs, uniform, T, first, top, last, pages, counts, fp32,
+                       !fp32 && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (q_stride_tok | q_stride_head) % 8 == 0};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (D == 128 && (reinterpret_cast<uintptr_t>(codes) & 7) == 0) return launch_select<4, true>(p, s);
-  return D <= 128 ? launch_select<4, false>(p, s) : launch_select<8, false>(p, s);
+  return launch_select(p, s);
 }
 
 }  // extern "C"

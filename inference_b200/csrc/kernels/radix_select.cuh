@@ -43,23 +43,24 @@ __device__ __forceinline__ void clear_bins(const Team<SIZE>& team, int* hist) {
 }
 __device__ __forceinline__ void count_key(int* hist, uint32_t key) { atomicAdd(&hist[key >> 21], 1); }
 
-// The bin in which the count from the top reaches `want`, in totals: {bin, what is left to find in it, its count, 0}. Ends with a barrier.
+// The bin in which the count from the top reaches `want`, in totals[32..]: {bin, what is left to find in it, its count, 0, 0}. Ends with a barrier.
 template <int SIZE>
 __device__ __forceinline__ void find_bin(const Team<SIZE>& team, const int* hist, int want, int* totals) {
   constexpr int PER = SELECT_BINS / SIZE;
   static_assert(SELECT_BINS % SIZE == 0 && PER >= 2 && SIZE <= 1024, "bins are shared out evenly");
-  // the thread of rank r holds the r-th run of PER bins from the top
+  // the thread of rank r adds up the r-th run of PER bins from the top, from a place of its own on so that neighbours meet in no bank
   const int* run = hist + SELECT_BINS - (team.rank + 1) * PER;
-  int mine[PER], sum = 0;
+  int sum = 0;
   if constexpr (PER % 4 == 0) {
 #pragma unroll
-    for (int j = 0; j < PER; j += 4) *reinterpret_cast<int4*>(mine + j) = *reinterpret_cast<const int4*>(run + j);
+    for (int j = 0; j < PER / 4; ++j) {
+      const int4 x = reinterpret_cast<const int4*>(run)[(j + team.lane() * PER / 32) & (PER / 4 - 1)];
+      sum += (x.x + x.y) + (x.z + x.w);
+    }
   } else {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) mine[j] = run[j];
+    for (int j = 0; j < PER; ++j) sum += run[j];
   }
-#pragma unroll
-  for (int j = 0; j < PER; ++j) sum += mine[j];
   int incl = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -71,11 +72,11 @@ __device__ __forceinline__ void find_bin(const Team<SIZE>& team, const int* hist
   int before = incl - sum;
   for (int w = 0; w < team.warp(); ++w) before += totals[w];
   if (before < want && want <= before + sum) {
-#pragma unroll
     for (int j = PER - 1; j >= 0; --j) {
-      if (before < want && want <= before + mine[j])
-        totals[32] = SELECT_BINS - (team.rank + 1) * PER + j, totals[33] = want - before, totals[34] = mine[j], totals[35] = 0;
-      before += mine[j];
+      const int mine = run[j];
+      if (before < want && want <= before + mine)
+        totals[32] = SELECT_BINS - (team.rank + 1) * PER + j, totals[33] = want - before, totals[34] = mine, totals[35] = totals[36] = 0;
+      before += mine;
     }
   }
   team.sync();
@@ -86,12 +87,13 @@ __device__ __forceinline__ void find_bin(const Team<SIZE>& team, const int* hist
 // free afterwards (behind a barrier of the team).
 template <int SIZE, typename Key>
 __device__ Threshold select_threshold(const Team<SIZE>& team, const Key& key, int n, int want, int* hist) {
-  int* totals = hist + SELECT_BINS;            // [32] of the warps, then find_bin's, then {key, ties}
+  int* totals = hist + SELECT_BINS;            // [32] of the warps, find_bin's five, {key, ties}
   find_bin(team, hist, want, totals);
   const uint32_t bin = (uint32_t)totals[32];
   const int left = totals[33], m = totals[34];
   if (m <= SIZE) {
     uint32_t* list = reinterpret_cast<uint32_t*>(hist);
+#pragma unroll 4
     for (int i = team.rank; i < n; i += SIZE) {
       const uint32_t k = key(i);
       if ((k >> 21) == bin) list[atomicAdd(&totals[35], 1)] = k;
@@ -101,10 +103,10 @@ __device__ Threshold select_threshold(const Team<SIZE>& team, const Key& key, in
       const uint32_t mine = list[team.rank];
       int above = 0, same = 0;
       for (int j = 0; j < m; ++j) above += list[j] > mine, same += list[j] == mine;
-      if (above < left && left <= above + same) totals[36] = (int)mine, totals[37] = left - above;      // one key fits: its owners write the same
+      if (above < left && left <= above + same) totals[37] = (int)mine, totals[38] = left - above;      // one key fits: its owners write the same
     }
     team.sync();
-    return Threshold{(uint32_t)totals[36], totals[37]};
+    return Threshold{(uint32_t)totals[37], totals[38]};
   }
   uint32_t prefix = bin << 21, mask = 0x7ffu << 21;
   want = left;
@@ -165,11 +167,89 @@ __device__ __forceinline__ PairSums sum_over_warps(const Team<SIZE>& team, int2 
 template <typename Key>
 __device__ __forceinline__ int2 count_run(const Key& key, const Threshold& t, int first, int last) {
   int above = 0, same = 0;
+#pragma unroll 4
   for (int i = first + (int)(threadIdx.x & 31); i < last; i += 32) {
     const uint32_t k = key(i);
     above += k > t.key, same += k == t.key;
   }
   return make_int2(__reduce_add_sync(0xffffffffu, above), __reduce_add_sync(0xffffffffu, same));
+}
+
+// A first digit of float_keys in proportion to the numbers between zero and the largest, for choices of few among many of one spread: a bin at the choice's border
+// holds a thousandth of them where one of exponent and two bits holds a tenth. Numbers below zero fall into the lowest bin. Where the largest is not a positive
+// finite number that can be divided by, the key's own digits serve.
+struct LinearDigit {
+  float scale;                                 // 0: the key's own digits
+  __device__ __forceinline__ explicit LinearDigit(uint32_t largest) {
+    const float top = __uint_as_float(largest & 0x7fffffffu);
+    scale = (largest & 0x80000000u) && top > 1e-30f && top < INFINITY ? (float)(SELECT_BINS - 1) / top : 0.f;
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t key) const {
+    if (scale == 0.f) return key >> 21;
+    return (key & 0x80000000u) ? min((uint32_t)(__uint_as_float(key & 0x7fffffffu) * scale), (uint32_t)SELECT_BINS - 1u) : 0u;
+  }
+};
+
+// The indexes of the `want` largest keys in ascending order, put(place, index), ties to the lowest index. largest: the largest key. Where a team has a thread for
+// each chosen key and for each in the border's bin, one pass gathers both and two counts put them into order. The caller clears the bins; the whole team calls it,
+// and the keys are written before it (it begins with a barrier).
+template <int SIZE, typename Key, typename Put>
+__device__ __forceinline__ void choose_in_order(const Team<SIZE>& team, const Key& key, int n, int want, uint32_t largest, int* hist, const Put& put) {
+  int* totals = hist + SELECT_BINS;
+  const LinearDigit digit(largest);
+  team.sync();
+  if (want <= SIZE) {
+#pragma unroll 4
+    for (int i = team.rank; i < n; i += SIZE) atomicAdd(&hist[digit(key(i))], 1);
+    team.sync();
+    find_bin(team, hist, want, totals);
+    const uint32_t bin = (uint32_t)totals[32];
+    const int left = totals[33], m = totals[34];
+    if (m <= SIZE) {
+      uint32_t* border = reinterpret_cast<uint32_t*>(hist);      // keys of the border's bin, their indexes, and what is chosen
+      int *border_at = hist + SIZE, *chosen = hist + 2 * SIZE;
+#pragma unroll 4
+      for (int i = team.rank; i < n; i += SIZE) {
+        const uint32_t k = key(i), d = digit(k);
+        if (d > bin) {
+          chosen[atomicAdd(&totals[36], 1)] = i;
+        } else if (d == bin) {
+          const int j = atomicAdd(&totals[35], 1);
+          border[j] = k, border_at[j] = i;
+        }
+      }
+      team.sync();
+      if (team.rank < m) {
+        const uint32_t mine = border[team.rank];
+        const int at = border_at[team.rank];
+        int above = 0;
+#pragma unroll 4
+        for (int j = 0; j < m; ++j) above += border[j] > mine || (border[j] == mine && border_at[j] < at);
+        if (above < left) chosen[want - left + above] = at;
+      }
+      team.sync();
+      if (team.rank < want) {
+        const int at = chosen[team.rank];
+        int place = 0;
+#pragma unroll 4
+        for (int j = 0; j < want; ++j) place += chosen[j] < at;
+        put(place, at);
+      }
+      return;
+    }
+    clear_bins(team, hist);
+    team.sync();
+  }
+  for (int i = team.rank; i < n; i += SIZE) count_key(hist, key(i));
+  team.sync();
+  const Threshold t = select_threshold(team, key, n, want, hist);
+  const int seg = ((n + SIZE - 1) / SIZE) * 32, lo = min(team.warp() * seg, n), hi = min(lo + seg, n);
+  const PairSums sums = sum_over_warps(team, count_run(key, t, lo, hi), reinterpret_cast<int2*>(hist));
+  int at = sums.before.x + min(sums.before.y, t.ties);
+  for_each_choice(key, t, lo, hi, sums.before.y, [&](int i, bool in, uint32_t ins) {
+    if (in) put(at + __popc(ins & ((1u << team.lane()) - 1u)), i);
+    at += __popc(ins);
+  });
 }
 
 }  // namespace swb
