@@ -1,11 +1,13 @@
 // Attention of new tokens over a paged cache, each on its own: over the pages that were selected for it, or over the whole cache with the weight that
 // every key receives added up.
 //
-// A problem is one query token, one key/value head and up to 16 of the query heads that share it; its keys are dealt out to `num_splits` blocks in tiles. A block
-// goes over its keys once with the running maximum and sum of the softmax in 32 bits, and leaves an un-normalised sum of values with both; the blocks of a
-// problem are joined by a second launch (none where a problem has one block and no weights are kept). Weights need the maximum and sum over all
-// keys, which are known at the end only: the scores are kept (4 bytes a key and query head, beside the keys' and values' 2 (D + Dv) a key), and the
-// second launch turns them into weights and adds up those of a key over heads and tokens, in a fixed order and without atomics.
+// A problem is up to 16 rows of queries with one key/value head: query heads that share it, of one token, or where tokens of a sequence read the same keys and the
+// heads are few, of several tokens. Its keys are dealt out to `num_splits` blocks. A block goes over its keys once with the running maximum and sum of the softmax in
+// 32 bits, and is left with an un-normalised sum of values and both. Up to 8 blocks of a problem are a cluster and join their parts from one another's
+// shared memory; more leave them in the workspace for a second launch. Weights need the maximum and sum over all keys, which are known at
+// the end only: the scores are kept (4 bytes a key and query head, beside the keys' and values' 2 (D + Dv) a key) and turned into weights there, by the
+// blocks themselves where every sequence has one token, else by the second launch, which adds up those of a key token by token and head by head. Every sum has
+// one order, and there are no atomics.
 //
 // Masked keys (behind what a token sees, on pages that are not there) take no part: their scores are -inf whatever the products were, and
 // their values are not multiplied at all, so that what the memory holds there does not matter.
@@ -21,7 +23,8 @@ SWB_REGISTER_STATUS_UNIT(attn_budget);
 
 namespace {
 
-constexpr int ROWS = 16;                     // query heads of a problem
+constexpr int ROWS = 16;                     // of queries in a problem
+constexpr int MAX_SPLITS = 64, MAX_CLUSTER = 8, MAX_GROUP = 128;
 
 struct BudgetParams {
   const void* q;
@@ -41,8 +44,11 @@ struct BudgetParams {
   const int* counts;         // [tokens, Hkv]
   int width;
   int num_splits;
-  float* part_o;             // [problems, num_splits, ROWS, Dv]
-  float* part_ml;            // [problems, num_splits, ROWS, 2]
+  int run;                   // tokens of a problem (more than one only without page lists)
+  int cluster;               // the splits of a problem are a cluster
+  int weigh_here;            // blocks add their weights themselves
+  float* part_o;             // [tokens, Hq, num_splits, Dv], null where blocks or clusters finish the output
+  float* part_ml;            // [tokens, Hq, num_splits, 2]: maximum (log2 units) and sum; null where nobody reads them
   float* scores;             // [tokens, Hq, capacity] in log2 units, where weights are kept
   long long capacity;
   float* weights;            // [num_seqs, Hkv, .], inner stride 1
@@ -62,6 +68,8 @@ __device__ __forceinline__ Token token_of(const BudgetParams& p, int t) {
   x.seen = max(min(p.kv_lens[x.seq] - (x.q_len - 1 - (t - x.q0)), p.max_blocks * p.bs), 0);
   return x;
 }
+
+__device__ __forceinline__ size_t part_at(const BudgetParams& p, int t, int head, int split) { return ((size_t)t * p.Hkv * p.G + head) * p.num_splits + split; }
 
 __device__ __forceinline__ void store_out(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store_out(bf16* p, float x) { *p = __float2bfloat16(x); }
@@ -158,22 +166,19 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_budget_plain_kernel(const 
     }
   }
   __syncthreads();
-  const size_t problem = ((size_t)t * p.Hkv + h) * p.head_tiles + ht;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     if (r >= rows) break;
+    const int head = h * p.G + g0 + r;
 #pragma unroll
     for (int c = 0; c < COLS; ++c) {
       const int d = c * PLAIN_THREADS + tid;
       if (d >= p.Dv) continue;
-      if (p.part_o) p.part_o[((problem * p.num_splits + split) * ROWS + r) * p.Dv + d] = o[c][r];
-      else store_out(reinterpret_cast<E*>(p.out) + t * p.out_stride_tok + (size_t)(h * p.G + g0 + r) * p.Dv + d, s_l[r] == 0.f ? 0.f : o[c][r] / s_l[r]);
+      if (p.part_o) p.part_o[part_at(p, t, head, split) * p.Dv + d] = o[c][r];
+      else store_out(reinterpret_cast<E*>(p.out) + t * p.out_stride_tok + (size_t)head * p.Dv + d, s_l[r] == 0.f ? 0.f : o[c][r] / s_l[r]);
     }
   }
-  if (p.part_o && tid < rows) {
-    float* ml = p.part_ml + ((problem * p.num_splits + split) * ROWS + tid) * 2;
-    ml[0] = s_m[tid], ml[1] = s_l[tid];
-  }
+  if (p.part_ml && tid < rows) *reinterpret_cast<float2*>(p.part_ml + part_at(p, t, h * p.G + g0 + tid, split) * 2) = make_float2(s_m[tid], s_l[tid]);
 }
 
 // ---- bf16, widths up to 128, pages of 16-key groups: matrix instructions fed by TMA ------------------------------------------------------------------------
@@ -186,13 +191,39 @@ constexpr int FW = 4, FS = 3;                       // warps; groups in a warp's
 constexpr int HALF_BYTES = 2048, GROUP_BYTES = 4 * HALF_BYTES;      // 16 rows of 64 columns; K low, K high, V low, V high
 constexpr int SQ_BYTES = ROWS * 256, LDO = 132;
 constexpr int FAST_SMEM = 1024 + FW * FS * GROUP_BYTES + SQ_BYTES + 256;
-static_assert(FW * ROWS * LDO * 4 + FW * ROWS * 8 <= FW * FS * GROUP_BYTES, "the warps' results fit where the ring was");
+constexpr int FINISH_FLOATS = FW * ROWS * LDO + FW * ROWS * 2 + ROWS * 2 + ROWS * 2 + ROWS * MAX_CLUSTER;
+static_assert(FINISH_FLOATS * 4 <= FW * FS * GROUP_BYTES, "the warps' results fit where the ring was");
 
 // 16-byte chunk c (0..15) of row r (0..15) of a K or V group: two boxes of 64 columns with the 128-byte swizzle
 __device__ __forceinline__ uint32_t group_off(int r, int c) { return (uint32_t)(((c >> 3) << 11) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 __device__ __forceinline__ uint32_t q_off(int r, int c) { return (uint32_t)(r * 256 + ((c ^ (r & 7)) << 4)); }
 
-template <int NT>         // eights of query heads: 1 or 2
+// Values behind the first `live` rows of a group are not multiplied: whole warp.
+__device__ __forceinline__ void zero_values(uint8_t* group, int live, int halves, int lane) {
+  for (int j = lane; j < (16 - live) * 8 * halves; j += 32) {
+    const int half = j / ((16 - live) * 8), at = j % ((16 - live) * 8);
+    *reinterpret_cast<uint4*>(group + (2 + half) * HALF_BYTES + live * 128 + at * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();                         // the next copy into the group comes behind these writes
+  __syncwarp();
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_cluster(uint32_t at, int rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(rank));
+  return remote;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t at) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+  return x;
+}
+
+template <int NT>         // eights of rows: 1 or 2
 __global__ void __launch_bounds__(FW * 32, 2) attn_budget_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const BudgetParams p) {
   pdl_launch_dependents();
   extern __shared__ uint8_t fast_smem[];
@@ -212,10 +243,23 @@ __global__ void __launch_bounds__(FW * 32, 2) attn_budget_kernel(const __grid_co
   }
   __syncthreads();
   pdl_wait(TL_ATTN_DECODE);
-  const int S = p.num_splits, split = blockIdx.x % S, y = blockIdx.x / S, hy = y % (p.Hkv * p.head_tiles), t = y / (p.Hkv * p.head_tiles);
-  const int h = hy / p.head_tiles, ht = hy % p.head_tiles, g0 = ht * ROWS, rows = min(ROWS, p.G - g0);
-  if (p.cu_q && t >= p.cu_q[p.num_seqs]) return;
-  const Token tok = token_of(p, t);
+  const int S = p.num_splits, split = blockIdx.x % S, y = blockIdx.x / S, per_token = p.Hkv * p.head_tiles, hy = y % per_token;
+  const int h = hy / p.head_tiles, g0 = hy % p.head_tiles * ROWS, heads = min(ROWS, p.G - g0);      // heads of a token
+  int t = y / per_token, tokens = 1;                // first token, and how many
+  Token tok;
+  if (p.run == 1) {
+    if (p.cu_q && t >= p.cu_q[p.num_seqs]) return;
+    tok = token_of(p, t);
+  } else {
+    const int runs = (p.uniform_q + p.run - 1) / p.run;
+    tok.seq = t / runs;
+    const int q0 = p.cu_q ? p.cu_q[tok.seq] : tok.seq * p.uniform_q, q1 = p.cu_q ? p.cu_q[tok.seq + 1] : q0 + p.uniform_q;
+    t = q0 + t % runs * p.run;
+    tokens = min(p.run, min(q1, p.tokens) - t);
+    if (tokens <= 0) return;
+    tok.seen = max(min(p.kv_lens[tok.seq] - (q1 - t - tokens), p.max_blocks * p.bs), 0);            // of the last token
+  }
+  const int rows = heads * tokens;                  // row r: token r / heads, head r % heads
   const int sub = p.bs >> 4;                        // groups of a page
   const size_t list = (size_t)t * p.Hkv + h;
   const int* pages = p.pages ? p.pages + list * p.width : nullptr;
@@ -225,7 +269,8 @@ __global__ void __launch_bounds__(FW * 32, 2) attn_budget_kernel(const __grid_co
   const int k_halves = (p.D + 63) >> 6, v_halves = (p.Dv + 63) >> 6, boxes = k_halves + v_halves;
   const int* table = p.table + tok.seq * p.table_stride;
 
-  // Rows and live keys of this warp's groups i0..i0 + 31, one to a lane.
+  // Rows of this warp's groups i0..i0 + 31, one to a lane, and how many keys from the group's first on the last token sees (what it sees behind the group counts
+  // up to 16: a row of a token before it sees less).
   int row_l = 0, live_l = 0;
   const auto locate = [&](int i0) {
     const int i = i0 + lane;
@@ -234,7 +279,7 @@ __global__ void __launch_bounds__(FW * 32, 2) attn_budget_kernel(const __grid_co
       const int g = lo + warp + i * FW, page = pages ? pages[g / sub] : g / sub, off = (g % sub) * 16;
       if (page >= 0 && page < p.max_blocks) {
         const int block = table[page];
-        live_l = (unsigned)block < (unsigned)p.num_blocks ? max(0, min(16, tok.seen - (page * p.bs + off))) : 0;
+        live_l = (unsigned)block < (unsigned)p.num_blocks ? max(0, min(16 + ROWS, tok.seen - (page * p.bs + off))) : 0;
         row_l = (block * p.Hkv + h) * p.bs + off;
       }
     }
@@ -262,7 +307,7 @@ __global__ void __launch_bounds__(FW * 32, 2) attn_budget_kernel(const __grid_co
     const int r = i >> 4, c = i & 15;
     uint4 x = make_uint4(0, 0, 0, 0);
     if (r < rows && c * 8 < p.D) {
-      const bf16* from = q + r * p.q_stride_head + c * 8;
+      const bf16* from = q + r / heads * p.q_stride_tok + r % heads * p.q_stride_head + c * 8;
       if (p.q_vec) {
         x = *reinterpret_cast<const uint4*>(from);
       } else {
@@ -289,11 +334,13 @@ __global__ void __launch_bounds__(FW * 32, 2) attn_budget_kernel(const __grid_co
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[x][i][0] = o[x][i][1] = o[x][i][2] = o[x][i][3] = 0.f;
   }
-  float* score[NT];                                 // of this lane's heads, at the block's first key
+  float* score[NT];                                 // of this lane's rows, at the block's first key
+  int behind[NT];                                   // keys that the problem's last token sees and this lane's row does not
 #pragma unroll
   for (int x = 0; x < NT; ++x) {
     const int r = gr + 8 * x;
-    score[x] = p.scores && r < rows ? p.scores + ((size_t)t * p.Hkv * p.G + h * p.G + g0 + r) * p.capacity + (size_t)lo * 16 : nullptr;
+    score[x] = p.scores && r < rows ? p.scores + ((size_t)(t + r / heads) * p.Hkv * p.G + h * p.G + g0 + r % heads) * p.capacity + (size_t)lo * 16 : nullptr;
+    behind[x] = r < rows ? tokens - 1 - r / heads : 0;
   }
   uint32_t phases = 0;
   int stage = 0;
@@ -308,14 +355,7 @@ __global__ void __launch_bounds__(FW * 32, 2) attn_budget_kernel(const __grid_co
       phases ^= 1u << stage;
       if (lane == stage) live_st = 0;               // nothing in flight there
       const uint32_t sK = smem_u32(ring + stage * GROUP_BYTES), sV = sK + 2 * HALF_BYTES;
-      if (live < 16) {                              // what lies behind the last live key is not multiplied
-        for (int j = lane; j < (16 - live) * 8 * v_halves; j += 32) {
-          const int half = j / ((16 - live) * 8), at = j % ((16 - live) * 8);
-          *reinterpret_cast<uint4*>(ring + stage * GROUP_BYTES + (2 + half) * HALF_BYTES + live * 128 + at * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
+      if (live < 16 && tokens == 1) zero_values(ring + stage * GROUP_BYTES, live, v_halves, lane);
       float s[2][4];
 #pragma unroll
       for (int x = 0; x < 2; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
@@ -335,7 +375,7 @@ __global__ void __launch_bounds__(FW * 32, 2) attn_budget_kernel(const __grid_co
         for (int e = 0; e < 4; ++e) {
           const int key = (e >> 1) * 8 + t4 * 2 + (e & 1);
           const float raw = score_transform(s[e >> 1][2 * x + (e & 1)], p.scale, p.softcap);
-          v[e] = key < live ? raw : -INFINITY;
+          v[e] = key < live - behind[x] ? raw : -INFINITY;
         }
         if (score[x]) {
           float* to = score[x] + (size_t)(warp + i * FW) * 16 + t4 * 2;
@@ -359,13 +399,37 @@ __global__ void __launch_bounds__(FW * 32, 2) attn_budget_kernel(const __grid_co
         l[x] += (v[0] + v[1]) + (v[2] + v[3]);
         pf[x][0] = pack_bf16(v[0], v[1]), pf[x][1] = pack_bf16(v[2], v[3]);
       }
+      if (live - (tokens - 1) >= 16 || tokens == 1) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j >= v_steps) break;
-        uint32_t a[4];
-        ldsm_x4_trans(sV + group_off((mi >> 1) * 8 + (lane & 7), j * 2 + (mi & 1)), a[0], a[1], a[2], a[3]);
+        for (int j = 0; j < 8; ++j) {
+          if (j >= v_steps) break;
+          uint32_t a[4];
+          ldsm_x4_trans(sV + group_off((mi >> 1) * 8 + (lane & 7), j * 2 + (mi & 1)), a[0], a[1], a[2], a[3]);
 #pragma unroll
-        for (int x = 0; x < NT; ++x) mma_16816(o[x][j], a, pf[x][0], pf[x][1]);
+          for (int x = 0; x < NT; ++x) mma_16816(o[x][j], a, pf[x][0], pf[x][1]);
+        }
+      } else {
+        // Some of the tokens do not see all of these keys: each has a product of its own, behind which the values that only later ones see are zeros, and takes its
+        // own columns from it.
+        for (int i = tokens - 1; i >= 0; --i) {
+          const int own = max(live - (tokens - 1 - i), 0);
+          if (own < 16) zero_values(ring + stage * GROUP_BYTES, own, v_halves, lane);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (j >= v_steps) break;
+            uint32_t a[4];
+            ldsm_x4_trans(sV + group_off((mi >> 1) * 8 + (lane & 7), j * 2 + (mi & 1)), a[0], a[1], a[2], a[3]);
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+              float c[4] = {0.f, 0.f, 0.f, 0.f};
+              mma_16816(c, a, pf[x][0], pf[x][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if ((8 * x + t4 * 2 + (e & 1)) / heads == i) o[x][j][e] += c[e];
+            }
+          }
+          __syncwarp();
+        }
       }
       __syncwarp();                                 // every lane has read the stage
     } else {
@@ -399,7 +463,13 @@ __global__ void __launch_bounds__(FW * 32, 2) attn_budget_kernel(const __grid_co
       for (int e = 0; e < 4; ++e) sO[(warp * ROWS + 8 * x + t4 * 2 + (e & 1)) * LDO + j * 16 + gr + (e >> 1) * 8] = o[x][j][e];
   }
   __syncthreads();
-  const size_t problem = ((size_t)t * p.Hkv + h) * p.head_tiles + ht;
+  float* sPart = sM + FW * ROWS * 2;                // [ROWS][2]: the block's maximum and sum
+  float* sAll = sPart + ROWS * 2;                   // [ROWS][2]: the problem's maximum, 1 / sum
+  float* sFactor = sAll + ROWS * 2;                 // [ROWS][MAX_CLUSTER]
+  const auto token_at = [&](int r) { return t + r / heads; };
+  const auto head_at = [&](int r) { return h * p.G + g0 + r % heads; };
+  const bool parts = p.part_o != nullptr;
+  bf16* out = reinterpret_cast<bf16*>(p.out);
   for (int i = tid; i < rows * p.Dv; i += FW * 32) {
     const int r = i / p.Dv, d = i % p.Dv;
     float M = -INFINITY, L = 0.f, x = 0.f;
@@ -412,14 +482,70 @@ __global__ void __launch_bounds__(FW * 32, 2) attn_budget_kernel(const __grid_co
       L = fmaf(e, sM[(w * ROWS + r) * 2 + 1], L);
       x = fmaf(e, sO[(w * ROWS + r) * LDO + d], x);
     }
-    if (p.part_o) {
-      const size_t at = (problem * S + split) * ROWS + r;
-      p.part_o[at * p.Dv + d] = x;
-      if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(M, L);
-    } else {
-      reinterpret_cast<bf16*>(p.out)[t * p.out_stride_tok + (size_t)(h * p.G + g0 + r) * p.Dv + d] = __float2bfloat16(L == 0.f ? 0.f : x / L);
+    if (parts) p.part_o[part_at(p, token_at(r), head_at(r), split) * p.Dv + d] = x;
+    else if (S == 1) out[token_at(r) * p.out_stride_tok + (size_t)head_at(r) * p.Dv + d] = __float2bfloat16(L == 0.f ? 0.f : x / L);
+    else sO[r * LDO + d] = x;                       // warp 0's, which this thread alone reads
+    if (d == 0) {
+      sPart[r * 2] = M, sPart[r * 2 + 1] = L;
+      sAll[r * 2] = base, sAll[r * 2 + 1] = L == 0.f ? 0.f : 1.f / L;
+      if (p.part_ml) *reinterpret_cast<float2*>(p.part_ml + part_at(p, token_at(r), head_at(r), split) * 2) = make_float2(M, L);
     }
   }
+  if (parts) return;
+  if (S > 1) {
+    cluster_barrier();
+    if (tid < rows) {
+      float m_of[MAX_CLUSTER], l_of[MAX_CLUSTER], M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int s = 0; s < MAX_CLUSTER; ++s) {
+        m_of[s] = -INFINITY, l_of[s] = 0.f;
+        if (s < S) {
+          const uint32_t at = in_cluster(smem_u32(sPart + tid * 2), s);
+          m_of[s] = ld_cluster(at), l_of[s] = ld_cluster(at + 4);
+        }
+        M = fmaxf(M, m_of[s]);
+      }
+      const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+      for (int s = 0; s < MAX_CLUSTER; ++s) L = fmaf(m_of[s] = exp2f(m_of[s] - base), l_of[s], L);
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      sAll[tid * 2] = base, sAll[tid * 2 + 1] = inv;
+#pragma unroll
+      for (int s = 0; s < MAX_CLUSTER; ++s) sFactor[tid * MAX_CLUSTER + s] = m_of[s] * inv;
+    }
+    __syncthreads();
+    for (int i = tid; i < (rows - split + S - 1) / S * p.Dv; i += FW * 32) {        // rows split, split + S, ...
+      const int r = split + i / p.Dv * S, d = i % p.Dv;
+      const uint32_t at = smem_u32(sO + r * LDO + d);
+      float x = 0.f;
+#pragma unroll
+      for (int s = 0; s < MAX_CLUSTER; ++s)
+        if (s < S) x = fmaf(sFactor[r * MAX_CLUSTER + s], ld_cluster(in_cluster(at, s)), x);
+      out[token_at(r) * p.out_stride_tok + (size_t)head_at(r) * p.Dv + d] = __float2bfloat16(x);
+    }
+  } else if (p.weigh_here) {
+    __syncthreads();
+  }
+  if (p.weigh_here) {                               // one token: row r is head r, and the block's scores are its own writes
+    float* w = p.weights + tok.seq * p.w_seq + h * p.w_head;
+    const float* from = p.scores + ((size_t)t * p.Hkv * p.G + h * p.G) * p.capacity;
+    const int end = min((lo + n) * 16, tok.seen);
+    for (int j0 = lo * 16 + tid; j0 < end; j0 += 4 * FW * 32) {
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+      for (int r = 0; r < rows; ++r) {
+        float x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = j0 + k * FW * 32 < end ? from[r * p.capacity + j0 + k * FW * 32] : 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] = fmaf(exp2f(x[k] - sAll[r * 2]), sAll[r * 2 + 1], sum[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (j0 + k * FW * 32 < end) w[j0 + k * FW * 32] += sum[k];
+    }
+  }
+  if (S > 1) cluster_barrier();                     // nobody's shared memory goes away while another block reads it
 }
 
 bool fast_fits(const BudgetParams& p, int fp32) {
@@ -435,90 +561,114 @@ int launch_fast(BudgetParams p, cudaStream_t s) {
   if (rc) return rc;
   rc = make_tmap_bf16_2d(&tv, p.v, rows, p.Dv, p.Dv, 16);
   if (rc) return rc;
-  auto kernel = p.G <= 8 ? attn_budget_kernel<1> : attn_budget_kernel<2>;
+  const bool one = p.G * p.run <= 8;
+  auto kernel = one ? attn_budget_kernel<1> : attn_budget_kernel<2>;
   static bool configured[2][64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !configured[p.G <= 8][dev]) {
+  if (dev < 0 || dev >= 64 || !configured[one][dev]) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FAST_SMEM);
     if (e != cudaSuccess) return -(int)e;
-    if (dev >= 0 && dev < 64) configured[p.G <= 8][dev] = true;
+    if (dev >= 0 && dev < 64) configured[one][dev] = true;
   }
-  return launch_kernel(kernel, dim3(p.num_splits * p.Hkv * p.head_tiles * p.tokens), dim3(FW * 32), FAST_SMEM, s, tk, tv, p);
+  const int problems = (p.run > 1 ? p.num_seqs * ((p.uniform_q + p.run - 1) / p.run) : p.tokens) * p.Hkv * p.head_tiles;
+  const dim3 grid(p.num_splits * problems), block(FW * 32);
+  if (!p.cluster) return launch_kernel(kernel, grid, block, FAST_SMEM, s, tk, tv, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = FAST_SMEM, cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.num_splits, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr, cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tk, tv, p);
+  return e == cudaSuccess ? 0 : -(int)e;
 }
 
 // ---- joining ------------------------------------------------------------------------------------------------------------------------------------------
-constexpr int JOIN_THREADS = 128, MAX_SPLITS = 64;
+constexpr int JOIN_THREADS = 128, WEIGH_KEYS = 4 * JOIN_THREADS;
+static_assert(MAX_GROUP <= JOIN_THREADS, "a block weighs a row to a thread");
 
-// {maximum, sum} of row r in each split of a problem -> factors of the splits' values, exp2(max - common) / sum: one warp, S <= 64.
-__device__ __forceinline__ void split_factors(const float* ml, int S, int lane, float* factor, float* common, float* inv_sum) {
+// {maximum, sum} of a row in each of its splits -> factors of the splits' values, exp2(max - common) / sum; by one warp.
+__device__ __forceinline__ void split_factors(const float* ml, int S, int lane, float* factor) {
   float m[2], l[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int s = lane + 32 * i;
-    const float2 x = s < S ? __ldcg(reinterpret_cast<const float2*>(ml + (size_t)s * ROWS * 2)) : make_float2(-INFINITY, 0.f);
+    const float2 x = s < S ? __ldcg(reinterpret_cast<const float2*>(ml) + s) : make_float2(-INFINITY, 0.f);
     m[i] = x.x, l[i] = x.y;
   }
   const float M = warp_max(fmaxf(m[0], m[1])), base = M == -INFINITY ? 0.f : M;
   const float e0 = exp2f(m[0] - base), e1 = exp2f(m[1] - base);
   const float L = warp_sum(fmaf(e0, l[0], e1 * l[1])), inv = L == 0.f ? 0.f : 1.f / L;
-  if (factor) {
-    if (lane < S) factor[lane] = e0 * inv;
-    if (lane + 32 < S) factor[lane + 32] = e1 * inv;
-  }
-  if (common && lane == 0) *common = base, *inv_sum = inv;
+  if (lane < S) factor[lane] = e0 * inv;
+  if (lane + 32 < S) factor[lane + 32] = e1 * inv;
 }
 
-// A block per problem: the parts of each row, weighed by their distance to the common maximum.
+// The first `join_blocks` blocks join the parts of one row each; the others weigh a run of keys of one (sequence, key/value head) each.
 template <typename E>
-__global__ void __launch_bounds__(JOIN_THREADS) attn_budget_join_kernel(const BudgetParams p) {
+__global__ void __launch_bounds__(JOIN_THREADS) attn_budget_finish_kernel(const BudgetParams p, int join_blocks) {
   pdl_launch_dependents();
-  __shared__ float s_w[ROWS][MAX_SPLITS];
-  const int tid = threadIdx.x, hy = blockIdx.x % (p.Hkv * p.head_tiles), t = blockIdx.x / (p.Hkv * p.head_tiles);
-  const int h = hy / p.head_tiles, ht = hy % p.head_tiles, g0 = ht * ROWS, rows = min(ROWS, p.G - g0), S = p.num_splits;
+  __shared__ float s_factor[MAX_SPLITS], s_all[MAX_GROUP * 2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, S = p.num_splits, Hq = p.Hkv * p.G;
   pdl_wait();
-  if (p.cu_q && t >= p.cu_q[p.num_seqs]) return;
-  const size_t problem = ((size_t)t * p.Hkv + h) * p.head_tiles + ht;
-  for (int r = tid >> 5; r < rows; r += JOIN_THREADS / 32) split_factors(p.part_ml + (problem * S * ROWS + r) * 2, S, tid & 31, s_w[r], nullptr, nullptr);
-  __syncthreads();
-  for (int i = tid; i < rows * p.Dv; i += JOIN_THREADS) {
-    const int r = i / p.Dv, d = i % p.Dv;
-    const float* o = p.part_o + (problem * S * ROWS + r) * p.Dv + d;
-    float x = 0.f;
+  if ((int)blockIdx.x < join_blocks) {
+    const int t = blockIdx.x / Hq, head = blockIdx.x % Hq;
+    if (p.cu_q && t >= p.cu_q[p.num_seqs]) return;
+    if (warp == 0) split_factors(p.part_ml + part_at(p, t, head, 0) * 2, S, lane, s_factor);
+    __syncthreads();
+    for (int d = tid; d < p.Dv; d += JOIN_THREADS) {
+      const float* o = p.part_o + part_at(p, t, head, 0) * p.Dv + d;
+      float x = 0.f;
+#pragma unroll 16
+      for (int s = 0; s < S; ++s) x = fmaf(s_factor[s], __ldcg(o + (size_t)s * p.Dv), x);
+      store_out(reinterpret_cast<E*>(p.out) + t * p.out_stride_tok + (size_t)head * p.Dv + d, x);
+    }
+    return;
+  }
+  const int blocks = (int)((p.capacity + WEIGH_KEYS - 1) / WEIGH_KEYS), i = blockIdx.x - join_blocks;
+  const int h = i / blocks % p.Hkv, seq = i / blocks / p.Hkv;
+  const long long j0 = (long long)(i % blocks) * WEIGH_KEYS + tid;
+  const int q0 = p.cu_q ? p.cu_q[seq] : seq * p.uniform_q, q1 = min(p.cu_q ? p.cu_q[seq + 1] : q0 + p.uniform_q, p.tokens);
+  const int total = p.kv_lens[seq], len = min(total, p.max_blocks * p.bs);
+  if (j0 - tid >= len) return;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  const int batch = MAX_GROUP / p.G;             // tokens whose rows a block has room for
+  for (int t0 = q0; t0 < q1; t0 += batch) {
+    const int pairs = min(batch, q1 - t0) * p.G;
+    __syncthreads();
+    if (tid < pairs) {                           // MAX_GROUP = JOIN_THREADS: a row to a thread
+      const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + part_at(p, t0 + tid / p.G, h * p.G + tid % p.G, 0);
+      float M = -INFINITY, L = 0.f;
 #pragma unroll 8
-    for (int s = 0; s < S; ++s) x = fmaf(s_w[r][s], __ldcg(o + (size_t)s * ROWS * p.Dv), x);
-    store_out(reinterpret_cast<E*>(p.out) + t * p.out_stride_tok + (size_t)(h * p.G + g0 + r) * p.Dv + d, x);
-  }
-}
-
-constexpr int WEIGH_THREADS = 256, MAX_GROUP = 128;
-
-// A block per (run of keys, key/value head, sequence): the weights of the sequence's new tokens, added up token by token and head by head.
-__global__ void __launch_bounds__(WEIGH_THREADS) attn_budget_weigh_kernel(const BudgetParams p) {
-  pdl_launch_dependents();
-  __shared__ float s_m[MAX_GROUP], s_inv[MAX_GROUP];
-  const int tid = threadIdx.x, h = blockIdx.y, seq = blockIdx.z, S = p.num_splits;
-  const long long j = (long long)blockIdx.x * WEIGH_THREADS + tid;
-  pdl_wait();
-  const int q0 = p.cu_q ? p.cu_q[seq] : seq * p.uniform_q, q1 = p.cu_q ? p.cu_q[seq + 1] : q0 + p.uniform_q;
-  const int len = min(p.kv_lens[seq], p.max_blocks * p.bs);
-  if ((long long)blockIdx.x * WEIGH_THREADS >= len) return;
-  float sum = 0.f;
-  for (int t = q0; t < q1; ++t) {
-    const int seen = p.kv_lens[seq] - (q1 - 1 - t);
-    __syncthreads();
-    for (int g = tid >> 5; g < p.G; g += WEIGH_THREADS / 32) {
-      const size_t problem = ((size_t)t * p.Hkv + h) * p.head_tiles + g / ROWS;
-      split_factors(p.part_ml + (problem * S * ROWS + g % ROWS) * 2, S, tid & 31, nullptr, &s_m[g], &s_inv[g]);
+      for (int s = 0; s < S; ++s) M = fmaxf(M, __ldcg(ml + s).x);
+      const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll 8
+      for (int s = 0; s < S; ++s) {
+        const float2 x = __ldcg(ml + s);
+        L = fmaf(exp2f(x.x - base), x.y, L);
+      }
+      s_all[tid * 2] = base, s_all[tid * 2 + 1] = L == 0.f ? 0.f : 1.f / L;
     }
     __syncthreads();
-    if (j < seen && j < len) {
-      const float* s = p.scores + ((size_t)t * p.Hkv + h) * p.G * p.capacity + j;
+    const float* s = p.scores + ((size_t)t0 * Hq + h * p.G) * p.capacity + j0;
 #pragma unroll 4
-      for (int g = 0; g < p.G; ++g) sum = fmaf(exp2f(__ldcg(s + g * p.capacity) - s_m[g]), s_inv[g], sum);
+    for (int i = 0; i < pairs; ++i) {
+      const int tok = i / p.G, seen = min(total - (q1 - 1 - t0 - tok), len);
+      const float m = s_all[i * 2], inv = s_all[i * 2 + 1];
+      const float* row = s + ((size_t)tok * Hq + i % p.G) * p.capacity;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float x = j0 + k * JOIN_THREADS < seen ? __ldcg(row + k * JOIN_THREADS) : -INFINITY;
+        sum[k] = fmaf(exp2f(x - m), x == -INFINITY ? 0.f : inv, sum[k]);       // (a row without a sum adds nothing to keys it does not see)
+      }
     }
   }
-  if (j < len) p.weights[seq * p.w_seq + h * p.w_head + j] += sum;
+  float* w = p.weights + seq * p.w_seq + h * p.w_head;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (j0 + k * JOIN_THREADS < len) w[j0 + k * JOIN_THREADS] += sum[k];
 }
 
 template <typename E>
@@ -539,13 +689,13 @@ int heads_in_tiles(int G) { return (G + ROWS - 1) / ROWS; }
 
 extern "C" {
 
-// Bytes of the workspace: the parts of the problems, and the scores where weights are kept (scores = 1; capacity: keys of the widest table row).
+// Bytes of the workspace: the parts of the rows, and the scores where weights are kept (scores = 1; capacity: keys of the widest table row).
 long long swb_attn_budget_workspace(int tokens, int Hkv, int G, int Dv, int num_splits, long long capacity, int scores) {
-  const long long parts = num_splits > 1 || scores ? (long long)tokens * Hkv * swb::heads_in_tiles(G) * num_splits * swb::ROWS * (Dv + 2) * 4 : 0;
-  return parts + (scores ? (long long)tokens * Hkv * G * capacity * 4 : 0);
+  const long long rows = (long long)tokens * Hkv * G;
+  return rows * 4 * (num_splits * (Dv + 2) + (scores ? capacity : 0)) + 16;
 }
 
-// See BudgetParams. dims: host int[16] = tokens, num_seqs, tokens of each sequence (without cu_q), table width, blocks, block_size, Hkv, G, D, Dv,
+// See BudgetParams. dims: host int[16] = tokens, num_seqs, tokens of each sequence (with cu_q: at most), table width, blocks, block_size, Hkv, G, D, Dv,
 // width of the page lists, splits, fp32, 0, 0, 0; strides: host long long[8] = q token and head, out token, table, weights sequence and head, 0, 0.
 // pages and counts, or weights, or neither.
 int swb_attn_budget(const int* dims, const long long* strides, const void* q, void* out, const void* k, const void* v, const int* table, const int* cu_q,
@@ -558,7 +708,7 @@ int swb_attn_budget(const int* dims, const long long* strides, const void* q, vo
   const int fp32 = dims[12];
   if (p.tokens <= 0 || p.num_seqs <= 0) return 0;
   if (p.num_seqs > 65535 || p.Hkv > 65535 || p.max_blocks < 1 || p.num_blocks < 1 || p.bs < 1 || p.Hkv < 1 || p.G < 1 || p.G > MAX_GROUP || p.D < 1 || p.D > 256 ||
-      p.Dv < 1 || p.Dv > 256 || p.num_splits < 1 || p.num_splits > MAX_SPLITS || (!cu_q && p.uniform_q < 1) || (pages && (!counts || p.width < 1 || weights)) || !q || !out ||
+      p.Dv < 1 || p.Dv > 256 || p.num_splits < 1 || p.num_splits > MAX_SPLITS || p.uniform_q < 1 || (pages && (!counts || p.width < 1 || weights)) || !q || !out ||
       !k || !v || !table || !kv_lens)
     return -3;
   p.head_tiles = heads_in_tiles(p.G);
@@ -566,21 +716,33 @@ int swb_attn_budget(const int* dims, const long long* strides, const void* q, vo
   p.q = q, p.out = out, p.k = k, p.v = v, p.table = table, p.cu_q = cu_q, p.kv_lens = kv_lens, p.pages = pages, p.counts = counts, p.weights = weights;
   p.q_stride_tok = strides[0], p.q_stride_head = strides[1], p.out_stride_tok = strides[2], p.table_stride = strides[3], p.w_seq = strides[4], p.w_head = strides[5];
   p.scale = scale, p.softcap = softcap, p.capacity = (long long)p.max_blocks * p.bs;
-  if (swb_attn_budget_workspace(p.tokens, p.Hkv, p.G, p.Dv, p.num_splits, p.capacity, weights != nullptr) > workspace_bytes) return -3;
-  if (p.num_splits > 1 || weights) {
-    const size_t rows = (size_t)p.tokens * p.Hkv * p.head_tiles * p.num_splits * ROWS;
-    p.part_o = reinterpret_cast<float*>(workspace);
-    p.part_ml = p.part_o + rows * p.Dv;
-    if (weights) p.scores = p.part_ml + rows * 2;
+  const bool fast = fast_fits(p, fp32);
+  // tokens of one sequence read the same keys: as many as rows allow share a problem
+  p.run = 1;
+  while (fast && !pages && p.run * 2 * p.G <= ROWS && p.run < p.uniform_q) p.run *= 2;
+  const long long problems = (p.run > 1 ? (long long)p.num_seqs * ((p.uniform_q + p.run - 1) / p.run) : p.tokens) * p.Hkv * p.head_tiles;
+  // Blocks of a cluster start together and wait for one another, which costs nothing while all of them fit the chip at once; behind that a second launch is cheaper
+  // (48 sequences of up to 8191 keys, 8 key/value heads, 4 splits: 305 us as clusters, 2xx with a second launch)
+  p.cluster = fast && p.num_splits > 1 && p.num_splits <= MAX_CLUSTER && problems * p.num_splits <= 2 * 148;
+  p.weigh_here = weights && fast && p.uniform_q == 1 && p.head_tiles == 1 && (p.cluster || p.num_splits == 1);
+  const bool join = p.num_splits > 1 && !p.cluster, weigh = weights && !p.weigh_here;
+  if (join || weights) {
+    if (swb_attn_budget_workspace(p.tokens, p.Hkv, p.G, p.Dv, p.num_splits, p.capacity, weights != nullptr) > workspace_bytes || !workspace) return -3;
+    const size_t rows = (size_t)p.tokens * p.Hkv * p.G, parts = rows * p.num_splits;
+    float* ws = reinterpret_cast<float*>(workspace);          // scores in front: rows of a multiple of 16 keys stay 64-byte aligned
+    if (weights) p.scores = ws, ws += rows * p.capacity;
+    ws += (4 - (rows * p.capacity * (weights != nullptr)) % 4) % 4;
+    if (join || weigh) p.part_ml = ws;
+    if (join) p.part_o = ws + parts * 2;
   }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  int rc = fast_fits(p, fp32) ? launch_fast(p, s) : fp32 ? launch_plain<float>(p, s) : launch_plain<bf16>(p, s);
-  if (rc || !p.part_o) return rc;
-  const dim3 grid(p.Hkv * p.head_tiles * p.tokens);
-  rc = fp32 ? launch_kernel(attn_budget_join_kernel<float>, grid, dim3(JOIN_THREADS), 0, s, p)
-            : launch_kernel(attn_budget_join_kernel<bf16>, grid, dim3(JOIN_THREADS), 0, s, p);
-  if (rc || !weights) return rc;
-  return launch_kernel(attn_budget_weigh_kernel, dim3((unsigned)((p.capacity + WEIGH_THREADS - 1) / WEIGH_THREADS), p.Hkv, p.num_seqs), dim3(WEIGH_THREADS), 0, s, p);
+  int rc = fast ? launch_fast(p, s) : fp32 ? launch_plain<float>(p, s) : launch_plain<bf16>(p, s);
+  if (rc || !(join || weigh)) return rc;
+  const int join_blocks = join ? p.tokens * p.Hkv * p.G : 0;
+  const long long blocks = join_blocks + (weigh ? (p.capacity + WEIGH_KEYS - 1) / WEIGH_KEYS * p.Hkv * p.num_seqs : 0);
+  if (blocks > INT_MAX) return -3;
+  return fp32 ? launch_kernel(attn_budget_finish_kernel<float>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, s, p, join_blocks)
+              : launch_kernel(attn_budget_finish_kernel<bf16>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, s, p, join_blocks);
 }
 
 }  // extern "C"

@@ -142,7 +142,7 @@ long long swb_evict_moves(int num_seqs, int Hkv, int capacity, int keep) {
   return (long long)num_seqs * Hkv * (1 + 2 * most);
 }
 
-// See EvictParams. dims: host int[12] = num_seqs, Hkv, table width, blocks, block_size, k row bytes, v row bytes, capacity, keep, recent, first, 0;
+// See EvictParams. dims: host int[11] = num_seqs, Hkv, table width, blocks, block_size, k row bytes, v row bytes, capacity, keep, recent, first;
 // strides: host long long[4] = weights sequence and head, positions sequence and head. moves: swb_evict_moves ints.
 int swb_evict(const int* dims, const long long* strides, void* k, void* v, const int* table, long long table_stride, const int* kv_lens, int* new_lens, const int* next,
               float* weights, int* positions, int* moves, void* stream) {

@@ -13,7 +13,7 @@ to the caller. Steps are described as in `paged_attention`: kv_lens int32 [num_s
 are the new tokens' ranges, or None where every sequence has max_q_len of them; rows behind the last range are left as they were."""
 from __future__ import annotations
 
-import ctypes
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -50,41 +50,59 @@ class PageSelection:
     counts: torch.Tensor
 
 
+# A decode step calls these once a layer: what is checked is read from each tensor once, and host arrays go to the library as packed bytes.
+_INTS = {n: struct.Struct(f"{n}i").pack for n in (9, 11, 14, 16)}
+_LONGS = {n: struct.Struct(f"{n}q").pack for n in (4, 8)}
+_KINDS = (torch.bfloat16, torch.float32)
+
+
 def _require(ok: bool, what: str) -> None:
     if not ok:
         raise KernelError(what)
 
 
-def _place(first: torch.Tensor, *others: torch.Tensor | None) -> None:
+def _place(*tensors: torch.Tensor | None) -> None:
     """All operands on the current device: launches go to its current stream."""
-    require_cuda(first, *others)
-    dev = torch.cuda.current_device()
-    for t in (first, *others):
-        if t is not None and t.device.index != dev:
+    dev = torch.cuda.current_device() if torch.cuda.is_initialized() else 0
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            require_cuda(t)
             raise KernelError(f"operands lie on {t.device}, the current device is cuda:{dev}")
 
 
-def _check_cache(kcache: torch.Tensor, vcache: torch.Tensor | None = None) -> None:
-    _require(kcache.dim() == 4 and kcache.dtype in (torch.bfloat16, torch.float32) and kcache.is_contiguous() and kcache.shape[3] <= MAX_WIDTH,
+def _check_cache(kcache: torch.Tensor, vcache: torch.Tensor | None = None) -> tuple[int, int, int, int, int]:
+    shape, kind = kcache.shape, kcache.dtype
+    _require(len(shape) == 4 and kind in _KINDS and kcache.is_contiguous() and shape[3] <= MAX_WIDTH,
              "pages are contiguous [blocks, kv heads, block_size, width] in bf16 or fp32, at most 256 wide")
-    _require(vcache is None or (vcache.dim() == 4 and vcache.dtype == kcache.dtype and vcache.is_contiguous() and vcache.shape[:3] == kcache.shape[:3]
-                                and vcache.shape[3] <= MAX_WIDTH), "value pages match the key pages in type, number, heads and block_size")
+    blocks, heads, bs, D = shape
+    if vcache is None:
+        return blocks, heads, bs, D, 0
+    other = vcache.shape
+    _require(len(other) == 4 and vcache.dtype == kind and vcache.is_contiguous() and other[:3] == shape[:3] and other[3] <= MAX_WIDTH,
+             "value pages match the key pages in type, number, heads and block_size")
+    return blocks, heads, bs, D, other[3]
 
 
-def _check_step(table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor | None, max_q_len: int, tokens: int | None) -> int:
-    n = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
-    _require(table.dtype == kv_lens.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == n and table.stride(1) == 1 and kv_lens.is_contiguous(),
-             "block_table is int32 [num_seqs, pages] with rows of unit stride, kv_lens int32 [num_seqs]")
-    _require(cu_q is None or (cu_q.dtype == torch.int32 and cu_q.shape == (n + 1,) and cu_q.is_contiguous()), "cu_q is int32 [num_seqs + 1]")
-    _require(max_q_len >= 1 and (cu_q is not None or tokens is None or tokens == n * max_q_len), "without cu_q every sequence has max_q_len tokens")
-    _require(n < 65536 and table.shape[1] >= 1, "at most 65535 sequences, of a page at least")
-    return n
+def _check_step(table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor | None, max_q_len: int, tokens: int) -> tuple[int, int]:
+    """Number of sequences and width of the table. tokens < 0: not known."""
+    lens, rows = kv_lens.shape, table.shape
+    _require(len(lens) == 1 and len(rows) == 2 and rows[0] == lens[0] < 65536 and rows[1] >= 1 and table.dtype == kv_lens.dtype == torch.int32 and table.stride(1) == 1
+             and kv_lens.is_contiguous(), "block_table is int32 [num_seqs, pages] with rows of unit stride, kv_lens int32 [num_seqs], up to 65535 sequences of a page at least")
+    n = lens[0]
+    if cu_q is None:
+        _require(max_q_len >= 1 and (tokens < 0 or tokens == n * max_q_len), "without cu_q every sequence has max_q_len >= 1 tokens")
+    else:
+        _require(max_q_len >= 1 and cu_q.dtype == torch.int32 and cu_q.shape == (n + 1,) and cu_q.is_contiguous(), "cu_q is int32 [num_seqs + 1], max_q_len >= 1")
+    return n, rows[1]
 
 
-def _check_rows(q: torch.Tensor, kv_heads: int, width: int) -> int:
-    _require(q.dim() == 3 and q.stride(2) == 1 and q.shape[2] == width and q.shape[1] % kv_heads == 0 and 1 <= q.shape[1] // kv_heads <= MAX_GROUP,
-             "q is [T, heads, width], unit inner stride, up to 128 heads to a key/value head")
-    return q.shape[1] // kv_heads
+def _check_rows(q: torch.Tensor, kv_heads: int, width: int) -> tuple[int, int, int, int]:
+    """Tokens, heads of a group, token and head strides."""
+    _require(q.dim() == 3, "q is [T, heads, width]")
+    (T, heads, D), (tok, head, inner) = q.shape, q.stride()
+    G = heads // max(kv_heads, 1)
+    _require(inner == 1 and D == width and heads == G * kv_heads and 1 <= G <= MAX_GROUP, "q is [T, heads, width], unit inner stride, up to 128 heads to a key/value head")
+    return T, G, tok, head
 
 
 def summarize_pages(kcache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, summaries: PageSummaries, *, cu_q: torch.Tensor | None,
@@ -93,12 +111,11 @@ def summarize_pages(kcache: torch.Tensor, block_table: torch.Tensor, kv_lens: to
     number). s = sum of a page's keys, a = max |s|: codes rint(127 s / a), scale a / (127 block_size); sums and quotient in 64 bits."""
     codes, scales = summaries.codes, summaries.scales
     _place(kcache, block_table, kv_lens, codes, scales, cu_q)
-    _check_cache(kcache)
-    n = _check_step(block_table, kv_lens, cu_q, max_q_len, None)
-    blocks, heads, bs, D = kcache.shape
+    blocks, heads, bs, D, _ = _check_cache(kcache)
+    n, per = _check_step(block_table, kv_lens, cu_q, max_q_len, -1)
     _require(codes.dtype == torch.int8 and codes.shape == (blocks, heads, D) and codes.is_contiguous() and scales.dtype == torch.float32
              and scales.shape == (blocks, heads) and scales.is_contiguous(), "summaries belong to these pages: int8 [blocks, kv heads, D], fp32 [blocks, kv heads]")
-    dims = (ctypes.c_int * 9)(n, max_q_len, block_table.shape[1], blocks, bs, heads, D, kcache.dtype == torch.float32, 0)
+    dims = _INTS[9](n, max_q_len, per, blocks, bs, heads, D, kcache.dtype == torch.float32, 0)
     check(kernels().swb_page_summaries(dims, kcache.data_ptr(), codes.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), ptr(cu_q),
                                        kv_lens.data_ptr(), stream_ptr()), "swb_page_summaries")
 
@@ -112,53 +129,66 @@ def select_pages(q: torch.Tensor, summaries: PageSummaries, block_table: torch.T
     group of the codes' dot product. A token whose queries are not all finite, or all zero, finds every page alike."""
     codes, scales = summaries.codes, summaries.scales
     _place(q, codes, scales, block_table, kv_lens, cu_q)
-    T = q.shape[0]
-    n = _check_step(block_table, kv_lens, cu_q, max_q_len, T)
-    _require(codes.dim() == 3 and codes.dtype == torch.int8 and codes.is_contiguous() and scales.dtype == torch.float32 and scales.shape == codes.shape[:2]
-             and scales.is_contiguous() and codes.shape[2] <= MAX_WIDTH, "summaries are int8 [blocks, kv heads, D] and fp32 [blocks, kv heads]")
-    blocks, heads, D = codes.shape
-    _require(q.dtype in (torch.bfloat16, torch.float32), "q is bf16 or fp32")
-    G = _check_rows(q, heads, D)
+    shape = codes.shape
+    _require(len(shape) == 3 and codes.dtype == torch.int8 and codes.is_contiguous() and scales.dtype == torch.float32 and scales.shape == shape[:2]
+             and scales.is_contiguous() and shape[2] <= MAX_WIDTH, "summaries are int8 [blocks, kv heads, D] and fp32 [blocks, kv heads]")
+    blocks, heads, D = shape
+    _require(q.dtype in _KINDS, "q is bf16 or fp32")
+    T, G, tok, head = _check_rows(q, heads, D)
+    n, per = _check_step(block_table, kv_lens, cu_q, max_q_len, T)
     _require(block_size >= 1 and top >= 0 and first >= 0 and last >= 1, "block_size >= 1, top >= 0, first >= 0, last >= 1")
-    lib = kernels()
-    _require(lib.swb_page_select_smem(block_table.shape[1], G, D) <= SELECT_SMEM, "a selection is made over at most 200 KB of scores (4 bytes a page)")
-    pages = torch.empty((T, heads, first + top + last), dtype=torch.int32, device=q.device)
+    lib, width = kernels(), first + top + last
+    _require(lib.swb_page_select_smem(per, G, D) <= SELECT_SMEM, "a selection is made over at most 200 KB of scores (4 bytes a page)")
+    pages = torch.empty((T, heads, width), dtype=torch.int32, device=q.device)
     counts = torch.empty((T, heads), dtype=torch.int32, device=q.device)
-    dims = (ctypes.c_int * 14)(T, n, max_q_len, block_table.shape[1], blocks, block_size, heads, G, D, first, top, last, q.dtype == torch.float32, 0)
-    check(lib.swb_page_select(dims, q.data_ptr(), q.stride(0), q.stride(1), codes.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), ptr(cu_q),
+    dims = _INTS[14](T, n, max_q_len, per, blocks, block_size, heads, G, D, first, top, last, q.dtype == torch.float32, 0)
+    check(lib.swb_page_select(dims, q.data_ptr(), tok, head, codes.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), ptr(cu_q),
                               kv_lens.data_ptr(), pages.data_ptr(), counts.data_ptr(), stream_ptr()), "swb_page_select")
     return PageSelection(pages, counts)
 
 
 def budget_splits(problems: int, keys: int, sms: int = 148) -> int:
-    """Blocks that share a problem's keys: two to an SM where problems (tokens * kv heads) are fewer, none of less than 64 keys."""
-    return max(1, min(2 * sms // max(1, problems), (keys + 63) // 64, MAX_SPLITS))
+    """Blocks that share a problem's keys (problems: tokens * kv heads). Two blocks fit an SM: enough of them for four rounds of all SMs, so that sequences of different
+    lengths even out, none of less than 64 keys. Up to 8 join within one launch; more take a second one, which pays where 8 would leave SMs idle over long caches."""
+    most = (keys + 63) // 64
+    splits = min(8, most, max(1, 8 * sms // max(1, problems)))
+    if problems * 8 < sms and keys >= 8192:
+        splits = min(MAX_SPLITS, most, 2 * sms // max(1, problems))
+    return max(1, splits)
 
 
-def _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, softcap, num_splits, out, keys, selection=None, weights=None) -> torch.Tensor:
-    _place(q, kcache, vcache, block_table, kv_lens, cu_q, out, weights)
-    _check_cache(kcache, vcache)
-    T, Hq, D = q.shape
-    n = _check_step(block_table, kv_lens, cu_q, max_q_len, T)
-    blocks, heads, bs, _ = kcache.shape
-    Dv = vcache.shape[3]
-    G = _check_rows(q, heads, kcache.shape[3])
-    _require(q.dtype == kcache.dtype, "queries and cache have one type")
+def _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, softcap, num_splits, out, pages, counts, weights) -> torch.Tensor:
+    _place(q, kcache, vcache, block_table, kv_lens, cu_q, out, weights, pages, counts)
+    blocks, heads, bs, D, Dv = _check_cache(kcache, vcache)
+    T, G, tok, head = _check_rows(q, heads, D)
+    n, per = _check_step(block_table, kv_lens, cu_q, max_q_len, T)
+    kind, columns, width, keys = q.dtype, G * heads * Dv, 0, per * bs
+    _require(kind == kcache.dtype, "queries and cache have one type")
+    w_seq = w_head = 0
+    if weights is not None:
+        _check_entries(weights, torch.float32, n, heads, keys, "weights")
+        w_seq, w_head, _ = weights.stride()
+    else:
+        listed = pages.shape
+        _require(len(listed) == 3 and pages.dtype == counts.dtype == torch.int32 and listed[:2] == (T, heads) == counts.shape and listed[2] >= 1 and pages.is_contiguous()
+                 and counts.is_contiguous(), "the selection is int32 [T, kv heads, N >= 1] and [T, kv heads], contiguous")
+        width = listed[2]
+        keys = min(width, per) * bs
     if out is None:
-        out = torch.empty((T, Hq * Dv), dtype=q.dtype, device=q.device)
-    _require(out.shape == (T, Hq * Dv) and out.dtype == q.dtype and out.stride(1) == 1, "out is [T, heads * value width] in the type of q, unit inner stride")
+        out = torch.empty((T, columns), dtype=kind, device=q.device)
+        out_stride = columns
+    else:
+        _require(out.shape == (T, columns) and out.dtype == kind and out.stride(1) == 1, "out is [T, heads * value width] in the type of q, unit inner stride")
+        out_stride = out.stride(0)
     splits = budget_splits(T * heads, keys) if num_splits is None else num_splits
     _require(1 <= splits <= MAX_SPLITS, "1 to 64 splits")
-    lib, capacity = kernels(), block_table.shape[1] * bs
-    nbytes = lib.swb_attn_budget_workspace(T, heads, G, Dv, splits, capacity, weights is not None)
+    lib = kernels()
+    nbytes = lib.swb_attn_budget_workspace(T, heads, G, Dv, splits, per * bs, weights is not None) if splits > 1 or weights is not None else 0
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None     # the call's own: two streams or graphs share none
-    width = selection.pages.shape[2] if selection is not None else 0
-    dims = (ctypes.c_int * 16)(T, n, max_q_len, block_table.shape[1], blocks, bs, heads, G, D, Dv, width, splits, q.dtype == torch.float32, 0, 0, 0)
-    w_seq, w_head = (weights.stride(0), weights.stride(1)) if weights is not None else (0, 0)
-    strides = (ctypes.c_longlong * 8)(q.stride(0), q.stride(1), out.stride(0), block_table.stride(0), w_seq, w_head, 0, 0)
+    dims = _INTS[16](T, n, max_q_len, per, blocks, bs, heads, G, D, Dv, width, splits, kind == torch.float32, 0, 0, 0)
+    strides = _LONGS[8](tok, head, out_stride, block_table.stride(0), w_seq, w_head, 0, 0)
     check(lib.swb_attn_budget(dims, strides, q.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), block_table.data_ptr(), ptr(cu_q), kv_lens.data_ptr(),
-                              ptr(selection.pages) if selection is not None else None, ptr(selection.counts) if selection is not None else None, ptr(weights), scale,
-                              softcap, ptr(ws), nbytes, stream_ptr()), "swb_attn_budget")
+                              ptr(pages), ptr(counts), ptr(weights), scale, softcap, ptr(ws), nbytes, stream_ptr()), "swb_attn_budget")
     return out
 
 
@@ -169,13 +199,7 @@ def selected_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tens
 
     q [T, Hq, D] and the caches of one type. softcap > 0: scores s become softcap tanh(s / softcap). Lists may come from elsewhere than `select_pages`: in any order; pages that
     a token does not see, or that are not in the table, add nothing; a page listed twice counts twice. A token without keys gets zeros."""
-    pages, counts = selection.pages, selection.counts
-    require_cuda(pages, counts)
-    _require(pages.dtype == counts.dtype == torch.int32 and pages.dim() == 3 and pages.shape[:2] == (q.shape[0], kcache.shape[1]) and counts.shape == pages.shape[:2]
-             and pages.shape[2] >= 1 and pages.is_contiguous() and counts.is_contiguous() and pages.device == counts.device == q.device,
-             "the selection is int32 [T, kv heads, N >= 1] and [T, kv heads], contiguous, beside q")
-    return _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, softcap, num_splits, out, min(pages.shape[2], block_table.shape[1]) * kcache.shape[2],
-                      selection=selection)
+    return _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, softcap, num_splits, out, selection.pages, selection.counts, None)
 
 
 def tracked_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, weights: torch.Tensor, *,
@@ -186,13 +210,20 @@ def tracked_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tenso
 
     For decode steps, and for the last tokens of a prompt. Each token reads its keys on its own, and scores are kept until the sums are
     known: 4 bytes a token, query head and key of the table's width."""
-    _require(weights.dim() == 3 and weights.dtype == torch.float32 and weights.stride(2) == 1 and weights.shape[:2] == (kv_lens.shape[0], kcache.shape[1])
-             and weights.shape[2] >= block_table.shape[1] * kcache.shape[2] and not _overlaps(weights), "weights are fp32 [num_seqs, kv heads, an entry for each the table has room for]")
-    return _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, softcap, num_splits, out, block_table.shape[1] * kcache.shape[2], weights=weights)
+    return _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, softcap, num_splits, out, None, None, weights)
+
+
+def _check_entries(x: torch.Tensor, kind: torch.dtype, num_seqs: int, heads: int, entries: int, name: str) -> None:
+    """x [num_seqs, heads, N] is written per (sequence, head): rows may be strided, but must not share memory (expanded or overlapping views)."""
+    _require(x.dim() == 3 and x.dtype == kind, f"{name} are {kind} [num_seqs, kv heads, N]")
+    (a, b, n), (sa, sb, inner) = x.shape, x.stride()
+    _require(inner == 1 and a == num_seqs and b == heads and n >= entries, f"{name} have an entry for each that the block table has room for, unit inner stride")
+    if sb * b > sa or sb < n:
+        _require(not _overlaps(x), f"rows of {name} share memory")
 
 
 def _overlaps(x: torch.Tensor) -> bool:
-    """Whether two rows of x [A, B, N] share memory (expanded or overlapping views), which calls that write them refuse."""
+    """Whether two rows of x [A, B, N] share memory."""
     (a, sa), (b, sb) = sorted(((x.shape[i], x.stride(i)) for i in (0, 1)), key=lambda e: e[1])
     return (a > 1 and sa < x.shape[2]) or (b > 1 and sb < (a - 1) * sa + x.shape[2])
 
@@ -207,20 +238,18 @@ def evict_tokens(kcache: torch.Tensor, vcache: torch.Tensor, block_table: torch.
     entries without a record, which stand in order in front of the next position (all of them before the first call); the call records those it keeps. Weights behind `keep` become 0, positions -1.
     Everything is done in place. Pages must not be shared with a sequence that is not to lose tokens, nor between sequences of the call (`PagedSequence.unshare`)."""
     _place(kcache, vcache, block_table, kv_lens, weights, positions, next_positions)
-    _check_cache(kcache, vcache)
-    n = _check_step(block_table, kv_lens, None, 1, None)
-    blocks, heads, bs, D = kcache.shape
-    for name, t, kind in (("weights", weights, torch.float32), ("positions", positions, torch.int32)):
-        _require(t.dim() == 3 and t.dtype == kind and t.stride(2) == 1 and t.shape[:2] == (n, heads) and t.shape[2] >= block_table.shape[1] * bs and not _overlaps(t),
-                 f"{name} are {kind} [num_seqs, kv heads, an entry for each the table has room for]")
+    blocks, heads, bs, D, Dv = _check_cache(kcache, vcache)
+    n, per = _check_step(block_table, kv_lens, None, 1, -1)
+    capacity, size = per * bs, 4 if kcache.dtype == torch.float32 else 2
+    _check_entries(weights, torch.float32, n, heads, capacity, "weights")
+    _check_entries(positions, torch.int32, n, heads, capacity, "positions")
     _require(next_positions.dtype == torch.int32 and next_positions.shape == (n,) and next_positions.is_contiguous(), "next_positions are int32 [num_seqs]")
-    _require(keep >= 1 and recent >= 0 and first >= 0 and recent + first <= keep, "0 <= first, recent; first + recent <= keep")
-    capacity, size = block_table.shape[1] * bs, kcache.element_size()
-    lib = kernels()
-    moves = torch.empty(lib.swb_evict_moves(n, heads, capacity, keep), dtype=torch.int32, device=kcache.device)
-    lens = torch.empty(n, dtype=torch.int32, device=kcache.device)
-    dims = (ctypes.c_int * 12)(n, heads, block_table.shape[1], blocks, bs, D * size, vcache.shape[3] * size, capacity, keep, recent, first, 0)
-    strides = (ctypes.c_longlong * 4)(weights.stride(0), weights.stride(1), positions.stride(0), positions.stride(1))
+    _require(keep >= 1 and recent >= 0 and first >= 0 and recent + first <= keep, "0 <= first, recent; 1 <= keep; first + recent <= keep")
+    lib, device = kernels(), kcache.device
+    moves = torch.empty(lib.swb_evict_moves(n, heads, capacity, keep), dtype=torch.int32, device=device)
+    lens = torch.empty(n, dtype=torch.int32, device=device)
+    dims = _INTS[11](n, heads, per, blocks, bs, D * size, Dv * size, capacity, keep, recent, first)
+    strides = _LONGS[4](*weights.stride()[:2], *positions.stride()[:2])
     check(lib.swb_evict(dims, strides, kcache.data_ptr(), vcache.data_ptr(), block_table.data_ptr(), block_table.stride(0), kv_lens.data_ptr(), lens.data_ptr(),
                         next_positions.data_ptr(), weights.data_ptr(), positions.data_ptr(), moves.data_ptr(), stream_ptr()), "swb_evict")
     return lens

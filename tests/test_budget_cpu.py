@@ -113,5 +113,5 @@ def test_rows_that_share_memory():
 
 
 def test_splits():
-    assert budget.budget_splits(8, 100000) == 37 and budget.budget_splits(8, 64) == 1 and budget.budget_splits(8, 65) == 2
-    assert budget.budget_splits(1, 10 ** 6) == 64 and budget.budget_splits(400, 10 ** 6) == 1 and budget.budget_splits(0, 0) == 1
+    assert budget.budget_splits(8, 100000) == 37 and budget.budget_splits(8, 64) == 1 and budget.budget_splits(8, 65) == 2 and budget.budget_splits(8, 8000) == 8
+    assert budget.budget_splits(1, 10 ** 6) == 64 and budget.budget_splits(400, 10 ** 6) == 2 and budget.budget_splits(0, 0) == 1 and budget.budget_splits(10 ** 6, 10 ** 6) == 1
