@@ -187,12 +187,16 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_budget_plain_kernel(const 
 // warp waits for another before the end. Group i of a block goes to warp i % 4. With queries as rows of 16, S = Q K^T leaves the weights of a head and pairs of
 // neighbouring keys in a thread, which is what the second operand of O^T = V^T P^T wants: nothing is moved in between, and heads
 // are the 8 columns of that product, so a group of up to 8 query heads wastes none of it.
-constexpr int FW = 4, FS = 3;                       // warps; groups in a warp's ring
+// What a block costs before its first group and behind its last (some 5 us: look-ups that wait for one another, the joining of its warps) is hidden by the other
+// blocks of its SM. Rings of three groups leave room for two blocks, rings of two for three; the bytes on their way are the same. Two groups where blocks are many and
+// short (500 tokens with 4 key/value heads and 64 pages each: 165 us with two blocks, 126 with three), three where they are few (512 blocks
+// of 128 pages: 94 us with two blocks, 111 with three, of which the last 68 blocks run alone).
+constexpr int FW = 4;                               // warps
 constexpr int HALF_BYTES = 2048, GROUP_BYTES = 4 * HALF_BYTES;      // 16 rows of 64 columns; K low, K high, V low, V high
 constexpr int SQ_BYTES = ROWS * 256, LDO = 132;
-constexpr int FAST_SMEM = 1024 + FW * FS * GROUP_BYTES + SQ_BYTES + 256;
+constexpr int fast_smem_bytes(int FS) { return 1024 + FW * FS * GROUP_BYTES + SQ_BYTES + 256; }
 constexpr int FINISH_FLOATS = FW * ROWS * LDO + FW * ROWS * 2 + ROWS * 2 + ROWS * 2 + ROWS * MAX_CLUSTER;
-static_assert(FINISH_FLOATS * 4 <= FW * FS * GROUP_BYTES, "the warps' results fit where the ring was");
+static_assert(FINISH_FLOATS * 4 <= FW * 2 * GROUP_BYTES, "the warps' results fit where the ring was");
 
 // 16-byte chunk c (0..15) of row r (0..15) of a K or V group: two boxes of 64 columns with the 128-byte swizzle
 __device__ __forceinline__ uint32_t group_off(int r, int c) { return (uint32_t)(((c >> 3) << 11) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
@@ -223,8 +227,8 @@ __device__ __forceinline__ float ld_cluster(uint32_t at) {
   return x;
 }
 
-template <int NT>         // eights of rows: 1 or 2
-__global__ void __launch_bounds__(FW * 32, 2) attn_budget_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const BudgetParams p) {
+template <int NT, int FS>         // eights of rows: 1 or 2; groups in a warp's ring: 3, or 2
+__global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budget_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const BudgetParams p) {
   pdl_launch_dependents();
   extern __shared__ uint8_t fast_smem[];
   uint8_t* smem = fast_smem + ((1024u - (smem_u32(fast_smem) & 1023u)) & 1023u);
@@ -562,20 +566,22 @@ int launch_fast(BudgetParams p, cudaStream_t s) {
   rc = make_tmap_bf16_2d(&tv, p.v, rows, p.Dv, p.Dv, 16);
   if (rc) return rc;
   const bool one = p.G * p.run <= 8;
-  auto kernel = one ? attn_budget_kernel<1> : attn_budget_kernel<2>;
-  static bool configured[2][64] = {};
+  const int problems = (p.run > 1 ? p.num_seqs * ((p.uniform_q + p.run - 1) / p.run) : p.tokens) * p.Hkv * p.head_tiles;
+  const bool many = one && (long long)problems * p.num_splits >= 9 * 148;
+  auto kernel = many ? attn_budget_kernel<1, 2> : one ? attn_budget_kernel<1, 3> : attn_budget_kernel<2, 3>;
+  const int smem = fast_smem_bytes(many ? 2 : 3), which = many ? 2 : one;
+  static bool configured[3][64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !configured[one][dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FAST_SMEM);
+  if (dev < 0 || dev >= 64 || !configured[which][dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return -(int)e;
-    if (dev >= 0 && dev < 64) configured[one][dev] = true;
+    if (dev >= 0 && dev < 64) configured[which][dev] = true;
   }
-  const int problems = (p.run > 1 ? p.num_seqs * ((p.uniform_q + p.run - 1) / p.run) : p.tokens) * p.Hkv * p.head_tiles;
   const dim3 grid(p.num_splits * problems), block(FW * 32);
-  if (!p.cluster) return launch_kernel(kernel, grid, block, FAST_SMEM, s, tk, tv, p);
+  if (!p.cluster) return launch_kernel(kernel, grid, block, smem, s, tk, tv, p);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = FAST_SMEM, cfg.stream = s;
+  cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = p.num_splits, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
@@ -587,7 +593,7 @@ int launch_fast(BudgetParams p, cudaStream_t s) {
 }
 
 // ---- joining ------------------------------------------------------------------------------------------------------------------------------------------
-constexpr int JOIN_THREADS = 128, WEIGH_KEYS = 4 * JOIN_THREADS;
+constexpr int JOIN_THREADS = 128;
 static_assert(MAX_GROUP <= JOIN_THREADS, "a block weighs a row to a thread");
 
 // {maximum, sum} of a row in each of its splits -> factors of the splits' values, exp2(max - common) / sum; by one warp.
@@ -606,8 +612,9 @@ __device__ __forceinline__ void split_factors(const float* ml, int S, int lane, 
   if (lane + 32 < S) factor[lane + 32] = e1 * inv;
 }
 
-// The first `join_blocks` blocks join the parts of one row each; the others weigh a run of keys of one (sequence, key/value head) each.
-template <typename E>
+// The first `join_blocks` blocks join the parts of one row each; the others weigh a run of keys of one (sequence, key/value head) each. KEYS of a thread: four for steps
+// of one token, whose few rows leave room for no more loads otherwise, one for several tokens, whose rows are many and blocks few.
+template <typename E, int KEYS>
 __global__ void __launch_bounds__(JOIN_THREADS) attn_budget_finish_kernel(const BudgetParams p, int join_blocks) {
   pdl_launch_dependents();
   __shared__ float s_factor[MAX_SPLITS], s_all[MAX_GROUP * 2];
@@ -627,13 +634,16 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_budget_finish_kernel(const 
     }
     return;
   }
-  const int blocks = (int)((p.capacity + WEIGH_KEYS - 1) / WEIGH_KEYS), i = blockIdx.x - join_blocks;
+  constexpr int RUN = KEYS * JOIN_THREADS;
+  const int blocks = (int)((p.capacity + RUN - 1) / RUN), i = blockIdx.x - join_blocks;
   const int h = i / blocks % p.Hkv, seq = i / blocks / p.Hkv;
-  const long long j0 = (long long)(i % blocks) * WEIGH_KEYS + tid;
+  const long long j0 = (long long)(i % blocks) * RUN + tid;
   const int q0 = p.cu_q ? p.cu_q[seq] : seq * p.uniform_q, q1 = min(p.cu_q ? p.cu_q[seq + 1] : q0 + p.uniform_q, p.tokens);
   const int total = p.kv_lens[seq], len = min(total, p.max_blocks * p.bs);
   if (j0 - tid >= len) return;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  float sum[KEYS];
+#pragma unroll
+  for (int k = 0; k < KEYS; ++k) sum[k] = 0.f;
   const int batch = MAX_GROUP / p.G;             // tokens whose rows a block has room for
   for (int t0 = q0; t0 < q1; t0 += batch) {
     const int pairs = min(batch, q1 - t0) * p.G;
@@ -653,13 +663,13 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_budget_finish_kernel(const 
     }
     __syncthreads();
     const float* s = p.scores + ((size_t)t0 * Hq + h * p.G) * p.capacity + j0;
-#pragma unroll 4
+#pragma unroll (KEYS == 1 ? 16 : 4)
     for (int i = 0; i < pairs; ++i) {
       const int tok = i / p.G, seen = min(total - (q1 - 1 - t0 - tok), len);
       const float m = s_all[i * 2], inv = s_all[i * 2 + 1];
       const float* row = s + ((size_t)tok * Hq + i % p.G) * p.capacity;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < KEYS; ++k) {
         const float x = j0 + k * JOIN_THREADS < seen ? __ldcg(row + k * JOIN_THREADS) : -INFINITY;
         sum[k] = fmaf(exp2f(x - m), x == -INFINITY ? 0.f : inv, sum[k]);       // (a row without a sum adds nothing to keys it does not see)
       }
@@ -667,7 +677,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_budget_finish_kernel(const 
   }
   float* w = p.weights + seq * p.w_seq + h * p.w_head;
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
+  for (int k = 0; k < KEYS; ++k)
     if (j0 + k * JOIN_THREADS < len) w[j0 + k * JOIN_THREADS] += sum[k];
 }
 
@@ -722,7 +732,7 @@ int swb_attn_budget(const int* dims, const long long* strides, const void* q, vo
   while (fast && !pages && p.run * 2 * p.G <= ROWS && p.run < p.uniform_q) p.run *= 2;
   const long long problems = (p.run > 1 ? (long long)p.num_seqs * ((p.uniform_q + p.run - 1) / p.run) : p.tokens) * p.Hkv * p.head_tiles;
   // Blocks of a cluster start together and wait for one another, which costs nothing while all of them fit the chip at once; behind that a second launch is cheaper
-  // (48 sequences of up to 8191 keys, 8 key/value heads, 4 splits: 305 us as clusters, 2xx with a second launch)
+  // (48 sequences of up to 8191 keys, 8 key/value heads, 4 splits: 305 us as clusters, 233 with a second launch)
   p.cluster = fast && p.num_splits > 1 && p.num_splits <= MAX_CLUSTER && problems * p.num_splits <= 2 * 148;
   p.weigh_here = weights && fast && p.uniform_q == 1 && p.head_tiles == 1 && (p.cluster || p.num_splits == 1);
   const bool join = p.num_splits > 1 && !p.cluster, weigh = weights && !p.weigh_here;
@@ -738,11 +748,12 @@ int swb_attn_budget(const int* dims, const long long* strides, const void* q, vo
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int rc = fast ? launch_fast(p, s) : fp32 ? launch_plain<float>(p, s) : launch_plain<bf16>(p, s);
   if (rc || !(join || weigh)) return rc;
-  const int join_blocks = join ? p.tokens * p.Hkv * p.G : 0;
-  const long long blocks = join_blocks + (weigh ? (p.capacity + WEIGH_KEYS - 1) / WEIGH_KEYS * p.Hkv * p.num_seqs : 0);
+  const int join_blocks = join ? p.tokens * p.Hkv * p.G : 0, run = JOIN_THREADS * (p.uniform_q == 1 ? 4 : 1);
+  const long long blocks = join_blocks + (weigh ? (p.capacity + run - 1) / run * p.Hkv * p.num_seqs : 0);
   if (blocks > INT_MAX) return -3;
-  return fp32 ? launch_kernel(attn_budget_finish_kernel<float>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, s, p, join_blocks)
-              : launch_kernel(attn_budget_finish_kernel<bf16>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, s, p, join_blocks);
+  auto kernel = fp32 ? (p.uniform_q == 1 ? attn_budget_finish_kernel<float, 4> : attn_budget_finish_kernel<float, 1>)
+                     : (p.uniform_q == 1 ? attn_budget_finish_kernel<bf16, 4> : attn_budget_finish_kernel<bf16, 1>);
+  return launch_kernel(kernel, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, s, p, join_blocks);
 }
 
 }  // extern "C"

@@ -147,14 +147,16 @@ def select_pages(q: torch.Tensor, summaries: PageSummaries, block_table: torch.T
     return PageSelection(pages, counts)
 
 
-def budget_splits(problems: int, keys: int, sms: int = 148) -> int:
-    """Blocks that share a problem's keys (problems: tokens * kv heads). Two blocks fit an SM: enough of them for four rounds of all SMs, so that sequences of different
-    lengths even out, none of less than 64 keys. Up to 8 join within one launch; more take a second one, which pays where 8 would leave SMs idle over long caches."""
-    most = (keys + 63) // 64
-    splits = min(8, most, max(1, 8 * sms // max(1, problems)))
-    if problems * 8 < sms and keys >= 8192:
-        splits = min(MAX_SPLITS, most, 2 * sms // max(1, problems))
-    return max(1, splits)
+def budget_splits(problems: int, keys: int, even: bool, sms: int = 148) -> int:
+    """Blocks that share a problem's keys (problems: tokens, or runs of a few of them, * kv heads; even: all have about as many keys). An SM holds two blocks or three.
+
+    Fewer problems than fit at once: as many splits as fit, up to 8, which join within the launch; more, joined by a second one, where 8 would leave SMs idle over
+    long caches. More problems: one block each, or where their lengths differ enough blocks of 512 keys and more to even out over seven rounds of the SMs."""
+    slots, problems = 2 * sms, max(1, problems)
+    fit = slots // problems
+    if not even and problems * keys >= slots * 4096:
+        return max(1, min(MAX_SPLITS, keys // 512, 21 * sms // problems))
+    return max(1, min((keys + 63) // 64, MAX_SPLITS if fit > 8 and problems * 8 < sms and keys >= 8192 else 8, fit))
 
 
 def _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, softcap, num_splits, out, pages, counts, weights) -> torch.Tensor:
@@ -180,7 +182,13 @@ def _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, 
     else:
         _require(out.shape == (T, columns) and out.dtype == kind and out.stride(1) == 1, "out is [T, heads * value width] in the type of q, unit inner stride")
         out_stride = out.stride(0)
-    splits = budget_splits(T * heads, keys) if num_splits is None else num_splits
+    if num_splits is None:
+        run = 1                                       # tokens of a sequence that share a problem
+        while weights is not None and run < max_q_len and run * 2 * G <= 16:
+            run *= 2
+        splits = budget_splits((T if run == 1 else n * -(-max_q_len // run)) * heads, keys, weights is None)
+    else:
+        splits = num_splits
     _require(1 <= splits <= MAX_SPLITS, "1 to 64 splits")
     lib = kernels()
     nbytes = lib.swb_attn_budget_workspace(T, heads, G, Dv, splits, per * bs, weights is not None) if splits > 1 or weights is not None else 0
