@@ -618,6 +618,8 @@ template <typename E, int KEYS>
 __global__ void __launch_bounds__(JOIN_THREADS) attn_budget_finish_kernel(const BudgetParams p, int join_blocks) {
   pdl_launch_dependents();
   __shared__ float s_factor[MAX_SPLITS], s_all[MAX_GROUP * 2];
+  __shared__ size_t s_row[MAX_GROUP];
+  __shared__ int s_seen[MAX_GROUP];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, S = p.num_splits, Hq = p.Hkv * p.G;
   pdl_wait();
   if ((int)blockIdx.x < join_blocks) {
@@ -641,44 +643,55 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_budget_finish_kernel(const 
   const int q0 = p.cu_q ? p.cu_q[seq] : seq * p.uniform_q, q1 = min(p.cu_q ? p.cu_q[seq + 1] : q0 + p.uniform_q, p.tokens);
   const int total = p.kv_lens[seq], len = min(total, p.max_blocks * p.bs);
   if (j0 - tid >= len) return;
-  float sum[KEYS];
+  float* w = p.weights + seq * p.w_seq + h * p.w_head;
+  float sum[KEYS], old[KEYS];
 #pragma unroll
-  for (int k = 0; k < KEYS; ++k) sum[k] = 0.f;
+  for (int k = 0; k < KEYS; ++k) sum[k] = 0.f, old[k] = j0 + k * JOIN_THREADS < len ? w[j0 + k * JOIN_THREADS] : 0.f;
   const int batch = MAX_GROUP / p.G;             // tokens whose rows a block has room for
   for (int t0 = q0; t0 < q1; t0 += batch) {
     const int pairs = min(batch, q1 - t0) * p.G;
     __syncthreads();
-    if (tid < pairs) {                           // MAX_GROUP = JOIN_THREADS: a row to a thread
-      const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + part_at(p, t0 + tid / p.G, h * p.G + tid % p.G, 0);
+    if (tid < pairs) {                           // MAX_GROUP <= JOIN_THREADS: a row to a thread
+      const int tok = tid / p.G;
+      const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + part_at(p, t0 + tok, h * p.G + tid % p.G, 0);
       float M = -INFINITY, L = 0.f;
-#pragma unroll 8
-      for (int s = 0; s < S; ++s) M = fmaxf(M, __ldcg(ml + s).x);
-      const float base = M == -INFINITY ? 0.f : M;
-#pragma unroll 8
-      for (int s = 0; s < S; ++s) {
-        const float2 x = __ldcg(ml + s);
-        L = fmaf(exp2f(x.x - base), x.y, L);
+      for (int s0 = 0; s0 < S; s0 += 8) {
+        float2 x[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) x[s] = s0 + s < S ? __ldcg(ml + s0 + s) : make_float2(-INFINITY, 0.f);
+        float top = M;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) top = fmaxf(top, x[s].x);
+        const float base = top == -INFINITY ? 0.f : top;
+        L *= exp2f(M - base);
+#pragma unroll
+        for (int s = 0; s < 8; ++s) L = fmaf(exp2f(x[s].x - base), x[s].y, L);
+        M = top;
       }
-      s_all[tid * 2] = base, s_all[tid * 2 + 1] = L == 0.f ? 0.f : 1.f / L;
+      s_all[tid * 2] = M == -INFINITY ? 0.f : M, s_all[tid * 2 + 1] = L == 0.f ? 0.f : 1.f / L;
+      s_row[tid] = ((size_t)(t0 + tok) * Hq + h * p.G + tid % p.G) * p.capacity;
+      s_seen[tid] = min(total - (q1 - 1 - t0 - tok), len);
     }
     __syncthreads();
-    const float* s = p.scores + ((size_t)t0 * Hq + h * p.G) * p.capacity + j0;
-#pragma unroll (KEYS == 1 ? 16 : 4)
-    for (int i = 0; i < pairs; ++i) {
-      const int tok = i / p.G, seen = min(total - (q1 - 1 - t0 - tok), len);
-      const float m = s_all[i * 2], inv = s_all[i * 2 + 1];
-      const float* row = s + ((size_t)tok * Hq + i % p.G) * p.capacity;
+    constexpr int U = 16 / KEYS;                 // rows whose scores are on their way together
+    for (int r0 = 0; r0 < pairs; r0 += U) {
+      float x[U][KEYS];
 #pragma unroll
-      for (int k = 0; k < KEYS; ++k) {
-        const float x = j0 + k * JOIN_THREADS < seen ? __ldcg(row + k * JOIN_THREADS) : -INFINITY;
-        sum[k] = fmaf(exp2f(x - m), x == -INFINITY ? 0.f : inv, sum[k]);       // (a row without a sum adds nothing to keys it does not see)
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < KEYS; ++k) x[u][k] = r0 + u < pairs && j0 + k * JOIN_THREADS < s_seen[min(r0 + u, MAX_GROUP - 1)] ? __ldcg(p.scores + s_row[r0 + u] + j0 + k * JOIN_THREADS) : -INFINITY;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float m = s_all[min(r0 + u, MAX_GROUP - 1) * 2], inv = s_all[min(r0 + u, MAX_GROUP - 1) * 2 + 1];
+#pragma unroll
+        for (int k = 0; k < KEYS; ++k)
+          if (x[u][k] != -INFINITY) sum[k] = fmaf(exp2f(x[u][k] - m), inv, sum[k]);        // keys that a row does not see get nothing of it, whatever its sum is
       }
     }
   }
-  float* w = p.weights + seq * p.w_seq + h * p.w_head;
 #pragma unroll
   for (int k = 0; k < KEYS; ++k)
-    if (j0 + k * JOIN_THREADS < len) w[j0 + k * JOIN_THREADS] += sum[k];
+    if (j0 + k * JOIN_THREADS < len) w[j0 + k * JOIN_THREADS] = old[k] + sum[k];
 }
 
 template <typename E>
