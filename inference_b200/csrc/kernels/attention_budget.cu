@@ -213,6 +213,7 @@ __device__ __forceinline__ void zero_values(uint8_t* group, int live, int halves
 }
 
 __device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

@@ -7,6 +7,8 @@
 #include "common.cuh"
 #include "radix_select.cuh"
 
+#include <climits>
+
 namespace swb {
 namespace {
 
@@ -26,109 +28,210 @@ struct EvictParams {
   long long p_seq, p_head;
   int capacity;              // entries of a row of weights and positions
   int keep, recent, first;
-  int* moves;                // per (sequence, head): count, then holes [max_moves], then sources [max_moves]
+  int* moves;                // per (sequence, head): holes [max_moves], then sources [max_moves]
   int max_moves;
 };
 
-constexpr int EVICT_THREADS = 512;
-constexpr int EVICT_CACHED = 40960;            // keys held in shared memory; longer rows are read again in every pass
+constexpr int EVICT_THREADS = 512, EVICT_WARPS = EVICT_THREADS / 32, EVICT_CLUSTER = 8;
+constexpr int EVICT_CACHED = 16384;            // keys that a block holds in shared memory; with more it computes them again in every pass
 
 __device__ __forceinline__ int entry_position(const int* pos, int i, int len, int next) {
   const int x = pos[i];
   return x >= 0 ? x : next - (len - i);
 }
 
-__global__ void __launch_bounds__(EVICT_THREADS, 2) evict_plan_kernel(const EvictParams p) {
+// Shared memory of the cluster's first block, or of another one.
+__device__ __forceinline__ uint32_t in_block(const void* at, int rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(at)), "r"(rank));
+  return remote;
+}
+__device__ __forceinline__ int load_from(const int* at, int rank) {
+  int x;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(x) : "r"(in_block(at, rank)) : "memory");
+  return x;
+}
+__device__ __forceinline__ void store_to(const void* at, int rank, uint32_t x) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(in_block(at, rank)), "r"(x) : "memory");
+}
+__device__ __forceinline__ int add_to(const int* at, int rank, int x) {
+  int old;
+  asm volatile("atom.shared::cluster.add.s32 %0, [%1], %2;" : "=r"(old) : "r"(in_block(at, rank)), "r"(x) : "memory");
+  return old;
+}
+
+// `blocks` blocks, a cluster, share a (sequence, head): each has an equal run of the entries in front of `keep` and one of those behind. The first one's histogram
+// gathers the others', and it finds the threshold for all; what is kept in front of a run follows from the keys above and equal to the threshold
+// there, so every block knows the places of its holes (not kept, in front of `keep`) and sources (kept, behind it) in the list of moves. The moves are
+// then shared out evenly. Counts are whole numbers: nothing depends on the order of the atomics.
+template <typename W>
+__global__ void __launch_bounds__(EVICT_THREADS, 2) evict_kernel(const EvictParams p, int blocks) {
   pdl_launch_dependents();
   extern __shared__ uint32_t evict_keys[];
   __shared__ __align__(16) int hist[SELECT_INTS];
+  __shared__ int s_count[4];                   // keys above and equal to the threshold, in front of and behind `keep`
   const Team<EVICT_THREADS> team(threadIdx.x);
-  const int h = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = blockIdx.x % blocks, h = blockIdx.x / blocks, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t below = (1u << lane) - 1u;
+  int* totals = hist + SELECT_BINS;
+  const auto meet = [&]() {
+    if (blocks > 1) {
+      __syncwarp();
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+      __syncthreads();
+    }
+  };
+  clear_bins(team, hist);
   pdl_wait();
   const int len = min(p.kv_lens[seq], min(p.max_blocks * p.bs, p.capacity)), keep = p.keep;
-  int* moves = p.moves + ((size_t)seq * p.Hkv + h) * (1 + 2 * (size_t)p.max_moves);
-  if (h == 0 && tid == 0) p.new_lens[seq] = min(p.kv_lens[seq], keep);
-  if (len <= keep) {
-    if (tid == 0) moves[0] = 0;
-    return;
-  }
+  if (h == 0 && rank == 0 && tid == 0) p.new_lens[seq] = min(p.kv_lens[seq], keep);
+  if (len <= keep) return;                     // the whole cluster
+  int* moves = p.moves + ((size_t)seq * p.Hkv + h) * 2 * (size_t)p.max_moves;      // holes, then sources
   float* w = p.weights + seq * p.w_seq + h * p.w_head;
   int* pos = p.positions + seq * p.p_seq + h * p.p_head;
   const int next = p.next[seq];
+  const auto cut = [&](int n, int r) { return (int)((long long)n * r / blocks); };
+  const int a0 = cut(keep, rank), na = cut(keep, rank + 1) - a0, b0 = keep + cut(len - keep, rank), nb = keep + cut(len - keep, rank + 1) - b0;
+  const auto entry = [&](int i) { return i < na ? a0 + i : b0 + i - na; };          // of this block's i-th key
   const auto fresh_key = [&](int i) -> uint32_t {
-    const int at = entry_position(pos, i, len, next);
-    return at < p.first || at >= next - p.recent ? 0xffffffffu : float_key(w[i]);
+    const int e = entry(i), at = entry_position(pos, e, len, next);
+    return at < p.first || at >= next - p.recent ? 0xffffffffu : float_key(w[e]);
   };
-  const bool cached = len <= EVICT_CACHED;
-  clear_bins(team, hist);
-  __syncthreads();
-  for (int i = tid; i < len; i += EVICT_THREADS) {
-    const uint32_t k = fresh_key(i);
-    if (cached) evict_keys[i] = k;
-    count_key(hist, k);
-  }
+  const bool cached = na + nb <= EVICT_CACHED;
   const auto key = [&](int i) -> uint32_t { return cached ? evict_keys[i] : fresh_key(i); };
-  __syncthreads();
-  const Threshold th = select_threshold(team, key, len, keep, hist);
-  // Every warp has a run of the entries in front of `keep` and one of those behind. What is kept in front of a run follows from the keys above and equal
-  // to the threshold there, and holes are what is not kept in front of `keep`, sources what is kept behind.
+  // histograms of `digit` of the keys that agree with prefix under mask, gathered in the first block; bin and rest in its totals
+  const auto find = [&](uint32_t prefix, uint32_t mask, int shift, uint32_t digit, int want) {
+#pragma unroll 4
+    for (int i = tid; i < na + nb; i += EVICT_THREADS) {
+      const uint32_t k = mask ? key(i) : fresh_key(i);
+      if (!mask && cached) evict_keys[i] = k;
+      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digit], 1);
+    }
+    __syncthreads();
+    if (rank > 0)
+      for (int i = tid; i < SELECT_BINS; i += EVICT_THREADS)
+        if (hist[i]) add_to(&hist[i], 0, hist[i]);
+    meet();
+    if (rank == 0) find_bin(team, hist, want, totals);
+    meet();
+  };
+  meet();                                      // all blocks run and their bins are clear
+  find(0u, 0u, 21, 0x7ffu, keep);
+  uint32_t prefix = (uint32_t)load_from(&totals[32], 0), mask = 0x7ffu;
+  int want = load_from(&totals[33], 0);
+  const int m = load_from(&totals[34], 0);
+  Threshold th;
+  if (m <= EVICT_THREADS) {                    // few enough to be ranked by one block
+    uint32_t* list = reinterpret_cast<uint32_t*>(hist);
+    meet();                                    // everybody has read the totals, and find_bin the bins
+#pragma unroll 4
+    for (int i = tid; i < na + nb; i += EVICT_THREADS) {
+      const uint32_t k = key(i);
+      if ((k >> 21) == prefix) store_to(&list[add_to(&totals[35], 0, 1)], 0, k);
+    }
+    meet();
+    if (rank == 0 && tid < m) {
+      const uint32_t mine = list[tid];
+      int above = 0, same = 0;
+      for (int j = 0; j < m; ++j) above += list[j] > mine, same += list[j] == mine;
+      if (above < want && want <= above + same) totals[37] = (int)mine, totals[38] = want - above;
+    }
+    meet();
+    th = Threshold{(uint32_t)load_from(&totals[37], 0), load_from(&totals[38], 0)};
+  } else {
+    prefix <<= 21, mask <<= 21;
+#pragma unroll 1
+    for (int round = 0; round < 2; ++round) {
+      const int shift = round == 0 ? 10 : 0;
+      const uint32_t digit = round == 0 ? 0x7ffu : 0x3ffu;
+      meet();                                  // everybody has read the totals
+      clear_bins(team, hist);
+      meet();
+      find(prefix, mask, shift, digit, want);
+      prefix |= (uint32_t)load_from(&totals[32], 0) << shift;
+      mask |= digit << shift;
+      want = load_from(&totals[33], 0);
+    }
+    th = Threshold{prefix, want};
+  }
+  // runs of this block's warps, and what lies in front of them
   const auto run = [&](int n) { return ((n + EVICT_THREADS - 1) / EVICT_THREADS) * 32; };
-  const int lo_a = min(warp * run(keep), keep), hi_a = min(lo_a + run(keep), keep);
-  const int lo_b = min(keep + warp * run(len - keep), len), hi_b = min(lo_b + run(len - keep), len);
-  const PairSums a = sum_over_warps(team, count_run(key, th, lo_a, hi_a), reinterpret_cast<int2*>(hist));
-  const PairSums b = sum_over_warps(team, count_run(key, th, lo_b, hi_b), reinterpret_cast<int2*>(hist) + 32);
-  const int kept_a = a.all.x + min(a.all.y, th.ties), total = keep - kept_a;
-  int hole_at = lo_a - (a.before.x + min(a.before.y, th.ties));
-  for_each_choice(key, th, lo_a, hi_a, a.before.y, [&](int i, bool in, uint32_t) {
+  const int lo_a = min(warp * run(na), na), hi_a = min(lo_a + run(na), na), lo_b = na + min(warp * run(nb), nb), hi_b = min(lo_b + run(nb), na + nb);
+  meet();                                      // the totals are read: their neighbours are written again
+  int2* slots = reinterpret_cast<int2*>(hist);
+  const PairSums a = sum_over_warps(team, count_run(key, th, lo_a, hi_a), slots);
+  const PairSums b = sum_over_warps(team, count_run(key, th, lo_b, hi_b), slots + 32);
+  if (tid == 0) s_count[0] = a.all.x, s_count[1] = a.all.y, s_count[2] = b.all.x, s_count[3] = b.all.y;
+  meet();
+  int above_a = a.before.x, same_a = a.before.y, above_b = b.before.x, same_b = b.before.y, all_above = 0, all_same = 0;
+  for (int r = 0; r < blocks; ++r) {
+    const int x = load_from(&s_count[0], r), y = load_from(&s_count[1], r);
+    all_above += x, all_same += y;
+    if (r < rank) above_a += x, same_a += y, above_b += load_from(&s_count[2], r), same_b += load_from(&s_count[3], r);
+  }
+  const int kept_a = all_above + min(all_same, th.ties), total = keep - kept_a;
+  int hole_at = a0 + lo_a - (above_a + min(same_a, th.ties));
+  for_each_choice(key, th, lo_a, hi_a, same_a, [&](int i, bool in, uint32_t) {
     const bool hole = i < hi_a && !in;
     const uint32_t holes = __ballot_sync(0xffffffffu, hole);
-    if (hole) moves[1 + hole_at + __popc(holes & ((1u << lane) - 1u))] = i;
+    if (hole) moves[hole_at + __popc(holes & below)] = entry(i);
     hole_at += __popc(holes);
   });
-  int source_at = a.all.x + b.before.x + min(a.all.y + b.before.y, th.ties) - kept_a;
-  for_each_choice(key, th, lo_b, hi_b, a.all.y + b.before.y, [&](int i, bool in, uint32_t ins) {
-    if (in) moves[1 + p.max_moves + source_at + __popc(ins & ((1u << lane) - 1u))] = i;
+  int source_at = all_above + above_b + min(all_same + same_b, th.ties) - kept_a;
+  for_each_choice(key, th, lo_b, hi_b, all_same + same_b, [&](int i, bool in, uint32_t ins) {
+    if (in) moves[p.max_moves + source_at + __popc(ins & below)] = entry(i);
     source_at += __popc(ins);
   });
-  if (tid == 0) moves[0] = total;
-  __syncthreads();
-  // weights and positions: records for what stays, then the moves, then the tail is cleared
-  for (int i = tid; i < keep; i += EVICT_THREADS)
-    if (pos[i] < 0) pos[i] = next - (len - i);
-  __syncthreads();
-  for (int m = tid; m < total; m += EVICT_THREADS) {
-    const int hole = moves[1 + m], from = moves[1 + p.max_moves + m];
-    w[hole] = w[from];
-    pos[hole] = entry_position(pos, from, len, next);
-  }
-  __syncthreads();
-  for (int i = keep + tid; i < len; i += EVICT_THREADS) w[i] = 0.f;
-  for (int i = keep + tid; i < p.capacity; i += EVICT_THREADS) pos[i] = -1;
-}
+  __syncthreads();                             // no key of this block is computed any more
+  for (int i = tid; i < na; i += EVICT_THREADS)          // what stays has a record from now on
+    if (pos[a0 + i] < 0) pos[a0 + i] = next - (len - (a0 + i));
+  meet();                                      // the list is complete
 
-constexpr int MOVE_WARPS = 8;
-
-// A warp per entry: its key row, then its value row, in words of type W.
-template <typename W>
-__global__ void __launch_bounds__(MOVE_WARPS * 32) evict_move_kernel(const EvictParams p) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int h = blockIdx.y, seq = blockIdx.z, lane = threadIdx.x & 31;
-  const int* moves = p.moves + ((size_t)seq * p.Hkv + h) * (1 + 2 * (size_t)p.max_moves);
-  const int m = blockIdx.x * MOVE_WARPS + (threadIdx.x >> 5);
-  if (m >= moves[0]) return;
-  const int hole = moves[1 + m], from = moves[1 + p.max_moves + m];
+  // 32 moves to a warp: a lane looks one up, then the warp copies their rows, four at a time
   const int* table = p.table + seq * p.table_stride;
-  const int to_block = table[hole / p.bs], from_block = table[from / p.bs];
-  if ((unsigned)to_block >= (unsigned)p.num_blocks || (unsigned)from_block >= (unsigned)p.num_blocks) return;
-  const size_t to = ((size_t)to_block * p.Hkv + h) * p.bs + hole % p.bs, fr = ((size_t)from_block * p.Hkv + h) * p.bs + from % p.bs;
-  const auto copy = [&](char* base, int bytes) {
-    const W* src = reinterpret_cast<const W*>(base + fr * bytes);
-    W* dst = reinterpret_cast<W*>(base + to * bytes);
-    for (int i = lane; i < bytes / (int)sizeof(W); i += 32) dst[i] = src[i];
-  };
-  copy(p.k, p.k_bytes);
-  copy(p.v, p.v_bytes);
+  const int k_words = p.k_bytes / (int)sizeof(W), words = k_words + p.v_bytes / (int)sizeof(W);
+  W* kc = reinterpret_cast<W*>(p.k);
+  W* vc = reinterpret_cast<W*>(p.v);
+  for (int m0 = (warp * blocks + rank) * 32; m0 < total; m0 += EVICT_WARPS * blocks * 32) {
+    long long to = -1, from = 0;
+    if (m0 + lane < total) {
+      const int hole = moves[m0 + lane], source = moves[p.max_moves + m0 + lane];
+      const int to_block = table[hole / p.bs], from_block = table[source / p.bs];
+      w[hole] = w[source];
+      pos[hole] = entry_position(pos, source, len, next);
+      if ((unsigned)to_block < (unsigned)p.num_blocks && (unsigned)from_block < (unsigned)p.num_blocks) {
+        to = ((long long)to_block * p.Hkv + h) * p.bs + hole % p.bs;
+        from = ((long long)from_block * p.Hkv + h) * p.bs + source % p.bs;
+      }
+    }
+    const int n = min(32, total - m0);
+    for (int j0 = 0; j0 < n; j0 += 4) {
+      long long t4[4], f4[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        t4[j] = __shfl_sync(0xffffffffu, to, (j0 + j) & 31), f4[j] = __shfl_sync(0xffffffffu, from, (j0 + j) & 31);
+        if (j0 + j >= n) t4[j] = -1;
+      }
+      for (int i = lane; i < words; i += 32) {
+        const bool is_k = i < k_words;
+        W* base = is_k ? kc + i : vc + (i - k_words);
+        const int row = is_k ? k_words : words - k_words;
+        W x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (t4[j] >= 0) x[j] = base[f4[j] * row];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (t4[j] >= 0) base[t4[j] * row] = x[j];
+      }
+    }
+  }
+  meet();                                      // what moved is read
+  for (int i = b0 + tid; i < b0 + nb; i += EVICT_THREADS) w[i] = 0.f;
+  const int c0 = keep + cut(p.capacity - keep, rank), c1 = keep + cut(p.capacity - keep, rank + 1);
+  for (int i = c0 + tid; i < c1; i += EVICT_THREADS) pos[i] = -1;
 }
 
 }  // namespace
@@ -136,10 +239,10 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) evict_move_kernel(const Evict
 
 extern "C" {
 
-// Ints of the list of moves: per (sequence, head) a count and two indexes for each of the entries that can move.
+// Ints of the list of moves: per (sequence, head) two indexes for each of the entries that can move.
 long long swb_evict_moves(int num_seqs, int Hkv, int capacity, int keep) {
   const long long most = capacity > keep ? (capacity - keep < keep ? capacity - keep : keep) : 0;
-  return (long long)num_seqs * Hkv * (1 + 2 * most);
+  return (long long)num_seqs * Hkv * 2 * most;
 }
 
 // See EvictParams. dims: host int[11] = num_seqs, Hkv, table width, blocks, block_size, k row bytes, v row bytes, capacity, keep, recent, first;
@@ -150,23 +253,33 @@ int swb_evict(const int* dims, const long long* strides, void* k, void* v, const
   const int seqs = dims[0], Hkv = dims[1], max_blocks = dims[2], blocks = dims[3], bs = dims[4], kb = dims[5], vb = dims[6], capacity = dims[7];
   const int keep = dims[8], recent = dims[9], first = dims[10];
   if (seqs <= 0) return 0;
-  if (seqs > 65535 || Hkv < 1 || Hkv > 65535 || bs < 1 || kb < 2 || vb < 2 || ((kb | vb) & 1) || keep < 1 || recent < 0 || first < 0 || first > keep - recent || blocks < 1 ||
-      max_blocks < 1 || !k || !v || !table || !kv_lens || !new_lens || !next || !weights || !positions || !moves)
-    return -3;
   const int most = capacity > keep ? (capacity - keep < keep ? capacity - keep : keep) : 0;
+  if (seqs > 65535 || Hkv < 1 || Hkv > 65535 || bs < 1 || kb < 2 || vb < 2 || ((kb | vb) & 1) || keep < 1 || recent < 0 || first < 0 || first > keep - recent || blocks < 1 ||
+      max_blocks < 1 || (long long)max_blocks * bs > INT_MAX || !k || !v || !table || !kv_lens || !new_lens || !next || !weights || !positions || (most && !moves))
+    return -3;
   const EvictParams p{reinterpret_cast<char*>(k), reinterpret_cast<char*>(v), kb, vb, table, table_stride, max_blocks, blocks, bs, Hkv, kv_lens, new_lens, next, weights,
                       strides[0], strides[1], positions, strides[2], strides[3], capacity, keep, recent, first, moves, most};
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const size_t smem = 4 * (size_t)(capacity < EVICT_CACHED ? capacity : EVICT_CACHED);
+  // a block for every 2048 entries where that fills the chip no further than one round
+  int share = 1;
+  while (share < EVICT_CLUSTER && share * 2048 < capacity && (long long)share * 2 * Hkv * seqs <= 2 * 148) share *= 2;
+  const int cached = capacity / share + 2;
+  const size_t smem = 4 * (size_t)(cached < EVICT_CACHED ? cached : EVICT_CACHED);
+  const bool wide = ((kb | vb) & 15) == 0 && ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
+  auto kernel = wide ? evict_kernel<uint4> : evict_kernel<uint16_t>;
   if (smem > 32 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(evict_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return -(int)e;
   }
-  int rc = launch_kernel(evict_plan_kernel, dim3(Hkv, seqs), dim3(EVICT_THREADS), smem, s, p);
-  if (rc || most == 0) return rc;
-  const dim3 grid((most + MOVE_WARPS - 1) / MOVE_WARPS, Hkv, seqs), block(MOVE_WARPS * 32);
-  const bool wide = ((kb | vb) & 15) == 0 && ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
-  return wide ? launch_kernel(evict_move_kernel<uint4>, grid, block, 0, s, p) : launch_kernel(evict_move_kernel<uint16_t>, grid, block, 0, s, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(Hkv * share, seqs), cfg.blockDim = dim3(EVICT_THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = share, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr, cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p, share);
+  return e == cudaSuccess ? 0 : -(int)e;
 }
 
 }  // extern "C"
