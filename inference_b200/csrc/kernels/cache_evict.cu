@@ -34,6 +34,7 @@ struct EvictParams {
 
 constexpr int EVICT_THREADS = 512, EVICT_WARPS = EVICT_THREADS / 32, EVICT_CLUSTER = 8;
 constexpr int EVICT_CACHED = 16384;            // keys that a block holds in shared memory; with more it computes them again in every pass
+constexpr int EVICT_LISTED = 1024;             // keys in the border's bin that one block can take apart alone
 
 __device__ __forceinline__ int entry_position(const int* pos, int i, int len, int next) {
   const int x = pos[i];
@@ -54,6 +55,9 @@ __device__ __forceinline__ int load_from(const int* at, int rank) {
 __device__ __forceinline__ void store_to(const void* at, int rank, uint32_t x) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(in_block(at, rank)), "r"(x) : "memory");
 }
+__device__ __forceinline__ void red_to(const int* at, int rank, int x) {
+  asm volatile("red.shared::cluster.add.s32 [%0], %1;" ::"r"(in_block(at, rank)), "r"(x) : "memory");
+}
 __device__ __forceinline__ int add_to(const int* at, int rank, int x) {
   int old;
   asm volatile("atom.shared::cluster.add.s32 %0, [%1], %2;" : "=r"(old) : "r"(in_block(at, rank)), "r"(x) : "memory");
@@ -69,7 +73,8 @@ __global__ void __launch_bounds__(EVICT_THREADS, 2) evict_kernel(const EvictPara
   pdl_launch_dependents();
   extern __shared__ uint32_t evict_keys[];
   __shared__ __align__(16) int hist[SELECT_INTS];
-  __shared__ int s_count[4];                   // keys above and equal to the threshold, in front of and behind `keep`
+  __shared__ uint32_t s_list[EVICT_LISTED];
+  __shared__ int s_listed, s_count[4];                   // keys above and equal to the threshold, in front of and behind `keep`
   const Team<EVICT_THREADS> team(threadIdx.x);
   const int rank = blockIdx.x % blocks, h = blockIdx.x / blocks, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t below = (1u << lane) - 1u;
@@ -103,7 +108,7 @@ __global__ void __launch_bounds__(EVICT_THREADS, 2) evict_kernel(const EvictPara
   const auto key = [&](int i) -> uint32_t { return cached ? evict_keys[i] : fresh_key(i); };
   // histograms of `digit` of the keys that agree with prefix under mask, gathered in the first block; bin and rest in its totals
   const auto find = [&](uint32_t prefix, uint32_t mask, int shift, uint32_t digit, int want) {
-#pragma unroll 4
+#pragma unroll 8
     for (int i = tid; i < na + nb; i += EVICT_THREADS) {
       const uint32_t k = mask ? key(i) : fresh_key(i);
       if (!mask && cached) evict_keys[i] = k;
@@ -112,7 +117,7 @@ __global__ void __launch_bounds__(EVICT_THREADS, 2) evict_kernel(const EvictPara
     __syncthreads();
     if (rank > 0)
       for (int i = tid; i < SELECT_BINS; i += EVICT_THREADS)
-        if (hist[i]) add_to(&hist[i], 0, hist[i]);
+        if (hist[i]) red_to(&hist[i], 0, hist[i]);
     meet();
     if (rank == 0) find_bin(team, hist, want, totals);
     meet();
@@ -123,23 +128,35 @@ __global__ void __launch_bounds__(EVICT_THREADS, 2) evict_kernel(const EvictPara
   int want = load_from(&totals[33], 0);
   const int m = load_from(&totals[34], 0);
   Threshold th;
-  if (m <= EVICT_THREADS) {                    // few enough to be ranked by one block
-    uint32_t* list = reinterpret_cast<uint32_t*>(hist);
-    meet();                                    // everybody has read the totals, and find_bin the bins
+  if (m <= EVICT_LISTED) {
+    // Every block gathers its own and asks for room in the first one's list once (an addition to another block's memory with an answer takes some 100 cycles,
+    // one behind the other). The first block then chooses by the other 21 bits.
+    if (tid == 0) s_listed = 0;
+    meet();                                    // everybody has read the totals
 #pragma unroll 4
     for (int i = tid; i < na + nb; i += EVICT_THREADS) {
       const uint32_t k = key(i);
-      if ((k >> 21) == prefix) store_to(&list[add_to(&totals[35], 0, 1)], 0, k);
+      if ((k >> 21) == prefix) s_list[atomicAdd(&s_listed, 1)] = k;
+    }
+    if (rank == 0) clear_bins(team, hist);
+    meet();                                    // the first block's list has its own keys and their number
+    if (rank > 0) {
+      const int own = s_listed;
+      __syncthreads();
+      if (tid == 0 && own) s_listed = add_to(&s_listed, 0, own);
+      __syncthreads();
+      for (int i = tid; i < own; i += EVICT_THREADS) store_to(&s_list[s_listed + i], 0, s_list[i]);
+    }
+    if (blocks > 1) meet();
+    if (rank == 0) {
+      const auto rest = [&](int i) { return s_list[i] << 11; };
+      for (int i = tid; i < m; i += EVICT_THREADS) count_key(hist, rest(i));
+      __syncthreads();
+      const Threshold t = select_threshold(team, rest, m, want, hist);
+      if (tid == 0) totals[39] = (int)(prefix << 21 | t.key >> 11), totals[40] = t.ties;
     }
     meet();
-    if (rank == 0 && tid < m) {
-      const uint32_t mine = list[tid];
-      int above = 0, same = 0;
-      for (int j = 0; j < m; ++j) above += list[j] > mine, same += list[j] == mine;
-      if (above < want && want <= above + same) totals[37] = (int)mine, totals[38] = want - above;
-    }
-    meet();
-    th = Threshold{(uint32_t)load_from(&totals[37], 0), load_from(&totals[38], 0)};
+    th = Threshold{(uint32_t)load_from(&totals[39], 0), load_from(&totals[40], 0)};
   } else {
     prefix <<= 21, mask <<= 21;
 #pragma unroll 1
@@ -165,12 +182,13 @@ __global__ void __launch_bounds__(EVICT_THREADS, 2) evict_kernel(const EvictPara
   const PairSums b = sum_over_warps(team, count_run(key, th, lo_b, hi_b), slots + 32);
   if (tid == 0) s_count[0] = a.all.x, s_count[1] = a.all.y, s_count[2] = b.all.x, s_count[3] = b.all.y;
   meet();
-  int above_a = a.before.x, same_a = a.before.y, above_b = b.before.x, same_b = b.before.y, all_above = 0, all_same = 0;
-  for (int r = 0; r < blocks; ++r) {
-    const int x = load_from(&s_count[0], r), y = load_from(&s_count[1], r);
-    all_above += x, all_same += y;
-    if (r < rank) above_a += x, same_a += y, above_b += load_from(&s_count[2], r), same_b += load_from(&s_count[3], r);
-  }
+  // lane r has block r's counts
+  int4 mine = make_int4(0, 0, 0, 0);
+  if (lane < blocks) mine = make_int4(load_from(&s_count[0], lane), load_from(&s_count[1], lane), load_from(&s_count[2], lane), load_from(&s_count[3], lane));
+  const auto all_of = [&](int x) { return __reduce_add_sync(0xffffffffu, x); };
+  const auto before = [&](int x) { return __reduce_add_sync(0xffffffffu, lane < rank ? x : 0); };
+  const int all_above = all_of(mine.x), all_same = all_of(mine.y);
+  const int above_a = a.before.x + before(mine.x), same_a = a.before.y + before(mine.y), above_b = b.before.x + before(mine.z), same_b = b.before.y + before(mine.w);
   const int kept_a = all_above + min(all_same, th.ties), total = keep - kept_a;
   int hole_at = a0 + lo_a - (above_a + min(same_a, th.ties));
   for_each_choice(key, th, lo_a, hi_a, same_a, [&](int i, bool in, uint32_t) {
@@ -189,44 +207,45 @@ __global__ void __launch_bounds__(EVICT_THREADS, 2) evict_kernel(const EvictPara
     if (pos[a0 + i] < 0) pos[a0 + i] = next - (len - (a0 + i));
   meet();                                      // the list is complete
 
-  // 32 moves to a warp: a lane looks one up, then the warp copies their rows, four at a time
+  // Up to 32 moves to a warp: its lanes look one up each, all at once, then it copies their rows, eight moves on their way together.
   const int* table = p.table + seq * p.table_stride;
   const int k_words = p.k_bytes / (int)sizeof(W), words = k_words + p.v_bytes / (int)sizeof(W);
   W* kc = reinterpret_cast<W*>(p.k);
   W* vc = reinterpret_cast<W*>(p.v);
-  for (int m0 = (warp * blocks + rank) * 32; m0 < total; m0 += EVICT_WARPS * blocks * 32) {
-    long long to = -1, from = 0;
-    if (m0 + lane < total) {
-      const int hole = moves[m0 + lane], source = moves[p.max_moves + m0 + lane];
+  const int stride = EVICT_WARPS * blocks;
+  for (int m0 = warp * blocks + rank; m0 < total; m0 += 32 * stride) {
+    const int m = m0 + lane * stride, n = min(32, (total - m0 + stride - 1) / stride);
+    long long to = -1, from = -1;              // rows, -1: none
+    float weight = 0.f;
+    int place = 0, target = -1;
+    if (m < total) {
+      const int hole = moves[m], source = moves[p.max_moves + m];
       const int to_block = table[hole / p.bs], from_block = table[source / p.bs];
-      w[hole] = w[source];
-      pos[hole] = entry_position(pos, source, len, next);
+      weight = w[source], place = entry_position(pos, source, len, next), target = hole;
       if ((unsigned)to_block < (unsigned)p.num_blocks && (unsigned)from_block < (unsigned)p.num_blocks) {
         to = ((long long)to_block * p.Hkv + h) * p.bs + hole % p.bs;
         from = ((long long)from_block * p.Hkv + h) * p.bs + source % p.bs;
       }
     }
-    const int n = min(32, total - m0);
-    for (int j0 = 0; j0 < n; j0 += 4) {
-      long long t4[4], f4[4];
+    for (int i0 = 0; i0 < words; i0 += 32) {
+      const int i = i0 + lane;
+      W* base = i < k_words ? kc + i : vc + (i - k_words);
+      const int row = i < k_words ? k_words : words - k_words;
+      for (int j0 = 0; j0 < n; j0 += 8) {
+        W x[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        t4[j] = __shfl_sync(0xffffffffu, to, (j0 + j) & 31), f4[j] = __shfl_sync(0xffffffffu, from, (j0 + j) & 31);
-        if (j0 + j >= n) t4[j] = -1;
-      }
-      for (int i = lane; i < words; i += 32) {
-        const bool is_k = i < k_words;
-        W* base = is_k ? kc + i : vc + (i - k_words);
-        const int row = is_k ? k_words : words - k_words;
-        W x[4];
+        for (int j = 0; j < 8; ++j) {
+          const long long f = __shfl_sync(0xffffffffu, from, j0 + j);
+          if (f >= 0 && i < words) x[j] = base[f * row];
+        }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (t4[j] >= 0) x[j] = base[f4[j] * row];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (t4[j] >= 0) base[t4[j] * row] = x[j];
+        for (int j = 0; j < 8; ++j) {
+          const long long t = __shfl_sync(0xffffffffu, to, j0 + j);
+          if (t >= 0 && i < words) base[t * row] = x[j];
+        }
       }
     }
+    if (target >= 0) w[target] = weight, pos[target] = place;
   }
   meet();                                      // what moved is read
   for (int i = b0 + tid; i < b0 + nb; i += EVICT_THREADS) w[i] = 0.f;
