@@ -19,7 +19,7 @@ from dataclasses import dataclass
 import torch
 
 from .._native import kernels
-from .runtime import KernelError, check, ptr, require_cuda, stream_ptr
+from .runtime import KernelError, check, ptr, require_cuda
 
 MAX_WIDTH, MAX_GROUP, MAX_SPLITS = 256, 128, 64
 SELECT_SMEM = 200 * 1024
@@ -61,13 +61,14 @@ def _require(ok: bool, what: str) -> None:
         raise KernelError(what)
 
 
-def _place(*tensors: torch.Tensor | None) -> None:
-    """All operands on the current device: launches go to its current stream."""
+def _place(*tensors: torch.Tensor | None) -> int:
+    """All operands on the current device; its current stream, which launches go to."""
     dev = torch.cuda.current_device() if torch.cuda.is_initialized() else 0
     for t in tensors:
         if t is not None and t.get_device() != dev:
             require_cuda(t)
             raise KernelError(f"operands lie on {t.device}, the current device is cuda:{dev}")
+    return torch._C._cuda_getCurrentRawStream(dev)          # (a Stream object takes 3 us to make)
 
 
 def _check_cache(kcache: torch.Tensor, vcache: torch.Tensor | None = None) -> tuple[int, int, int, int, int]:
@@ -110,14 +111,14 @@ def summarize_pages(kcache: torch.Tensor, block_table: torch.Tensor, kv_lens: to
     """Fills the summaries of the pages that the step's new tokens complete: the last tokens of each sequence, already in the cache (max_q_len bounds their
     number). s = sum of a page's keys, a = max |s|: codes rint(127 s / a), scale a / (127 block_size); sums and quotient in 64 bits."""
     codes, scales = summaries.codes, summaries.scales
-    _place(kcache, block_table, kv_lens, codes, scales, cu_q)
+    stream = _place(kcache, block_table, kv_lens, codes, scales, cu_q)
     blocks, heads, bs, D, _ = _check_cache(kcache)
     n, per = _check_step(block_table, kv_lens, cu_q, max_q_len, -1)
     _require(codes.dtype == torch.int8 and codes.shape == (blocks, heads, D) and codes.is_contiguous() and scales.dtype == torch.float32
              and scales.shape == (blocks, heads) and scales.is_contiguous(), "summaries belong to these pages: int8 [blocks, kv heads, D], fp32 [blocks, kv heads]")
     dims = _INTS[9](n, max_q_len, per, blocks, bs, heads, D, kcache.dtype == torch.float32, 0)
     check(kernels().swb_page_summaries(dims, kcache.data_ptr(), codes.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), ptr(cu_q),
-                                       kv_lens.data_ptr(), stream_ptr()), "swb_page_summaries")
+                                       kv_lens.data_ptr(), stream), "swb_page_summaries")
 
 
 def select_pages(q: torch.Tensor, summaries: PageSummaries, block_table: torch.Tensor, kv_lens: torch.Tensor, *, cu_q: torch.Tensor | None, max_q_len: int,
@@ -128,7 +129,7 @@ def select_pages(q: torch.Tensor, summaries: PageSummaries, block_table: torch.T
     q [T, Hq, D] bf16 or fp32 (token and head strides free). The group's queries are rounded to 8-bit codes of one step, max |q| / 127; score = the page's scale * max over the
     group of the codes' dot product. A token whose queries are not all finite, or all zero, finds every page alike."""
     codes, scales = summaries.codes, summaries.scales
-    _place(q, codes, scales, block_table, kv_lens, cu_q)
+    stream = _place(q, codes, scales, block_table, kv_lens, cu_q)
     shape = codes.shape
     _require(len(shape) == 3 and codes.dtype == torch.int8 and codes.is_contiguous() and scales.dtype == torch.float32 and scales.shape == shape[:2]
              and scales.is_contiguous() and shape[2] <= MAX_WIDTH, "summaries are int8 [blocks, kv heads, D] and fp32 [blocks, kv heads]")
@@ -143,7 +144,7 @@ def select_pages(q: torch.Tensor, summaries: PageSummaries, block_table: torch.T
     counts = torch.empty((T, heads), dtype=torch.int32, device=q.device)
     dims = _INTS[14](T, n, max_q_len, per, blocks, block_size, heads, G, D, first, top, last, q.dtype == torch.float32, 0)
     check(lib.swb_page_select(dims, q.data_ptr(), tok, head, codes.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), ptr(cu_q),
-                              kv_lens.data_ptr(), pages.data_ptr(), counts.data_ptr(), stream_ptr()), "swb_page_select")
+                              kv_lens.data_ptr(), pages.data_ptr(), counts.data_ptr(), stream), "swb_page_select")
     return PageSelection(pages, counts)
 
 
@@ -160,7 +161,7 @@ def budget_splits(problems: int, keys: int, even: bool, sms: int = 148) -> int:
 
 
 def _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, softcap, num_splits, out, pages, counts, weights) -> torch.Tensor:
-    _place(q, kcache, vcache, block_table, kv_lens, cu_q, out, weights, pages, counts)
+    stream = _place(q, kcache, vcache, block_table, kv_lens, cu_q, out, weights, pages, counts)
     blocks, heads, bs, D, Dv = _check_cache(kcache, vcache)
     T, G, tok, head = _check_rows(q, heads, D)
     n, per = _check_step(block_table, kv_lens, cu_q, max_q_len, T)
@@ -196,7 +197,7 @@ def _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, 
     dims = _INTS[16](T, n, max_q_len, per, blocks, bs, heads, G, D, Dv, width, splits, kind == torch.float32, 0, 0, 0)
     strides = _LONGS[8](tok, head, out_stride, block_table.stride(0), w_seq, w_head, 0, 0)
     check(lib.swb_attn_budget(dims, strides, q.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), block_table.data_ptr(), ptr(cu_q), kv_lens.data_ptr(),
-                              ptr(pages), ptr(counts), ptr(weights), scale, softcap, ptr(ws), nbytes, stream_ptr()), "swb_attn_budget")
+                              ptr(pages), ptr(counts), ptr(weights), scale, softcap, ptr(ws), nbytes, stream), "swb_attn_budget")
     return out
 
 
@@ -245,7 +246,7 @@ def evict_tokens(kcache: torch.Tensor, vcache: torch.Tensor, block_table: torch.
     and lie behind `keep` move in order into the holes in front of it: their rows of both caches, weight and position. positions int32 [num_seqs, kv heads, N]: -1 for
     entries without a record, which stand in order in front of the next position (all of them before the first call); the call records those it keeps. Weights behind `keep` become 0, positions -1.
     Everything is done in place. Pages must not be shared with a sequence that is not to lose tokens, nor between sequences of the call (`PagedSequence.unshare`)."""
-    _place(kcache, vcache, block_table, kv_lens, weights, positions, next_positions)
+    stream = _place(kcache, vcache, block_table, kv_lens, weights, positions, next_positions)
     blocks, heads, bs, D, Dv = _check_cache(kcache, vcache)
     n, per = _check_step(block_table, kv_lens, None, 1, -1)
     capacity, size = per * bs, 4 if kcache.dtype == torch.float32 else 2
@@ -259,5 +260,5 @@ def evict_tokens(kcache: torch.Tensor, vcache: torch.Tensor, block_table: torch.
     dims = _INTS[11](n, heads, per, blocks, bs, D * size, Dv * size, capacity, keep, recent, first)
     strides = _LONGS[4](*weights.stride()[:2], *positions.stride()[:2])
     check(lib.swb_evict(dims, strides, kcache.data_ptr(), vcache.data_ptr(), block_table.data_ptr(), block_table.stride(0), kv_lens.data_ptr(), lens.data_ptr(),
-                        next_positions.data_ptr(), weights.data_ptr(), positions.data_ptr(), moves.data_ptr(), stream_ptr()), "swb_evict")
+                        next_positions.data_ptr(), weights.data_ptr(), positions.data_ptr(), moves.data_ptr(), stream), "swb_evict")
     return lens

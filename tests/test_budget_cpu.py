@@ -27,9 +27,8 @@ class _NoKernels:
 @pytest.fixture(autouse=True)
 def on_the_cpu(monkeypatch):
     monkeypatch.setattr(budget, "kernels", lambda: _NoKernels())
-    monkeypatch.setattr(budget, "_place", lambda *a: None)
+    monkeypatch.setattr(budget, "_place", lambda *a: 0)
     monkeypatch.setattr(budget, "require_cuda", lambda *a: None)
-    monkeypatch.setattr(budget, "stream_ptr", lambda: 0)
 
 
 def _args():
