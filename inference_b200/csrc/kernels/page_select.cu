@@ -29,10 +29,11 @@ struct SummaryParams {
 
 constexpr int SUMMARY_WARPS = 4;
 
-// rint(127 s / a). The quotient of the 32-bit numbers is off by less than 4 2^-24 127: only where it comes that near a half are the 64-bit numbers divided.
-__device__ __forceinline__ int8_t summary_code(double s, double a) {
-  const float r = __fdiv_rn(127.f * (float)s, (float)a), q = rintf(r);
-  if (fabsf(fabsf(r - q) - 0.5f) > 1e-4f && (float)a > 1e-30f && (float)a < 1e30f) return (int8_t)(int)q;
+// rint(127 s / a), where step = 127 / a in 32 bits. The product of 32-bit numbers is off by less than 4 2^-24 127: only where it comes that near a half are the 64-bit
+// numbers divided.
+__device__ __forceinline__ int8_t summary_code(double s, double a, float step) {
+  const float r = (float)s * step, q = rintf(r);
+  if (fabsf(fabsf(r - q) - 0.5f) > 1e-4f && step < 1e30f && step > 1e-30f) return (int8_t)(int)q;
   return (int8_t)(int)rint(127.0 * s / a);
 }
 
@@ -111,9 +112,10 @@ __global__ void __launch_bounds__(SUMMARY_WARPS * 32) page_summary_quads_kernel(
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) a = fmax(a, __shfl_xor_sync(0xffffffffu, a, o));
   uint32_t codes = 0u;
+  const float step = __fdiv_rn(127.f, (float)a);
 #pragma unroll
   for (int c = 0; c < 4; ++c)
-    if (!bad && a > 0.0) codes |= (uint32_t)(uint8_t)summary_code(s[c], a) << (8 * c);
+    if (!bad && a > 0.0) codes |= (uint32_t)(uint8_t)summary_code(s[c], a, step) << (8 * c);
   if (live) reinterpret_cast<uint32_t*>(p.codes + at * p.D)[lane] = codes;
   if (lane == 0) p.scales[at] = bad ? NAN : (float)(a / (127.0 * p.bs));
 }
@@ -151,7 +153,7 @@ __global__ void __launch_bounds__(SUMMARY_WARPS * 32) page_summary_kernel(const 
 #pragma unroll
   for (int c = 0; c < COLS; ++c) {
     const int d = c * 32 + lane;
-    if (d < p.D) p.codes[at * p.D + d] = bad || a == 0.0 ? (int8_t)0 : summary_code(s[c], a);
+    if (d < p.D) p.codes[at * p.D + d] = bad || a == 0.0 ? (int8_t)0 : summary_code(s[c], a, __fdiv_rn(127.f, (float)a));
   }
   if (lane == 0) p.scales[at] = bad ? NAN : (float)(a / (127.0 * p.bs));
 }

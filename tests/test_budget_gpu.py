@@ -277,6 +277,35 @@ def test_page_summaries(kv, D, bs, kind):
     assert torch.equal(sums.codes.cpu(), want_c) and torch.equal(sums.scales.cpu().nan_to_num(nan=-7.0), want_s.nan_to_num(nan=-7.0))
 
 
+@pytest.mark.parametrize("D,bs", [(128, 16), (64, 32), (96, 4), (128, 80)])
+def test_summaries_at_the_borders(D, bs):
+    """Pages whose sums cancel, lie on halves of the step, differ by little, pass the range of 32 bits or have none."""
+    ops = _ops()
+    c = Cache([40 * bs], [1], heads=1, kv_heads=1, D=D, bs=bs)
+    k, at = c.k, c.table[0].long()
+    g = _gen(D)
+    k[at[0]] *= 1e-3                                          # small numbers beside large ones that cancel
+    k[at[0], 0, 0], k[at[0], 0, 1] = 300.0, -300.0
+    k[at[1]] = 0
+    k[at[1], 0, 0] = (torch.arange(D, device=CUDA) - D // 2).bfloat16()
+    k[at[1], 0, 0, 0] = 254.0                                 # 127 x / 254: every odd number is a half
+    k[at[2]] = 3e38
+    k[at[2], 0, :, 1] = 1.5e38
+    k[at[3]] = 0
+    k[at[4]] = torch.randint(-2, 3, k[at[4]].shape, device=CUDA, generator=g).bfloat16() * 2.0 ** -130      # below the normal numbers of 32 bits
+    k[at[5]] = 1.0
+    k[at[5], 0, 0, 3] = 1.0 + 2.0 ** -7
+    k[at[6], 0, bs - 1, D - 1] = float("nan")
+    k[at[7], 0, 1, 1], k[at[7], 0, 2, 1] = float("inf"), float("-inf")
+    k[at[8]] = torch.where(torch.rand(k[at[8]].shape, device=CUDA, generator=g) < 0.5, 1.0, 2.0 ** -20).bfloat16()
+    sums = ops.PageSummaries.empty(k)
+    ops.summarize_pages(k, c.table, c.kv_lens, sums, cu_q=None, max_q_len=40 * bs)
+    for page in range(40):
+        code, scale = _summary(k[at[page], 0].cpu())
+        got = float(sums.scales[at[page], 0])
+        assert torch.equal(sums.codes[at[page], 0].cpu(), code) and (got == scale or (math.isnan(got) and math.isnan(scale))), page
+
+
 def test_summaries_of_single_steps_are_those_of_the_prompt():
     ops = _ops()
     c = Cache([70], [1], kv_heads=2)
