@@ -75,21 +75,51 @@ __device__ __forceinline__ void store_out(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store_out(bf16* p, float x) { *p = __float2bfloat16(x); }
 
 // ---- any types and widths: 32-bit arithmetic on ordinary cores --------------------------------------------------------------------------------------
-constexpr int PLAIN_TILE = 32, PLAIN_THREADS = 128;
+constexpr int PLAIN_TILE = 32, PLAIN_THREADS = 128, PLAIN_WARPS = PLAIN_THREADS / 32;
 
-template <typename E, int COLS>       // COLS * 128 >= Dv
+__device__ __forceinline__ int plain_ldk(int D) { return (D + 3) / 4 * 4 + 4; }      // lanes with neighbouring keys meet in no bank
+
+// One tile of rows of `width` numbers into shared memory as 32-bit numbers, rows ld apart (a warp a row at a time, eight rows on their way), zeros where a key is masked and
+// behind the row's end. VEC: four numbers at a time.
+template <typename E, bool VEC>
+__device__ __forceinline__ void plain_fetch(float* to, int ld, const E* from, int width, const long long* rows) {
+  constexpr int STEP = VEC ? 4 : 1, KEYS = PLAIN_TILE / PLAIN_WARPS;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, padded = (width + 3) / 4 * 4;
+  for (int d = lane * STEP; d < padded; d += 32 * STEP) {
+    float4 x[KEYS];
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+      const long long row = rows[warp + i * PLAIN_WARPS];
+      x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row >= 0 && d < width) {
+        if constexpr (VEC) x[i] = load_row4(from + row * width + d);
+        else x[i].x = to_f(from[row * width + d]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+      float* at = to + (warp + i * PLAIN_WARPS) * ld + d;
+      if constexpr (VEC) *reinterpret_cast<float4*>(at) = x[i];
+      else *at = x[i].x;
+    }
+  }
+}
+
+// R: rows that a problem can have, 4, 8 or 16. COLS * 128 >= Dv.
+template <typename E, int COLS, int R, bool VEC>
 __global__ void __launch_bounds__(PLAIN_THREADS) attn_budget_plain_kernel(const BudgetParams p) {
   pdl_launch_dependents();
-  extern __shared__ float plain_smem[];
-  const int ldk = p.D + 1;
-  float* sq = plain_smem;                          // [ROWS][D]
-  float* sk = sq + ROWS * p.D;                     // [PLAIN_TILE][D + 1]
-  float* sp = sk + PLAIN_TILE * ldk;               // [PLAIN_TILE][ROWS]
+  extern __shared__ __align__(16) float plain_smem[];
+  const int ldk = plain_ldk(p.D), D4 = ldk - 4, ldv = (p.Dv + 3) / 4 * 4;
+  float* sq = plain_smem;                          // [R][D4], zeros behind a row's end
+  float* sk = sq + R * D4;                         // [PLAIN_TILE][ldk]
+  float* sv = sk + PLAIN_TILE * ldk;               // [PLAIN_TILE][ldv]
+  float* sp = sv + PLAIN_TILE * ldv;               // [PLAIN_TILE][R]
   __shared__ long long s_row[PLAIN_TILE];          // first row of the key's page + its place, -1: masked
   __shared__ float s_m[ROWS], s_l[ROWS], s_alpha[ROWS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int split = blockIdx.x % p.num_splits, y = blockIdx.x / p.num_splits, hy = y % (p.Hkv * p.head_tiles), t = y / (p.Hkv * p.head_tiles);
-  const int h = hy / p.head_tiles, ht = hy % p.head_tiles, g0 = ht * ROWS, rows = min(ROWS, p.G - g0);
+  const int h = hy / p.head_tiles, ht = hy % p.head_tiles, g0 = ht * ROWS, rows = min(R, p.G - g0);
   pdl_wait();
   if (p.cu_q && t >= p.cu_q[p.num_seqs]) return;
   const Token tok = token_of(p, t);
@@ -99,15 +129,14 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_budget_plain_kernel(const 
   const int tiles = (total + PLAIN_TILE - 1) / PLAIN_TILE, per = (tiles + p.num_splits - 1) / p.num_splits;
   const int t_lo = split * per, t_hi = min(tiles, t_lo + per);
   const E* q = reinterpret_cast<const E*>(p.q) + t * p.q_stride_tok + (size_t)(h * p.G + g0) * p.q_stride_head;
-  for (int i = tid; i < rows * p.D; i += PLAIN_THREADS) sq[i] = to_f(q[(i / p.D) * p.q_stride_head + i % p.D]);
-  if (tid < ROWS) s_m[tid] = -INFINITY, s_l[tid] = 0.f;
-  float o[COLS][ROWS];
+  for (int r = warp; r < R; r += PLAIN_WARPS)
+    for (int d = lane; d < D4; d += 32) sq[r * D4 + d] = r < rows && d < p.D ? to_f(q[r * p.q_stride_head + d]) : 0.f;
+  if (tid < ROWS) s_m[tid] = -INFINITY, s_l[tid] = 0.f, s_alpha[tid] = 1.f;
+  float o[COLS][R];
 #pragma unroll
   for (int c = 0; c < COLS; ++c)
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) o[c][r] = 0.f;
-  const E* kc = reinterpret_cast<const E*>(p.k);
-  const E* vc = reinterpret_cast<const E*>(p.v);
+    for (int r = 0; r < R; ++r) o[c][r] = 0.f;
   for (int tile = t_lo; tile < t_hi; ++tile) {
     __syncthreads();
     if (tid < PLAIN_TILE) {
@@ -124,22 +153,36 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_budget_plain_kernel(const 
       s_row[tid] = row;
     }
     __syncthreads();
-    for (int i = tid; i < PLAIN_TILE * p.D; i += PLAIN_THREADS) {
-      const int key = i / p.D, d = i % p.D;
-      sk[key * ldk + d] = s_row[key] >= 0 ? to_f(kc[s_row[key] * p.D + d]) : 0.f;
-    }
+    plain_fetch<E, VEC>(sk, ldk, reinterpret_cast<const E*>(p.k), p.D, s_row);
+    plain_fetch<E, VEC>(sv, ldv, reinterpret_cast<const E*>(p.v), p.Dv, s_row);
     __syncthreads();
     // lane = key, a warp every fourth row
-    for (int r = warp; r < rows; r += PLAIN_THREADS / 32) {
-      float s = 0.f;
-      for (int d = 0; d < p.D; ++d) s = fmaf(sq[r * p.D + d], sk[lane * ldk + d], s);
-      const bool live = s_row[lane] >= 0;
-      s = live ? score_transform(s, p.scale, p.softcap) : -INFINITY;
-      const int j = tile * PLAIN_TILE + lane;
-      if (p.scores && j < total) p.scores[((size_t)t * p.Hkv * p.G + h * p.G + g0 + r) * p.capacity + j] = s;
-      const float m0 = s_m[r], m1 = fmaxf(m0, warp_max(s)), base = m1 == -INFINITY ? 0.f : m1;
-      const float e = exp2f(s - base), sum = warp_sum(e);
-      sp[lane * ROWS + r] = live ? e : 0.f;
+    constexpr int MINE = R / PLAIN_WARPS;
+    float s[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) s[i] = 0.f;
+    for (int d = 0; d < D4; d += 4) {
+      const float4 k = *reinterpret_cast<const float4*>(sk + lane * ldk + d);
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(sq + (warp + i * PLAIN_WARPS) * D4 + d);
+        s[i] = fmaf(x.x, k.x, s[i]), s[i] = fmaf(x.y, k.y, s[i]), s[i] = fmaf(x.z, k.z, s[i]), s[i] = fmaf(x.w, k.w, s[i]);
+      }
+    }
+    const bool live = s_row[lane] >= 0;
+    const int j = tile * PLAIN_TILE + lane;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      const int r = warp + i * PLAIN_WARPS;
+      if (r >= rows) {
+        sp[lane * R + r] = 0.f;
+        continue;
+      }
+      const float x = live ? score_transform(s[i], p.scale, p.softcap) : -INFINITY;
+      if (p.scores && j < total) p.scores[((size_t)t * p.Hkv * p.G + h * p.G + g0 + r) * p.capacity + j] = x;
+      const float m0 = s_m[r], m1 = fmaxf(m0, warp_max(x)), base = m1 == -INFINITY ? 0.f : m1;
+      const float e = exp2f(x - base), sum = warp_sum(e);
+      sp[lane * R + r] = live ? e : 0.f;
       __syncwarp();                                // s_m is read by all lanes before lane 0 writes it
       if (lane == 0) {
         const float alpha = exp2f(m0 - base);
@@ -148,26 +191,28 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_budget_plain_kernel(const 
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-      if (r < rows) {
+    for (int r = 0; r < R; ++r) {
+      const float alpha = s_alpha[r];
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) o[c][r] *= s_alpha[r];
-      }
-    for (int key = 0; key < PLAIN_TILE; ++key) {
-      if (s_row[key] < 0) continue;
+      for (int c = 0; c < COLS; ++c) o[c][r] *= alpha;
+    }
+#pragma unroll 4
+    for (int key = 0; key < PLAIN_TILE; ++key) {   // masked keys have zeros in both
+      float w[R];
+#pragma unroll
+      for (int r = 0; r < R; r += 4) *reinterpret_cast<float4*>(w + r) = *reinterpret_cast<const float4*>(sp + key * R + r);
 #pragma unroll
       for (int c = 0; c < COLS; ++c) {
         const int d = c * PLAIN_THREADS + tid;
-        const float x = d < p.Dv ? to_f(vc[s_row[key] * p.Dv + d]) : 0.f;
+        const float x = d < p.Dv ? sv[key * ldv + d] : 0.f;
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r)
-          if (r < rows) o[c][r] = fmaf(sp[key * ROWS + r], x, o[c][r]);
+        for (int r = 0; r < R; ++r) o[c][r] = fmaf(w[r], x, o[c][r]);
       }
     }
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
+  for (int r = 0; r < R; ++r) {
     if (r >= rows) break;
     const int head = h * p.G + g0 + r;
 #pragma unroll
@@ -695,15 +740,27 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_budget_finish_kernel(const 
     if (j0 + k * JOIN_THREADS < len) w[j0 + k * JOIN_THREADS] = old[k] + sum[k];
 }
 
-template <typename E>
+template <typename E, int R, bool VEC>
 int launch_plain(const BudgetParams& p, cudaStream_t s) {
-  const size_t smem = 4 * ((size_t)ROWS * p.D + (size_t)PLAIN_TILE * (p.D + 1) + PLAIN_TILE * ROWS);
-  auto kernel = p.Dv <= 128 ? attn_budget_plain_kernel<E, 1> : attn_budget_plain_kernel<E, 2>;
+  const int ldk = (p.D + 3) / 4 * 4 + 4, ldv = (p.Dv + 3) / 4 * 4;
+  const size_t smem = 4 * ((size_t)R * (ldk - 4) + (size_t)PLAIN_TILE * (ldk + ldv + R));
+  auto kernel = p.Dv <= 128 ? attn_budget_plain_kernel<E, 1, R, VEC> : attn_budget_plain_kernel<E, 2, R, VEC>;
   if (smem > 40 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return -(int)e;
   }
   return launch_kernel(kernel, dim3(p.num_splits * p.Hkv * p.head_tiles * p.tokens), dim3(PLAIN_THREADS), smem, s, p);
+}
+
+template <typename E, bool VEC>
+int launch_plain(const BudgetParams& p, cudaStream_t s) {
+  return p.G <= 4 ? launch_plain<E, 4, VEC>(p, s) : p.G <= 8 ? launch_plain<E, 8, VEC>(p, s) : launch_plain<E, 16, VEC>(p, s);
+}
+
+template <typename E>
+int launch_plain(const BudgetParams& p, cudaStream_t s) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v);
+  return (p.D | p.Dv) % 4 == 0 && at % (4 * sizeof(E)) == 0 ? launch_plain<E, true>(p, s) : launch_plain<E, false>(p, s);
 }
 
 int heads_in_tiles(int G) { return (G + ROWS - 1) / ROWS; }

@@ -174,6 +174,7 @@ struct SelectParams {
   int* counts;               // [tokens, Hkv]
   int fp32;                  // type of q
   int q_vec;                 // bf16 rows of 16-byte alignment
+  int share;                 // blocks of a problem
 };
 
 constexpr int SELECT_THREADS = 256, SELECT_WARPS = SELECT_THREADS / 32;
@@ -213,8 +214,9 @@ __device__ __forceinline__ int8_t query_code(float x, float a, bool fp32) {
 // codes sixteen loads touched each line four times, and the look-ups in the cache's tags bound the kernel): the lane of page g and quarter t holds columns 64 j + 16 t and on,
 // for two steps, and the queries' codes are read in the same order, so the order of the columns within a step is another than the instruction's and the sum the same.
 // Then the tokens are shared out among teams of warps, each of which chooses among its token's scores.
+// CL: p.share blocks, a cluster, score a part of the pages each into the first one's memory, and that one chooses (few problems over long caches).
 // Shared memory: the teams' histograms, codes of the queries [TT, G, 32 KS], keys [TT, pages].
-template <int TT, int KS, bool FULL, int GP>
+template <int TT, int KS, bool FULL, int GP, bool CL>
 __global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 ? 4 : 3) page_select_kernel(const SelectParams p) {
   constexpr int TEAM = SELECT_THREADS / TT, LD = 32 * KS;
   pdl_launch_dependents();
@@ -229,7 +231,8 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 ? 4 : 3)
   uint32_t* keys = reinterpret_cast<uint32_t*>(qc + TT * p.G * LD);
   // blocks that run together share what they read: the tokens of a prompt a head's codes, the heads of a decode step a page's memory
   const int runs = (p.uniform_q + TT - 1) / TT, all_runs = runs * p.num_seqs;
-  const int h = TT > 1 ? blockIdx.x / all_runs : blockIdx.x % p.Hkv, run = TT > 1 ? blockIdx.x % all_runs : blockIdx.x / p.Hkv, seq = run / runs;
+  const int share = CL ? p.share : 1, rank = CL ? blockIdx.x % share : 0, x = CL ? blockIdx.x / share : blockIdx.x;
+  const int h = TT > 1 ? x / all_runs : x % p.Hkv, run = TT > 1 ? x % all_runs : x / p.Hkv, seq = run / runs;
   if (tid < TT) s_bad[tid] = 0, s_largest[tid] = 0u;
   pdl_wait();
   const int q0 = p.cu_q ? p.cu_q[seq] : seq * p.uniform_q, q1 = p.cu_q ? p.cu_q[seq + 1] : q0 + p.uniform_q;
@@ -244,7 +247,7 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 ? 4 : 3)
   const int t = t0 + team.id, n = t < min(q1, p.tokens) ? pages_of(t) : 0;
   int* out = p.pages + ((size_t)t * p.Hkv + h) * width;
   if (team.rank == 0) s_cand[team.id] = n > width ? n - p.first - p.last : 0;
-  if (t < min(q1, p.tokens)) {
+  if (rank == 0 && t < min(q1, p.tokens)) {
     if (team.rank == 0) p.counts[(size_t)t * p.Hkv + h] = min(n, width);
     if (n <= width) {
       for (int i = team.rank; i < width; i += TEAM) out[i] = i < n ? i : -1;
@@ -332,11 +335,19 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 ? 4 : 3)
     const int block = i < cand ? table[i] : -1;
     return (unsigned)block < (unsigned)p.num_blocks ? block : -1;
   };
+  uint32_t first_keys = 0;                         // of the cluster's first block
+  if (CL) {
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(first_keys) : "r"(smem_u32(keys)));
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");        // it runs
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
   // keeps the score of candidate i for a token, which has `most` of them
   const auto keep = [&](int tok, int most, int i, int best, float scale, bool there) -> uint32_t {
     if (i >= most) return 0u;
     const uint32_t k = float_key(there ? __fmul_rn((float)best, scale) : -INFINITY);
-    keys[tok * p.max_blocks + i] = k;
+    if (CL) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(first_keys + 4u * i), "r"(k) : "memory");
+    else keys[tok * p.max_blocks + i] = k;
     return k;
   };
   // the largest key of each token, where a thread keeps keys of several
@@ -425,24 +436,36 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 ? 4 : 3)
   // while 16 pages are scored the next 16 are on their way, and the blocks of the 32 behind them
   uint32_t even[KS][4], odd[KS][4];
   const auto scales_of = [&](int block) { return block >= 0 ? p.scales[(size_t)block * p.Hkv + h] : 0.f; };
-  int i0 = warp * 32, block = locate(i0 + lane), next = locate(i0 + SELECT_THREADS + lane);
+  const int step = SELECT_THREADS * share;
+  int i0 = rank * SELECT_THREADS + warp * 32, block = locate(i0 + lane), next = locate(i0 + step + lane);
   float scale = scales_of(block);
   if (i0 < cand) fetch(even, block, 0);
-  for (; i0 < cand; i0 += SELECT_THREADS) {
+  for (; i0 < cand; i0 += step) {
     const uint32_t there = __ballot_sync(0xffffffffu, block >= 0);
     fetch(odd, block, 1);
     score(even, i0, 0, scale, there);
     const float here = scale;
     block = next;
-    next = locate(i0 + 2 * SELECT_THREADS + lane);
+    next = locate(i0 + 2 * step + lane);
     scale = scales_of(block);
-    if (i0 + SELECT_THREADS < cand) fetch(even, block, 0);
+    if (i0 + step < cand) fetch(even, block, 0);
     score(odd, i0, 1, here, there);
   }
 #pragma unroll
   for (int x = 0; x < NT; ++x)
     if (most_of[x] > 0 && largest[x]) atomicMax(&s_largest[x * (8 / Gp) + tok0], largest[x]);
   __syncthreads();
+  if (CL) {
+    if (rank > 0 && tid == 0) {
+      uint32_t to;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(smem_u32(s_largest)));
+      asm volatile("red.shared::cluster.max.u32 [%0], %1;" ::"r"(to), "r"(s_largest[0]) : "memory");
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank > 0) return;
+  }
   if (n <= width) return;                          // whole teams leave
   const int want = n - p.first - p.last;           // this token's candidates
   const uint32_t* own = keys + team.id * p.max_blocks;
@@ -458,19 +481,35 @@ int select_tokens(int uniform, int G, int pages) {
   return TT;
 }
 
-template <int TT, int KS, bool FULL, int GP>
+template <int TT, int KS, bool FULL, int GP, bool CL = false>
 int launch_select(const SelectParams& p, cudaStream_t s) {
   const size_t smem = TT * ((size_t)SELECT_INTS * 4 + (size_t)p.G * 32 * KS + 4 * (size_t)p.max_blocks);
-  auto kernel = page_select_kernel<TT, KS, FULL, GP>;
+  auto kernel = page_select_kernel<TT, KS, FULL, GP, CL>;
   if (smem > 47 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return -(int)e;
   }
-  return launch_kernel(kernel, dim3((unsigned)(p.num_seqs * ((p.uniform_q + TT - 1) / TT) * p.Hkv)), dim3(SELECT_THREADS), smem, s, p);
+  const dim3 grid((unsigned)(p.num_seqs * ((p.uniform_q + TT - 1) / TT) * p.Hkv * (CL ? p.share : 1)));
+  if (!CL) return launch_kernel(kernel, grid, dim3(SELECT_THREADS), smem, s, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid, cfg.blockDim = dim3(SELECT_THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.share, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr, cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  return e == cudaSuccess ? 0 : -(int)e;
 }
 
 template <int KS, bool FULL, int GP>
-int launch_select(const SelectParams& p, cudaStream_t s) {
+int launch_select(SelectParams p, cudaStream_t s) {
+  // few problems over many pages: up to 8 blocks each, of 256 pages and more
+  const long long problems = (long long)p.num_seqs * p.uniform_q * p.Hkv;
+  p.share = 1;
+  while (p.share < 8 && p.share * 512 <= p.max_blocks && problems * p.share * 2 <= 2 * 148) p.share *= 2;
+  if (p.share > 1) return launch_select<1, KS, FULL, GP, true>(p, s);
   const int TT = select_tokens(p.uniform_q, p.G, p.max_blocks);
   if constexpr (GP != 8)
     if (TT == 4) return launch_select<4, KS, FULL, GP>(p, s);
@@ -518,14 +557,14 @@ int swb_page_select(const int* dims, const void* q, long long q_stride_tok, long
   const int T = dims[0], seqs = dims[1], uniform = dims[2], max_blocks = dims[3], blocks = dims[4], bs = dims[5], Hkv = dims[6], G = dims[7], D = dims[8];
   const int first = dims[9], top = dims[10], last = dims[11], fp32 = dims[12];
   if (T <= 0 || seqs <= 0) return 0;
-  if ((long long)seqs * uniform * Hkv > INT_MAX || bs < 1 || Hkv < 1 || G < 1 || D < 1 || blocks < 1 || max_blocks < 1 || first < 0 || top < 0 || last < 1 || uniform < 1 || D > 256 || (long long)max_blocks * bs > INT_MAX || !q || !codes ||
+  if ((long long)seqs * uniform * Hkv > INT_MAX / 8 || bs < 1 || Hkv < 1 || G < 1 || D < 1 || blocks < 1 || max_blocks < 1 || first < 0 || top < 0 || last < 1 || uniform < 1 || D > 256 || (long long)max_blocks * bs > INT_MAX || !q || !codes ||
       !scales || !table || !kv_lens || !pages || !counts)
     return -3;
   const long long smem = swb_page_select_smem(max_blocks, G, D);
   if (smem > 200 * 1024) return -3;
   const SelectParams p{q, q_stride_tok, q_stride_head, reinterpret_cast<const int8_t*>(codes), reinterpret_cast<const float*>(scales), table, table_stride,
                        max_blocks, blocks, bs, Hkv, G, D, cu_q, kv_lens, seqs, uniform, T, first, top, last, pages, counts, fp32,
-                       !fp32 && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (q_stride_tok | q_stride_head) % 8 == 0};
+                       !fp32 && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (q_stride_tok | q_stride_head) % 8 == 0, 1};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return launch_select(p, s);
 }

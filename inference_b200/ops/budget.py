@@ -148,12 +148,15 @@ def select_pages(q: torch.Tensor, summaries: PageSummaries, block_table: torch.T
     return PageSelection(pages, counts)
 
 
-def budget_splits(problems: int, keys: int, even: bool, sms: int = 148) -> int:
-    """Blocks that share a problem's keys (problems: tokens, or runs of a few of them, * kv heads; even: all have about as many keys). An SM holds two blocks or three.
+def budget_splits(problems: int, keys: int, even: bool, tensor_cores: bool = True, sms: int = 148) -> int:
+    """Blocks that share a problem's keys (problems: tokens, or runs of a few of them, * kv heads; even: all have about as many keys). An SM holds two or three blocks of the
+    kernel on tensor cores, more of the plain one.
 
     Fewer problems than fit at once: as many splits as fit, up to 8, which join within the launch; more, joined by a second one, where 8 would leave SMs idle over
     long caches. More problems: one block each, or where their lengths differ enough blocks of 512 keys and more to even out over seven rounds of the SMs."""
     slots, problems = 2 * sms, max(1, problems)
+    if not tensor_cores:
+        return max(1, min(MAX_SPLITS, (keys + 63) // 64, 8 * sms // problems))
     fit = slots // problems
     if not even and problems * keys >= slots * 4096:
         return max(1, min(MAX_SPLITS, keys // 512, 21 * sms // problems))
@@ -183,20 +186,21 @@ def _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, 
     else:
         _require(out.shape == (T, columns) and out.dtype == kind and out.stride(1) == 1, "out is [T, heads * value width] in the type of q, unit inner stride")
         out_stride = out.stride(0)
-    if num_splits is None:
-        run = 1                                       # tokens of a sequence that share a problem
-        while weights is not None and run < max_q_len and run * 2 * G <= 16:
-            run *= 2
-        splits = budget_splits((T if run == 1 else n * -(-max_q_len // run)) * heads, keys, weights is None)
-    else:
-        splits = num_splits
+    k_ptr, v_ptr = kcache.data_ptr(), vcache.data_ptr()
+    fast = kind is torch.bfloat16 and (D | Dv) % 8 == 0 and D <= 128 and Dv <= 128 and bs % 16 == 0 and (k_ptr | v_ptr) % 16 == 0 and blocks * heads * bs < 2 ** 31
+    run = 1                                               # tokens of a sequence that share a problem
+    while fast and weights is not None and run < max_q_len and run * 2 * G <= 16:
+        run *= 2
+    problems = (T if run == 1 else n * -(-max_q_len // run)) * heads * -(-G // 16)
+    splits = budget_splits(problems, keys, weights is None, fast) if num_splits is None else num_splits
     _require(1 <= splits <= MAX_SPLITS, "1 to 64 splits")
-    lib = kernels()
-    nbytes = lib.swb_attn_budget_workspace(T, heads, G, Dv, splits, per * bs, weights is not None) if splits > 1 or weights is not None else 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None     # the call's own: two streams or graphs share none
+    lib, ws, nbytes = kernels(), None, 0
+    if weights is not None or not (splits == 1 or (fast and splits <= 8 and problems * splits <= 296)):      # else blocks finish their results, or clusters do
+        nbytes = lib.swb_attn_budget_workspace(T, heads, G, Dv, splits, per * bs, weights is not None)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)        # the call's own: two streams or graphs share none
     dims = _INTS[16](T, n, max_q_len, per, blocks, bs, heads, G, D, Dv, width, splits, kind == torch.float32, 0, 0, 0)
     strides = _LONGS[8](tok, head, out_stride, block_table.stride(0), w_seq, w_head, 0, 0)
-    check(lib.swb_attn_budget(dims, strides, q.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), block_table.data_ptr(), ptr(cu_q), kv_lens.data_ptr(),
+    check(lib.swb_attn_budget(dims, strides, q.data_ptr(), out.data_ptr(), k_ptr, v_ptr, block_table.data_ptr(), ptr(cu_q), kv_lens.data_ptr(),
                               ptr(pages), ptr(counts), ptr(weights), scale, softcap, ptr(ws), nbytes, stream), "swb_attn_budget")
     return out
 

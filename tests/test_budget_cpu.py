@@ -115,4 +115,5 @@ def test_splits():
     assert budget.budget_splits(8, 100000, True) == 37 and budget.budget_splits(8, 64, True) == 1 and budget.budget_splits(8, 65, False) == 2
     assert budget.budget_splits(8, 8000, False) == 8 and budget.budget_splits(64, 8000, True) == 4 and budget.budget_splits(1, 10 ** 6, True) == 64
     assert budget.budget_splits(400, 10 ** 6, True) == 1 and budget.budget_splits(400, 8192, False) == 7 and budget.budget_splits(10 ** 6, 10 ** 6, False) == 1
+    assert budget.budget_splits(64, 4000, True, False) == 18 and budget.budget_splits(8, 100, False, False) == 2 and budget.budget_splits(5000, 4000, False, False) == 1
     assert budget.budget_splits(0, 0, True) == 1 and budget.budget_splits(0, 0, False) == 1
