@@ -158,6 +158,22 @@ __global__ void __launch_bounds__(SUMMARY_WARPS * 32) page_summary_kernel(const 
   if (lane == 0) p.scales[at] = bad ? NAN : (float)(a / (127.0 * p.bs));
 }
 
+// codes * scales as 32-bit numbers, four at a time where rows allow.
+__global__ void __launch_bounds__(256) page_values_kernel(const int8_t* codes, const float* scales, float* out, long long n, int D, int four) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long step = (long long)gridDim.x * 256;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (four ? n / 4 : n); i += step) {
+    if (four) {
+      const char4 c = reinterpret_cast<const char4*>(codes)[i];
+      const float s = scales[n <= 0xffffffffll ? (uint32_t)i / (uint32_t)(D / 4) : i / (D / 4)];
+      reinterpret_cast<float4*>(out)[i] = make_float4(c.x * s, c.y * s, c.z * s, c.w * s);
+    } else {
+      out[i] = codes[i] * scales[i / D];
+    }
+  }
+}
+
 struct SelectParams {
   const void* q;
   long long q_stride_tok, q_stride_head;
@@ -229,6 +245,7 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 ? 4 : 3)
   int* hist = reinterpret_cast<int*>(select_smem) + team.id * SELECT_INTS;
   int8_t* qc = reinterpret_cast<int8_t*>(select_smem + TT * SELECT_INTS * 4);
   uint32_t* keys = reinterpret_cast<uint32_t*>(qc + TT * p.G * LD);
+  const int ldkeys = (p.max_blocks + 3) & ~3;
   // blocks that run together share what they read: the tokens of a prompt a head's codes, the heads of a decode step a page's memory
   const int runs = (p.uniform_q + TT - 1) / TT, all_runs = runs * p.num_seqs;
   const int share = CL ? p.share : 1, rank = CL ? blockIdx.x % share : 0, x = CL ? blockIdx.x / share : blockIdx.x;
@@ -347,7 +364,7 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 ? 4 : 3)
     if (i >= most) return 0u;
     const uint32_t k = float_key(there ? __fmul_rn((float)best, scale) : -INFINITY);
     if (CL) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(first_keys + 4u * i), "r"(k) : "memory");
-    else keys[tok * p.max_blocks + i] = k;
+    else keys[tok * ldkeys + i] = k;
     return k;
   };
   // the largest key of each token, where a thread keeps keys of several
@@ -468,9 +485,7 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 ? 4 : 3)
   }
   if (n <= width) return;                          // whole teams leave
   const int want = n - p.first - p.last;           // this token's candidates
-  const uint32_t* own = keys + team.id * p.max_blocks;
-  const auto key = [&](int i) { return own[i]; };
-  choose_in_order(team, key, want, p.top, s_largest[team.id], hist, [&](int place, int i) { out[p.first + place] = p.first + i; });
+  choose_in_order(team, keys + team.id * ldkeys, want, p.top, s_largest[team.id], hist, [&](int place, int i) { out[p.first + place] = p.first + i; });
 }
 
 // Tokens of a block: as many as the 16 columns of two products hold (4 at most), where sequences have them, as long as the scores leave room for two blocks on an SM.
@@ -483,7 +498,7 @@ int select_tokens(int uniform, int G, int pages) {
 
 template <int TT, int KS, bool FULL, int GP, bool CL = false>
 int launch_select(const SelectParams& p, cudaStream_t s) {
-  const size_t smem = TT * ((size_t)SELECT_INTS * 4 + (size_t)p.G * 32 * KS + 4 * (size_t)p.max_blocks);
+  const size_t smem = TT * ((size_t)SELECT_INTS * 4 + (size_t)p.G * 32 * KS + 4 * (size_t)((p.max_blocks + 3) & ~3));
   auto kernel = page_select_kernel<TT, KS, FULL, GP, CL>;
   if (smem > 47 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -546,8 +561,20 @@ int swb_page_summaries(const int* dims, const void* k, void* codes, void* scales
   return fp32 ? launch_kernel(page_summary_kernel<float, 8>, grid, block, 0, s, p) : launch_kernel(page_summary_kernel<bf16, 8>, grid, block, 0, s, p);
 }
 
+// out [rows, D] = codes [rows, D] * scales [rows].
+int swb_page_values(const void* codes, const void* scales, float* out, long long rows, int D, void* stream) {
+  using namespace swb;
+  if (rows <= 0) return 0;
+  if (D < 1 || !codes || !scales || !out) return -3;
+  const long long n = rows * D;
+  const int four = D % 4 == 0 && (reinterpret_cast<uintptr_t>(codes) & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const long long want = (n / (four ? 4 : 1) + 255) / 256, blocks = want < 8 * 148 ? want : 8 * 148;
+  return launch_kernel(page_values_kernel, dim3((unsigned)(blocks < 1 ? 1 : blocks)), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), reinterpret_cast<const int8_t*>(codes),
+                       reinterpret_cast<const float*>(scales), out, n, D, four);
+}
+
 // Bytes of shared memory that a selection over `pages` pages needs; above the limit of a block it is refused.
-long long swb_page_select_smem(int pages, int G, int D) { return 4ll * swb::SELECT_INTS + (long long)G * (D <= 128 ? 128 : 256) + 4ll * pages; }
+long long swb_page_select_smem(int pages, int G, int D) { return 4ll * swb::SELECT_INTS + (long long)G * (D <= 128 ? 128 : 256) + 4ll * ((pages + 3) & ~3); }
 
 // See SelectParams. dims: host int[14] = tokens, num_seqs, tokens of each sequence (with cu_q: at most), table width, blocks, block_size, Hkv, G, D, first,
 // top, last, fp32, 0.

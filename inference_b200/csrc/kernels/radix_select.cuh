@@ -190,17 +190,25 @@ struct LinearDigit {
   }
 };
 
-// The indexes of the `want` largest keys in ascending order, put(place, index), ties to the lowest index. largest: the largest key. Where a team has a thread for
-// each chosen key and for each in the border's bin, one pass gathers both and two counts put them into order. The caller clears the bins; the whole team calls it,
-// and the keys are written before it (it begins with a barrier).
-template <int SIZE, typename Key, typename Put>
-__device__ __forceinline__ void choose_in_order(const Team<SIZE>& team, const Key& key, int n, int want, uint32_t largest, int* hist, const Put& put) {
+// The indexes of the `want` largest of n keys in ascending order, put(place, index), ties to the lowest index. keys: shared memory of 16-byte alignment, read in fours (up to
+// three behind the last are read and not used); largest: the largest of them. Where a team has a thread for each chosen key and for each in the border's bin, one pass
+// gathers both and two counts put them into order. The caller clears the bins; the whole team calls it, and the keys are written before it (it begins with a barrier).
+template <int SIZE, typename Put>
+__device__ __forceinline__ void choose_in_order(const Team<SIZE>& team, const uint32_t* keys, int n, int want, uint32_t largest, int* hist, const Put& put) {
   int* totals = hist + SELECT_BINS;
   const LinearDigit digit(largest);
+  const auto each = [&](const auto& visit) {
+    for (int i = team.rank * 4; i < n; i += SIZE * 4) {
+      const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
+      visit(i, k.x);
+      if (i + 1 < n) visit(i + 1, k.y);
+      if (i + 2 < n) visit(i + 2, k.z);
+      if (i + 3 < n) visit(i + 3, k.w);
+    }
+  };
   team.sync();
   if (want <= SIZE) {
-#pragma unroll 4
-    for (int i = team.rank; i < n; i += SIZE) atomicAdd(&hist[digit(key(i))], 1);
+    each([&](int, uint32_t k) { atomicAdd(&hist[digit(k)], 1); });
     team.sync();
     find_bin(team, hist, want, totals);
     const uint32_t bin = (uint32_t)totals[32];
@@ -208,16 +216,16 @@ __device__ __forceinline__ void choose_in_order(const Team<SIZE>& team, const Ke
     if (m <= SIZE) {
       uint32_t* border = reinterpret_cast<uint32_t*>(hist);      // keys of the border's bin, their indexes, and what is chosen
       int *border_at = hist + SIZE, *chosen = hist + 2 * SIZE;
-#pragma unroll 4
-      for (int i = team.rank; i < n; i += SIZE) {
-        const uint32_t k = key(i), d = digit(k);
+      each([&](int i, uint32_t k) {
+        const uint32_t d = digit(k);
+        if (d < bin) return;
         if (d > bin) {
           chosen[atomicAdd(&totals[36], 1)] = i;
-        } else if (d == bin) {
+        } else {
           const int j = atomicAdd(&totals[35], 1);
           border[j] = k, border_at[j] = i;
         }
-      }
+      });
       team.sync();
       if (team.rank < m) {
         const uint32_t mine = border[team.rank];
@@ -230,9 +238,12 @@ __device__ __forceinline__ void choose_in_order(const Team<SIZE>& team, const Ke
       team.sync();
       if (team.rank < want) {
         const int at = chosen[team.rank];
-        int place = 0;
-#pragma unroll 4
-        for (int j = 0; j < want; ++j) place += chosen[j] < at;
+        int place = 0, j = 0;
+        for (; j + 4 <= want; j += 4) {
+          const int4 x = *reinterpret_cast<const int4*>(chosen + j);
+          place += (x.x < at) + (x.y < at) + (x.z < at) + (x.w < at);
+        }
+        for (; j < want; ++j) place += chosen[j] < at;
         put(place, at);
       }
       return;
@@ -240,8 +251,9 @@ __device__ __forceinline__ void choose_in_order(const Team<SIZE>& team, const Ke
     clear_bins(team, hist);
     team.sync();
   }
-  for (int i = team.rank; i < n; i += SIZE) count_key(hist, key(i));
+  each([&](int, uint32_t k) { count_key(hist, k); });
   team.sync();
+  const auto key = [&](int i) { return keys[i]; };
   const Threshold t = select_threshold(team, key, n, want, hist);
   const int seg = ((n + SIZE - 1) / SIZE) * 32, lo = min(team.warp() * seg, n), hi = min(lo + seg, n);
   const PairSums sums = sum_over_warps(team, count_run(key, t, lo, hi), reinterpret_cast<int2*>(hist));

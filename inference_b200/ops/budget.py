@@ -40,7 +40,12 @@ class PageSummaries:
 
     def values(self) -> torch.Tensor:
         """The mean keys that the summaries stand for, fp32 [blocks, kv heads, D]."""
-        return self.codes * self.scales[..., None]
+        codes, scales = self.codes, self.scales
+        stream = _place(codes, scales)
+        _check_summaries(codes, scales)
+        out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
+        check(kernels().swb_page_values(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), scales.numel(), codes.shape[2], stream), "swb_page_values")
+        return out
 
 
 @dataclass
@@ -84,6 +89,13 @@ def _check_cache(kcache: torch.Tensor, vcache: torch.Tensor | None = None) -> tu
     return blocks, heads, bs, D, other[3]
 
 
+def _check_summaries(codes: torch.Tensor, scales: torch.Tensor) -> tuple[int, int, int]:
+    shape = codes.shape
+    _require(len(shape) == 3 and codes.dtype == torch.int8 and codes.is_contiguous() and scales.dtype == torch.float32 and scales.shape == shape[:2]
+             and scales.is_contiguous() and shape[2] <= MAX_WIDTH, "summaries are contiguous int8 [blocks, kv heads, D] and fp32 [blocks, kv heads], at most 256 wide")
+    return shape
+
+
 def _check_step(table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor | None, max_q_len: int, tokens: int) -> tuple[int, int]:
     """Number of sequences and width of the table. tokens < 0: not known."""
     lens, rows = kv_lens.shape, table.shape
@@ -114,8 +126,7 @@ def summarize_pages(kcache: torch.Tensor, block_table: torch.Tensor, kv_lens: to
     stream = _place(kcache, block_table, kv_lens, codes, scales, cu_q)
     blocks, heads, bs, D, _ = _check_cache(kcache)
     n, per = _check_step(block_table, kv_lens, cu_q, max_q_len, -1)
-    _require(codes.dtype == torch.int8 and codes.shape == (blocks, heads, D) and codes.is_contiguous() and scales.dtype == torch.float32
-             and scales.shape == (blocks, heads) and scales.is_contiguous(), "summaries belong to these pages: int8 [blocks, kv heads, D], fp32 [blocks, kv heads]")
+    _require(_check_summaries(codes, scales) == (blocks, heads, D), "summaries belong to these pages: [blocks, kv heads, D]")
     dims = _INTS[9](n, max_q_len, per, blocks, bs, heads, D, kcache.dtype == torch.float32, 0)
     check(kernels().swb_page_summaries(dims, kcache.data_ptr(), codes.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), ptr(cu_q),
                                        kv_lens.data_ptr(), stream), "swb_page_summaries")
@@ -130,10 +141,7 @@ def select_pages(q: torch.Tensor, summaries: PageSummaries, block_table: torch.T
     group of the codes' dot product. A token whose queries are not all finite, or all zero, finds every page alike."""
     codes, scales = summaries.codes, summaries.scales
     stream = _place(q, codes, scales, block_table, kv_lens, cu_q)
-    shape = codes.shape
-    _require(len(shape) == 3 and codes.dtype == torch.int8 and codes.is_contiguous() and scales.dtype == torch.float32 and scales.shape == shape[:2]
-             and scales.is_contiguous() and shape[2] <= MAX_WIDTH, "summaries are int8 [blocks, kv heads, D] and fp32 [blocks, kv heads]")
-    blocks, heads, D = shape
+    blocks, heads, D = _check_summaries(codes, scales)
     _require(q.dtype in _KINDS, "q is bf16 or fp32")
     T, G, tok, head = _check_rows(q, heads, D)
     n, per = _check_step(block_table, kv_lens, cu_q, max_q_len, T)

@@ -274,6 +274,7 @@ def test_page_summaries(kv, D, bs, kind):
                     code, scale = _summary(c.k[at, h].cpu())
                     want_c[at, h], want_s[at, h] = code, scale
     ops.summarize_pages(c.k, c.table, c.kv_lens, sums, cu_q=cu, max_q_len=max(new))
+    assert torch.equal(sums.values().nan_to_num(nan=-7.0), (sums.codes * sums.scales[..., None]).nan_to_num(nan=-7.0))
     assert torch.equal(sums.codes.cpu(), want_c) and torch.equal(sums.scales.cpu().nan_to_num(nan=-7.0), want_s.nan_to_num(nan=-7.0))
 
 
