@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
     const int q0 = p.cu_q ? p.cu_q[tok.seq] : tok.seq * p.uniform_q, q1 = p.cu_q ? p.cu_q[tok.seq + 1] : q0 + p.uniform_q;
     t = q0 + t % runs * p.run;
     tokens = min(p.run, min(q1, p.tokens) - t);
-    if (tokens <= 0) return;
+    if (tokens <= 0 || t < 0) return;
     tok.seen = max(min(p.kv_lens[tok.seq] - (q1 - t - tokens), p.max_blocks * p.bs), 0);            // of the last token
   }
   const int rows = heads * tokens;                  // row r: token r / heads, head r % heads
@@ -686,7 +686,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_budget_finish_kernel(const 
   const int blocks = (int)((p.capacity + RUN - 1) / RUN), i = blockIdx.x - join_blocks;
   const int h = i / blocks % p.Hkv, seq = i / blocks / p.Hkv;
   const long long j0 = (long long)(i % blocks) * RUN + tid;
-  const int q0 = p.cu_q ? p.cu_q[seq] : seq * p.uniform_q, q1 = min(p.cu_q ? p.cu_q[seq + 1] : q0 + p.uniform_q, p.tokens);
+  const int q0 = max(p.cu_q ? p.cu_q[seq] : seq * p.uniform_q, 0), q1 = p.cu_q ? p.cu_q[seq + 1] : q0 + p.uniform_q;
+  const int q_end = min(min(q1, p.tokens), q0 + p.uniform_q);      // tokens whose scores are there
   const int total = p.kv_lens[seq], len = min(total, p.max_blocks * p.bs);
   if (j0 - tid >= len) return;
   float* w = p.weights + seq * p.w_seq + h * p.w_head;
@@ -694,8 +695,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_budget_finish_kernel(const 
 #pragma unroll
   for (int k = 0; k < KEYS; ++k) sum[k] = 0.f, old[k] = j0 + k * JOIN_THREADS < len ? w[j0 + k * JOIN_THREADS] : 0.f;
   const int batch = MAX_GROUP / p.G;             // tokens whose rows a block has room for
-  for (int t0 = q0; t0 < q1; t0 += batch) {
-    const int pairs = min(batch, q1 - t0) * p.G;
+  for (int t0 = q0; t0 < q_end; t0 += batch) {
+    const int pairs = min(batch, q_end - t0) * p.G;
     __syncthreads();
     if (tid < pairs) {                           // MAX_GROUP <= JOIN_THREADS: a row to a thread
       const int tok = tid / p.G;

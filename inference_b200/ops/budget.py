@@ -10,7 +10,8 @@ Two ways to spend less than the whole cache on a new token, both beside `paged_a
 Caches are one layer's pages [blocks, kv heads, block_size, width] with the block tables of `PagedSequence`. bf16, or fp32 in the 32-bit mode; widths up to 256.
 Calls run on the current stream, take no host reads and can be captured into graphs; buffers that a call fills (summaries, weights, positions, the cache) belong
 to the caller. Steps are described as in `paged_attention`: kv_lens int32 [num_seqs] counts a sequence's tokens with the new ones, cu_q int32 [num_seqs + 1]
-are the new tokens' ranges, or None where every sequence has max_q_len of them; rows behind the last range are left as they were."""
+are the new tokens' ranges within the rows of q and max_q_len bounds a sequence's number (None: every sequence has max_q_len of them); rows behind the last range
+are left as they were. Lengths beyond a table's pages count as the table's end, and pages whose number is not in the cache are passed over."""
 from __future__ import annotations
 
 import struct
@@ -257,7 +258,8 @@ def evict_tokens(kcache: torch.Tensor, vcache: torch.Tensor, block_table: torch.
     sequence's next token), and of the others those of largest weight (fp32 [num_seqs, kv heads, N], as `tracked_attention` adds them up; ties: the lowest index). Entries that stay
     and lie behind `keep` move in order into the holes in front of it: their rows of both caches, weight and position. positions int32 [num_seqs, kv heads, N]: -1 for
     entries without a record, which stand in order in front of the next position (all of them before the first call); the call records those it keeps. Weights behind `keep` become 0, positions -1.
-    Everything is done in place. Pages must not be shared with a sequence that is not to lose tokens, nor between sequences of the call (`PagedSequence.unshare`)."""
+    Everything is done in place. Pages must not be
+    shared with a sequence that is not to lose tokens, nor between sequences of the call."""
     stream = _place(kcache, vcache, block_table, kv_lens, weights, positions, next_positions)
     blocks, heads, bs, D, Dv = _check_cache(kcache, vcache)
     n, per = _check_step(block_table, kv_lens, None, 1, -1)

@@ -608,3 +608,101 @@ def test_results_do_not_change_from_call_to_call():
         got = [ops.tracked_attention(c.q, c.k, c.v, c.table, c.kv_lens, weights, scale=0.1, **c.step), weights]
         first = first or got
         assert all(torch.equal(x, y) for x, y in zip(got, first))
+
+
+@pytest.mark.parametrize("heads,kv", [(8, 2), (14, 2), (24, 2)])
+def test_streams_beside_each_other(heads, kv):
+    """The same calls on two streams at once, each with tensors of its own, give what they give one after the other."""
+    ops = _ops()
+    caches = [Cache([900, 300 + 40 * i], [3, 3], heads=heads, kv_heads=kv, seed=i) for i in range(2)]
+
+    def work(c):
+        sums = ops.PageSummaries.empty(c.k)
+        ops.summarize_pages(c.k, c.table, c.kv_lens, sums, cu_q=None, max_q_len=900)
+        sel = ops.select_pages(c.q, sums, c.table, c.kv_lens, block_size=16, top=5, **c.step)
+        weights = torch.zeros(2, kv, c.per * 16, device=CUDA)
+        return [sums.values().nan_to_num(), sel.pages, sel.counts, ops.selected_attention(c.q, c.k, c.v, c.table, c.kv_lens, sel, scale=0.1, **c.step),
+                ops.tracked_attention(c.q, c.k, c.v, c.table, c.kv_lens, weights, scale=0.1, **c.step), weights]
+
+    want = [work(c) for c in caches]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in caches]
+    for _ in range(10):
+        got = []
+        for c, s in zip(caches, streams):
+            with torch.cuda.stream(s):
+                got.append(work(c))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for a, b in zip(got, want) for x, y in zip(a, b))
+
+
+def test_nothing_to_do():
+    """No sequences, no new tokens, empty sequences."""
+    ops = _ops()
+    c = Cache([0, 40], [1, 1])
+    none = torch.zeros(0, 8, 128, dtype=torch.bfloat16, device=CUDA)
+    empty = {"cu_q": torch.zeros(3, dtype=torch.int32, device=CUDA), "max_q_len": 4}
+    weights = torch.zeros(2, 2, c.per * 16, device=CUDA)
+    sums = ops.PageSummaries.empty(c.k)
+    ops.summarize_pages(c.k, c.table, c.kv_lens, sums, **empty)
+    assert sums.scales.eq(0).all()
+    sel = ops.select_pages(none, sums, c.table, c.kv_lens, block_size=16, top=2, **empty)
+    assert sel.pages.shape == (0, 2, 7)
+    assert ops.selected_attention(none, c.k, c.v, c.table, c.kv_lens, sel, scale=1.0, **empty).shape == (0, 1024)
+    assert ops.tracked_attention(none, c.k, c.v, c.table, c.kv_lens, weights, scale=1.0, **empty).shape == (0, 1024) and weights.eq(0).all()
+    lens = torch.zeros(0, dtype=torch.int32, device=CUDA)
+    assert ops.tracked_attention(none, c.k, c.v, c.table[:0], lens, weights[:0], scale=1.0, cu_q=None, max_q_len=1).shape == (0, 1024)
+    assert ops.evict_tokens(c.k, c.v, c.table[:0], lens, weights[:0], weights[:0].int(), lens, keep=4, recent=1).shape == (0,)
+    pages = torch.full((2, 2, 3), -1, dtype=torch.int32, device=CUDA)
+    out = ops.selected_attention(c.q, c.k, c.v, c.table, c.kv_lens, ops.PageSelection(pages, torch.zeros(2, 2, dtype=torch.int32, device=CUDA)), scale=1.0, **c.step)
+    assert out.eq(0).all()
+
+
+def test_lengths_behind_the_table_and_below_zero():
+    """A length that the table has no pages for counts as the table's end; one below zero as none. New tokens that max_q_len does not cover are the caller's mistake, but nothing
+    is read or written out of place for them."""
+    ops = _ops()
+    c = Cache([64, 64], [1, 1], extra_pages=0)
+    kv = torch.tensor([1000, -5], dtype=torch.int32, device=CUDA)
+    weights = torch.zeros(2, 2, 64, device=CUDA)
+    out = ops.tracked_attention(c.q, c.k, c.v, c.table, kv, weights, scale=0.1, **c.step)
+    c.lens = [64, 0]
+    _check_attention(c, out, lambda t, b, h, seen: range(seen), 0.1, weights=weights, before=torch.zeros_like(weights))
+    sums = ops.PageSummaries.empty(c.k)
+    ops.summarize_pages(c.k, c.table, kv, sums, cu_q=None, max_q_len=2000)
+    sel = ops.select_pages(c.q, sums, c.table, kv, block_size=16, top=1, first=1, last=1, **c.step)
+    assert sel.counts.tolist() == [[3, 3], [0, 0]]
+    positions = torch.full((2, 2, 64), -1, dtype=torch.int32, device=CUDA)
+    assert ops.evict_tokens(c.k, c.v, c.table, kv, weights, positions, kv.clone(), keep=50, recent=0).tolist() == [50, -5]
+    assert (positions[0, :, :50] >= 0).all() and (positions[1] == -1).all()
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+def test_a_cache_behind_two_to_the_31_numbers(kind):
+    """Pages whose first number lies behind 2^31: addresses are 64-bit."""
+    ops = _ops()
+    D, bs, kv = 128, 16, 2
+    blocks = 2 ** 31 // (kv * bs * D) + 40
+    k = torch.zeros(blocks, kv, bs, D, dtype=kind, device=CUDA)
+    v = torch.zeros_like(k)
+    g = _gen(8)
+    tail = torch.arange(blocks - 20, blocks, device=CUDA)
+    k[tail] = torch.randn(20, kv, bs, D, device=CUDA, generator=g).to(kind)
+    v[tail] = torch.randn(20, kv, bs, D, device=CUDA, generator=g).to(kind)
+    c = Cache([300], [1], heads=8, kv_heads=kv, kind=kind, extra_pages=1)
+    c.k, c.v, c.blocks, c.table = k, v, blocks, tail[torch.randperm(20, device=CUDA, generator=g)].to(torch.int32)[None]
+    weights = torch.zeros(1, kv, 320, device=CUDA)
+    out = ops.tracked_attention(c.q, k, v, c.table, c.kv_lens, weights, scale=0.1, **c.step)
+    _check_attention(c, out, lambda t, b, h, seen: range(seen), 0.1, weights=weights, before=torch.zeros_like(weights))
+    sums = ops.PageSummaries.empty(k)
+    ops.summarize_pages(k, c.table, c.kv_lens, sums, cu_q=None, max_q_len=300)
+    for page in (0, 17):
+        code, scale = _summary(k[c.table[0, page].long(), 1].cpu())
+        assert torch.equal(sums.codes[c.table[0, page].long(), 1].cpu(), code) and float(sums.scales[c.table[0, page].long(), 1]) == scale
+    sel = ops.select_pages(c.q, sums, c.table, c.kv_lens, block_size=bs, top=4, **c.step)
+    assert sel.pages[0, 0].tolist() == _select(c, sums, 0, 0, 0, 300, 4, 1, 4)
+    rows = c.row("k", 0, range(300))
+    positions = torch.full((1, kv, 320), -1, dtype=torch.int32, device=CUDA)
+    ops.evict_tokens(k, v, c.table, c.kv_lens, weights, positions, c.kv_lens.clone(), keep=100, recent=10)
+    for h in range(kv):
+        assert torch.equal(c.row("k", 0, range(100))[h], rows[h, positions[0, h, :100].long()])
