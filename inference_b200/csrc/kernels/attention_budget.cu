@@ -48,7 +48,7 @@ struct BudgetParams {
   int cluster;               // the splits of a problem are a cluster
   int weigh_here;            // blocks add their weights themselves
   float* part_o;             // [tokens, Hq, num_splits, Dv], null where blocks or clusters finish the output
-  float* part_ml;            // [tokens, Hq, num_splits, 2]: maximum (log2 units) and sum; null where nobody reads them
+  float* part_ml;            // [tokens, Hq, num_splits, 2]: maximum (log2 units) and sum, of a cluster's problem [tokens, Hq, 2]; null where nobody reads them
   float* scores;             // [tokens, Hq, capacity] in log2 units, where weights are kept
   long long capacity;
   float* weights;            // [num_seqs, Hkv, .], inner stride 1
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
     if (d == 0) {
       sPart[r * 2] = M, sPart[r * 2 + 1] = L;
       sAll[r * 2] = base, sAll[r * 2 + 1] = L == 0.f ? 0.f : 1.f / L;
-      if (p.part_ml) *reinterpret_cast<float2*>(p.part_ml + part_at(p, token_at(r), head_at(r), split) * 2) = make_float2(M, L);
+      if (p.part_ml && !p.cluster) *reinterpret_cast<float2*>(p.part_ml + part_at(p, token_at(r), head_at(r), split) * 2) = make_float2(M, L);
     }
   }
   if (parts) return;
@@ -560,6 +560,7 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
       for (int s = 0; s < MAX_CLUSTER; ++s) L = fmaf(m_of[s] = exp2f(m_of[s] - base), l_of[s], L);
       const float inv = L == 0.f ? 0.f : 1.f / L;
       sAll[tid * 2] = base, sAll[tid * 2 + 1] = inv;
+      if (p.part_ml && split == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)token_at(tid) * p.Hkv * p.G + head_at(tid)) * 2) = make_float2(M, L);
 #pragma unroll
       for (int s = 0; s < MAX_CLUSTER; ++s) sFactor[tid * MAX_CLUSTER + s] = m_of[s] * inv;
     }
@@ -658,8 +659,8 @@ __device__ __forceinline__ void split_factors(const float* ml, int S, int lane, 
   if (lane + 32 < S) factor[lane + 32] = e1 * inv;
 }
 
-// The first `join_blocks` blocks join the parts of one row each; the others weigh a run of keys of one (sequence, key/value head) each. KEYS of a thread: four for steps
-// of one token, whose few rows leave room for no more loads otherwise, one for several tokens, whose rows are many and blocks few.
+// The first `join_blocks` blocks join the parts of one row each; the others weigh a run of keys of one (sequence, key/value head) each. KEYS of a thread: four for
+// steps of one token, whose rows are few and blocks many, one for several tokens, whose rows are many and blocks few.
 template <typename E, int KEYS>
 __global__ void __launch_bounds__(JOIN_THREADS) attn_budget_finish_kernel(const BudgetParams p, int join_blocks) {
   pdl_launch_dependents();
@@ -720,7 +721,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_budget_finish_kernel(const 
       s_seen[tid] = min(total - (q1 - 1 - t0 - tok), len);
     }
     __syncthreads();
-    constexpr int U = 16 / KEYS;                 // rows whose scores are on their way together
+    constexpr int U = KEYS == 1 ? 32 : 4;        // rows whose scores are on their way together
     for (int r0 = 0; r0 < pairs; r0 += U) {
       float x[U][KEYS];
 #pragma unroll
@@ -823,6 +824,7 @@ int swb_attn_budget(const int* dims, const long long* strides, const void* q, vo
   const int join_blocks = join ? p.tokens * p.Hkv * p.G : 0, run = JOIN_THREADS * (p.uniform_q == 1 ? 4 : 1);
   const long long blocks = join_blocks + (weigh ? (p.capacity + run - 1) / run * p.Hkv * p.num_seqs : 0);
   if (blocks > INT_MAX) return -3;
+  if (p.cluster) p.num_splits = 1;               // the cluster left one pair a row
   auto kernel = fp32 ? (p.uniform_q == 1 ? attn_budget_finish_kernel<float, 4> : attn_budget_finish_kernel<float, 1>)
                      : (p.uniform_q == 1 ? attn_budget_finish_kernel<bf16, 4> : attn_budget_finish_kernel<bf16, 1>);
   return launch_kernel(kernel, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, s, p, join_blocks);
