@@ -240,7 +240,7 @@ constexpr int FW = 4;                               // warps
 constexpr int HALF_BYTES = 2048, GROUP_BYTES = 4 * HALF_BYTES;      // 16 rows of 64 columns; K low, K high, V low, V high
 constexpr int SQ_BYTES = ROWS * 256, LDO = 132;
 constexpr int fast_smem_bytes(int FS) { return 1024 + FW * FS * GROUP_BYTES + SQ_BYTES + 256; }
-constexpr int FINISH_FLOATS = FW * ROWS * LDO + FW * ROWS * 2 + ROWS * 2 + ROWS * 2 + ROWS * MAX_CLUSTER;
+constexpr int FINISH_FLOATS = FW * ROWS * LDO + FW * ROWS * 2 + ROWS * 2 + ROWS * 2 + ROWS * MAX_CLUSTER + ROWS * FW;
 static_assert(FINISH_FLOATS * 4 <= FW * 2 * GROUP_BYTES, "the warps' results fit where the ring was");
 
 // 16-byte chunk c (0..15) of row r (0..15) of a K or V group: two boxes of 64 columns with the 128-byte swizzle
@@ -516,29 +516,33 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
   float* sPart = sM + FW * ROWS * 2;                // [ROWS][2]: the block's maximum and sum
   float* sAll = sPart + ROWS * 2;                   // [ROWS][2]: the problem's maximum, 1 / sum
   float* sFactor = sAll + ROWS * 2;                 // [ROWS][MAX_CLUSTER]
+  float* sWarps = sFactor + ROWS * MAX_CLUSTER;     // [ROWS][FW]
   const auto token_at = [&](int r) { return t + r / heads; };
   const auto head_at = [&](int r) { return h * p.G + g0 + r % heads; };
   const bool parts = p.part_o != nullptr;
   bf16* out = reinterpret_cast<bf16*>(p.out);
-  for (int i = tid; i < rows * p.Dv; i += FW * 32) {
-    const int r = i / p.Dv, d = i % p.Dv;
-    float M = -INFINITY, L = 0.f, x = 0.f;
+  if (tid < rows) {                                 // a row's warps, weighed by their distance to the common maximum
+    float m_of[FW], M = -INFINITY, L = 0.f;
 #pragma unroll
-    for (int w = 0; w < FW; ++w) M = fmaxf(M, sM[(w * ROWS + r) * 2]);
+    for (int w = 0; w < FW; ++w) M = fmaxf(M, m_of[w] = sM[(w * ROWS + tid) * 2]);
     const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
-    for (int w = 0; w < FW; ++w) {
-      const float e = exp2f(sM[(w * ROWS + r) * 2] - base);
-      L = fmaf(e, sM[(w * ROWS + r) * 2 + 1], L);
-      x = fmaf(e, sO[(w * ROWS + r) * LDO + d], x);
-    }
-    if (parts) p.part_o[part_at(p, token_at(r), head_at(r), split) * p.Dv + d] = x;
-    else if (S == 1) out[token_at(r) * p.out_stride_tok + (size_t)head_at(r) * p.Dv + d] = __float2bfloat16(L == 0.f ? 0.f : x / L);
-    else sO[r * LDO + d] = x;                       // warp 0's, which this thread alone reads
-    if (d == 0) {
-      sPart[r * 2] = M, sPart[r * 2 + 1] = L;
-      sAll[r * 2] = base, sAll[r * 2 + 1] = L == 0.f ? 0.f : 1.f / L;
-      if (p.part_ml && !p.cluster) *reinterpret_cast<float2*>(p.part_ml + part_at(p, token_at(r), head_at(r), split) * 2) = make_float2(M, L);
+    for (int w = 0; w < FW; ++w) L = fmaf(m_of[w] = exp2f(m_of[w] - base), sM[(w * ROWS + tid) * 2 + 1], L);
+    const float inv = L == 0.f ? 0.f : 1.f / L, f = !parts && S == 1 ? inv : 1.f;
+    *reinterpret_cast<float4*>(sWarps + tid * 4) = make_float4(m_of[0] * f, m_of[1] * f, m_of[2] * f, m_of[3] * f);
+    sPart[tid * 2] = M, sPart[tid * 2 + 1] = L;
+    sAll[tid * 2] = base, sAll[tid * 2 + 1] = inv;
+    if (p.part_ml && !p.cluster) *reinterpret_cast<float2*>(p.part_ml + part_at(p, token_at(tid), head_at(tid), split) * 2) = make_float2(M, L);
+  }
+  __syncthreads();
+  for (int r = 0; r < rows; ++r) {
+    const float4 f = *reinterpret_cast<const float4*>(sWarps + r * 4);
+    for (int d = tid; d < p.Dv; d += FW * 32) {
+      float* o4 = sO + r * LDO + d;
+      const float x = fmaf(f.x, o4[0], f.y * o4[ROWS * LDO]) + fmaf(f.z, o4[2 * ROWS * LDO], f.w * o4[3 * ROWS * LDO]);
+      if (parts) p.part_o[part_at(p, token_at(r), head_at(r), split) * p.Dv + d] = x;
+      else if (S == 1) out[token_at(r) * p.out_stride_tok + (size_t)head_at(r) * p.Dv + d] = __float2bfloat16(x);
+      else o4[0] = x;                               // warp 0's, which this thread alone reads
     }
   }
   if (parts) return;
@@ -565,17 +569,16 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
       for (int s = 0; s < MAX_CLUSTER; ++s) sFactor[tid * MAX_CLUSTER + s] = m_of[s] * inv;
     }
     __syncthreads();
-    for (int i = tid; i < (rows - split + S - 1) / S * p.Dv; i += FW * 32) {        // rows split, split + S, ...
-      const int r = split + i / p.Dv * S, d = i % p.Dv;
-      const uint32_t at = smem_u32(sO + r * LDO + d);
-      float x = 0.f;
+    for (int r = split; r < rows; r += S)
+      for (int d = tid; d < p.Dv; d += FW * 32) {
+        const uint32_t at = smem_u32(sO + r * LDO + d);
+        float o_of[MAX_CLUSTER], x = 0.f;
 #pragma unroll
-      for (int s = 0; s < MAX_CLUSTER; ++s)
-        if (s < S) x = fmaf(sFactor[r * MAX_CLUSTER + s], ld_cluster(in_cluster(at, s)), x);
-      out[token_at(r) * p.out_stride_tok + (size_t)head_at(r) * p.Dv + d] = __float2bfloat16(x);
-    }
-  } else if (p.weigh_here) {
-    __syncthreads();
+        for (int s = 0; s < MAX_CLUSTER; ++s) o_of[s] = s < S ? ld_cluster(in_cluster(at, s)) : 0.f;
+#pragma unroll
+        for (int s = 0; s < MAX_CLUSTER; ++s) x = fmaf(sFactor[r * MAX_CLUSTER + s], o_of[s], x);
+        out[token_at(r) * p.out_stride_tok + (size_t)head_at(r) * p.Dv + d] = __float2bfloat16(x);
+      }
   }
   if (p.weigh_here) {                               // one token: row r is head r, and the block's scores are its own writes
     float* w = p.weights + tok.seq * p.w_seq + h * p.w_head;
