@@ -130,12 +130,9 @@ def _declare_kernels(lib: ctypes.CDLL) -> None:
     sig("swb_head_mix", [c_void_p, c_ll, c_void_p, c_void_p, c_ll, c_void_p, c_ll, c_int, c_int, c_int, c_int, c_int, c_void_p])
     sig("swb_page_summaries", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_void_p, c_void_p])
     sig("swb_page_values", [c_void_p, c_void_p, c_void_p, c_ll, c_int, c_void_p])
-    sig("swb_page_select_smem", [c_int, c_int, c_int], c_ll)
     sig("swb_page_select", [c_void_p, c_void_p, c_ll, c_ll, c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p])
-    sig("swb_attn_budget_workspace", [c_int, c_int, c_int, c_int, c_int, c_ll, c_int], c_ll)
     sig("swb_attn_budget", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                             c_float, c_float, c_void_p, c_ll, c_void_p])
-    sig("swb_evict_moves", [c_int, c_int, c_int, c_int], c_ll)
     sig("swb_evict", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p])
     sig("swb_attn_simple", [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_int, c_int, c_void_p, c_void_p,
                             c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_int, c_float,

@@ -775,15 +775,10 @@ int heads_in_tiles(int G) { return (G + ROWS - 1) / ROWS; }
 
 extern "C" {
 
-// Bytes of the workspace: the parts of the rows, and the scores where weights are kept (scores = 1; capacity: keys of the widest table row).
-long long swb_attn_budget_workspace(int tokens, int Hkv, int G, int Dv, int num_splits, long long capacity, int scores) {
-  const long long rows = (long long)tokens * Hkv * G;
-  return rows * 4 * (num_splits * (Dv + 2) + (scores ? capacity : 0)) + 16;
-}
-
 // See BudgetParams. dims: host int[16] = tokens, num_seqs, tokens of each sequence (with cu_q: at most), table width, blocks, block_size, Hkv, G, D, Dv,
 // width of the page lists, splits, fp32, 0, 0, 0; strides: host long long[8] = q token and head, out token, table, weights sequence and head, 0, 0.
-// pages and counts, or weights, or neither.
+// pages and counts, or weights, or neither. workspace (16-byte aligned), where results are joined by a second launch or weights are kept: 4 tokens Hq (splits (Dv + 2) +
+// keys of the table, with weights) + 16 bytes.
 int swb_attn_budget(const int* dims, const long long* strides, const void* q, void* out, const void* k, const void* v, const int* table, const int* cu_q,
                     const int* kv_lens, const int* pages, const int* counts, float* weights, float scale, float softcap, void* workspace, long long workspace_bytes,
                     void* stream) {
@@ -813,9 +808,10 @@ int swb_attn_budget(const int* dims, const long long* strides, const void* q, vo
   p.weigh_here = weights && fast && p.uniform_q == 1 && p.head_tiles == 1 && (p.cluster || p.num_splits == 1);
   const bool join = p.num_splits > 1 && !p.cluster, weigh = weights && !p.weigh_here;
   if (join || weights) {
-    if (swb_attn_budget_workspace(p.tokens, p.Hkv, p.G, p.Dv, p.num_splits, p.capacity, weights != nullptr) > workspace_bytes || !workspace) return -3;
+    // workspace: the parts of the rows, and the scores where weights are kept, in front of them
     const size_t rows = (size_t)p.tokens * p.Hkv * p.G, parts = rows * p.num_splits;
-    float* ws = reinterpret_cast<float*>(workspace);          // scores in front: rows of a multiple of 16 keys stay 64-byte aligned
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || (long long)(4 * (parts * (p.Dv + 2) + (weights ? rows * p.capacity : 0)) + 16) > workspace_bytes) return -3;
+    float* ws = reinterpret_cast<float*>(workspace);
     if (weights) p.scores = ws, ws += rows * p.capacity;
     ws += (4 - (rows * p.capacity * (weights != nullptr)) % 4) % 4;
     if (join || weigh) p.part_ml = ws;

@@ -258,15 +258,10 @@ __global__ void __launch_bounds__(EVICT_THREADS, 2) evict_kernel(const EvictPara
 
 extern "C" {
 
-// Ints of the list of moves: per (sequence, head) two indexes for each of the entries that can move.
-long long swb_evict_moves(int num_seqs, int Hkv, int capacity, int keep) {
-  const long long most = capacity > keep ? (capacity - keep < keep ? capacity - keep : keep) : 0;
-  return (long long)num_seqs * Hkv * 2 * most;
-}
-
 // See EvictParams. dims: host int[11] = num_seqs, Hkv, table width, blocks, block_size, k row bytes, v row bytes, capacity, keep, recent, first;
-// strides: host long long[4] = weights sequence and head, positions sequence and head. moves: swb_evict_moves ints.
-int swb_evict(const int* dims, const long long* strides, void* k, void* v, const int* table, long long table_stride, const int* kv_lens, int* new_lens, const int* next,
+// sizes: host long long[5] = strides of weights (sequence and head) and positions, ints that `moves` has room for: two for each of the entries that can move, min(keep,
+// capacity - keep), per (sequence, head).
+int swb_evict(const int* dims, const long long* sizes, void* k, void* v, const int* table, long long table_stride, const int* kv_lens, int* new_lens, const int* next,
               float* weights, int* positions, int* moves, void* stream) {
   using namespace swb;
   const int seqs = dims[0], Hkv = dims[1], max_blocks = dims[2], blocks = dims[3], bs = dims[4], kb = dims[5], vb = dims[6], capacity = dims[7];
@@ -274,10 +269,10 @@ int swb_evict(const int* dims, const long long* strides, void* k, void* v, const
   if (seqs <= 0) return 0;
   const int most = capacity > keep ? (capacity - keep < keep ? capacity - keep : keep) : 0;
   if (seqs > 65535 || Hkv < 1 || Hkv > 65535 || bs < 1 || kb < 2 || vb < 2 || ((kb | vb) & 1) || keep < 1 || recent < 0 || first < 0 || first > keep - recent || blocks < 1 ||
-      max_blocks < 1 || (long long)max_blocks * bs > INT_MAX || !k || !v || !table || !kv_lens || !new_lens || !next || !weights || !positions || (most && !moves))
+      max_blocks < 1 || (long long)max_blocks * bs > INT_MAX || !k || !v || !table || !kv_lens || !new_lens || !next || !weights || !positions || (most && !moves) || sizes[4] < 2ll * seqs * Hkv * most)
     return -3;
   const EvictParams p{reinterpret_cast<char*>(k), reinterpret_cast<char*>(v), kb, vb, table, table_stride, max_blocks, blocks, bs, Hkv, kv_lens, new_lens, next, weights,
-                      strides[0], strides[1], positions, strides[2], strides[3], capacity, keep, recent, first, moves, most};
+                      sizes[0], sizes[1], positions, sizes[2], sizes[3], capacity, keep, recent, first, moves, most};
   // a block for every 2048 entries where that fills the chip no further than one round
   int share = 1;
   while (share < EVICT_CLUSTER && share * 2048 < capacity && (long long)share * 2 * Hkv * seqs <= 2 * 148) share *= 2;

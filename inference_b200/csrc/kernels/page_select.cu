@@ -220,15 +220,17 @@ __device__ __forceinline__ float load_query(const SelectParams& p, long long at)
 
 // rint(127 x / a), |x| <= a. Where both are bf16, 127 x has 15 bits and the quotient, a fraction over a's 8 bits and powers of two, is either a
 // half exactly or further from one than 2^-16 of itself: its rounding to 32 bits moves nothing across. Other numbers are divided in 64 bits.
+// (Near the end of the 32-bit range both are made smaller first, by a power of two.)
 __device__ __forceinline__ int8_t query_code(float x, float a, bool fp32) {
-  return fp32 ? (int8_t)(int)rint(127.0 * (double)x / (double)a) : (int8_t)(int)rintf(__fdiv_rn(127.f * x, a));
+  if (fp32) return (int8_t)(int)rint(127.0 * (double)x / (double)a);
+  const float s = a > 0x1p100f ? 0x1p-64f : 1.f;
+  return (int8_t)(int)rintf(__fdiv_rn(127.f * (x * s), a * s));
 }
 
 // A block per (run of TT tokens of a sequence, head). The dot products are 8-bit matrix products: 16 rows are pages, 8 columns the tokens' query heads (a token's heads
 // are filled up to a power of two, with copies of its first, which change no maximum; GP is that power where it is known), so that a head's neighbours are a thread's own or a shuffle away and
-// every thread ends with one page's score for one token. A page's row is fetched 16 codes at a time (a load of a warp then touches eight lines; with 8
-// codes sixteen loads touched each line four times, and the look-ups in the cache's tags bound the kernel): the lane of page g and quarter t holds columns 64 j + 16 t and on,
-// for two steps, and the queries' codes are read in the same order, so the order of the columns within a step is another than the instruction's and the sum the same.
+// every thread ends with one page's score for one token. A page's row is fetched 16 codes at a time (8 at a time took 8 % longer
+// over a prompt): the lane of page g and quarter t holds columns 64 j + 16 t and on, for two steps, and the queries' codes are read in the same order, so the order of the columns within a step is another than the instruction's and the sum the same.
 // Then the tokens are shared out among teams of warps, each of which chooses among its token's scores.
 // CL: p.share blocks, a cluster, score a part of the pages each into the first one's memory, and that one chooses (few problems over long caches).
 // Shared memory: the teams' histograms, codes of the queries [TT, G, 32 KS], keys [TT, pages].
@@ -573,9 +575,6 @@ int swb_page_values(const void* codes, const void* scales, float* out, long long
                        reinterpret_cast<const float*>(scales), out, n, D, four);
 }
 
-// Bytes of shared memory that a selection over `pages` pages needs; above the limit of a block it is refused.
-long long swb_page_select_smem(int pages, int G, int D) { return 4ll * swb::SELECT_INTS + (long long)G * (D <= 128 ? 128 : 256) + 4ll * ((pages + 3) & ~3); }
-
 // See SelectParams. dims: host int[14] = tokens, num_seqs, tokens of each sequence (with cu_q: at most), table width, blocks, block_size, Hkv, G, D, first,
 // top, last, fp32, 0.
 int swb_page_select(const int* dims, const void* q, long long q_stride_tok, long long q_stride_head, const void* codes, const void* scales, const int* table,
@@ -587,8 +586,8 @@ int swb_page_select(const int* dims, const void* q, long long q_stride_tok, long
   if ((long long)seqs * uniform * Hkv > INT_MAX / 8 || bs < 1 || Hkv < 1 || G < 1 || D < 1 || blocks < 1 || max_blocks < 1 || first < 0 || top < 0 || last < 1 || uniform < 1 || D > 256 || (long long)max_blocks * bs > INT_MAX || !q || !codes ||
       !scales || !table || !kv_lens || !pages || !counts)
     return -3;
-  const long long smem = swb_page_select_smem(max_blocks, G, D);
-  if (smem > 200 * 1024) return -3;
+  // a token's histogram, codes and scores in one block's shared memory
+  if (4ll * SELECT_INTS + (long long)G * (D <= 128 ? 128 : 256) + 4ll * ((max_blocks + 3) & ~3) > 200 * 1024) return -3;
   const SelectParams p{q, q_stride_tok, q_stride_head, reinterpret_cast<const int8_t*>(codes), reinterpret_cast<const float*>(scales), table, table_stride,
                        max_blocks, blocks, bs, Hkv, G, D, cu_q, kv_lens, seqs, uniform, T, first, top, last, pages, counts, fp32,
                        !fp32 && (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (q_stride_tok | q_stride_head) % 8 == 0, 1};

@@ -23,7 +23,7 @@ from .._native import kernels
 from .runtime import KernelError, check, ptr, require_cuda
 
 MAX_WIDTH, MAX_GROUP, MAX_SPLITS = 256, 128, 64
-SELECT_SMEM = 200 * 1024
+MAX_PAGES = 40000         # of a selection: the scores of a token lie in one block's shared memory
 
 
 @dataclass
@@ -58,7 +58,7 @@ class PageSelection:
 
 # A decode step calls these once a layer: what is checked is read from each tensor once, and host arrays go to the library as packed bytes.
 _INTS = {n: struct.Struct(f"{n}i").pack for n in (9, 11, 14, 16)}
-_LONGS = {n: struct.Struct(f"{n}q").pack for n in (4, 8)}
+_LONGS = {n: struct.Struct(f"{n}q").pack for n in (5, 8)}
 _KINDS = (torch.bfloat16, torch.float32)
 
 
@@ -147,12 +147,12 @@ def select_pages(q: torch.Tensor, summaries: PageSummaries, block_table: torch.T
     T, G, tok, head = _check_rows(q, heads, D)
     n, per = _check_step(block_table, kv_lens, cu_q, max_q_len, T)
     _require(block_size >= 1 and top >= 0 and first >= 0 and last >= 1, "block_size >= 1, top >= 0, first >= 0, last >= 1")
-    lib, width = kernels(), first + top + last
-    _require(lib.swb_page_select_smem(per, G, D) <= SELECT_SMEM, "a selection is made over at most 200 KB of scores (4 bytes a page)")
-    pages = torch.empty((T, heads, width), dtype=torch.int32, device=q.device)
-    counts = torch.empty((T, heads), dtype=torch.int32, device=q.device)
+    _require(per <= MAX_PAGES, "a selection is made over at most 40000 pages")
+    width, rows = first + top + last, T * heads
+    both = torch.empty(rows * (width + 1), dtype=torch.int32, device=q.device)
+    pages, counts = both.as_strided((T, heads, width), (heads * width, width, 1)), both.as_strided((T, heads), (heads, 1), rows * width)
     dims = _INTS[14](T, n, max_q_len, per, blocks, block_size, heads, G, D, first, top, last, q.dtype == torch.float32, 0)
-    check(lib.swb_page_select(dims, q.data_ptr(), tok, head, codes.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), ptr(cu_q),
+    check(kernels().swb_page_select(dims, q.data_ptr(), tok, head, codes.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), ptr(cu_q),
                               kv_lens.data_ptr(), pages.data_ptr(), counts.data_ptr(), stream), "swb_page_select")
     return PageSelection(pages, counts)
 
@@ -203,13 +203,13 @@ def _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, 
     problems = (T if run == 1 else n * -(-max_q_len // run)) * heads * -(-G // 16)
     splits = budget_splits(problems, keys, weights is None, fast) if num_splits is None else num_splits
     _require(1 <= splits <= MAX_SPLITS, "1 to 64 splits")
-    lib, ws, nbytes = kernels(), None, 0
+    ws, nbytes = None, 0
     if weights is not None or not (splits == 1 or (fast and splits <= 8 and problems * splits <= 296)):      # else blocks finish their results, or clusters do
-        nbytes = lib.swb_attn_budget_workspace(T, heads, G, Dv, splits, per * bs, weights is not None)
+        nbytes = 4 * T * G * heads * (splits * (Dv + 2) + (0 if weights is None else per * bs)) + 16
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)        # the call's own: two streams or graphs share none
     dims = _INTS[16](T, n, max_q_len, per, blocks, bs, heads, G, D, Dv, width, splits, kind == torch.float32, 0, 0, 0)
     strides = _LONGS[8](tok, head, out_stride, block_table.stride(0), w_seq, w_head, 0, 0)
-    check(lib.swb_attn_budget(dims, strides, q.data_ptr(), out.data_ptr(), k_ptr, v_ptr, block_table.data_ptr(), ptr(cu_q), kv_lens.data_ptr(),
+    check(kernels().swb_attn_budget(dims, strides, q.data_ptr(), out.data_ptr(), k_ptr, v_ptr, block_table.data_ptr(), ptr(cu_q), kv_lens.data_ptr(),
                               ptr(pages), ptr(counts), ptr(weights), scale, softcap, ptr(ws), nbytes, stream), "swb_attn_budget")
     return out
 
@@ -268,11 +268,11 @@ def evict_tokens(kcache: torch.Tensor, vcache: torch.Tensor, block_table: torch.
     _check_entries(positions, torch.int32, n, heads, capacity, "positions")
     _require(next_positions.dtype == torch.int32 and next_positions.shape == (n,) and next_positions.is_contiguous(), "next_positions are int32 [num_seqs]")
     _require(keep >= 1 and recent >= 0 and first >= 0 and recent + first <= keep, "0 <= first, recent; 1 <= keep; first + recent <= keep")
-    lib, device = kernels(), kcache.device
-    moves = torch.empty(lib.swb_evict_moves(n, heads, capacity, keep), dtype=torch.int32, device=device)
+    device, room = kcache.device, 2 * n * heads * max(0, min(keep, capacity - keep))
+    moves = torch.empty(room, dtype=torch.int32, device=device)
     lens = torch.empty(n, dtype=torch.int32, device=device)
     dims = _INTS[11](n, heads, per, blocks, bs, D * size, Dv * size, capacity, keep, recent, first)
-    strides = _LONGS[4](*weights.stride()[:2], *positions.stride()[:2])
-    check(lib.swb_evict(dims, strides, kcache.data_ptr(), vcache.data_ptr(), block_table.data_ptr(), block_table.stride(0), kv_lens.data_ptr(), lens.data_ptr(),
+    sizes = _LONGS[5](*weights.stride()[:2], *positions.stride()[:2], room)
+    check(kernels().swb_evict(dims, sizes, kcache.data_ptr(), vcache.data_ptr(), block_table.data_ptr(), block_table.stride(0), kv_lens.data_ptr(), lens.data_ptr(),
                         next_positions.data_ptr(), weights.data_ptr(), positions.data_ptr(), moves.data_ptr(), stream), "swb_evict")
     return lens

@@ -9,17 +9,6 @@ B, T, H, KV, D, BS, N = 2, 2, 4, 2, 16, 4, 8
 
 
 class _NoKernels:
-    """Sizes are answered, launches are not."""
-
-    def swb_page_select_smem(self, pages, G, D):
-        return 8448 + G * 128 + 4 * pages
-
-    def swb_attn_budget_workspace(self, *a):
-        return 64
-
-    def swb_evict_moves(self, *a):
-        return 64
-
     def __getattr__(self, name):
         raise AssertionError(f"{name} was launched")
 
@@ -103,6 +92,18 @@ def test_tensors_on_the_cpu_are_refused(monkeypatch):
     for name in ALL:
         with pytest.raises(KernelError, match="CUDA tensors"):
             _call(name, _args())
+
+
+def test_tensors_on_another_device_are_refused(monkeypatch):
+    class Elsewhere:
+        is_cuda, device = True, "cuda:1"
+
+        def get_device(self):
+            return 1
+
+    monkeypatch.undo()
+    with pytest.raises(KernelError, match="the current device is cuda:0"):
+        budget._place(None, Elsewhere())
 
 
 def test_rows_that_share_memory():

@@ -354,6 +354,8 @@ def test_select_pages(heads, kv, D, bs, top, first, last, kind):
     sums.scales[c.table[2, 20:30].long()] = 0.0              # ties
     c.q[3].zero_()
     c.q[4, 0, 0] = float("inf")
+    c.q[6] *= 2.0 ** 124                                      # 127 of them pass the range of 32 bits
+    c.q[7] *= 2.0 ** -128
     c.table[3, 4] = c.blocks + 7
     got = ops.select_pages(c.q, sums, c.table, c.kv_lens, block_size=bs, top=top, first=first, last=last, **c.step)
     pages, counts = got.pages.cpu(), got.counts.cpu()
