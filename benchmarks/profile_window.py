@@ -14,6 +14,7 @@ with cudaProfilerStart/Stop so that `ncu --profile-from-start off` sees only tho
   --what q4k_chain  one gate-up link of a chain of Q4_K products (T from --shape "Tx..", 28672 x 4096)
   --what conv_sums  one implicit-GEMM convolution that adds up its output's group sums (832 x 1216 x 128 -> 128)
   --what last_conv  group norm, SiLU and the last convolution of a decoder (832 x 1216 x 128 -> 8)
+  --what operator  one pass of a case of perf/operators.py (--case: its name)
   --what vae      one FLUX-class VAE decode, 128 x 128 latents -> 1024 x 1024 (about 115 launches, 1.3 GB live)
 """
 import argparse
@@ -44,6 +45,7 @@ def main():
     ap.add_argument("--depth-single", type=int, default=4)
     ap.add_argument("--layers", type=int, default=32)
     ap.add_argument("--reps", type=int, default=1)
+    ap.add_argument("--case", default="selected_server")
     args = ap.parse_args()
     from inference_b200 import ops
 
@@ -125,6 +127,12 @@ def main():
         cu = torch.tensor([0, q_len], dtype=torch.int32, device=dev)
         kvl = torch.tensor([ctx + q_len], dtype=torch.int32, device=dev)
         window(lambda: ops.paged_attention(q, kc, vc, table, kvl, cu_q=cu, max_q_len=q_len, scale=D ** -0.5, causal=True), reps=args.reps)
+    elif args.what == "operator":
+        from perf import operators
+
+        operators.own = True
+        state = operators.prepare(next(c for c in operators.listed() if c["name"] == args.case), 1)
+        window(lambda: operators.run(state), reps=args.reps)
     elif args.what == "vae":
         from inference_b200.models.vae import VaeConfig, VaeDecoderGpu
 

@@ -667,7 +667,8 @@ __device__ __forceinline__ void split_factors(const float* ml, int S, int lane, 
 template <typename E, int KEYS>
 __global__ void __launch_bounds__(JOIN_THREADS) attn_budget_finish_kernel(const BudgetParams p, int join_blocks) {
   pdl_launch_dependents();
-  __shared__ float s_factor[MAX_SPLITS], s_all[MAX_GROUP * 2];
+  __shared__ float s_factor[MAX_SPLITS];
+  __shared__ __align__(8) float s_all[MAX_GROUP * 2];
   __shared__ size_t s_row[MAX_GROUP];
   __shared__ int s_seen[MAX_GROUP];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, S = p.num_splits, Hq = p.Hkv * p.G;
@@ -725,18 +726,25 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_budget_finish_kernel(const 
     }
     __syncthreads();
     constexpr int U = KEYS == 1 ? 32 : 4;        // rows whose scores are on their way together
+    const bool alike = KEYS > 1;                 // one token: its rows see the same keys
+    bool in[KEYS];
+#pragma unroll
+    for (int k = 0; k < KEYS; ++k) in[k] = j0 + k * JOIN_THREADS < s_seen[0];
     for (int r0 = 0; r0 < pairs; r0 += U) {
       float x[U][KEYS];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        const int r = min(r0 + u, pairs - 1);
+        const float* row = p.scores + s_row[r] + j0;
 #pragma unroll
-        for (int k = 0; k < KEYS; ++k) x[u][k] = r0 + u < pairs && j0 + k * JOIN_THREADS < s_seen[min(r0 + u, MAX_GROUP - 1)] ? __ldcg(p.scores + s_row[r0 + u] + j0 + k * JOIN_THREADS) : -INFINITY;
+        for (int k = 0; k < KEYS; ++k) x[u][k] = r0 + u < pairs && (alike ? in[k] : j0 < s_seen[r]) ? __ldcg(row + k * JOIN_THREADS) : -INFINITY;
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float m = s_all[min(r0 + u, MAX_GROUP - 1) * 2], inv = s_all[min(r0 + u, MAX_GROUP - 1) * 2 + 1];
+        const float2 total_of = *reinterpret_cast<const float2*>(s_all + min(r0 + u, pairs - 1) * 2);
 #pragma unroll
         for (int k = 0; k < KEYS; ++k)
-          if (x[u][k] != -INFINITY) sum[k] = fmaf(exp2f(x[u][k] - m), inv, sum[k]);        // keys that a row does not see get nothing of it, whatever its sum is
+          if (x[u][k] != -INFINITY) sum[k] = fmaf(exp2f(x[u][k] - total_of.x), total_of.y, sum[k]);      // keys that a row does not see get nothing of it, whatever its sum is
       }
     }
   }
