@@ -234,8 +234,10 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_budget_plain_kernel(const 
 // are the 8 columns of that product, so a group of up to 8 query heads wastes none of it.
 // What a block costs before its first group and behind its last (some 5 us: look-ups that wait for one another, the joining of its warps) is hidden by the other
 // blocks of its SM. Rings of three groups leave room for two blocks, rings of two for three; the bytes on their way are the same. Two groups where blocks are many and
-// short (500 tokens with 4 key/value heads and 64 pages each: 165 us with two blocks, 126 with three), three where they are few (512 blocks
-// of 128 pages: 94 us with two blocks, 111 with three, of which the last 68 blocks run alone).
+// short (500 tokens with 4 key/value heads and 64 pages each: 165 us with two blocks, 126 with three; 123 now, 8.5 TB/s through the second-level cache), three where
+// they are few (512 blocks of 128 pages: 94 us with two blocks, 5.7 TB/s, 111 with three, of which the last 68 blocks run alone). 48 sequences of up to 8191
+// keys, 8 key/value heads, in 8 splits: 201 us, 6.1 TB/s, and 17 for their weights. Warps that take equal runs of all problems' keys one behind the other, and fill their
+// rings across problems, took 112, 252 and 155 us: SMs differ in what they get of a busy memory, and nothing evens that out then.
 constexpr int FW = 4;                               // warps
 constexpr int HALF_BYTES = 2048, GROUP_BYTES = 4 * HALF_BYTES;      // 16 rows of 64 columns; K low, K high, V low, V high
 constexpr int SQ_BYTES = ROWS * 256, LDO = 132;

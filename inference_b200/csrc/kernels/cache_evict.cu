@@ -55,8 +55,10 @@ __device__ __forceinline__ int load_from(const int* at, int rank) {
 __device__ __forceinline__ void store_to(const void* at, int rank, uint32_t x) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(in_block(at, rank)), "r"(x) : "memory");
 }
-__device__ __forceinline__ void red_to(const int* at, int rank, int x) {
-  asm volatile("red.shared::cluster.add.s32 [%0], %1;" ::"r"(in_block(at, rank)), "r"(x) : "memory");
+__device__ __forceinline__ int4 load4_from(const int* at, int rank) {
+  int4 x;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(in_block(at, rank)) : "memory");
+  return x;
 }
 __device__ __forceinline__ int add_to(const int* at, int rank, int x) {
   int old;
@@ -65,16 +67,19 @@ __device__ __forceinline__ int add_to(const int* at, int rank, int x) {
 }
 
 // `blocks` blocks, a cluster, share a (sequence, head): each has an equal run of the entries in front of `keep` and one of those behind. The first one's histogram
-// gathers the others', and it finds the threshold for all; what is kept in front of a run follows from the keys above and equal to the threshold
+// takes the others' in, and it finds the threshold for all; what is kept in front of a run follows from the keys above and equal to the threshold
 // there, so every block knows the places of its holes (not kept, in front of `keep`) and sources (kept, behind it) in the list of moves. The moves are
 // then shared out evenly. Counts are whole numbers: nothing depends on the order of the atomics.
+// What bounds it is the chain of steps that wait for one another (16 384 keys fit a block, so a pass over them is short): 64 sequences of up to 4608 keys to 4096, 8
+// heads, of which a quarter has anything to lose: 30 us, a third of them for the moves (4 TB/s while they last, of rows of 256 bytes in random places); 2 sequences of
+// 30 000 keys to 4000 with 8 blocks a head: 36 us. Two launches, a plan by one block a head and moves by many, took 56 and 93 us.
 template <typename W>
 __global__ void __launch_bounds__(EVICT_THREADS, 2) evict_kernel(const EvictParams p, int blocks) {
   pdl_launch_dependents();
   extern __shared__ uint32_t evict_keys[];
   __shared__ __align__(16) int hist[SELECT_INTS];
   __shared__ uint32_t s_list[EVICT_LISTED];
-  __shared__ int s_listed, s_count[4];                   // keys above and equal to the threshold, in front of and behind `keep`
+  __shared__ int s_listed, s_count[4];         // length of the list; keys above and equal to the threshold, in front of and behind `keep`
   const Team<EVICT_THREADS> team(threadIdx.x);
   const int rank = blockIdx.x % blocks, h = blockIdx.x / blocks, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t below = (1u << lane) - 1u;
@@ -114,11 +119,18 @@ __global__ void __launch_bounds__(EVICT_THREADS, 2) evict_kernel(const EvictPara
       if (!mask && cached) evict_keys[i] = k;
       if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digit], 1);
     }
-    __syncthreads();
-    if (rank > 0)
-      for (int i = tid; i < SELECT_BINS; i += EVICT_THREADS)
-        if (hist[i]) red_to(&hist[i], 0, hist[i]);
     meet();
+    if (rank == 0 && blocks > 1) {             // four bins to a thread, of all blocks at once
+      static_assert(SELECT_BINS == 4 * EVICT_THREADS, "bins are shared out evenly");
+      int4 x[EVICT_CLUSTER];
+#pragma unroll
+      for (int r = 1; r < EVICT_CLUSTER; ++r) x[r] = r < blocks ? load4_from(hist + tid * 4, r) : make_int4(0, 0, 0, 0);
+      int4 sum = reinterpret_cast<int4*>(hist)[tid];
+#pragma unroll
+      for (int r = 1; r < EVICT_CLUSTER; ++r) sum.x += x[r].x, sum.y += x[r].y, sum.z += x[r].z, sum.w += x[r].w;
+      reinterpret_cast<int4*>(hist)[tid] = sum;
+      __syncthreads();
+    }
     if (rank == 0) find_bin(team, hist, want, totals);
     meet();
   };
@@ -273,7 +285,7 @@ int swb_evict(const int* dims, const long long* sizes, void* k, void* v, const i
     return -3;
   const EvictParams p{reinterpret_cast<char*>(k), reinterpret_cast<char*>(v), kb, vb, table, table_stride, max_blocks, blocks, bs, Hkv, kv_lens, new_lens, next, weights,
                       sizes[0], sizes[1], positions, sizes[2], sizes[3], capacity, keep, recent, first, moves, most};
-  // a block for every 2048 entries where that fills the chip no further than one round
+  // a block for every 2048 entries where that fills the chip no further than one round (with up to four rounds, 64 sequences take as long)
   int share = 1;
   while (share < EVICT_CLUSTER && share * 2048 < capacity && (long long)share * 2 * Hkv * seqs <= 2 * 148) share *= 2;
   const int cached = capacity / share + 2;

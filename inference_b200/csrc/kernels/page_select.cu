@@ -57,7 +57,8 @@ __device__ __forceinline__ float two_sum(float x, float y, float& rest) {
 
 // bf16 pages up to 128 wide, widths and page sizes of a multiple of four: a lane has four columns, all rows of a page on their way at once. Sums of four rows are formed
 // in 32 bits with what each addition leaves out beside them (a change of type to 64 bits runs at a sixteenth of the rate, and 16 of them a column bound the
-// kernel: 81 us for 120 000 tokens of 8 heads), then added in 64 bits. A page with a sum that is not finite in 32 bits takes the other way.
+// kernel: 81 us for 120 000 tokens of 8 heads, 61 this way, 4.1 TB/s, three of four instructions a cycle), then added in 64 bits. A page with a sum that is not finite in 32
+// bits takes the other way.
 __global__ void __launch_bounds__(SUMMARY_WARPS * 32) page_summary_quads_kernel(const SummaryParams p) {
   pdl_launch_dependents();
   pdl_wait();
@@ -234,6 +235,8 @@ __device__ __forceinline__ int8_t query_code(float x, float a, bool fp32) {
 // Then the tokens are shared out among teams of warps, each of which chooses among its token's scores.
 // CL: p.share blocks, a cluster, score a part of the pages each into the first one's memory, and that one chooses (few problems over long caches).
 // Shared memory: the teams' histograms, codes of the queries [TT, G, 32 KS], keys [TT, pages].
+// 64 sequences of up to 1025 pages, 8 heads: 20 us (54 MB: 2.7 TB/s), most of it latency, of the look-ups and the first rows (half) and of the choice's steps (a quarter).
+// 1000 tokens of a prompt over 1063 pages: 104 us, of which scores and choice have about the same part; 2 instructions a cycle, 278 MB through the second-level cache.
 template <int TT, int KS, bool FULL, int GP, bool CL>
 __global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 ? 4 : 3) page_select_kernel(const SelectParams p) {
   constexpr int TEAM = SELECT_THREADS / TT, LD = 32 * KS;
@@ -534,7 +537,7 @@ int launch_select(SelectParams p, cudaStream_t s) {
 }
 
 // Groups of 3 or 4 and of 5 to 8 heads of 128 columns have kernels of their own: without the choice of the reduction and the ends of rows in the loop they
-// issue half the instructions, which bound them.
+// issue fewer instructions a page.
 int launch_select(const SelectParams& p, cudaStream_t s) {
   if (p.D == 128 && (reinterpret_cast<uintptr_t>(p.codes) & 15) == 0 && p.G > 2 && p.G <= 8) return p.G <= 4 ? launch_select<4, true, 4>(p, s) : launch_select<4, true, 8>(p, s);
   return p.D <= 128 ? launch_select<4, false, 0>(p, s) : launch_select<8, false, 0>(p, s);
