@@ -23,6 +23,16 @@ class PagedKvPool:
         self.data = torch.zeros((num_layers, 2, num_blocks, kv_heads, block_size, head_dim), dtype=dtype,
                                 device=device)
         self.allocator = BlockAllocator(num_blocks)
+        self.summaries: list | None = None      # of the pages of each layer (`with_summaries`)
+
+    def with_summaries(self) -> list:
+        """8-bit summaries of every layer's key pages, for decode steps on a page budget (`ops.PageSummaries`, a thirty-second of the keys). They go by
+        block like the pages: forks share them, a page that is taken back and filled again is summarised again, and a copied page is one that is about to be filled."""
+        if self.summaries is None:
+            from ..ops import PageSummaries
+
+            self.summaries = [PageSummaries.empty(self.data[layer, 0]) for layer in range(self.num_layers)]
+        return self.summaries
 
     @property
     def bytes(self) -> int:

@@ -13,6 +13,7 @@ from typing import Callable
 import torch
 
 from ..models.llama import LlamaGpu
+from ..ops import PageBudget
 from .kv_pool import PagedKvPool, PagedSequence
 from .runner import ModelRunner
 
@@ -33,6 +34,7 @@ class EngineConfig:
     prefill_token_budget: int = 16384   # tokens per prefill forward (bounds activation memory)
     kv_bytes: int | None = None          # None: size the pool for max_batch * max_seq_len tokens
     use_graphs: bool = True
+    page_budget: PageBudget | None = None    # decode steps read that many pages of each context (None: all of it)
 
 
 class LlmEngine:
@@ -52,7 +54,7 @@ class LlmEngine:
         else:
             self.pool = PagedKvPool(m.num_layers, nblocks, model.hkv, m.head_dim, c.block_size, device=model.device)
         self.runner = ModelRunner(model, self.pool, max_batch=c.max_batch, max_seq_len=c.max_seq_len,
-                                  use_graphs=c.use_graphs)
+                                  use_graphs=c.use_graphs, page_budget=c.page_budget)
 
     def new_sequence(self) -> PagedSequence:
         return PagedSequence(self.pool)

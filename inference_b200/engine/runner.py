@@ -14,6 +14,7 @@ import os
 import numpy as np
 import torch
 
+from ..contracts.errors import Unsupported
 from ..models.llama import LlamaGpu, StepInputs, splits_for as _splits_for
 from ..utils import tracing
 from ..utils.graphs import recording
@@ -42,8 +43,15 @@ class ModelRunner:
     MULTI_STEPS = 256
 
     def __init__(self, model: LlamaGpu, pool: PagedKvPool, max_batch: int = 64, max_seq_len: int = 8192,
-                 use_graphs: bool = True):
+                 use_graphs: bool = True, page_budget=None):
+        """page_budget (`ops.PageBudget`): decode steps read the pages that are selected for each token and key/value head; prompts read everything.
+        For the decoders of the Llama family on one uniform pool."""
         self.model, self.pool = model, pool
+        self.page_budget = page_budget
+        if page_budget is not None and not (isinstance(model, LlamaGpu) and isinstance(pool, PagedKvPool)):
+            raise Unsupported("a page budget needs a decoder of the Llama family on a uniform pool")
+        if page_budget is not None:
+            pool.with_summaries()
         self.max_batch, self.max_seq_len = max_batch, max_seq_len
         self.max_blocks = (max_seq_len + pool.block_size - 1) // pool.block_size
         # models whose layers differ in KV heads or visible keys choose their splits themselves (one per layer)
@@ -86,6 +94,9 @@ class ModelRunner:
         self.d2h_bytes_last = 0
         self.launches_last = 0
 
+    def _summaries(self) -> list | None:
+        return self.pool.summaries if self.page_budget is not None else None
+
     # ---- prefill (eager, ragged) ------------------------------------------------------------------
     def prefill(self, seqs: list[PagedSequence], new_tokens: list[list[int]], *, want_logits: bool = False,
                 all_positions: bool = False, embed_overrides: list[tuple[list[int], torch.Tensor] | None] | None = None,
@@ -126,6 +137,7 @@ class ModelRunner:
             num_seqs=len(seqs), decode=decode, fresh_prefill=fresh and not decode,
             attn_splits=self._splits(len(seqs), max(kvl)) if decode else 1,
             logits_rows=None if all_positions else d_rows,
+            page_budget=self.page_budget, summaries=self._summaries(),
             spans=[(len(t), n) for t, n in zip(new_tokens, kvl)])
         if self._stateful:
             inp.state_slots = d_states
@@ -280,7 +292,8 @@ class ModelRunner:
             inp = StepInputs(input_ids=self._ids[r0:r1], positions=self._pos[r0:r1], slot_mapping=self._slots[r0:r1],
                              block_table=self._table[r0:r1], kv_lens=self._kvl[r0:r1], cu_q=None, max_q_len=1,
                              num_seqs=r1 - r0, decode=True, attn_splits=splits, logits_rows=None,
-                             state_slots=self._states[r0:r1] if self._stateful else None)
+                             state_slots=self._states[r0:r1] if self._stateful else None,
+                             page_budget=self.page_budget, summaries=self._summaries())
             part = self.model.forward_hidden(inp, self.pool.data)
             # the model may hand back a view of a workspace that the next sub-step reuses
             parts.append(part.clone() if cap < B else part)

@@ -45,6 +45,8 @@ class StepInputs:
     #                                           to the residual stream at those rows after decoder layer l (Qwen3-VL)
     state_slots: torch.Tensor | None = None    # int32 [num_seqs]: slot of each sequence's recurrent state (-1 = do not
     #                                           touch any: a padding row); None for models without recurrent layers
+    page_budget: "ops.PageBudget | None" = None    # decode steps read the pages that it selects for each token ...
+    summaries: list | None = None              # ... by these summaries, one `ops.PageSummaries` a layer, which every step keeps up
     spans: list[tuple[int, int]] | None = None # host copy of (new tokens, context length) per sequence; None in a decode
     #                                           step (one token each, lengths change under a captured graph)
 
@@ -400,7 +402,7 @@ class LlamaGpu:
         D = cfg.head_dim
         eps, woff = cfg.rms_norm_eps, cfg.norm_weight_offset
         T = inp.input_ids.numel()
-        if self._use_tp_prefill(T) and inp.embed_rows is None and inp.rope_table is None and inp.deepstack is None:
+        if self._use_tp_prefill(T) and inp.summaries is None and inp.embed_rows is None and inp.rope_table is None and inp.deepstack is None:
             return self._forward_hidden_tp_prefill(inp, kv_pool)
         rope_pos, rope_cos, rope_sin = inp.positions, self.cos, self.sin
         if inp.rope_table is not None:
@@ -456,7 +458,17 @@ class LlamaGpu:
                               q_norm=L.q_norm, k_norm=L.k_norm, norm_eps=eps, norm_w_offset=woff,
                               block_size=block_size)
             q = qkv[:, :q_cols].view(T, self.hq, D)
-            if inp.fresh_prefill and inp.cu_q is not None and not cfg.attn_logit_softcap and self.dense_prefill:
+            if inp.summaries is not None:
+                ops.summarize_pages(kv_pool[li, 0], inp.block_table, inp.kv_lens, inp.summaries[li], cu_q=inp.cu_q, max_q_len=inp.max_q_len)
+                n += 1
+            if inp.page_budget is not None and inp.decode:
+                budget = inp.page_budget
+                chosen = ops.select_pages(q, inp.summaries[li], inp.block_table, inp.kv_lens, cu_q=inp.cu_q, max_q_len=inp.max_q_len, block_size=block_size,
+                                          top=budget.top, first=budget.first, last=budget.last)
+                attn = ops.selected_attention(q, kv_pool[li, 0], kv_pool[li, 1], inp.block_table, inp.kv_lens, chosen, cu_q=inp.cu_q,
+                                              max_q_len=inp.max_q_len, scale=cfg.attn_scale, softcap=cfg.attn_logit_softcap or 0.0)
+                n += 1
+            elif inp.fresh_prefill and inp.cu_q is not None and not cfg.attn_logit_softcap and self.dense_prefill:
                 # no earlier context: causal attention straight from the projection output on the tcgen05 kernel
                 kv_cols = self.hkv * D
                 attn = ops.varlen_causal_attention(q, qkv[:, q_cols:q_cols + kv_cols].view(T, self.hkv, D),

@@ -49,6 +49,17 @@ class PageSummaries:
         return out
 
 
+@dataclass(frozen=True)
+class PageBudget:
+    """How many pages a new token reads: the first ones, the last ones (its own among them) and the best of those between (`select_pages`)."""
+    top: int
+    first: int = 1
+    last: int = 4
+
+    def __post_init__(self):
+        _require(self.top >= 0 and self.first >= 0 and self.last >= 1, "top >= 0, first >= 0, last >= 1")
+
+
 @dataclass
 class PageSelection:
     """pages int32 [T, kv heads, N]: places in the sequence (page p holds tokens p * block_size and on), -1 behind the first counts int32 [T, kv heads]."""

@@ -708,3 +708,96 @@ def test_a_cache_behind_two_to_the_31_numbers(kind):
     ops.evict_tokens(k, v, c.table, c.kv_lens, weights, positions, c.kv_lens.clone(), keep=100, recent=10)
     for h in range(kv):
         assert torch.equal(c.row("k", 0, range(100))[h], rows[h, positions[0, h, :100].long()])
+
+
+# ---- in the engine ------------------------------------------------------------------------------------------------------------------------------------
+def _engine(budget, *, use_graphs=True, seed=0, **over):
+    from inference_b200.engine.llm_engine import EngineConfig, LlmEngine
+    from inference_b200.models import ModelConfig
+    from inference_b200.models.llama import LlamaGpu
+
+    cfg = ModelConfig.from_json({"hidden_size": 512, "intermediate_size": 1024, "num_hidden_layers": 3, "num_attention_heads": 4, "num_key_value_heads": 2, "head_dim": 128,
+                                 "vocab_size": 2048, "rms_norm_eps": 1e-5, "rope_theta": 10000.0, **over})
+    model = LlamaGpu(cfg, device=torch.device("cuda")).init_random(seed=seed)
+    return LlmEngine(model, EngineConfig(max_batch=8, max_seq_len=1024, use_graphs=use_graphs, page_budget=budget))
+
+
+def _prompts():
+    g = torch.Generator().manual_seed(4)
+    return [torch.randint(0, 2048, (n,), generator=g).tolist() for n in (600, 37, 256, 15)]
+
+
+@pytest.mark.parametrize("over", [{}, {"model_type": "gemma2", "attn_logit_softcapping": 50.0, "query_pre_attn_scalar": 128}])
+def test_a_page_budget_that_holds_every_page_changes_nothing_but_roundings(over):
+    ops = _ops()
+    runs = []
+    for budget in (None, ops.PageBudget(top=64)):
+        eng = _engine(budget, **over)
+        seqs = [eng.new_sequence() for _ in _prompts()]
+        got = [eng.runner.prefill(seqs, _prompts(), want_logits=True)]
+        for step in range(20):
+            got.append(eng.runner.decode(seqs, [(7 * step + i) % 2048 for i in range(4)], want_logits=True).clone())
+        runs.append(got)
+    assert torch.equal(runs[0][0], runs[1][0])       # prompts read everything in either case
+    for a, b in zip(*runs):
+        assert (a - b).abs().max() <= 0.03 * a.abs().max()       # bf16 weights of the products are rounded in another order
+
+
+def test_steps_on_a_page_budget_are_the_same_from_a_graph_and_without():
+    ops = _ops()
+    budget = ops.PageBudget(top=3, first=1, last=2)
+    got = [_engine(budget, use_graphs=graphs).generate_batch(_prompts(), max_new_tokens=40).tokens for graphs in (True, False)]
+    assert got[0] == got[1]
+    assert all(len(t) == 40 for t in got[0])
+
+
+def test_a_page_budget_reads_what_its_summaries_select():
+    """Every layer's summaries are those of its pages after prompts, steps, a rollback and new steps; a fork finds them; and a step's attention is that of the pages they select."""
+    ops = _ops()
+    eng = _engine(ops.PageBudget(top=2, first=1, last=1))
+    seq = eng.new_sequence()
+    prompt = _prompts()[0]
+    eng.runner.prefill([seq], [prompt])
+    for i in range(30):
+        eng.runner.decode([seq], [i])
+    seq.truncate(603)                                 # within a page that was full
+    eng.runner.prefill([seq], [[9] * 40], want_logits=True)
+    seen = []
+    real = ops.selected_attention
+
+    def spy(q, k, v, table, lens, sel, **kw):
+        out = real(q, k, v, table, lens, sel, **kw)
+        seen.append((q.clone(), k, v, table, lens.clone(), sel, kw, out.clone()))
+        return out
+
+    eng.runner.use_graphs = False
+    ops.selected_attention = spy
+    try:
+        eng.runner.decode([seq], [5])
+    finally:
+        ops.selected_attention = real
+    assert len(seen) == 3
+    full = seq.length // 16
+    for layer, (q, k, v, table, lens, sel, kw, out) in enumerate(seen):
+        for page in range(full):
+            at = seq.blocks[page]
+            for h in range(2):
+                code, scale = _summary(eng.pool.data[layer, 0, at, h].cpu())
+                assert torch.equal(eng.pool.summaries[layer].codes[at, h].cpu(), code) and float(eng.pool.summaries[layer].scales[at, h]) == scale
+        c = Cache([seq.length], [1], heads=4, kv_heads=2)
+        c.k, c.v, c.table, c.q, c.blocks = k, v, table, q, k.shape[0]
+        for h in range(2):
+            assert sel.pages[0, h].tolist() == _select(c, eng.pool.summaries[layer], 0, 0, h, seq.length, 2, 1, 1)
+        host = sel.pages.cpu()
+        _check_attention(c, out, lambda t, b, h, n: [p * 16 + i for p in host[t, h].tolist() for i in range(16) if p * 16 + i < n], kw["scale"])
+
+
+def test_a_page_budget_needs_a_uniform_pool():
+    from inference_b200.contracts.errors import Unsupported
+    from inference_b200.engine.runner import ModelRunner
+
+    ops = _ops()
+    with pytest.raises(ops.KernelError):
+        ops.PageBudget(top=1, last=0)
+    with pytest.raises(Unsupported):
+        ModelRunner(object(), object(), page_budget=ops.PageBudget(top=1))
