@@ -341,7 +341,8 @@ def _select(c, sums, t, b, h, seen, top, first, last):
 
 
 @pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("heads,kv,D,bs", [(8, 2, 128, 16), (4, 4, 64, 16), (12, 1, 96, 32), (40, 1, 128, 16), (6, 2, 40, 16), (3, 1, 17, 5), (16, 8, 256, 16)])
+@pytest.mark.parametrize("heads,kv,D,bs", [(8, 2, 128, 16), (4, 4, 64, 16), (12, 1, 96, 32), (40, 1, 128, 16), (6, 2, 40, 16), (3, 1, 17, 5), (16, 8, 256, 16), (16, 2, 128, 16),
+                                           (6, 2, 128, 16), (5, 1, 128, 32), (4, 2, 128, 16)])
 @pytest.mark.parametrize("top,first,last", [(3, 1, 2), (0, 2, 1), (20, 0, 1), (1, 0, 3)])
 def test_select_pages(heads, kv, D, bs, top, first, last, kind):
     ops = _ops()
@@ -366,18 +367,19 @@ def test_select_pages(heads, kv, D, bs, top, first, last, kind):
             assert counts[t, h] == len(want)
 
 
+@pytest.mark.parametrize("G", [1, 2, 4, 7, 12])
 @pytest.mark.parametrize("pages,top", [(5000, 60), (4097, 4090), (300, 299), (2049, 1)])
-def test_selection_among_many_pages(pages, top):
+def test_selection_among_many_pages(pages, top, G):
     ops = _ops()
     g = _gen(pages)
-    c = Cache([16], [1], heads=4, kv_heads=2)
+    c = Cache([16], [1], heads=2 * G, kv_heads=2)
     c.lens, c.per, c.blocks = [pages * 16], pages, pages
     c.kv_lens, c.table = torch.tensor([pages * 16], dtype=torch.int32, device=CUDA), torch.randperm(pages, device=CUDA, generator=g).to(torch.int32)[None]
     # few codes: many scores are alike
     sums = ops.PageSummaries(torch.randint(-1, 2, (pages, 2, 128), device=CUDA, generator=g).to(torch.int8) * (torch.arange(128, device=CUDA) < 3).to(torch.int8),
                              torch.randint(1, 3, (pages, 2), device=CUDA, generator=g).float())
     got = ops.select_pages(c.q, sums, c.table, c.kv_lens, block_size=16, top=top, first=0, last=1, **c.step)
-    q = c.q[0].double().view(2, 2, 128)
+    q = c.q[0].double().view(2, G, 128)
     qc = torch.round(127 * q / q.abs().amax((1, 2), keepdim=True))
     score = (torch.einsum("hgd,phd->hgp", qc, sums.codes.double()).amax(1) * sums.scales.double().T)[:, c.table[0].long()]
     want = score[:, :-1].sort(dim=-1, descending=True, stable=True).indices[:, :top].sort(-1).values
@@ -460,6 +462,48 @@ def test_evict_from_long_caches(n, keep):
     src[~stay[:keep]] = stay[keep:].nonzero()[:, 0] + keep
     assert out.tolist() == [keep] and torch.equal(pos[0, 0, :keep].long(), src) and torch.equal(w[0, 0, :keep], old_w[0, 0, src])
     assert torch.equal(c.row("k", 0, range(keep))[0], rows[src])
+
+
+def test_eviction_from_a_graph():
+    """One capture, replayed as the cache grows again: as the same calls one after the other."""
+    ops = _ops()
+    results = []
+    for graphed in (False, True):
+        c = Cache([200, 150], [1, 1], seed=11, extra_pages=1)
+        g = _gen(12)
+        weights = torch.rand(2, 2, c.per * 16, device=CUDA, generator=g)
+        positions = torch.full((2, 2, c.per * 16), -1, dtype=torch.int32, device=CUDA)
+        kv, nxt = c.kv_lens.clone(), c.kv_lens.clone()
+
+        def body():
+            return ops.evict_tokens(c.k, c.v, c.table, kv, weights, positions, nxt, keep=100, recent=8, first=2)
+
+        state = [t.clone() for t in (c.k, c.v, weights, positions)]
+        if graphed:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                body()
+            torch.cuda.current_stream().wait_stream(side)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                lens = body()
+            for t, old in zip((c.k, c.v, weights, positions), state):
+                t.copy_(old)
+        seen = []
+        for step in range(4):
+            if graphed:
+                graph.replay()
+            else:
+                lens = body()
+            seen += [lens.clone(), weights.clone(), positions.clone(), c.k.clone(), c.v.clone()]
+            kv.copy_(lens + 37)                               # new tokens, with weights of their own
+            nxt += 37
+            weights[:, :, 100:137] = torch.rand(2, 2, 37, device=CUDA, generator=_gen(step))
+        results.append(seen)
+    for a, b in zip(*results):
+        assert torch.equal(a.nan_to_num(nan=-7.0), b.nan_to_num(nan=-7.0)) if a.is_floating_point() else torch.equal(a, b)
 
 
 # ---- together -----------------------------------------------------------------------------------------------------------------------------------------
