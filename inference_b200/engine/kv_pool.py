@@ -27,8 +27,11 @@ class PagedKvPool:
 
     def with_summaries(self) -> list:
         """8-bit summaries of every layer's key pages, for decode steps on a page budget (`ops.PageSummaries`, a thirty-second of the keys). They go by
-        block like the pages: forks share them, a page that is taken back and filled again is summarised again, and a copied page is one that is about to be filled."""
+        block like the pages: forks share them, a page that is taken back and filled again is summarised again, and a copied page is one that is about to be filled. Asked for while no page is in use: those
+        that are filled already would have none."""
         if self.summaries is None:
+            if self.allocator.live_blocks():
+                raise ValueError("summaries of a pool whose pages are in use already")
             from ..ops import PageSummaries
 
             self.summaries = [PageSummaries.empty(self.data[layer, 0]) for layer in range(self.num_layers)]

@@ -44,8 +44,8 @@ class ModelRunner:
 
     def __init__(self, model: LlamaGpu, pool: PagedKvPool, max_batch: int = 64, max_seq_len: int = 8192,
                  use_graphs: bool = True, page_budget=None):
-        """page_budget (`ops.PageBudget`): decode steps read the pages that are selected for each token and key/value head; prompts read everything.
-        For the decoders of the Llama family on one uniform pool."""
+        """page_budget (`ops.PageBudget`): steps of as few tokens a sequence as a decode step (one, drafts that are verified, a prompt of that length) read the pages
+        that are selected for each token and key/value head; longer and ragged ones read everything. For the decoders of the Llama family on one uniform pool."""
         self.model, self.pool = model, pool
         self.page_budget = page_budget
         if page_budget is not None and not (isinstance(model, LlamaGpu) and isinstance(pool, PagedKvPool)):
@@ -83,7 +83,7 @@ class ModelRunner:
         self._multi_meta = torch.zeros((self.MULTI_STEPS, self._n_meta), dtype=torch.int32, device=dev)
         self._multi_out = torch.zeros(self.MULTI_STEPS * max_batch, dtype=torch.int64, device=dev)
         self._step = torch.zeros(1, dtype=torch.int32, device=dev)
-        self._graphs: dict[tuple[int, int, bool], _DecodeGraph] = {}
+        self._graphs: dict[tuple[int, int, bool | str, bool], _DecodeGraph] = {}
         self._meta_copy_done = None
         self.pad_batches = self.use_graphs      # decode batches are padded to a bucket so graphs are reused
         # SWB_DECODE_SPLIT=n runs a decode batch of more than n rows as consecutive sub-steps of at most n rows, so
@@ -95,7 +95,8 @@ class ModelRunner:
         self.launches_last = 0
 
     def _summaries(self) -> list | None:
-        return self.pool.summaries if self.page_budget is not None else None
+        """Kept up by every runner of a pool that has them: another one may select by them."""
+        return getattr(self.pool, "summaries", None) if isinstance(self.model, LlamaGpu) else None
 
     # ---- prefill (eager, ragged) ------------------------------------------------------------------
     def prefill(self, seqs: list[PagedSequence], new_tokens: list[list[int]], *, want_logits: bool = False,
@@ -335,7 +336,7 @@ class ModelRunner:
             self._meta_copy_done.record()
         self.h2d_bytes_last = self._host_meta.numel() * 4
         splits = self._splits(Bp, max_kv)
-        key = (Bp, splits, want_logits)
+        key = (Bp, splits, want_logits, self._summaries() is not None)
         if not self.use_graphs or self.model.device.type != "cuda":
             toks, logits = self._decode_body(Bp, splits, want_logits)
             self.launches_last = self.model.launches
@@ -396,7 +397,7 @@ class ModelRunner:
                 out[k].copy_(toks)
             self.launches_last = self.model.launches * n_steps
             return out
-        key = (B, splits, "feedback")
+        key = (B, splits, "feedback", self._summaries() is not None)
         g = self._graphs.get(key)
         if g is None:
             self._multi_meta[0].copy_(host_all[0], non_blocking=True)

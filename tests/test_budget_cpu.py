@@ -118,3 +118,13 @@ def test_splits():
     assert budget.budget_splits(400, 10 ** 6, True) == 1 and budget.budget_splits(400, 8192, False) == 7 and budget.budget_splits(10 ** 6, 10 ** 6, False) == 1
     assert budget.budget_splits(64, 4000, True, False) == 18 and budget.budget_splits(8, 100, False, False) == 2 and budget.budget_splits(5000, 4000, False, False) == 1
     assert budget.budget_splits(0, 0, True) == 1 and budget.budget_splits(0, 0, False) == 1
+
+
+def test_summaries_are_asked_for_before_a_pool_is_used():
+    from inference_b200.engine.kv_pool import PagedKvPool, PagedSequence
+
+    pool = PagedKvPool(1, 4, 1, 64, device="cpu")
+    PagedSequence(pool).reserve(1)
+    with pytest.raises(ValueError):
+        pool.with_summaries()
+    assert pool.summaries is None

@@ -836,6 +836,34 @@ def test_a_page_budget_reads_what_its_summaries_select():
         _check_attention(c, out, lambda t, b, h, n: [p * 16 + i for p in host[t, h].tolist() for i in range(16) if p * 16 + i < n], kw["scale"])
 
 
+def test_runners_of_one_pool_keep_its_summaries_up():
+    """One runner with a budget, one without (made, and its step captured, before the pool had summaries): what the second one writes is summarised too."""
+    from inference_b200.engine.runner import ModelRunner
+
+    ops = _ops()
+    eng = _engine(None)
+    plain = eng.runner
+    seq = eng.new_sequence()
+    plain.prefill([seq], [_prompts()[1]])
+    plain.decode([seq], [3])
+    with pytest.raises(ValueError):
+        ModelRunner(eng.model, eng.pool, max_batch=8, max_seq_len=1024, page_budget=ops.PageBudget(top=2))
+    seq.release()
+    short = ModelRunner(eng.model, eng.pool, max_batch=8, max_seq_len=1024, page_budget=ops.PageBudget(top=2))
+    seq = eng.new_sequence()
+    for i, run in enumerate((plain, short, plain)):
+        run.prefill([seq], [_prompts()[i]])
+        for token in range(20):
+            run.decode([seq], [token])
+    torch.cuda.synchronize()
+    for layer in range(3):
+        for page in range(seq.length // 16):
+            at = seq.blocks[page]
+            for h in range(2):
+                code, scale = _summary(eng.pool.data[layer, 0, at, h].cpu())
+                assert torch.equal(eng.pool.summaries[layer].codes[at, h].cpu(), code) and float(eng.pool.summaries[layer].scales[at, h]) == scale
+
+
 def test_a_page_budget_needs_a_uniform_pool():
     from inference_b200.contracts.errors import Unsupported
     from inference_b200.engine.runner import ModelRunner
