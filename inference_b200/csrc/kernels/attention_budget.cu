@@ -53,7 +53,8 @@ struct BudgetParams {
   long long capacity;
   float* weights;            // [num_seqs, Hkv, .], inner stride 1
   long long w_seq, w_head;
-  int q_vec;                 // rows of q are 16-byte aligned
+  int q_vec, out_vec;        // rows of q are 16-byte aligned, those of out 8-byte
+  int whole_rows;            // a TMA box holds whole rows (widths are multiples of 64), else 64 columns
 };
 
 // What a query token is: its sequence and the keys it sees.
@@ -259,6 +260,18 @@ __device__ __forceinline__ void zero_values(uint8_t* group, int live, int halves
   __syncwarp();
 }
 
+// Whether all values of rows from..to - 1 of a group are finite: whole warp.
+__device__ __forceinline__ bool finite_values(const uint8_t* group, int from, int to, int halves, int lane) {
+  bool finite = true;
+  for (int half = 0; half < halves; ++half)
+    for (int j = lane; j < (to - from) * 8; j += 32) {
+      const uint4 x = *reinterpret_cast<const uint4*>(group + (2 + half) * HALF_BYTES + from * 128 + j * 16);
+#pragma unroll
+      for (const uint32_t w : {x.x, x.y, x.z, x.w}) finite = finite && (w & 0x7f80u) != 0x7f80u && (w & 0x7f800000u) != 0x7f800000u;
+    }
+  return __all_sync(0xffffffffu, finite);
+}
+
 __device__ __forceinline__ void cluster_barrier() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -269,9 +282,14 @@ __device__ __forceinline__ uint32_t in_cluster(uint32_t at, int rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(rank));
   return remote;
 }
-__device__ __forceinline__ float ld_cluster(uint32_t at) {
-  float x;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+__device__ __forceinline__ float2 ld_cluster2(uint32_t at) {
+  float2 x;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(at) : "memory");
+  return x;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t at) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at) : "memory");
   return x;
 }
 
@@ -344,6 +362,13 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
     if (lane == stage) live_st = live;
     if (live == 0) return;                          // nothing is read of a group without live keys
     if (lane == 0) mbar_arrive_expect_tx(&full[stage], (uint32_t)boxes * HALF_BYTES);
+    if (p.whole_rows) {
+      if (lane == 0) {
+        tma_load_3d(ring + stage * GROUP_BYTES, &tmap_k, &full[stage], 0, row, 0);
+        tma_load_3d(ring + stage * GROUP_BYTES + 2 * HALF_BYTES, &tmap_v, &full[stage], 0, row, 0);
+      }
+      return;
+    }
     __syncwarp();
     if (lane < boxes) {
       const bool is_k = lane < k_halves;
@@ -407,7 +432,7 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
       phases ^= 1u << stage;
       if (lane == stage) live_st = 0;               // nothing in flight there
       const uint32_t sK = smem_u32(ring + stage * GROUP_BYTES), sV = sK + 2 * HALF_BYTES;
-      if (live < 16 && tokens == 1) zero_values(ring + stage * GROUP_BYTES, live, v_halves, lane);
+      if (live < 16) zero_values(ring + stage * GROUP_BYTES, live, v_halves, lane);
       float s[2][4];
 #pragma unroll
       for (int x = 0; x < 2; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
@@ -420,38 +445,51 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
         mma_16816(s[1], qf[kk], b2, b3);
       }
       uint32_t pf[NT][2];
+      float v[NT][4], base[NT];                     // keys 2 t4, 2 t4 + 1, 8 + 2 t4, 9 + 2 t4 of head gr + 8 x
 #pragma unroll
       for (int x = 0; x < NT; ++x) {
-        float v[4];                                 // keys 2 t4, 2 t4 + 1, 8 + 2 t4, 9 + 2 t4 of head gr + 8 x
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int key = (e >> 1) * 8 + t4 * 2 + (e & 1);
           const float raw = score_transform(s[e >> 1][2 * x + (e & 1)], p.scale, p.softcap);
-          v[e] = key < live - behind[x] ? raw : -INFINITY;
+          v[x][e] = key < live - behind[x] ? raw : -INFINITY;
         }
         if (score[x]) {
           float* to = score[x] + (size_t)(warp + i * FW) * 16 + t4 * 2;
-          *reinterpret_cast<float2*>(to) = make_float2(v[0], v[1]);
-          *reinterpret_cast<float2*>(to + 8) = make_float2(v[2], v[3]);
+          *reinterpret_cast<float2*>(to) = make_float2(v[x][0], v[x][1]);
+          *reinterpret_cast<float2*>(to + 8) = make_float2(v[x][2], v[x][3]);
         }
-        float top = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float now = fmaxf(m[x], top), base = now == -INFINITY ? 0.f : now;
-        if (__any_sync(0xffffffffu, now > m[x])) {  // otherwise every factor is one
-          const float alpha = exp2f(m[x] - base);
+        base[x] = fmaxf(fmaxf(v[x][0], v[x][1]), fmaxf(v[x][2], v[x][3]));
+      }
+      bool more = false;
+#pragma unroll
+      for (int x = 0; x < NT; ++x) base[x] = fmaxf(base[x], __shfl_xor_sync(0xffffffffu, base[x], 1));
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+        base[x] = fmaxf(m[x], fmaxf(base[x], __shfl_xor_sync(0xffffffffu, base[x], 2)));
+        more = more || base[x] > m[x];
+      }
+      if (__any_sync(0xffffffffu, more)) {          // otherwise every factor is one
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+          const float alpha = exp2f(m[x] - (base[x] == -INFINITY ? 0.f : base[x]));
+          m[x] = base[x];
           l[x] *= alpha;
           const float a0 = __shfl_sync(0xffffffffu, alpha, t4 * 8), a1 = __shfl_sync(0xffffffffu, alpha, t4 * 8 + 4);
 #pragma unroll
           for (int j = 0; j < 8; ++j) o[x][j][0] *= a0, o[x][j][1] *= a1, o[x][j][2] *= a0, o[x][j][3] *= a1;
-          m[x] = now;
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = exp2f(v[e] - base);
-        l[x] += (v[0] + v[1]) + (v[2] + v[3]);
-        pf[x][0] = pack_bf16(v[0], v[1]), pf[x][1] = pack_bf16(v[2], v[3]);
       }
-      if (live - (tokens - 1) >= 16 || tokens == 1) {
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+        if (base[x] == -INFINITY) base[x] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[x][e] = exp2f(v[x][e] - base[x]);
+        l[x] += (v[x][0] + v[x][1]) + (v[x][2] + v[x][3]);
+        pf[x][0] = pack_bf16(v[x][0], v[x][1]), pf[x][1] = pack_bf16(v[x][2], v[x][3]);
+      }
+      // Keys that some of the tokens do not see weigh nothing for those, which is enough where their values are numbers.
+      if (live - (tokens - 1) >= 16 || tokens == 1 || finite_values(ring + stage * GROUP_BYTES, max(live - (tokens - 1), 0), min(live, 16), v_halves, lane)) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (j >= v_steps) break;
@@ -461,8 +499,7 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
           for (int x = 0; x < NT; ++x) mma_16816(o[x][j], a, pf[x][0], pf[x][1]);
         }
       } else {
-        // Some of the tokens do not see all of these keys: each has a product of its own, behind which the values that only later ones see are zeros, and takes its
-        // own columns from it.
+        // Each token has a product of its own, behind which the values that only later ones see are zeros, and takes its own columns from it.
         for (int i = tokens - 1; i >= 0; --i) {
           const int own = max(live - (tokens - 1 - i), 0);
           if (own < 16) zero_values(ring + stage * GROUP_BYTES, own, v_halves, lane);
@@ -537,14 +574,27 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
     if (p.part_ml && !p.cluster) *reinterpret_cast<float2*>(p.part_ml + part_at(p, token_at(tid), head_at(tid), split) * 2) = make_float2(M, L);
   }
   __syncthreads();
-  for (int r = 0; r < rows; ++r) {
+  const int d = lane * 4;                           // a row to a warp, four columns to a lane
+  const auto store = [&](int r, float4 x) {
+    bf16* to = out + token_at(r) * p.out_stride_tok + (size_t)head_at(r) * p.Dv + d;
+    if (p.out_vec) *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
+    else to[0] = __float2bfloat16(x.x), to[1] = __float2bfloat16(x.y), to[2] = __float2bfloat16(x.z), to[3] = __float2bfloat16(x.w);
+  };
+#pragma unroll 4
+  for (int r = warp; r < rows; r += FW) {
+    if (d >= p.Dv) break;
     const float4 f = *reinterpret_cast<const float4*>(sWarps + r * 4);
-    for (int d = tid; d < p.Dv; d += FW * 32) {
-      float* o4 = sO + r * LDO + d;
-      const float x = fmaf(f.x, o4[0], f.y * o4[ROWS * LDO]) + fmaf(f.z, o4[2 * ROWS * LDO], f.w * o4[3 * ROWS * LDO]);
-      if (parts) p.part_o[part_at(p, token_at(r), head_at(r), split) * p.Dv + d] = x;
-      else if (S == 1) out[token_at(r) * p.out_stride_tok + (size_t)head_at(r) * p.Dv + d] = __float2bfloat16(x);
-      else o4[0] = x;                               // warp 0's, which this thread alone reads
+    float4* at = reinterpret_cast<float4*>(sO + r * LDO + d);
+    const float4 x0 = at[0], x1 = at[ROWS * LDO / 4], x2 = at[2 * ROWS * LDO / 4], x3 = at[3 * ROWS * LDO / 4];
+    const auto sum = [&](float a, float b, float c, float e) { return fmaf(f.x, a, f.y * b) + fmaf(f.z, c, f.w * e); };
+    const float4 x = make_float4(sum(x0.x, x1.x, x2.x, x3.x), sum(x0.y, x1.y, x2.y, x3.y), sum(x0.z, x1.z, x2.z, x3.z), sum(x0.w, x1.w, x2.w, x3.w));
+    if (parts) {
+      float2* to = reinterpret_cast<float2*>(p.part_o + part_at(p, token_at(r), head_at(r), split) * p.Dv + d);
+      to[0] = make_float2(x.x, x.y), to[1] = make_float2(x.z, x.w);
+    } else if (S == 1) {
+      store(r, x);
+    } else {
+      at[0] = x;                                    // warp 0's, which this thread alone reads
     }
   }
   if (parts) return;
@@ -557,7 +607,8 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
         m_of[s] = -INFINITY, l_of[s] = 0.f;
         if (s < S) {
           const uint32_t at = in_cluster(smem_u32(sPart + tid * 2), s);
-          m_of[s] = ld_cluster(at), l_of[s] = ld_cluster(at + 4);
+          const float2 x = ld_cluster2(at);
+          m_of[s] = x.x, l_of[s] = x.y;
         }
         M = fmaxf(M, m_of[s]);
       }
@@ -571,16 +622,20 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
       for (int s = 0; s < MAX_CLUSTER; ++s) sFactor[tid * MAX_CLUSTER + s] = m_of[s] * inv;
     }
     __syncthreads();
-    for (int r = split; r < rows; r += S)
-      for (int d = tid; d < p.Dv; d += FW * 32) {
-        const uint32_t at = smem_u32(sO + r * LDO + d);
-        float o_of[MAX_CLUSTER], x = 0.f;
+#pragma unroll 2
+    for (int r = split + S * warp; r < rows; r += S * FW) {
+      if (d >= p.Dv) break;
+      const uint32_t at = smem_u32(sO + r * LDO + d);
+      float4 o_of[MAX_CLUSTER], x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int s = 0; s < MAX_CLUSTER; ++s) o_of[s] = s < S ? ld_cluster(in_cluster(at, s)) : 0.f;
+      for (int s = 0; s < MAX_CLUSTER; ++s) o_of[s] = s < S ? ld_cluster4(in_cluster(at, s)) : x;
 #pragma unroll
-        for (int s = 0; s < MAX_CLUSTER; ++s) x = fmaf(sFactor[r * MAX_CLUSTER + s], o_of[s], x);
-        out[token_at(r) * p.out_stride_tok + (size_t)head_at(r) * p.Dv + d] = __float2bfloat16(x);
+      for (int s = 0; s < MAX_CLUSTER; ++s) {
+        const float f = sFactor[r * MAX_CLUSTER + s];
+        x.x = fmaf(f, o_of[s].x, x.x), x.y = fmaf(f, o_of[s].y, x.y), x.z = fmaf(f, o_of[s].z, x.z), x.w = fmaf(f, o_of[s].w, x.w);
       }
+      store(r, x);
+    }
   }
   if (p.weigh_here) {                               // one token: row r is head r, and the block's scores are its own writes
     float* w = p.weights + tok.seq * p.w_seq + h * p.w_head;
@@ -610,12 +665,15 @@ bool fast_fits(const BudgetParams& p, int fp32) {
 }
 
 int launch_fast(BudgetParams p, cudaStream_t s) {
+  p.out_vec = (reinterpret_cast<uintptr_t>(p.out) & 7) == 0 && p.out_stride_tok % 4 == 0;
   p.q_vec = (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 && p.q_stride_tok % 8 == 0 && p.q_stride_head % 8 == 0;
   CUtensorMap tk, tv;
   const int rows = p.num_blocks * p.Hkv * p.bs;
-  int rc = make_tmap_bf16_2d(&tk, p.k, rows, p.D, p.D, 16);
+  p.whole_rows = (p.D | p.Dv) % 64 == 0;
+  const auto make_tmap = p.whole_rows ? make_tmap_bf16_blocks : make_tmap_bf16_2d;
+  int rc = make_tmap(&tk, p.k, rows, p.D, p.D, 16);
   if (rc) return rc;
-  rc = make_tmap_bf16_2d(&tv, p.v, rows, p.Dv, p.Dv, 16);
+  rc = make_tmap(&tv, p.v, rows, p.Dv, p.Dv, 16);
   if (rc) return rc;
   const bool one = p.G * p.run <= 8;
   const int problems = (p.run > 1 ? p.num_seqs * ((p.uniform_q + p.run - 1) / p.run) : p.tokens) * p.Hkv * p.head_tiles;
