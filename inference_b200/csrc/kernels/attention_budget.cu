@@ -293,7 +293,8 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t at) {
   return x;
 }
 
-template <int NT, int FS>         // eights of rows: 1 or 2; groups in a warp's ring: 3, or 2
+// NT: eights of rows, 1 or 2; FS: groups in a warp's ring, 3 or 2; WIDE: keys and values are 128 wide, so that all steps of a product are known and its loads run ahead
+template <int NT, int FS, bool WIDE>
 __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budget_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const BudgetParams p) {
   pdl_launch_dependents();
   extern __shared__ uint8_t fast_smem[];
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
     ldsm_x4(smem_u32(sQ) + q_off((mi & 1) * 8 + (lane & 7), kk * 2 + (mi >> 1)), qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3]);
     if (NT == 1) qf[kk][1] = qf[kk][3] = 0u;        // rows 8..15 are no heads
   }
-  const int k_steps = (p.D + 15) >> 4, v_steps = (p.Dv + 15) >> 4;
+  const int k_steps = WIDE ? 8 : (p.D + 15) >> 4, v_steps = WIDE ? 8 : (p.Dv + 15) >> 4;
 
   float o[NT][8][4], m[NT], l[NT];
 #pragma unroll
@@ -675,12 +676,15 @@ int launch_fast(BudgetParams p, cudaStream_t s) {
   if (rc) return rc;
   rc = make_tmap(&tv, p.v, rows, p.Dv, p.Dv, 16);
   if (rc) return rc;
-  const bool one = p.G * p.run <= 8;
+  const bool one = p.G * p.run <= 8, wide = p.D == 128 && p.Dv == 128;
   const int problems = (p.run > 1 ? p.num_seqs * ((p.uniform_q + p.run - 1) / p.run) : p.tokens) * p.Hkv * p.head_tiles;
   const bool many = one && (long long)problems * p.num_splits >= 9 * 148;
-  auto kernel = many ? attn_budget_kernel<1, 2> : one ? attn_budget_kernel<1, 3> : attn_budget_kernel<2, 3>;
-  const int smem = fast_smem_bytes(many ? 2 : 3), which = many ? 2 : one;
-  static bool configured[3][64] = {};
+  const int smem = fast_smem_bytes(many ? 2 : 3), which = (many ? 2 : one) + 3 * wide;
+  using Kernel = decltype(&attn_budget_kernel<1, 2, true>);
+  static constexpr Kernel kernels[6] = {attn_budget_kernel<2, 3, false>, attn_budget_kernel<1, 3, false>, attn_budget_kernel<1, 2, false>,
+                                        attn_budget_kernel<2, 3, true>, attn_budget_kernel<1, 3, true>, attn_budget_kernel<1, 2, true>};
+  const Kernel kernel = kernels[which];
+  static bool configured[6][64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !configured[which][dev]) {
