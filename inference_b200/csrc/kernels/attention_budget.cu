@@ -448,13 +448,29 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
       uint32_t pf[NT][2];
       float v[NT][4], base[NT];                     // keys 2 t4, 2 t4 + 1, 8 + 2 t4, 9 + 2 t4 of head gr + 8 x
 #pragma unroll
-      for (int x = 0; x < NT; ++x) {
+      for (int x = 0; x < NT; ++x)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = (e >> 1) * 8 + t4 * 2 + (e & 1);
-          const float raw = score_transform(s[e >> 1][2 * x + (e & 1)], p.scale, p.softcap);
-          v[x][e] = key < live - behind[x] ? raw : -INFINITY;
-        }
+        for (int e = 0; e < 4; ++e) v[x][e] = s[e >> 1][2 * x + (e & 1)];
+      if (p.softcap > 0.f) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[x][e] = score_transform(v[x][e], p.scale, p.softcap);
+      } else {
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[x][e] = score_transform(v[x][e], p.scale, 0.f);
+      }
+      if (live - (tokens - 1) < 16) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if ((e >> 1) * 8 + t4 * 2 + (e & 1) >= live - behind[x]) v[x][e] = -INFINITY;
+      }
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
         if (score[x]) {
           float* to = score[x] + (size_t)(warp + i * FW) * 16 + t4 * 2;
           *reinterpret_cast<float2*>(to) = make_float2(v[x][0], v[x][1]);
