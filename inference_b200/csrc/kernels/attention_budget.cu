@@ -272,6 +272,13 @@ __device__ __forceinline__ bool finite_values(const uint8_t* group, int from, in
   return __all_sync(0xffffffffu, finite);
 }
 
+// 2^x for x <= 0 within 2 ulp; weights below 2^-126 of the largest are zeros.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ void cluster_barrier() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -501,7 +508,7 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
       for (int x = 0; x < NT; ++x) {
         if (base[x] == -INFINITY) base[x] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[x][e] = exp2f(v[x][e] - base[x]);
+        for (int e = 0; e < 4; ++e) v[x][e] = exp2_fast(v[x][e] - base[x]);
         l[x] += (v[x][0] + v[x][1]) + (v[x][2] + v[x][3]);
         pf[x][0] = pack_bf16(v[x][0], v[x][1]), pf[x][1] = pack_bf16(v[x][2], v[x][3]);
       }
