@@ -749,15 +749,19 @@ __device__ __forceinline__ void split_factors(const float* ml, int S, int lane, 
   if (lane + 32 < S) factor[lane + 32] = e1 * inv;
 }
 
-// The first `join_blocks` blocks join the parts of one row each; the others weigh a run of keys of one (sequence, key/value head) each. KEYS of a thread: four for
-// steps of one token, whose rows are few and blocks many, one for several tokens, whose rows are many and blocks few.
-template <typename E, int KEYS>
-__global__ void __launch_bounds__(JOIN_THREADS) attn_budget_finish_kernel(const BudgetParams p, int join_blocks) {
+// The first `join_blocks` blocks join the parts of one row each; the others weigh keys of one (sequence, key/value head) each, V neighbouring ones to a lane. SPLIT: the
+// block's warps share 32 V keys and each takes a part of the rows, whose sums are added up in one order (16 tokens, 4 heads of a group, 6001 keys: 20 us with a key to a
+// lane and all 64 rows one behind the other, 7 so); else each warp has keys of its own. Rows are then few and blocks many and short: an SM holds 16 of them, so that
+// their look-ups hide one another (48 sequences of up to 8191 keys, 8 key/value heads of 4 heads: 21 us with 8 blocks, 17 with 16).
+template <typename E, int V, bool SPLIT>
+__global__ void __launch_bounds__(JOIN_THREADS, SPLIT ? 1 : 16) attn_budget_finish_kernel(const BudgetParams p, int join_blocks) {
   pdl_launch_dependents();
+  constexpr int WARPS = JOIN_THREADS / 32, RUN = 32 * V * (SPLIT ? 1 : WARPS), U = V == 1 ? 16 : SPLIT ? 8 : 2;      // U: rows whose scores are on their way together
   __shared__ float s_factor[MAX_SPLITS];
   __shared__ __align__(8) float s_all[MAX_GROUP * 2];
   __shared__ size_t s_row[MAX_GROUP];
   __shared__ int s_seen[MAX_GROUP];
+  __shared__ float s_sum[WARPS][32 * V];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, S = p.num_splits, Hq = p.Hkv * p.G;
   pdl_wait();
   if ((int)blockIdx.x < join_blocks) {
@@ -774,70 +778,117 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_budget_finish_kernel(const 
     }
     return;
   }
-  constexpr int RUN = KEYS * JOIN_THREADS;
   const int blocks = (int)((p.capacity + RUN - 1) / RUN), i = blockIdx.x - join_blocks;
   const int h = i / blocks % p.Hkv, seq = i / blocks / p.Hkv;
-  const long long j0 = (long long)(i % blocks) * RUN + tid;
+  const int first = i % blocks * RUN, at = ((SPLIT ? 0 : warp * 32) + lane) * V;      // of the block, and of this lane behind it
   const int q0 = max(p.cu_q ? p.cu_q[seq] : seq * p.uniform_q, 0), q1 = p.cu_q ? p.cu_q[seq + 1] : q0 + p.uniform_q;
   const int q_end = min(min(q1, p.tokens), q0 + p.uniform_q);      // tokens whose scores are there
-  const int total = p.kv_lens[seq], len = min(total, p.max_blocks * p.bs);
-  if (j0 - tid >= len) return;
-  float* w = p.weights + seq * p.w_seq + h * p.w_head;
-  float sum[KEYS], old[KEYS];
+  const int total = p.kv_lens[seq], len = (int)min((long long)total, p.capacity);
+  if (first >= len) return;
+  const int room = len - first - at;
+  const size_t j0 = (size_t)first + at;
+  float* w = p.weights + seq * p.w_seq + h * p.w_head + j0;
+  const bool whole = V == 4 && room >= 4 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+  float sum[V], old[V];
 #pragma unroll
-  for (int k = 0; k < KEYS; ++k) sum[k] = 0.f, old[k] = j0 + k * JOIN_THREADS < len ? w[j0 + k * JOIN_THREADS] : 0.f;
+  for (int k = 0; k < V; ++k) sum[k] = 0.f, old[k] = 0.f;
+  if (!SPLIT || warp == 0) {
+    if (whole) {
+      const float4 x = *reinterpret_cast<const float4*>(w);
+      old[0] = x.x, old[V > 1] = x.y, old[V / 2] = x.z, old[V - 1] = x.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) old[k] = k < room ? w[k] : 0.f;
+    }
+  }
+  constexpr int STEP = SPLIT ? WARPS : 1;
   const int batch = MAX_GROUP / p.G;             // tokens whose rows a block has room for
   for (int t0 = q0; t0 < q_end; t0 += batch) {
     const int pairs = min(batch, q_end - t0) * p.G;
     __syncthreads();
     if (tid < pairs) {                           // MAX_GROUP <= JOIN_THREADS: a row to a thread
       const int tok = tid / p.G;
-      const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + part_at(p, t0 + tok, h * p.G + tid % p.G, 0);
-      float M = -INFINITY, L = 0.f;
-      for (int s0 = 0; s0 < S; s0 += 8) {
-        float2 x[8];
-#pragma unroll
-        for (int s = 0; s < 8; ++s) x[s] = s0 + s < S ? __ldcg(ml + s0 + s) : make_float2(-INFINITY, 0.f);
-        float top = M;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) top = fmaxf(top, x[s].x);
-        const float base = top == -INFINITY ? 0.f : top;
-        L *= exp2f(M - base);
-#pragma unroll
-        for (int s = 0; s < 8; ++s) L = fmaf(exp2f(x[s].x - base), x[s].y, L);
-        M = top;
-      }
-      s_all[tid * 2] = M == -INFINITY ? 0.f : M, s_all[tid * 2 + 1] = L == 0.f ? 0.f : 1.f / L;
       s_row[tid] = ((size_t)(t0 + tok) * Hq + h * p.G + tid % p.G) * p.capacity;
       s_seen[tid] = min(total - (q1 - 1 - t0 - tok), len);
     }
     __syncthreads();
-    constexpr int U = KEYS == 1 ? 32 : 4;        // rows whose scores are on their way together
-    const bool alike = KEYS > 1;                 // one token: its rows see the same keys
-    bool in[KEYS];
-#pragma unroll
-    for (int k = 0; k < KEYS; ++k) in[k] = j0 + k * JOIN_THREADS < s_seen[0];
-    for (int r0 = 0; r0 < pairs; r0 += U) {
-      float x[U][KEYS];
+    float x[U][V];
+    const auto load = [&](int r0) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int r = min(r0 + u, pairs - 1);
-        const float* row = p.scores + s_row[r] + j0;
-#pragma unroll
-        for (int k = 0; k < KEYS; ++k) x[u][k] = r0 + u < pairs && (alike ? in[k] : j0 < s_seen[r]) ? __ldcg(row + k * JOIN_THREADS) : -INFINITY;
+        const int r = min(r0 + u * STEP, pairs - 1), left = r0 + u * STEP < pairs ? s_seen[r] - first - at : 0;      // keys that the row sees; behind them nothing is written
+        if constexpr (V == 4) {
+          const float4 y = left > 0 ? __ldcg(reinterpret_cast<const float4*>(p.scores + s_row[r] + j0)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          x[u][0] = left > 0 ? y.x : -INFINITY, x[u][1] = left > 1 ? y.y : -INFINITY, x[u][2] = left > 2 ? y.z : -INFINITY, x[u][3] = left > 3 ? y.w : -INFINITY;
+        } else {
+          x[u][0] = left > 0 ? __ldcg(p.scores + s_row[r] + j0) : -INFINITY;
+        }
       }
+    };
+    int r0 = SPLIT ? warp : 0;
+    if constexpr (SPLIT) load(r0);               // on their way while the rows' sums are
+    if (tid < pairs) {
+      const int tok = tid / p.G;
+      const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + part_at(p, t0 + tok, h * p.G + tid % p.G, 0);
+      float M = -INFINITY, L = 0.f;
+      for (int s0 = 0; s0 < S; s0 += 8) {
+        float2 y[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) y[s] = s0 + s < S ? __ldcg(ml + s0 + s) : make_float2(-INFINITY, 0.f);
+        float top = M;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) top = fmaxf(top, y[s].x);
+        const float base = top == -INFINITY ? 0.f : top;
+        L *= exp2f(M - base);
+#pragma unroll
+        for (int s = 0; s < 8; ++s) L = fmaf(exp2f(y[s].x - base), y[s].y, L);
+        M = top;
+      }
+      s_all[tid * 2] = M == -INFINITY ? 0.f : M, s_all[tid * 2 + 1] = L == 0.f ? 0.f : 1.f / L;
+    }
+    __syncthreads();
+    if constexpr (!SPLIT) load(r0);
+    while (r0 < pairs) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float2 total_of = *reinterpret_cast<const float2*>(s_all + min(r0 + u, pairs - 1) * 2);
+        const float2 all = *reinterpret_cast<const float2*>(s_all + min(r0 + u * STEP, pairs - 1) * 2);
 #pragma unroll
-        for (int k = 0; k < KEYS; ++k)
-          if (x[u][k] != -INFINITY) sum[k] = fmaf(exp2f(x[u][k] - total_of.x), total_of.y, sum[k]);      // keys that a row does not see get nothing of it, whatever its sum is
+        for (int k = 0; k < V; ++k)
+          if (x[u][k] != -INFINITY) sum[k] = fmaf(exp2_fast(x[u][k] - all.x), all.y, sum[k]);      // keys that a row does not see get nothing of it, whatever its sum is
       }
+      r0 += U * STEP;
+      if (r0 < pairs) load(r0);
     }
   }
+  if constexpr (SPLIT) {
 #pragma unroll
-  for (int k = 0; k < KEYS; ++k)
-    if (j0 + k * JOIN_THREADS < len) w[j0 + k * JOIN_THREADS] = old[k] + sum[k];
+    for (int k = 0; k < V; ++k) s_sum[warp][k * 32 + lane] = sum[k];
+    __syncthreads();
+    if (warp) return;
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+#pragma unroll
+      for (int o = 1; o < WARPS; ++o) sum[k] += s_sum[o][k * 32 + lane];
+  }
+  if (whole) {
+    *reinterpret_cast<float4*>(w) = make_float4(old[0] + sum[0], old[V > 1] + sum[V > 1], old[V / 2] + sum[V / 2], old[V - 1] + sum[V - 1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (k < room) w[k] = old[k] + sum[k];
+  }
+}
+
+template <typename E>
+int launch_finish(const BudgetParams& p, bool join, bool weigh, cudaStream_t s) {
+  const bool four = p.capacity % 4 == 0;         // rows of scores start on 16 bytes
+  const bool split = p.uniform_q * (long long)p.G >= 16;
+  const int join_blocks = join ? p.tokens * p.Hkv * p.G : 0, run = 32 * (four ? 4 : 1) * (split ? 1 : JOIN_THREADS / 32);
+  const long long blocks = join_blocks + (weigh ? (p.capacity + run - 1) / run * p.Hkv * p.num_seqs : 0);
+  if (blocks > INT_MAX) return -3;
+  auto kernel = four ? (split ? attn_budget_finish_kernel<E, 4, true> : attn_budget_finish_kernel<E, 4, false>)
+                     : (split ? attn_budget_finish_kernel<E, 1, true> : attn_budget_finish_kernel<E, 1, false>);
+  return launch_kernel(kernel, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, s, p, join_blocks);
 }
 
 template <typename E, int R, bool VEC>
@@ -915,13 +966,8 @@ int swb_attn_budget(const int* dims, const long long* strides, const void* q, vo
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int rc = fast ? launch_fast(p, s) : fp32 ? launch_plain<float>(p, s) : launch_plain<bf16>(p, s);
   if (rc || !(join || weigh)) return rc;
-  const int join_blocks = join ? p.tokens * p.Hkv * p.G : 0, run = JOIN_THREADS * (p.uniform_q == 1 ? 4 : 1);
-  const long long blocks = join_blocks + (weigh ? (p.capacity + run - 1) / run * p.Hkv * p.num_seqs : 0);
-  if (blocks > INT_MAX) return -3;
   if (p.cluster) p.num_splits = 1;               // the cluster left one pair a row
-  auto kernel = fp32 ? (p.uniform_q == 1 ? attn_budget_finish_kernel<float, 4> : attn_budget_finish_kernel<float, 1>)
-                     : (p.uniform_q == 1 ? attn_budget_finish_kernel<bf16, 4> : attn_budget_finish_kernel<bf16, 1>);
-  return launch_kernel(kernel, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, s, p, join_blocks);
+  return fp32 ? launch_finish<float>(p, join, weigh, s) : launch_finish<bf16>(p, join, weigh, s);
 }
 
 }  // extern "C"
