@@ -488,9 +488,15 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 ? 4 : 3)
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (rank > 0) return;
   }
-  if (n <= width) return;                          // whole teams leave
-  const int want = n - p.first - p.last;           // this token's candidates
-  choose_in_order(team, keys + team.id * ldkeys, want, p.top, s_largest[team.id], hist, [&](int place, int i) { out[p.first + place] = p.first + i; });
+  // The team's and its token's numbers once more: kept over the scores, where registers are short, they are spilled.
+  int self = threadIdx.x;
+  if constexpr (TT > 1) asm volatile("mov.u32 %0, %%tid.x;" : "=r"(self));
+  const Team<TEAM> choosing(self);
+  const int of = s_cand[choosing.id];              // this token's candidates
+  if (of == 0) return;                             // whole teams leave
+  int* to = p.pages + ((size_t)(t0 + choosing.id) * p.Hkv + h) * (p.first + p.top + p.last) + p.first;
+  choose_in_order(choosing, keys + choosing.id * ldkeys, of, p.top, s_largest[choosing.id], reinterpret_cast<int*>(select_smem) + choosing.id * SELECT_INTS,
+                  [&](int place, int i) { to[place] = p.first + i; });
 }
 
 // Tokens of a block: as many as the 16 columns of two products hold (4 at most), where sequences have them, as long as the scores leave room for two blocks on an SM.

@@ -47,7 +47,7 @@ __device__ __forceinline__ void count_key(int* hist, uint32_t key) { atomicAdd(&
 template <int SIZE>
 __device__ __forceinline__ void find_bin(const Team<SIZE>& team, const int* hist, int want, int* totals) {
   constexpr int PER = SELECT_BINS / SIZE;
-  static_assert(SELECT_BINS % SIZE == 0 && PER >= 2 && SIZE <= 1024, "bins are shared out evenly");
+  static_assert(SELECT_BINS % SIZE == 0 && PER >= 2 && PER <= 32, "bins are shared out evenly, a thread's among a warp");
   // the thread of rank r adds up the r-th run of PER bins from the top, from a place of its own on so that neighbours meet in no bank
   const int* run = hist + SELECT_BINS - (team.rank + 1) * PER;
   int sum = 0;
@@ -71,7 +71,24 @@ __device__ __forceinline__ void find_bin(const Team<SIZE>& team, const int* hist
   team.sync();
   int before = incl - sum;
   for (int w = 0; w < team.warp(); ++w) before += totals[w];
-  if (before < want && want <= before + sum) {
+  // one thread's run holds the place: its warp looks at the bins, a lane each, or it does so itself where they are few
+  const bool here = before < want && want <= before + sum;
+  if constexpr (PER >= 16) {
+    const uint32_t owner = __ballot_sync(0xffffffffu, here);
+    if (owner) {
+      const int lane = __ffs(owner) - 1, start = __shfl_sync(0xffffffffu, before, lane);
+      const int bin = SELECT_BINS - (team.warp() * 32 + lane) * PER - 1 - team.lane();
+      const int mine = team.lane() < PER ? hist[bin] : 0;
+      int to = mine;
+#pragma unroll
+      for (int o = 1; o < PER; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, to, o);
+        if (team.lane() >= o) to += v;
+      }
+      if (team.lane() < PER && start + to - mine < want && want <= start + to)
+        totals[32] = bin, totals[33] = want - start - to + mine, totals[34] = mine, totals[35] = totals[36] = 0;
+    }
+  } else if (here) {
     for (int j = PER - 1; j >= 0; --j) {
       const int mine = run[j];
       if (before < want && want <= before + mine)
@@ -191,8 +208,8 @@ struct LinearDigit {
 };
 
 // The indexes of the `want` largest of n keys in ascending order, put(place, index), ties to the lowest index. keys: shared memory of 16-byte alignment, read in fours (up to
-// three behind the last are read and not used); largest: the largest of them. Where a team has a thread for each chosen key and for each in the border's bin, one pass
-// gathers both and two counts put them into order. The caller clears the bins; the whole team calls it, and the keys are written before it (it begins with a barrier).
+// three behind the last are read and not used); largest: the largest of them. Where a team has a thread for each key in the border's bin and for each chosen one, or
+// for every other, one pass gathers both and two counts put them into order. The caller clears the bins; the whole team calls it, and the keys are written before it (it begins with a barrier).
 template <int SIZE, typename Put>
 __device__ __forceinline__ void choose_in_order(const Team<SIZE>& team, const uint32_t* keys, int n, int want, uint32_t largest, int* hist, const Put& put) {
   int* totals = hist + SELECT_BINS;
@@ -207,7 +224,8 @@ __device__ __forceinline__ void choose_in_order(const Team<SIZE>& team, const ui
     }
   };
   team.sync();
-  if (want <= SIZE) {
+  constexpr int MOST = SIZE < 256 ? 2 * SIZE : SIZE;      // of few threads each puts two in order (with 256 that costs registers, and 8 % of 64 sequences' selections)
+  if (want <= MOST) {
     each([&](int, uint32_t k) { atomicAdd(&hist[digit(k)], 1); });
     team.sync();
     find_bin(team, hist, want, totals);
@@ -236,8 +254,9 @@ __device__ __forceinline__ void choose_in_order(const Team<SIZE>& team, const ui
         if (above < left) chosen[want - left + above] = at;
       }
       team.sync();
-      if (team.rank < want) {
-        const int at = chosen[team.rank];
+#pragma unroll 1
+      for (int i = team.rank; i < want; i += SIZE) {
+        const int at = chosen[i];
         int place = 0, j = 0;
         for (; j + 4 <= want; j += 4) {
           const int4 x = *reinterpret_cast<const int4*>(chosen + j);
@@ -245,6 +264,7 @@ __device__ __forceinline__ void choose_in_order(const Team<SIZE>& team, const ui
         }
         for (; j < want; ++j) place += chosen[j] < at;
         put(place, at);
+        if constexpr (MOST == SIZE) break;
       }
       return;
     }
