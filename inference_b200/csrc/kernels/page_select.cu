@@ -238,7 +238,7 @@ __device__ __forceinline__ int8_t query_code(float x, float a, bool fp32) {
 // 64 sequences of up to 1025 pages, 8 heads: 20 us (54 MB: 2.7 TB/s), most of it latency, of the look-ups and the first rows (half) and of the choice's steps (a quarter).
 // 1000 tokens of a prompt over 1063 pages: 104 us, of which scores and choice have about the same part; 2 instructions a cycle, 278 MB through the second-level cache.
 template <int TT, int KS, bool FULL, int GP, bool CL>
-__global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 ? 4 : 3) page_select_kernel(const SelectParams p) {
+__global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 && !CL ? 4 : 3) page_select_kernel(const SelectParams p) {
   constexpr int TEAM = SELECT_THREADS / TT, LD = 32 * KS;
   pdl_launch_dependents();
   extern __shared__ __align__(16) uint8_t select_smem[];
@@ -489,8 +489,9 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 ? 4 : 3)
     if (rank > 0) return;
   }
   // The team's and its token's numbers once more: kept over the scores, where registers are short, they are spilled.
-  int self = threadIdx.x;
-  if constexpr (TT > 1) asm volatile("mov.u32 %0, %%tid.x;" : "=r"(self));
+  int self;
+  asm volatile("mov.u32 %0, %%tid.x;" : "=r"(self));
+  __builtin_assume(self >= 0 && self < SELECT_THREADS);
   const Team<TEAM> choosing(self);
   const int of = s_cand[choosing.id];              // this token's candidates
   if (of == 0) return;                             // whole teams leave
