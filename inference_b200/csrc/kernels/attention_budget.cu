@@ -233,12 +233,14 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_budget_plain_kernel(const 
 // warp waits for another before the end. Group i of a block goes to warp i % 4. With queries as rows of 16, S = Q K^T leaves the weights of a head and pairs of
 // neighbouring keys in a thread, which is what the second operand of O^T = V^T P^T wants: nothing is moved in between, and heads
 // are the 8 columns of that product, so a group of up to 8 query heads wastes none of it.
-// What a block costs before its first group and behind its last (some 5 us: look-ups that wait for one another, the joining of its warps) is hidden by the other
+// A group is some 1300 cycles of a warp's steps behind one another (products 270 and 200, weights 350, the next copies 260); a chain of loads and products whose
+// length is not known when compiled took 500 cycles more (selected pages of 500 tokens: 120 us, and 97 with it known), a soft cap's branch at every score 130.
+// What a block costs before its first group and behind its last (some 4 us: look-ups that wait for one another, the joining of its warps) is hidden by the other
 // blocks of its SM. Rings of three groups leave room for two blocks, rings of two for three; the bytes on their way are the same. Two groups where blocks are many and
-// short (500 tokens with 4 key/value heads and 64 pages each: 165 us with two blocks, 126 with three; 123 now, 8.5 TB/s through the second-level cache), three where
-// they are few (512 blocks of 128 pages: 94 us with two blocks, 5.7 TB/s, 111 with three, of which the last 68 blocks run alone). 48 sequences of up to 8191
-// keys, 8 key/value heads, in 8 splits: 201 us, 6.1 TB/s, and 17 for their weights. Warps that take equal runs of all problems' keys one behind the other, and fill their
-// rings across problems, took 112, 252 and 155 us: SMs differ in what they get of a busy memory, and nothing evens that out then.
+// short (500 tokens with 4 key/value heads and 64 pages each: 90 us, 11.7 TB/s through the second-level cache; before the steps were shortened 126, and 165 with two
+// blocks), three where they are few (512 blocks of 128 pages: 87 us, 6.2 TB/s, 95 % of what a copy gets; with three blocks the last 68 of them run alone). 48 sequences of up
+// to 8191 keys, 8 key/value heads, in 8 splits: 192 us, 6.4 TB/s, and 17 for their weights. Warps that take equal runs of all problems' keys one behind the other, and fill
+// their rings across problems, took 112 us where these took 94: SMs differ in what they get of a busy memory, and nothing evens that out then.
 constexpr int FW = 4;                               // warps
 constexpr int HALF_BYTES = 2048, GROUP_BYTES = 4 * HALF_BYTES;      // 16 rows of 64 columns; K low, K high, V low, V high
 constexpr int SQ_BYTES = ROWS * 256, LDO = 132;
@@ -949,7 +951,7 @@ int swb_attn_budget(const int* dims, const long long* strides, const void* q, vo
   while (fast && !pages && p.run * 2 * p.G <= ROWS && p.run < p.uniform_q) p.run *= 2;
   const long long problems = (p.run > 1 ? (long long)p.num_seqs * ((p.uniform_q + p.run - 1) / p.run) : p.tokens) * p.Hkv * p.head_tiles;
   // Blocks of a cluster start together and wait for one another, which costs nothing while all of them fit the chip at once; behind that a second launch is cheaper
-  // (48 sequences of up to 8191 keys, 8 key/value heads, 4 splits: 305 us as clusters, 233 with a second launch)
+  // (48 sequences of up to 8191 keys, 8 key/value heads, 4 splits: 305 us as clusters, 213 with a second launch)
   p.cluster = fast && p.num_splits > 1 && p.num_splits <= MAX_CLUSTER && problems * p.num_splits <= 2 * 148;
   p.weigh_here = weights && fast && p.uniform_q == 1 && p.head_tiles == 1 && (p.cluster || p.num_splits == 1);
   const bool join = p.num_splits > 1 && !p.cluster, weigh = weights && !p.weigh_here;

@@ -236,7 +236,8 @@ __device__ __forceinline__ int8_t query_code(float x, float a, bool fp32) {
 // CL: p.share blocks, a cluster, score a part of the pages each into the first one's memory, and that one chooses (few problems over long caches).
 // Shared memory: the teams' histograms, codes of the queries [TT, G, 32 KS], keys [TT, pages].
 // 64 sequences of up to 1025 pages, 8 heads: 20 us (54 MB: 2.7 TB/s), most of it latency, of the look-ups and the first rows (half) and of the choice's steps (a quarter).
-// 1000 tokens of a prompt over 1063 pages: 104 us, of which scores and choice have about the same part; 2 instructions a cycle, 278 MB through the second-level cache.
+// 1000 tokens of a prompt over 1063 pages: 90 us, of which scores and choice have about the same part; 2 instructions a cycle, 250 MB through the second-level cache. Registers are
+// what is short: 100 spilled bytes in the loop over pages cost 15 us, and two blocks an SM with none 10.
 template <int TT, int KS, bool FULL, int GP, bool CL>
 __global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 && !CL ? 4 : 3) page_select_kernel(const SelectParams p) {
   constexpr int TEAM = SELECT_THREADS / TT, LD = 32 * KS;

@@ -241,8 +241,8 @@ def tracked_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tenso
     """Attention of every new token over all keys that it sees -> [T, Hq * Dv], which also adds the softmax weights of the step, summed over its tokens and the query heads of
     a group, to weights fp32 [num_seqs, kv heads, >= table pages * block_size] (unit inner stride; entry j of a row belongs to cache entry j).
 
-    For decode steps, and for the last tokens of a prompt. Each token reads its keys on its own, and scores are kept until the sums are
-    known: 4 bytes a token, query head and key of the table's width."""
+    For decode steps, and for the last tokens of a prompt: keys are read once for every 16 rows (tokens * heads of a group) of a sequence, and scores are kept until the sums
+    are known, 4 bytes a token, query head and key of the table's width."""
     return _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, softcap, num_splits, out, None, None, weights)
 
 
