@@ -386,6 +386,28 @@ def test_selection_among_many_pages(pages, top, G):
     assert torch.equal(got.pages[0, :, :top].long(), want) and (got.pages[0, :, top] == pages - 1).all()
 
 
+@pytest.mark.parametrize("G,tokens", [(4, 9), (8, 5), (2, 6)])
+@pytest.mark.parametrize("pages,top", [(700, 63), (700, 64), (700, 65), (700, 128), (700, 129), (600, 256), (600, 257), (1300, 300)])
+def test_selection_of_a_prompt_among_many_pages(pages, top, G, tokens):
+    """Several tokens to a block, each chosen for by a part of its threads; many scores are alike, and the last tokens see other numbers of pages than the first."""
+    ops = _ops()
+    g = _gen(pages + top)
+    n = pages * 16 - 13
+    q = torch.randn(tokens, 2 * G, 128, device=CUDA, generator=g).bfloat16()
+    lens, table = torch.tensor([n], dtype=torch.int32, device=CUDA), torch.randperm(pages, device=CUDA, generator=g).to(torch.int32)[None]
+    sums = ops.PageSummaries(torch.randint(-1, 2, (pages, 2, 128), device=CUDA, generator=g).to(torch.int8) * (torch.arange(128, device=CUDA) < 3).to(torch.int8),
+                             torch.randint(1, 3, (pages, 2), device=CUDA, generator=g).float())
+    got = ops.select_pages(q, sums, table, lens, cu_q=None, max_q_len=tokens, block_size=16, top=top, first=1, last=2)
+    grouped = q.double().view(tokens, 2, G, 128)
+    qc = torch.round(127 * grouped / grouped.abs().amax((2, 3), keepdim=True))
+    score = (torch.einsum("thgd,phd->thgp", qc, sums.codes.double()).amax(2) * sums.scales.double().T)[:, :, table[0].long()]
+    for t in range(tokens):
+        seen = -(-(n - (tokens - 1 - t)) // 16)
+        best = score[t, :, 1:seen - 2].sort(dim=-1, descending=True, stable=True).indices[:, :top].sort(-1).values + 1
+        ends = torch.tensor([seen - 2, seen - 1], device=CUDA).expand(2, 2)
+        assert torch.equal(got.pages[t].long(), torch.cat((torch.zeros(2, 1, dtype=torch.long, device=CUDA), best, ends), 1)), t
+
+
 # ---- eviction -----------------------------------------------------------------------------------------------------------------------------------------
 def _evict(k, v, w, pos, n, nxt, keep, recent, first):
     """One head's rows [n, ...] as lists; the rule, entry by entry."""
