@@ -952,8 +952,9 @@ int swb_attn_budget(const int* dims, const long long* strides, const void* q, vo
   const long long problems = (p.run > 1 ? (long long)p.num_seqs * ((p.uniform_q + p.run - 1) / p.run) : p.tokens) * p.Hkv * p.head_tiles;
   // Blocks of a cluster start together and wait for one another, which costs nothing while all of them fit the chip at once; behind that a second launch is cheaper
   // (48 sequences of up to 8191 keys, 8 key/value heads, 4 splits: 305 us as clusters, 213 with a second launch)
-  p.cluster = fast && p.num_splits > 1 && p.num_splits <= MAX_CLUSTER && problems * p.num_splits <= 2 * 148;
-  p.weigh_here = weights && fast && p.uniform_q == 1 && p.head_tiles == 1 && (p.cluster || p.num_splits == 1);
+  const bool own_weights = fast && p.uniform_q == 1 && p.head_tiles == 1;       // else there is a second launch in any case
+  p.cluster = fast && p.num_splits > 1 && p.num_splits <= MAX_CLUSTER && problems * p.num_splits <= 2 * 148 && (!weights || own_weights);
+  p.weigh_here = weights && own_weights && (p.cluster || p.num_splits == 1);
   const bool join = p.num_splits > 1 && !p.cluster, weigh = weights && !p.weigh_here;
   if (join || weights) {
     // workspace: the parts of the rows, and the scores where weights are kept, in front of them
