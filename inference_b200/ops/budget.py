@@ -160,7 +160,7 @@ def select_pages(q: torch.Tensor, summaries: PageSummaries, block_table: torch.T
     _require(block_size >= 1 and top >= 0 and first >= 0 and last >= 1, "block_size >= 1, top >= 0, first >= 0, last >= 1")
     _require(per <= MAX_PAGES, "a selection is made over at most 40000 pages")
     width, rows = first + top + last, T * heads
-    both = torch.empty(rows * (width + 1), dtype=torch.int32, device=q.device)
+    both = q.new_empty(rows * (width + 1), dtype=torch.int32)
     pages, counts = both.as_strided((T, heads, width), (heads * width, width, 1)), both.as_strided((T, heads), (heads, 1), rows * width)
     dims = _INTS[14](T, n, max_q_len, per, blocks, block_size, heads, G, D, first, top, last, q.dtype == torch.float32, 0)
     check(kernels().swb_page_select(dims, q.data_ptr(), tok, head, codes.data_ptr(), scales.data_ptr(), block_table.data_ptr(), block_table.stride(0), ptr(cu_q),
@@ -201,7 +201,7 @@ def _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, 
         width = listed[2]
         keys = min(width, per) * bs
     if out is None:
-        out = torch.empty((T, columns), dtype=kind, device=q.device)
+        out = q.new_empty((T, columns))
         out_stride = columns
     else:
         _require(out.shape == (T, columns) and out.dtype == kind and out.stride(1) == 1, "out is [T, heads * value width] in the type of q, unit inner stride")
@@ -217,7 +217,7 @@ def _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, 
     ws, nbytes = None, 0
     if weights is not None or not (splits == 1 or (fast and splits <= 8 and problems * splits <= 296)):      # else blocks finish their results, or clusters do
         nbytes = 4 * T * G * heads * (splits * (Dv + 2) + (0 if weights is None else per * bs)) + 16
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)        # the call's own: two streams or graphs share none
+        ws = q.new_empty(nbytes, dtype=torch.uint8)        # the call's own: two streams or graphs share none
     dims = _INTS[16](T, n, max_q_len, per, blocks, bs, heads, G, D, Dv, width, splits, kind == torch.float32, 0, 0, 0)
     strides = _LONGS[8](tok, head, out_stride, block_table.stride(0), w_seq, w_head, 0, 0)
     check(kernels().swb_attn_budget(dims, strides, q.data_ptr(), out.data_ptr(), k_ptr, v_ptr, block_table.data_ptr(), ptr(cu_q), kv_lens.data_ptr(),
