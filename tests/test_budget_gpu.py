@@ -307,6 +307,23 @@ def test_summaries_at_the_borders(D, bs):
         assert torch.equal(sums.codes[at[page], 0].cpu(), code) and (got == scale or (math.isnan(got) and math.isnan(scale))), page
 
 
+@pytest.mark.parametrize("bs", [16, 20, 3])
+@pytest.mark.parametrize("low,high", [(0, 254), (0, 0), (0, 3), (250, 254), (100, 150)])
+def test_summaries_of_any_finite_numbers(low, high, bs):
+    """bf16 numbers of any sign and fraction whose exponents are `low` to `high`: below the normal range, near the end of it, and far apart."""
+    ops = _ops()
+    g = _gen(bs + low)
+    bits = torch.randint(0, 2, (12, 2, bs, 64), device=CUDA, generator=g) << 15 | torch.randint(low, high + 1, (12, 2, bs, 64), device=CUDA, generator=g) << 7
+    k = (bits | torch.randint(0, 128, bits.shape, device=CUDA, generator=g)).to(torch.int32).to(torch.int16).view(torch.bfloat16)
+    table, lens = torch.randperm(12, device=CUDA, generator=g).to(torch.int32)[None], torch.tensor([12 * bs], dtype=torch.int32, device=CUDA)
+    sums = ops.PageSummaries.empty(k)
+    ops.summarize_pages(k, table, lens, sums, cu_q=None, max_q_len=12 * bs)
+    for page in range(12):
+        for h in range(2):
+            code, scale = _summary(k[page, h].cpu())
+            assert torch.equal(sums.codes[page, h].cpu(), code) and float(sums.scales[page, h]) == scale, (page, h)
+
+
 def test_summaries_of_single_steps_are_those_of_the_prompt():
     ops = _ops()
     c = Cache([70], [1], kv_heads=2)
