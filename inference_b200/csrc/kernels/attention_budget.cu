@@ -57,6 +57,9 @@ struct BudgetParams {
   int whole_rows;            // a TMA box holds whole rows (widths are multiples of 64), else 64 columns
 };
 
+// Cached tokens of a sequence; a length that the table has no pages for is the table's end, and the last new token's place is there.
+__device__ __forceinline__ int length_of(const BudgetParams& p, int seq) { return min(p.kv_lens[seq], p.max_blocks * p.bs); }
+
 // What a query token is: its sequence and the keys it sees.
 struct Token {
   int seq, q0, q_len, seen;
@@ -66,7 +69,7 @@ __device__ __forceinline__ Token token_of(const BudgetParams& p, int t) {
   x.seq = seq_of_token(p.cu_q, p.num_seqs, p.uniform_q, t);
   x.q0 = p.cu_q ? p.cu_q[x.seq] : x.seq * p.uniform_q;
   x.q_len = p.cu_q ? p.cu_q[x.seq + 1] - x.q0 : p.uniform_q;
-  x.seen = max(min(p.kv_lens[x.seq] - (x.q_len - 1 - (t - x.q0)), p.max_blocks * p.bs), 0);
+  x.seen = max(length_of(p, x.seq) - (x.q_len - 1 - (t - x.q0)), 0);
   return x;
 }
 
@@ -337,7 +340,7 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
     t = q0 + t % runs * p.run;
     tokens = min(p.run, min(q1, p.tokens) - t);
     if (tokens <= 0 || t < 0) return;
-    tok.seen = max(min(p.kv_lens[tok.seq] - (q1 - t - tokens), p.max_blocks * p.bs), 0);            // of the last token
+    tok.seen = max(length_of(p, tok.seq) - (q1 - t - tokens), 0);            // of the last token
   }
   const int rows = heads * tokens;                  // row r: token r / heads, head r % heads
   const int sub = p.bs >> 4;                        // groups of a page
@@ -786,7 +789,7 @@ __global__ void __launch_bounds__(JOIN_THREADS, SPLIT ? 1 : 16) attn_budget_fini
   const int first = i % blocks * RUN, at = ((SPLIT ? 0 : warp * 32) + lane) * V;      // of the block, and of this lane behind it
   const int q0 = max(p.cu_q ? p.cu_q[seq] : seq * p.uniform_q, 0), q1 = p.cu_q ? p.cu_q[seq + 1] : q0 + p.uniform_q;
   const int q_end = min(min(q1, p.tokens), q0 + p.uniform_q);      // tokens whose scores are there
-  const int total = p.kv_lens[seq], len = (int)min((long long)total, p.capacity);
+  const int len = length_of(p, seq);
   if (first >= len) return;
   const int room = len - first - at;
   const size_t j0 = (size_t)first + at;
@@ -812,7 +815,7 @@ __global__ void __launch_bounds__(JOIN_THREADS, SPLIT ? 1 : 16) attn_budget_fini
     if (tid < pairs) {                           // MAX_GROUP <= JOIN_THREADS: a row to a thread
       const int tok = tid / p.G;
       s_row[tid] = ((size_t)(t0 + tok) * Hq + h * p.G + tid % p.G) * p.capacity;
-      s_seen[tid] = min(total - (q1 - 1 - t0 - tok), len);
+      s_seen[tid] = len - (q1 - 1 - t0 - tok);
     }
     __syncthreads();
     float x[U][V];

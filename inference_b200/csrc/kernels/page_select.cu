@@ -237,9 +237,9 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 && !CL ?
   const int q0 = p.cu_q ? p.cu_q[seq] : seq * p.uniform_q, q1 = p.cu_q ? p.cu_q[seq + 1] : q0 + p.uniform_q;
   const int t0 = q0 + (run % runs) * TT;
   if (t0 < 0 || t0 >= min(q1, p.tokens)) return;
-  const int len = p.kv_lens[seq], width = p.first + p.top + p.last;
+  const int len = min(p.kv_lens[seq], p.max_blocks * p.bs), width = p.first + p.top + p.last;
   const auto pages_of = [&](int t) {               // pages that token t sees
-    const int seen = min(len - (q1 - 1 - t), p.max_blocks * p.bs);
+    const int seen = len - (q1 - 1 - t);
     return seen > 0 ? (seen + p.bs - 1) / p.bs : 0;
   };
   // this team's token: what needs no scores

@@ -1,7 +1,7 @@
 """Operators of long caches on a budget where their definitions are easily missed: calls that the documentation allows and that differ from the usual ones."""
 import pytest
 import torch
-from test_budget_gpu import CUDA, Cache, _ops
+from test_budget_gpu import CUDA, Cache, _check_attention, _gen, _ops, _select
 
 pytestmark = pytest.mark.gpu
 
@@ -19,3 +19,27 @@ def test_pages_that_are_not_there_weigh_nothing_beside_a_key_that_is_no_number(s
     there = torch.tensor([j // 16 != 2 for j in range(100)], device=CUDA)
     assert weights[0, 1, :100][there].isnan().all() and weights[0, 0].isfinite().all()
     assert weights[0, :, 32:48].eq(0).all() and weights[0, :, 100:].eq(0).all()
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv", [(8, 2), (4, 4), (24, 2)])
+@pytest.mark.parametrize("q_lens", [(20, 7), (20, 20)])
+def test_lengths_behind_the_table_of_several_tokens(q_lens, heads, kv, kind):
+    """They count as the table's end: the last token sees all of it and the ones in front of it a key less each, in either type and however tokens share their keys."""
+    ops = _ops()
+    c = Cache([64, 30], q_lens, heads=heads, kv_heads=kv, kind=kind, extra_pages=0)
+    lens = torch.tensor([1000, 30], dtype=torch.int32, device=CUDA)
+    for splits in (None, 1, 3, 9):
+        weights = torch.zeros(2, kv, 64, device=CUDA)
+        out = ops.tracked_attention(c.q, c.k, c.v, c.table, lens, weights, scale=0.1, num_splits=splits, **c.step)
+        _check_attention(c, out, lambda t, b, h, seen: range(seen), 0.1, weights=weights, before=torch.zeros_like(weights))
+    g = _gen(heads)
+    sums = ops.PageSummaries(torch.randint(-127, 128, (c.blocks, kv, 128), device=CUDA, generator=g).to(torch.int8), torch.rand(c.blocks, kv, device=CUDA, generator=g))
+    some = ops.select_pages(c.q, sums, c.table, lens, block_size=16, top=1, first=0, last=1, **c.step)
+    for t, b, seen in c.tokens():
+        for h in range(kv):
+            want = _select(c, sums, t, b, h, seen, 1, 0, 1)
+            assert some.pages[t, h].tolist() == want + [-1] * (2 - len(want)) and some.counts[t, h] == len(want)
+    out = ops.selected_attention(c.q, c.k, c.v, c.table, lens, some, scale=0.1, **c.step)
+    host = some.pages.cpu()
+    _check_attention(c, out, lambda t, b, h, seen: [p * 16 + i for p in host[t, h].tolist() if p >= 0 for i in range(16) if p * 16 + i < seen], 0.1)
