@@ -207,6 +207,7 @@ def _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, 
     else:
         _require(out.shape == (T, columns) and out.dtype == kind and out.stride(1) == 1, "out is [T, heads * value width] in the type of q, unit inner stride")
         out_stride = out.stride(0)
+        _require(out_stride >= columns or T <= 1, "rows of out share memory")
     k_ptr, v_ptr = kcache.data_ptr(), vcache.data_ptr()
     fast = kind is torch.bfloat16 and (D | Dv) % 8 == 0 and D <= 128 and Dv <= 128 and bs % 16 == 0 and (k_ptr | v_ptr) % 16 == 0 and blocks * heads * bs < 2 ** 31
     run = 1                                               # tokens of a sequence that share a problem
