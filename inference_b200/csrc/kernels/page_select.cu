@@ -570,7 +570,7 @@ int swb_page_select(const int* dims, const void* q, long long q_stride_tok, long
   const int T = dims[0], seqs = dims[1], uniform = dims[2], max_blocks = dims[3], blocks = dims[4], bs = dims[5], Hkv = dims[6], G = dims[7], D = dims[8];
   const int first = dims[9], top = dims[10], last = dims[11], fp32 = dims[12];
   if (T <= 0 || seqs <= 0) return 0;
-  if ((long long)seqs * uniform * Hkv > INT_MAX / 8 || bs < 1 || Hkv < 1 || G < 1 || D < 1 || blocks < 1 || max_blocks < 1 || first < 0 || top < 0 || last < 1 || uniform < 1 || D > 256 || (long long)max_blocks * bs > INT_MAX || !q || !codes ||
+  if ((long long)seqs * uniform * Hkv > INT_MAX / 8 || bs < 1 || Hkv < 1 || G < 1 || D < 1 || blocks < 1 || max_blocks < 1 || first < 0 || top < 0 || last < 1 || (long long)first + top + last > INT_MAX || uniform < 1 || D > 256 || (long long)max_blocks * bs > INT_MAX || !q || !codes ||
       !scales || !table || !kv_lens || !pages || !counts)
     return -3;
   // a token's histogram, codes and scores in one block's shared memory

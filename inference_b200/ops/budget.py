@@ -161,6 +161,7 @@ def select_pages(q: torch.Tensor, summaries: PageSummaries, block_table: torch.T
     _require(block_size >= 1 and top >= 0 and first >= 0 and last >= 1, "block_size >= 1, top >= 0, first >= 0, last >= 1")
     _require(per <= MAX_PAGES, "a selection is made over at most 40000 pages")
     width, rows = first + top + last, T * heads
+    _require(width < 2 ** 31, "a selection lists fewer than 2^31 pages")
     both = q.new_empty(rows * (width + 1), dtype=torch.int32)
     pages, counts = both.as_strided((T, heads, width), (heads * width, width, 1)), both.as_strided((T, heads), (heads, 1), rows * width)
     dims = _INTS[14](T, n, max_q_len, per, blocks, block_size, heads, G, D, first, top, last, q.dtype == torch.float32, 0)

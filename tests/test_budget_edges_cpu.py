@@ -16,3 +16,20 @@ def test_results_whose_rows_share_memory_are_refused(name, stride):
     a["out"] = a["out"].as_strided((T, H * D), (H * D, 1))
     with pytest.raises(AssertionError, match="was launched"):
         _call(name, a)
+
+
+@pytest.mark.parametrize("top,first,last", [(2 ** 31 - 1, 1, 4), (2 ** 31, 0, 1), (2 ** 30, 2 ** 30, 1), (1, 2 ** 31 - 2, 1), (1, 0, 2 ** 40)])
+def test_selections_whose_width_passes_32_bits_are_refused(top, first, last):
+    a = _args() | {"top": top, "first": first, "last": last}
+    with pytest.raises(KernelError, match="2\\^31"):
+        _call("select", a)
+
+
+def test_the_library_refuses_a_selection_whose_width_passes_32_bits():
+    """Whoever calls it: the check stands in front of the launch (the pointers are not read)."""
+    from inference_b200._native import kernels
+    from inference_b200.ops.budget import _INTS
+
+    at = 1 << 20
+    dims = _INTS[14](1, 1, 1, 8, 20, 4, KV, 2, D, 2 ** 30, 2 ** 30, 1, 0, 0)
+    assert kernels().swb_page_select(dims, at, D, D, at, at, at, 8, None, at, at, at, None) == -3
