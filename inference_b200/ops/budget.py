@@ -115,6 +115,7 @@ def _check_step(table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor |
     _require(len(lens) == 1 and len(rows) == 2 and rows[0] == lens[0] < 65536 and rows[1] >= 1 and table.dtype == kv_lens.dtype == torch.int32 and table.stride(1) == 1
              and kv_lens.is_contiguous(), "block_table is int32 [num_seqs, pages] with rows of unit stride, kv_lens int32 [num_seqs], up to 65535 sequences of a page at least")
     n = lens[0]
+    _require(max_q_len < 2 ** 31, "max_q_len is below 2^31")
     if cu_q is None:
         _require(max_q_len >= 1 and (tokens < 0 or tokens == n * max_q_len), "without cu_q every sequence has max_q_len >= 1 tokens")
     else:
@@ -158,7 +159,7 @@ def select_pages(q: torch.Tensor, summaries: PageSummaries, block_table: torch.T
     _require(q.dtype in _KINDS, "q is bf16 or fp32")
     T, G, tok, head = _check_rows(q, heads, D)
     n, per = _check_step(block_table, kv_lens, cu_q, max_q_len, T)
-    _require(block_size >= 1 and top >= 0 and first >= 0 and last >= 1, "block_size >= 1, top >= 0, first >= 0, last >= 1")
+    _require(1 <= block_size < 2 ** 31 and top >= 0 and first >= 0 and last >= 1, "1 <= block_size < 2^31, top >= 0, first >= 0, last >= 1")
     _require(per <= MAX_PAGES, "a selection is made over at most 40000 pages")
     width, rows = first + top + last, T * heads
     _require(width < 2 ** 31, "a selection lists fewer than 2^31 pages")
@@ -281,7 +282,7 @@ def evict_tokens(kcache: torch.Tensor, vcache: torch.Tensor, block_table: torch.
     _check_entries(weights, torch.float32, n, heads, capacity, "weights")
     _check_entries(positions, torch.int32, n, heads, capacity, "positions")
     _require(next_positions.dtype == torch.int32 and next_positions.shape == (n,) and next_positions.is_contiguous(), "next_positions are int32 [num_seqs]")
-    _require(keep >= 1 and recent >= 0 and first >= 0 and recent + first <= keep, "0 <= first, recent; 1 <= keep; first + recent <= keep")
+    _require(1 <= keep < 2 ** 31 and recent >= 0 and first >= 0 and recent + first <= keep, "0 <= first, recent; 1 <= keep < 2^31; first + recent <= keep")
     device, room = kcache.device, 2 * n * heads * max(0, min(keep, capacity - keep))
     moves = torch.empty(room, dtype=torch.int32, device=device)
     lens = torch.empty(n, dtype=torch.int32, device=device)

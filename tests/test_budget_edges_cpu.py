@@ -33,3 +33,12 @@ def test_the_library_refuses_a_selection_whose_width_passes_32_bits():
     at = 1 << 20
     dims = _INTS[14](1, 1, 1, 8, 20, 4, KV, 2, D, 2 ** 30, 2 ** 30, 1, 0, 0)
     assert kernels().swb_page_select(dims, at, D, D, at, at, at, 8, None, at, at, at, None) == -3
+
+
+@pytest.mark.parametrize("name,key", [("summaries", "max_q"), ("select", "max_q"), ("selected", "max_q"), ("tracked", "max_q"), ("select", "bs"), ("evict", "keep")])
+def test_sizes_behind_32_bits_are_refused_as_arguments(name, key):
+    a = _args() | {key: 2 ** 31}
+    if key == "max_q":
+        a["cu"] = torch.zeros(B + 1, dtype=torch.int32)
+    with pytest.raises(KernelError):
+        _call(name, a)
