@@ -42,8 +42,9 @@ __device__ __forceinline__ long long summary_place(const SummaryParams& p, int h
   const int seq = blockIdx.z;
   const int q_len = p.cu_q ? p.cu_q[seq + 1] - p.cu_q[seq] : p.uniform_q;
   const int len = min(p.kv_lens[seq], p.max_blocks * p.bs);
-  const int page = max(len - q_len, 0) / p.bs + blockIdx.x;      // the first page that the new tokens can complete, and on
-  if ((page + 1) * p.bs > len || q_len <= 0) return -1;
+  if (len <= 0 || q_len <= 0) return -1;
+  const unsigned page = (unsigned)(max(len - q_len, 0) / p.bs) + blockIdx.x;      // the first page that the new tokens can complete, and on
+  if (page >= (unsigned)(len / p.bs)) return -1;
   const int block = p.table[seq * p.table_stride + page];
   return (unsigned)block < (unsigned)p.num_blocks ? (long long)block * p.Hkv + h : -1;
 }
@@ -538,7 +539,7 @@ int swb_page_summaries(const int* dims, const void* k, void* codes, void* scales
   using namespace swb;
   const int seqs = dims[0], max_q = dims[1], max_blocks = dims[2], blocks = dims[3], bs = dims[4], Hkv = dims[5], D = dims[6], fp32 = dims[7];
   if (seqs <= 0 || max_q <= 0 || max_blocks <= 0) return 0;
-  if (bs < 1 || Hkv < 1 || D < 1 || D > 256 || blocks < 1 || seqs > 65535 || !k || !codes || !scales || !table || !kv_lens) return -3;
+  if (bs < 1 || Hkv < 1 || D < 1 || D > 256 || blocks < 1 || seqs > 65535 || (long long)max_blocks * bs > INT_MAX || !k || !codes || !scales || !table || !kv_lens) return -3;
   const SummaryParams p{k, reinterpret_cast<int8_t*>(codes), reinterpret_cast<float*>(scales), table, table_stride, max_blocks, blocks, bs, Hkv, D, cu_q, kv_lens, seqs, max_q};
   // n new tokens complete at most (n + bs - 1) / bs pages
   const dim3 grid((max_q - 1) / bs + 1, (Hkv + SUMMARY_WARPS - 1) / SUMMARY_WARPS, seqs);

@@ -42,3 +42,12 @@ def test_sizes_behind_32_bits_are_refused_as_arguments(name, key):
         a["cu"] = torch.zeros(B + 1, dtype=torch.int32)
     with pytest.raises(KernelError):
         _call(name, a)
+
+
+def test_the_library_refuses_summaries_of_a_table_for_2_to_the_31_tokens():
+    """As it refuses such a table for the other operators: places in a sequence are 32-bit numbers. (The pointers are not read.)"""
+    from inference_b200._native import kernels
+    from inference_b200.ops.budget import _INTS
+
+    at = 1 << 20
+    assert kernels().swb_page_summaries(_INTS[9](1, 1, 2 ** 27, 20, 16, KV, D, 0, 0), at, at, at, at, 2 ** 27, None, at, None) == -3
