@@ -311,6 +311,7 @@ __global__ void __launch_bounds__(SELECT_THREADS, KS == 8 ? 2 : TT == 1 && !CL ?
   __syncthreads();
 
   constexpr int NT = TT == 4 ? 2 : 1;              // products beside each other: TT Gp <= 8 NT, or one token in turns of 8 heads
+  static_assert(TT == 1 || TT * GP <= 8 * NT, "every token of a block has columns");
   const int gr = lane >> 2, t4 = lane & 3;
   int Gp = GP ? GP : 1;
   while (!GP && Gp < p.G && Gp < 8) Gp <<= 1;
@@ -516,9 +517,11 @@ int launch_select(SelectParams p, cudaStream_t s) {
   while (p.share < 8 && p.share * 512 <= p.max_blocks && problems * p.share * 2 <= 2 * 148) p.share *= 2;
   if (p.share > 1) return launch_select<1, KS, FULL, GP, true>(p, s);
   const int TT = select_tokens(p.uniform_q, p.G, p.max_blocks);
-  if constexpr (GP != 8)
+  if constexpr (GP != 8) {                         // eight heads fill a product's columns with one token
     if (TT == 4) return launch_select<4, KS, FULL, GP>(p, s);
-  return TT == 2 ? launch_select<2, KS, FULL, GP>(p, s) : launch_select<1, KS, FULL, GP>(p, s);
+    if (TT == 2) return launch_select<2, KS, FULL, GP>(p, s);
+  }
+  return launch_select<1, KS, FULL, GP>(p, s);
 }
 
 // Groups of 3 or 4 and of 5 to 8 heads of 128 columns have kernels of their own: without the choice of the reduction and the ends of rows in the loop they
