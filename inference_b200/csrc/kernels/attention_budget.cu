@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
     if (p.cu_q && t >= p.cu_q[p.num_seqs]) return;
     tok = token_of(p, t);
   } else {
-    const int runs = (p.uniform_q + p.run - 1) / p.run;
+    const int runs = (p.uniform_q - 1) / p.run + 1;
     tok.seq = t / runs;
     const int q0 = p.cu_q ? p.cu_q[tok.seq] : tok.seq * p.uniform_q, q1 = p.cu_q ? p.cu_q[tok.seq + 1] : q0 + p.uniform_q;
     t = q0 + t % runs * p.run;
@@ -706,7 +706,7 @@ int launch_fast(BudgetParams p, cudaStream_t s) {
   rc = make_tmap(&tv, p.v, rows, p.Dv, p.Dv, 16);
   if (rc) return rc;
   const bool one = p.G * p.run <= 8, wide = p.D == 128 && p.Dv == 128;
-  const int problems = (p.run > 1 ? p.num_seqs * ((p.uniform_q + p.run - 1) / p.run) : p.tokens) * p.Hkv * p.head_tiles;
+  const int problems = (p.run > 1 ? p.num_seqs * ((p.uniform_q - 1) / p.run + 1) : p.tokens) * p.Hkv * p.head_tiles;
   const bool many = one && (long long)problems * p.num_splits >= 9 * 148;
   const int smem = fast_smem_bytes(many ? 2 : 3), which = (many ? 2 : one) + 3 * wide;
   using Kernel = decltype(&attn_budget_kernel<1, 2, true>);
@@ -788,7 +788,7 @@ __global__ void __launch_bounds__(JOIN_THREADS, SPLIT ? 1 : 16) attn_budget_fini
   const int h = i / blocks % p.Hkv, seq = i / blocks / p.Hkv;
   const int first = i % blocks * RUN, at = ((SPLIT ? 0 : warp * 32) + lane) * V;      // of the block, and of this lane behind it
   const int q0 = max(p.cu_q ? p.cu_q[seq] : seq * p.uniform_q, 0), q1 = p.cu_q ? p.cu_q[seq + 1] : q0 + p.uniform_q;
-  const int q_end = min(min(q1, p.tokens), q0 + p.uniform_q);      // tokens whose scores are there
+  const int q_end = q0 + min(min(q1, p.tokens) - q0, p.uniform_q);      // tokens whose scores are there
   const int len = length_of(p, seq);
   if (first >= len) return;
   const int room = len - first - at;
@@ -953,7 +953,8 @@ int swb_attn_budget(const int* dims, const long long* strides, const void* q, vo
   // tokens of one sequence read the same keys: as many as rows allow share a problem
   p.run = 1;
   while (fast && !pages && p.run * 2 * p.G <= ROWS && p.run < p.uniform_q) p.run *= 2;
-  const long long problems = (p.run > 1 ? (long long)p.num_seqs * ((p.uniform_q + p.run - 1) / p.run) : p.tokens) * p.Hkv * p.head_tiles;
+  const long long problems = (p.run > 1 ? (long long)p.num_seqs * ((p.uniform_q - 1) / p.run + 1) : p.tokens) * p.Hkv * p.head_tiles;
+  if (problems > INT_MAX / p.num_splits) return -3;
   // Blocks of a cluster start together and wait for one another, which costs nothing while all of them fit the chip at once; behind that a second launch is cheaper
   // (48 sequences of up to 8191 keys, 8 key/value heads, 4 splits: 305 us as clusters, 213 with a second launch)
   const bool own_weights = fast && p.uniform_q == 1 && p.head_tiles == 1;       // else there is a second launch in any case

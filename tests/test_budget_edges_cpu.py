@@ -51,3 +51,14 @@ def test_the_library_refuses_summaries_of_a_table_for_2_to_the_31_tokens():
 
     at = 1 << 20
     assert kernels().swb_page_summaries(_INTS[9](1, 1, 2 ** 27, 20, 16, KV, D, 0, 0), at, at, at, at, 2 ** 27, None, at, None) == -3
+
+
+def test_the_library_refuses_a_grid_of_more_than_2_to_the_31_blocks():
+    """Tokens that share their keys are dealt out by the longest step a sequence may have, which can be many more blocks than there are tokens."""
+    from inference_b200._native import kernels
+    from inference_b200.ops.budget import _INTS, _LONGS
+
+    at, seqs, most = 1 << 20, 65535, 2 ** 20
+    dims = _INTS[16](8, seqs, most, 1, 20, 16, 1, 1, 128, 128, 0, 1, 0, 0, 0, 0)
+    strides = _LONGS[8](128, 128, 128, 1, 16, 16, 0, 0)
+    assert kernels().swb_attn_budget(dims, strides, at, at, at, at, at, at, at, None, None, at, 1.0, 0.0, at, 1 << 20, None) == -3

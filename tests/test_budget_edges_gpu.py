@@ -43,3 +43,14 @@ def test_lengths_behind_the_table_of_several_tokens(q_lens, heads, kv, kind):
     out = ops.selected_attention(c.q, c.k, c.v, c.table, lens, some, scale=0.1, **c.step)
     host = some.pages.cpu()
     _check_attention(c, out, lambda t, b, h, seen: [p * 16 + i for p in host[t, h].tolist() if p >= 0 for i in range(16) if p * 16 + i < seen], 0.1)
+
+
+def test_the_largest_bound_of_a_step():
+    """max_q_len is a bound, and the largest number is one."""
+    ops = _ops()
+    c = Cache([40, 70, 20], [2, 3, 1], heads=24, kv_heads=2)
+    for kind in (torch.bfloat16, torch.float32):
+        c.q, c.k, c.v, c.kind = c.q.to(kind), c.k.to(kind), c.v.to(kind), kind
+        weights = torch.zeros(3, 2, c.per * 16, device=CUDA)
+        out = ops.tracked_attention(c.q, c.k, c.v, c.table, c.kv_lens, weights, scale=0.1, cu_q=c.cu, max_q_len=2 ** 31 - 1)
+        _check_attention(c, out, lambda t, b, h, seen: range(seen), 0.1, weights=weights, before=torch.zeros_like(weights))
