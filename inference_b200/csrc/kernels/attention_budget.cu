@@ -60,6 +60,9 @@ struct BudgetParams {
 // Cached tokens of a sequence; a length that the table has no pages for is the table's end, and the last new token's place is there.
 __device__ __forceinline__ int length_of(const BudgetParams& p, int seq) { return min(p.kv_lens[seq], p.max_blocks * p.bs); }
 
+// Rows of q in front of the first sequence's and behind the last one's.
+__device__ __forceinline__ bool of_no_sequence(const BudgetParams& p, int t) { return p.cu_q && (t < p.cu_q[0] || t >= p.cu_q[p.num_seqs]); }
+
 // What a query token is: its sequence and the keys it sees.
 struct Token {
   int seq, q0, q_len, seen;
@@ -125,7 +128,7 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_budget_plain_kernel(const 
   const int split = blockIdx.x % p.num_splits, y = blockIdx.x / p.num_splits, hy = y % (p.Hkv * p.head_tiles), t = y / (p.Hkv * p.head_tiles);
   const int h = hy / p.head_tiles, ht = hy % p.head_tiles, g0 = ht * ROWS, rows = min(R, p.G - g0);
   pdl_wait();
-  if (p.cu_q && t >= p.cu_q[p.num_seqs]) return;
+  if (of_no_sequence(p, t)) return;
   const Token tok = token_of(p, t);
   const size_t list = (size_t)t * p.Hkv + h;
   const int count = p.pages ? min(max(p.counts[list], 0), p.width) : 0;
@@ -331,7 +334,7 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
   int t = y / per_token, tokens = 1;                // first token, and how many
   Token tok;
   if (p.run == 1) {
-    if (p.cu_q && t >= p.cu_q[p.num_seqs]) return;
+    if (of_no_sequence(p, t)) return;
     tok = token_of(p, t);
   } else {
     const int runs = (p.uniform_q - 1) / p.run + 1;
@@ -772,7 +775,7 @@ __global__ void __launch_bounds__(JOIN_THREADS, SPLIT ? 1 : 16) attn_budget_fini
   pdl_wait();
   if ((int)blockIdx.x < join_blocks) {
     const int t = blockIdx.x / Hq, head = blockIdx.x % Hq;
-    if (p.cu_q && t >= p.cu_q[p.num_seqs]) return;
+    if (of_no_sequence(p, t)) return;
     if (warp == 0) split_factors(p.part_ml + part_at(p, t, head, 0) * 2, S, lane, s_factor);
     __syncthreads();
     for (int d = tid; d < p.Dv; d += JOIN_THREADS) {

@@ -10,8 +10,8 @@ Two ways to spend less than the whole cache on a new token, both beside `paged_a
 Caches are one layer's pages [blocks, kv heads, block_size, width] with the block tables of `PagedSequence`. bf16, or fp32 in the 32-bit mode; widths up to 256.
 Calls run on the current stream, take no host reads and can be captured into graphs; buffers that a call fills (summaries, weights, positions, the cache) belong
 to the caller. Steps are described as in `paged_attention`: kv_lens int32 [num_seqs] counts a sequence's tokens with the new ones, cu_q int32 [num_seqs + 1]
-are the new tokens' ranges within the rows of q and max_q_len bounds a sequence's number (None: every sequence has max_q_len of them); rows behind the last range
-are left as they were. Lengths beyond a table's pages count as the table's end (the last new token sees the whole table, the one before it a key less), and pages whose
+are the new tokens' ranges within the rows of q and max_q_len bounds a sequence's number (None: every sequence has max_q_len of them); rows in front of the first range
+and behind the last are left as they were. Lengths beyond a table's pages count as the table's end (the last new token sees the whole table, the one before it a key less), and pages whose
 number is not in the cache are passed over."""
 from __future__ import annotations
 

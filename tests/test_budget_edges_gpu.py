@@ -54,3 +54,24 @@ def test_the_largest_bound_of_a_step():
         weights = torch.zeros(3, 2, c.per * 16, device=CUDA)
         out = ops.tracked_attention(c.q, c.k, c.v, c.table, c.kv_lens, weights, scale=0.1, cu_q=c.cu, max_q_len=2 ** 31 - 1)
         _check_attention(c, out, lambda t, b, h, seen: range(seen), 0.1, weights=weights, before=torch.zeros_like(weights))
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads", [8, 24])
+@pytest.mark.parametrize("splits", [1, 2, 9])
+def test_rows_in_front_of_the_first_sequence_stay(splits, heads, kind):
+    """As those behind the last one do: rows of no sequence."""
+    ops = _ops()
+    c = Cache([40, 70], [2, 3], heads=heads, kind=kind, behind=5)
+    at, front = torch.full((10, 2), 3, dtype=torch.int32, device=CUDA), c.cu + 3
+    pages = torch.arange(3, dtype=torch.int32, device=CUDA).expand(10, 2, 3).contiguous()
+    q = c.q
+    weights, out = torch.zeros(2, 2, c.per * 16, device=CUDA), torch.full((10, heads * 128), 7.0, dtype=kind, device=CUDA)
+    some = out.clone()
+    ops.tracked_attention(q, c.k, c.v, c.table, c.kv_lens, weights, scale=0.1, num_splits=splits, out=out, cu_q=front, max_q_len=3)
+    ops.selected_attention(q, c.k, c.v, c.table, c.kv_lens, ops.PageSelection(pages, at), scale=0.1, num_splits=splits, out=some, cu_q=front, max_q_len=3)
+    for x in (out, some):
+        assert x[:3].eq(7).all() and x[8:].eq(7).all()
+    c.q = q[3:]
+    _check_attention(c, out[3:], lambda t, b, h, seen: range(seen), 0.1, weights=weights, before=torch.zeros_like(weights))
+    _check_attention(c, some[3:], lambda t, b, h, seen: range(min(seen, 48)), 0.1)
