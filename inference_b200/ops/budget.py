@@ -243,7 +243,9 @@ def tracked_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tenso
                       cu_q: torch.Tensor | None, max_q_len: int, scale: float, softcap: float = 0.0, num_splits: int | None = None,
                       out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of every new token over all keys that it sees -> [T, Hq * Dv], which also adds the softmax weights of the step, summed over its tokens and the query heads of
-    a group, to weights fp32 [num_seqs, kv heads, >= table pages * block_size] (unit inner stride; entry j of a row belongs to cache entry j).
+    a group, to weights fp32 [num_seqs, kv heads, >= table pages * block_size] (unit inner stride; entry j of a row belongs to cache entry j). Entries behind a sequence's
+    length are not touched. A new token's entry starts from what the row holds: a caller who takes tokens back (drafts that were not accepted) sets their weights to 0, as
+    `weights.masked_fill_(torch.arange(N) >= kv_lens[:, None, None], 0)` does for all sequences.
 
     For decode steps, and for the last tokens of a prompt: keys are read once for every 16 rows (tokens * heads of a group) of a sequence, and scores are kept until the sums
     are known, 4 bytes a token, query head and key of the table's width."""
@@ -272,8 +274,9 @@ def evict_tokens(kcache: torch.Tensor, vcache: torch.Tensor, block_table: torch.
     A head keeps the entries whose position is below `first` or among the last `recent` in front of next_positions int32 [num_seqs] (the position of the
     sequence's next token), and of the others those of largest weight (fp32 [num_seqs, kv heads, N], as `tracked_attention` adds them up; ties: the lowest index). Entries that stay
     and lie behind `keep` move in order into the holes in front of it: their rows of both caches, weight and position. positions int32 [num_seqs, kv heads, N]: -1 for
-    entries without a record, which stand in order in front of the next position (all of them before the first call); the call records those it keeps. Weights behind `keep` become 0, positions -1.
-    Everything is done in place. Pages must not be
+    entries without a record, which stand in order in front of the next position (all of them before the first call); the call records those it keeps. Of a sequence that
+    shrinks the weights of entries keep to L - 1 (L: its length) become 0 and the positions from `keep` to the row's end -1; weights behind L stay as they were, and so does all of a
+    sequence of no more than `keep` tokens. Everything is done in place. Pages must not be
     shared with a sequence that is not to lose tokens, nor between sequences of the call."""
     stream = _place(kcache, vcache, block_table, kv_lens, weights, positions, next_positions)
     blocks, heads, bs, D, Dv = _check_cache(kcache, vcache)

@@ -75,3 +75,40 @@ def test_rows_in_front_of_the_first_sequence_stay(splits, heads, kind):
     c.q = q[3:]
     _check_attention(c, out[3:], lambda t, b, h, seen: range(seen), 0.1, weights=weights, before=torch.zeros_like(weights))
     _check_attention(c, some[3:], lambda t, b, h, seen: range(min(seen, 48)), 0.1)
+
+
+@pytest.mark.parametrize("cleared", [True, False])
+def test_evictions_after_tokens_were_taken_back(cleared):
+    """Weights of drafts that were taken back are the caller's to clear, whether or not the sequence shrinks then: an eviction leaves what lies behind a sequence's length, and
+    the tokens that are appended there go on from it. Cleared, everything is as if the drafts had never been."""
+    ops = _ops()
+    keep, results = 60, []
+    for drafts in (0, 7):
+        c = Cache([100, 50], [1, 1], seed=3, filler=0.0)
+        weights = torch.zeros(2, 2, c.per * 16, device=CUDA)
+        positions = torch.full((2, 2, c.per * 16), -1, dtype=torch.int32, device=CUDA)
+        lens = c.kv_lens.clone()
+
+        def step(q, c=c, weights=weights, lens=lens):
+            return ops.tracked_attention(q, c.k, c.v, c.table, lens, weights, scale=0.1, cu_q=None, max_q_len=q.shape[0] // 2)
+
+        step(c.q)
+        if drafts:
+            lens += drafts
+            step(torch.randn(2 * drafts, 8, 128, device=CUDA, generator=_gen(5)).bfloat16())
+            lens -= drafts
+            stale = weights.clone()
+            at = torch.arange(c.per * 16, device=CUDA)
+            assert (stale[0, :, 100:107] > 0).all() and (stale[1, :, 50:57] > 0).all()
+            weights.copy_(seen)                        # what the drafts gave to the entries that stay is theirs: here only the rest is looked at
+            weights += stale * (at >= lens[:, None, None])
+            if cleared:
+                weights.masked_fill_(at >= lens[:, None, None], 0)
+        seen = weights.clone()
+        lens.copy_(ops.evict_tokens(c.k, c.v, c.table, lens, weights, positions, torch.tensor([100, 50], dtype=torch.int32, device=CUDA), keep=keep, recent=5, first=2))
+        assert lens.tolist() == [60, 50]
+        assert weights[0, :, keep:100].eq(0).all() and positions[0, :, keep:].eq(-1).all() and positions[1].eq(-1).all()
+        assert torch.equal(weights[0, :, 100:], seen[0, :, 100:]) and torch.equal(weights[1], seen[1])
+        results.append((weights.clone(), positions.clone(), c.k.clone(), c.v.clone()))
+    same = [torch.equal(a, b) for a, b in zip(*results)]
+    assert same == [cleared, True, True, True]
