@@ -44,8 +44,8 @@ class ModelRunner:
 
     def __init__(self, model: LlamaGpu, pool: PagedKvPool, max_batch: int = 64, max_seq_len: int = 8192,
                  use_graphs: bool = True, page_budget=None):
-        """page_budget (`ops.PageBudget`): steps of as few tokens a sequence as a decode step (one, drafts that are verified, a prompt of that length) read the pages
-        that are selected for each token and key/value head; longer and ragged ones read everything. For the decoders of the Llama family on one uniform pool."""
+        """page_budget (`ops.PageBudget`): decode steps, and steps that verify drafts (`prefill` with all_positions), read the pages that are selected for each token and
+        key/value head, however many tokens they have; prompts read everything, in whatever pieces they come. For the decoders of the Llama family on one uniform pool."""
         self.model, self.pool = model, pool
         self.page_budget = page_budget
         if page_budget is not None and not (isinstance(model, LlamaGpu) and isinstance(pool, PagedKvPool)):
@@ -108,7 +108,8 @@ class ModelRunner:
         image placeholders of a vision-language prompt). mrope_overrides[i] = (positions [3, len(new_tokens[i])], next
         position, rows within new_tokens[i], taps) gives those tokens three-axis rotary positions and adds taps[l] to
         the residual stream at `rows` after decoder layer l; the sequence's later tokens continue at `next position`
-        (kept on the sequence as `rope_delta`). want[i] = places within new_tokens[i]: returns the fp32 logits of exactly
+        (kept on the sequence as `rope_delta`). all_positions: the fp32 logits of every token, as a step that verifies drafts asks for; with a page budget such a step reads what
+        decode steps would. want[i] = places within new_tokens[i]: returns the fp32 logits of exactly
         these places, sequence by sequence [sum of len(want[i]), vocab]."""
         dev = self.model.device
         ids, pos, slots, cu, kvl, rows = [], [], [], [0], [], []
@@ -138,7 +139,7 @@ class ModelRunner:
             num_seqs=len(seqs), decode=decode, fresh_prefill=fresh and not decode,
             attn_splits=self._splits(len(seqs), max(kvl)) if decode else 1,
             logits_rows=None if all_positions else d_rows,
-            page_budget=self.page_budget, summaries=self._summaries(),
+            page_budget=self.page_budget if all_positions else None, summaries=self._summaries(),
             spans=[(len(t), n) for t, n in zip(new_tokens, kvl)])
         if self._stateful:
             inp.state_slots = d_states

@@ -45,7 +45,7 @@ class StepInputs:
     #                                           to the residual stream at those rows after decoder layer l (Qwen3-VL)
     state_slots: torch.Tensor | None = None    # int32 [num_seqs]: slot of each sequence's recurrent state (-1 = do not
     #                                           touch any: a padding row); None for models without recurrent layers
-    page_budget: "ops.PageBudget | None" = None    # decode steps read the pages that it selects for each token ...
+    page_budget: "ops.PageBudget | None" = None    # not None: the step reads the pages that it selects for each token ...
     summaries: list | None = None              # ... by these summaries, one `ops.PageSummaries` a layer, which every step keeps up
     spans: list[tuple[int, int]] | None = None # host copy of (new tokens, context length) per sequence; None in a decode
     #                                           step (one token each, lengths change under a captured graph)
@@ -461,7 +461,7 @@ class LlamaGpu:
             if inp.summaries is not None:
                 ops.summarize_pages(kv_pool[li, 0], inp.block_table, inp.kv_lens, inp.summaries[li], cu_q=inp.cu_q, max_q_len=inp.max_q_len)
                 n += 1
-            if inp.page_budget is not None and inp.decode:
+            if inp.page_budget is not None:
                 budget = inp.page_budget
                 chosen = ops.select_pages(q, inp.summaries[li], inp.block_table, inp.kv_lens, cu_q=inp.cu_q, max_q_len=inp.max_q_len, block_size=block_size,
                                           top=budget.top, first=budget.first, last=budget.last)

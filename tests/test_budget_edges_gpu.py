@@ -1,7 +1,7 @@
 """Operators of long caches on a budget where their definitions are easily missed: calls that the documentation allows and that differ from the usual ones."""
 import pytest
 import torch
-from test_budget_gpu import CUDA, Cache, _check_attention, _gen, _ops, _select
+from test_budget_gpu import CUDA, Cache, _check_attention, _engine, _gen, _ops, _prompts, _select
 
 pytestmark = pytest.mark.gpu
 
@@ -112,3 +112,57 @@ def test_evictions_after_tokens_were_taken_back(cleared):
         results.append((weights.clone(), positions.clone(), c.k.clone(), c.v.clone()))
     same = [torch.equal(a, b) for a, b in zip(*results)]
     assert same == [cleared, True, True, True]
+
+
+# ---- in the engine ------------------------------------------------------------------------------------------------------------------------------------
+@pytest.fixture
+def read_by_pages(monkeypatch):
+    """What selected_attention was called with, and gave."""
+    ops, seen = _ops(), []
+    real = ops.selected_attention
+
+    def spy(q, k, v, table, lens, sel, **kw):
+        out = real(q, k, v, table, lens, sel, **kw)
+        seen.append((q.clone(), k, v, table.clone(), lens.clone(), sel, kw, out.clone()))
+        return out
+
+    monkeypatch.setattr(ops, "selected_attention", spy)
+    return seen
+
+
+def test_a_prompt_reads_everything_in_whatever_pieces_it_comes(read_by_pages):
+    ops = _ops()
+    pieces = [_prompts()[0], [5, 6, 7], _prompts()[1], [1, 2], [3, 4, 5, 6, 7, 8, 9, 10]]
+    runs = []
+    for budget in (None, ops.PageBudget(top=1, first=0, last=1)):
+        eng = _engine(budget)
+        seq = eng.new_sequence()
+        runs.append([eng.runner.prefill([seq], [p], want_logits=True) for p in pieces])
+        runs[-1].append(eng.runner.prefill([seq], [[11, 12, 13]], want=[[0, 2]]))
+    assert all(torch.equal(a, b) for a, b in zip(*runs)) and not read_by_pages
+
+
+@pytest.mark.parametrize("drafts", [0, 1, 4, 8, 20])
+def test_verified_drafts_read_what_decode_steps_would(drafts, read_by_pages):
+    """However many there are, of one sequence or of several with numbers of their own, in front of and behind the end of a page; and after a rollback."""
+    ops = _ops()
+    eng = _engine(ops.PageBudget(top=2, first=1, last=1))
+    seqs = [eng.new_sequence(), eng.new_sequence()]
+    eng.runner.prefill(seqs, [_prompts()[0], _prompts()[2]])
+    ids = [[7 + i for i in range(drafts + 1)], [9, 8]]
+    for group, new in ((seqs[:1], ids[:1]), (seqs, ids)):
+        base = [s.length for s in group]
+        read_by_pages.clear()
+        got = eng.runner.prefill(group, new, all_positions=True)
+        assert got.shape == (sum(map(len, new)), 2048) and len(read_by_pages) == 3
+        for layer, (q, k, v, table, lens, sel, kw, out) in enumerate(read_by_pages):
+            c = Cache([s.length for s in group], [len(n) for n in new], heads=4, kv_heads=2)
+            c.k, c.v, c.table, c.q, c.blocks = k, v, table, q, k.shape[0]
+            host = sel.pages.cpu()
+            for t, b, seen in c.tokens():
+                for h in range(2):
+                    want = _select(c, eng.pool.summaries[layer], t, b, h, seen, 2, 1, 1)
+                    assert host[t, h].tolist() == want + [-1] * (4 - len(want))
+            _check_attention(c, out, lambda t, b, h, n: [p * 16 + i for p in host[t, h].tolist() if p >= 0 for i in range(16) if p * 16 + i < n], kw["scale"])
+        for s, n in zip(group, base):
+            s.truncate(n + 1)
