@@ -45,7 +45,7 @@ class ModelRunner:
     def __init__(self, model: LlamaGpu, pool: PagedKvPool, max_batch: int = 64, max_seq_len: int = 8192,
                  use_graphs: bool = True, page_budget=None):
         """page_budget (`ops.PageBudget`): decode steps, and steps that verify drafts (`prefill` with all_positions), read the pages that are selected for each token and
-        key/value head, however many tokens they have; prompts read everything, in whatever pieces they come. For the decoders of the Llama family on one uniform pool."""
+        key/value head, however many tokens they have; prompts read everything, in whatever pieces they come (one token a sequence is a decode step). For the decoders of the Llama family on one uniform pool."""
         self.model, self.pool = model, pool
         self.page_budget = page_budget
         if page_budget is not None and not (isinstance(model, LlamaGpu) and isinstance(pool, PagedKvPool)):
@@ -139,7 +139,7 @@ class ModelRunner:
             num_seqs=len(seqs), decode=decode, fresh_prefill=fresh and not decode,
             attn_splits=self._splits(len(seqs), max(kvl)) if decode else 1,
             logits_rows=None if all_positions else d_rows,
-            page_budget=self.page_budget if all_positions else None, summaries=self._summaries(),
+            page_budget=self.page_budget if all_positions or max_q == 1 else None, summaries=self._summaries(),
             spans=[(len(t), n) for t, n in zip(new_tokens, kvl)])
         if self._stateful:
             inp.state_slots = d_states

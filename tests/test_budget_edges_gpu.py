@@ -142,6 +142,19 @@ def test_a_prompt_reads_everything_in_whatever_pieces_it_comes(read_by_pages):
     assert all(torch.equal(a, b) for a, b in zip(*runs)) and not read_by_pages
 
 
+def test_more_sequences_than_a_decode_batch_are_a_step_too(read_by_pages):
+    from inference_b200.engine.backend import GpuBackend
+
+    ops = _ops()
+    eng = _engine(ops.PageBudget(top=1, first=1, last=1))
+    backend = GpuBackend(eng.runner)
+    seqs = [backend.new_sequence() for _ in range(9)]
+    backend.forward(seqs, [[i + k for k in range(50 + 4 * i)] for i in range(9)])
+    assert not read_by_pages
+    backend.forward_greedy(seqs, [[i] for i in range(9)])
+    assert len(read_by_pages) == 3 and all(x[0].shape[0] == 9 for x in read_by_pages)
+
+
 @pytest.mark.parametrize("drafts", [0, 1, 4, 8, 20])
 def test_verified_drafts_read_what_decode_steps_would(drafts, read_by_pages):
     """However many there are, of one sequence or of several with numbers of their own, in front of and behind the end of a page; and after a rollback."""
