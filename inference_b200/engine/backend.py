@@ -84,7 +84,26 @@ class GpuBackend:
     def _is_decode(self, seqs, new_tokens) -> bool:
         return all(len(t) == 1 for t in new_tokens) and len(seqs) <= self.runner.max_batch
 
+    def _apart(self, seqs, new_tokens) -> list[list[int]] | None:
+        """On a page budget: the sequences with one new token and those with more, where a step has both. The first are decode steps, which read what they would
+        without the prompts beside them."""
+        if getattr(self.runner, "page_budget", None) is None:
+            return None
+        one = [len(t) == 1 and getattr(s, "pending_embeds", None) is None and getattr(s, "pending_mrope", None) is None for s, t in zip(seqs, new_tokens)]
+        return None if all(one) or not any(one) else [[i for i, x in enumerate(one) if x == first] for first in (True, False)]
+
+    @staticmethod
+    def _each(parts, run, *lists) -> list:
+        """run(...) of each part's rows of `lists`; its results in the rows' own order."""
+        out = [None] * len(lists[0])
+        for part in parts:
+            for i, x in zip(part, run(*([rows[i] for i in part] for rows in lists))):
+                out[i] = x
+        return out
+
     def forward(self, seqs, new_tokens, all_positions=False):
+        if not all_positions and (parts := self._apart(seqs, new_tokens)):
+            return self._each(parts, self.forward, seqs, new_tokens)
         ov, mr = _take_overrides(seqs), _take_mrope(seqs)
         if ov is None and mr is None and not all_positions and self._is_decode(seqs, new_tokens):
             logits = self.runner.decode(seqs, [t[0] for t in new_tokens], want_logits=True)
@@ -104,12 +123,21 @@ class GpuBackend:
         return out
 
     def forward_greedy(self, seqs, new_tokens):
+        if parts := self._apart(seqs, new_tokens):
+            return self._each(parts, self.forward_greedy, seqs, new_tokens)
         ov, mr = _take_overrides(seqs), _take_mrope(seqs)
         if ov is None and mr is None and self._is_decode(seqs, new_tokens):
             return [int(x) for x in self.runner.decode(seqs, [t[0] for t in new_tokens]).tolist()]
         return [int(x) for x in self.runner.prefill(seqs, new_tokens, embed_overrides=ov, mrope_overrides=mr).tolist()]
 
     def forward_at(self, seqs, new_tokens, want):
+        if parts := self._apart(seqs, new_tokens):
+            def run(s, n, w):
+                got = self.forward_at(s, n, w)
+                return got.split([len(x) for x in w]) if got is not None else [None] * len(s)
+
+            rows = [x for x in self._each(parts, run, seqs, new_tokens, want) if x is not None]
+            return torch.cat(rows) if rows else None
         if self._is_decode(seqs, new_tokens):
             rows = [i for i, w in enumerate(want) for _ in w]
             logits = self.runner.decode(seqs, [t[0] for t in new_tokens], want_logits=True)

@@ -179,3 +179,37 @@ def test_verified_drafts_read_what_decode_steps_would(drafts, read_by_pages):
             _check_attention(c, out, lambda t, b, h, n: [p * 16 + i for p in host[t, h].tolist() if p >= 0 for i in range(16) if p * 16 + i < n], kw["scale"])
         for s, n in zip(group, base):
             s.truncate(n + 1)
+
+
+def test_decode_steps_read_the_same_with_prompts_beside_them(read_by_pages):
+    """A chunk of another sequence's prompt in the same call changes neither's result, and results keep the order of the call."""
+    from inference_b200.engine.backend import GpuBackend
+
+    ops = _ops()
+    runs = []
+    for together in (True, False):
+        eng = _engine(ops.PageBudget(top=2, first=1, last=1))
+        backend = GpuBackend(eng.runner)
+        seqs = [backend.new_sequence() for _ in range(3)]
+        backend.forward(seqs, [_prompts()[2], _prompts()[0], _prompts()[2][:100]])
+        news, wants, got = [[5], _prompts()[1], [6]], [[0], [3, 36], [0, 0]], []
+        order, call = range(3), [seqs, news]
+        if together:
+            got += [x.clone() for x in backend.forward(*call)]       # rows of a decode graph's own output, which the next step writes again
+            got += [torch.tensor(backend.forward_greedy(*call))]
+            got += [backend.forward_at(*call, wants)]
+            assert backend.forward_at(*call, [[], [], []]) is None and backend.forward_at(*call, [[], [1], []]).shape == (1, 2048)
+        else:
+            steps, prompt = [0, 2], [1]
+
+            def apart(f, *lists):
+                return {i: x for part in (steps, prompt) for i, x in zip(part, f(*([y[i] for i in part] for y in lists)))}
+
+            parts = apart(backend.forward, *call)
+            got += [parts[i].clone() for i in order]
+            parts = apart(backend.forward_greedy, *call)
+            got += [torch.tensor([parts[i] for i in order])]
+            one, more = backend.forward_at([seqs[0], seqs[2]], [news[0], news[2]], [wants[0], wants[2]]), backend.forward_at([seqs[1]], [news[1]], [wants[1]])
+            got += [torch.cat([one[:1], more, one[1:]])]
+        runs.append(got)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
