@@ -402,7 +402,7 @@ class LlamaGpu:
         D = cfg.head_dim
         eps, woff = cfg.rms_norm_eps, cfg.norm_weight_offset
         T = inp.input_ids.numel()
-        if self._use_tp_prefill(T) and inp.summaries is None and inp.embed_rows is None and inp.rope_table is None and inp.deepstack is None:
+        if self._use_tp_prefill(T) and inp.page_budget is None and inp.embed_rows is None and inp.rope_table is None and inp.deepstack is None:
             return self._forward_hidden_tp_prefill(inp, kv_pool)
         rope_pos, rope_cos, rope_sin = inp.positions, self.cos, self.sin
         if inp.rope_table is not None:
@@ -680,6 +680,9 @@ class LlamaGpu:
                               q_norm=L.q_norm, k_norm=L.k_norm, norm_eps=eps, norm_w_offset=woff,
                               block_size=block_size)
             q = qkv[:, :q_cols].view(T, self.hq, D)
+            if inp.summaries is not None:
+                ops.summarize_pages(kv_pool[li, 0], inp.block_table, inp.kv_lens, inp.summaries[li], cu_q=inp.cu_q, max_q_len=inp.max_q_len)
+                n += 1
             if inp.fresh_prefill and inp.cu_q is not None and not cfg.attn_logit_softcap and self.dense_prefill:
                 # no earlier context: causal attention straight from the projection output on the tcgen05 kernel
                 kv_cols = self.hkv * D

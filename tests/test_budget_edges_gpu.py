@@ -1,7 +1,7 @@
 """Operators of long caches on a budget where their definitions are easily missed: calls that the documentation allows and that differ from the usual ones."""
 import pytest
 import torch
-from test_budget_gpu import CUDA, Cache, _check_attention, _engine, _gen, _ops, _prompts, _select
+from test_budget_gpu import CUDA, Cache, _check_attention, _engine, _gen, _ops, _prompts, _select, _summary
 
 pytestmark = pytest.mark.gpu
 
@@ -213,3 +213,42 @@ def test_decode_steps_read_the_same_with_prompts_beside_them(read_by_pages):
             got += [torch.cat([one[:1], more, one[1:]])]
         runs.append(got)
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+class _OneRank:
+    """The row-parallel products and the sums over ranks of a fused prefill, where there is one rank: all rows are its own."""
+
+    def __init__(self):
+        self.partial, self.used = None, 0
+
+    def my_rows(self, T):
+        return 0, T
+
+    def gemm_scatter_rows(self, x, w):
+        self.partial = _ops().linear_any(x, w)
+
+    def reduce_norm_gather(self, T, res, weight, eps, woff, reduce=True):
+        self.used += 1
+        return _ops().rmsnorm(self.partial, weight, eps, residual=res, w_offset=woff) if reduce else _ops().rmsnorm(res, weight, eps, w_offset=woff)
+
+
+def test_the_fused_prefill_of_several_ranks_keeps_summaries_up(monkeypatch):
+    """Prompts on a page budget take it as they do without one; what it writes is summarised."""
+    ops = _ops()
+    eng, ctx = _engine(ops.PageBudget(top=2, first=1, last=1)), _OneRank()
+    monkeypatch.setattr(eng.model, "_use_tp_prefill", lambda T: T > 16)
+    monkeypatch.setattr(eng.model, "_tp_prefill_context", lambda: ctx)
+    seqs = [eng.new_sequence(), eng.new_sequence()]
+    for new in ([_prompts()[0], _prompts()[1]], [_prompts()[1], _prompts()[2]]):
+        eng.runner.prefill(seqs, new)
+    assert ctx.used == 2 * (1 + 2 * 3)
+    eng.runner.prefill(seqs, [list(range(12))] * 2, all_positions=True)      # reads by pages, which the fused prefill does not
+    assert ctx.used == 2 * (1 + 2 * 3)
+    torch.cuda.synchronize()
+    for layer in range(3):
+        sums = eng.pool.summaries[layer]
+        for seq in seqs:
+            for at in seq.blocks[:seq.length // 16]:
+                for h in range(2):
+                    code, scale = _summary(eng.pool.data[layer, 0, at, h].cpu())
+                    assert torch.equal(sums.codes[at, h].cpu(), code) and float(sums.scales[at, h]) == scale
