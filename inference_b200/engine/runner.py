@@ -98,6 +98,10 @@ class ModelRunner:
         """Kept up by every runner of a pool that has them: another one may select by them."""
         return getattr(self.pool, "summaries", None) if isinstance(self.model, LlamaGpu) else None
 
+    def _step_splits(self, batch: int, max_kv: int):
+        """Of a decode step. On a page budget it reads as many pages however long the context is, so that contexts that grow share a graph."""
+        return 1 if self.page_budget is not None else self._splits(batch, max_kv)
+
     # ---- prefill (eager, ragged) ------------------------------------------------------------------
     def prefill(self, seqs: list[PagedSequence], new_tokens: list[list[int]], *, want_logits: bool = False,
                 all_positions: bool = False, embed_overrides: list[tuple[list[int], torch.Tensor] | None] | None = None,
@@ -336,7 +340,7 @@ class ModelRunner:
             self._meta_copy_done = torch.cuda.Event()
             self._meta_copy_done.record()
         self.h2d_bytes_last = self._host_meta.numel() * 4
-        splits = self._splits(Bp, max_kv)
+        splits = self._step_splits(Bp, max_kv)
         key = (Bp, splits, want_logits, self._summaries() is not None)
         if not self.use_graphs or self.model.device.type != "cuda":
             toks, logits = self._decode_body(Bp, splits, want_logits)
@@ -383,7 +387,7 @@ class ModelRunner:
         for s in seqs:
             s.fed(None)
         self.h2d_bytes_last = host_all.numel() * 4
-        splits = self._splits(B, max_kv)
+        splits = self._step_splits(B, max_kv)
         first = torch.tensor(tokens, dtype=torch.int64)
         if dev.type != "cuda" or not self.use_graphs:
             out = torch.empty((n_steps, B), dtype=torch.int64, device=dev)

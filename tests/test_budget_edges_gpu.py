@@ -252,3 +252,18 @@ def test_the_fused_prefill_of_several_ranks_keeps_summaries_up(monkeypatch):
                 for h in range(2):
                     code, scale = _summary(eng.pool.data[layer, 0, at, h].cpu())
                     assert torch.equal(sums.codes[at, h].cpu(), code) and float(sums.scales[at, h]) == scale
+
+
+def test_contexts_that_grow_replay_the_graph_of_their_batch():
+    """What a step on a page budget reads does not follow from the context's length, so neither do its graphs."""
+    ops = _ops()
+    eng = _engine(ops.PageBudget(top=1))
+    seq = eng.new_sequence()
+    for n in (30, 300, 500):
+        eng.runner.prefill([seq], [list(range(n))])
+        eng.runner.decode([seq], [1])
+    assert eng.runner.captures == 1
+    eng.runner.decode_multi([seq], [1], 2)
+    eng.runner.prefill([seq], [list(range(100))])
+    eng.runner.decode_multi([seq], [1], 2)
+    assert eng.runner.captures == 2
