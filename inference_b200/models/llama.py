@@ -462,9 +462,9 @@ class LlamaGpu:
                 ops.summarize_pages(kv_pool[li, 0], inp.block_table, inp.kv_lens, inp.summaries[li], cu_q=inp.cu_q, max_q_len=inp.max_q_len)
                 n += 1
             if inp.page_budget is not None:
-                budget = inp.page_budget
+                budget, all_pages = inp.page_budget, inp.block_table.shape[1]      # what goes past the table's pages selects nothing more
                 chosen = ops.select_pages(q, inp.summaries[li], inp.block_table, inp.kv_lens, cu_q=inp.cu_q, max_q_len=inp.max_q_len, block_size=block_size,
-                                          top=budget.top, first=budget.first, last=budget.last)
+                                          top=min(budget.top, all_pages), first=min(budget.first, all_pages), last=min(budget.last, all_pages))
                 attn = ops.selected_attention(q, kv_pool[li, 0], kv_pool[li, 1], inp.block_table, inp.kv_lens, chosen, cu_q=inp.cu_q,
                                               max_q_len=inp.max_q_len, scale=cfg.attn_scale, softcap=cfg.attn_logit_softcap or 0.0)
                 n += 1

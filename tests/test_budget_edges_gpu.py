@@ -267,3 +267,19 @@ def test_contexts_that_grow_replay_the_graph_of_their_batch():
     eng.runner.prefill([seq], [list(range(100))])
     eng.runner.decode_multi([seq], [1], 2)
     assert eng.runner.captures == 2
+
+
+def test_a_budget_beyond_the_table_takes_the_tables_room(read_by_pages):
+    """A large number is the natural way to say everything: lists are as long as the table's pages ask for."""
+    ops = _ops()
+    runs = []
+    for budget in (ops.PageBudget(top=64), ops.PageBudget(top=10 ** 6), ops.PageBudget(top=0, first=10 ** 6), ops.PageBudget(top=1, last=2 ** 40)):
+        eng = _engine(budget, use_graphs=False)
+        seq = eng.new_sequence()
+        eng.runner.prefill([seq], [_prompts()[0]])
+        read_by_pages.clear()
+        runs.append(eng.runner.decode([seq], [3], want_logits=True).clone())
+        assert len(read_by_pages) == 3
+        for x in read_by_pages:
+            assert x[5].pages.shape[2] <= 64 + 64 + 1 and x[5].counts.eq(38).all()
+    assert all(torch.equal(x, runs[0]) for x in runs)
