@@ -16,6 +16,7 @@ import torch
 
 from ..contracts.errors import Unsupported
 from ..models.llama import LlamaGpu, StepInputs, splits_for as _splits_for
+from ..ops import budget
 from ..utils import tracing
 from ..utils.graphs import recording
 from .kv_pool import PagedKvPool, PagedSequence
@@ -50,10 +51,13 @@ class ModelRunner:
         self.page_budget = page_budget
         if page_budget is not None and not (isinstance(model, LlamaGpu) and isinstance(pool, PagedKvPool)):
             raise Unsupported("a page budget needs a decoder of the Llama family on a uniform pool")
-        if page_budget is not None:
-            pool.with_summaries()
         self.max_batch, self.max_seq_len = max_batch, max_seq_len
         self.max_blocks = (max_seq_len + pool.block_size - 1) // pool.block_size
+        if page_budget is not None:
+            if self.max_blocks > budget.MAX_PAGES or pool.head_dim > budget.MAX_WIDTH or model.hq // model.hkv > budget.MAX_GROUP:
+                raise Unsupported(f"a page budget takes contexts of up to {budget.MAX_PAGES} pages, heads of up to {budget.MAX_WIDTH} numbers and up to {budget.MAX_GROUP} of them "
+                                  "to a key/value head")
+            pool.with_summaries()
         # models whose layers differ in KV heads or visible keys choose their splits themselves (one per layer)
         self._splits = getattr(model, "decode_splits", None) or \
             (lambda batch, max_kv: _splits_for(batch, model.hkv, max_kv))

@@ -62,3 +62,20 @@ def test_the_library_refuses_a_grid_of_more_than_2_to_the_31_blocks():
     dims = _INTS[16](8, seqs, most, 1, 20, 16, 1, 1, 128, 128, 0, 1, 0, 0, 0, 0)
     strides = _LONGS[8](128, 128, 128, 1, 16, 16, 0, 0)
     assert kernels().swb_attn_budget(dims, strides, at, at, at, at, at, at, at, None, None, at, 1.0, 0.0, at, 1 << 20, None) == -3
+
+
+@pytest.mark.parametrize("max_seq_len,heads,kv_heads,width", [(16 * 40000 + 1, 8, 2, 64), (1024, 129, 1, 16), (1024, 8, 2, 264)])
+def test_a_page_budget_that_no_step_could_keep_is_refused_with_its_runner(max_seq_len, heads, kv_heads, width):
+    """Contexts of more pages than a selection is made over, more query heads to a key/value head and wider heads than its operators take: at once, not at the first step."""
+    from inference_b200.contracts.errors import Unsupported
+    from inference_b200.engine.kv_pool import PagedKvPool
+    from inference_b200.engine.runner import ModelRunner
+    from inference_b200.models.llama import LlamaGpu
+    from inference_b200.ops import PageBudget
+
+    model = LlamaGpu.__new__(LlamaGpu)
+    model.hq, model.hkv = heads, kv_heads
+    pool = PagedKvPool(1, 2, kv_heads, width, device="cpu")
+    with pytest.raises(Unsupported):
+        ModelRunner(model, pool, max_batch=1, max_seq_len=max_seq_len, page_budget=PageBudget(top=1))
+    assert pool.summaries is None
