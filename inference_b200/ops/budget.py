@@ -7,6 +7,8 @@ Two ways to spend less than the whole cache on a new token, both beside `paged_a
   keep less    `tracked_attention` reads the whole cache and adds up the weight that each entry receives, `evict_tokens` lets the entries of least
                weight go and closes their holes
 
+Both go together as long as pages are summarised again behind an eviction.
+
 Caches are one layer's pages [blocks, kv heads, block_size, width] with the block tables of `PagedSequence`. bf16, or fp32 in the 32-bit mode; widths up to 256.
 Calls run on the current stream, take no host reads and can be captured into graphs; buffers that a call fills (summaries, weights, positions, the cache) belong
 to the caller. Steps are described as in `paged_attention`: kv_lens int32 [num_seqs] counts a sequence's tokens with the new ones, cu_q int32 [num_seqs + 1]
@@ -276,7 +278,8 @@ def evict_tokens(kcache: torch.Tensor, vcache: torch.Tensor, block_table: torch.
     and lie behind `keep` move in order into the holes in front of it: their rows of both caches, weight and position. positions int32 [num_seqs, kv heads, N]: -1 for
     entries without a record, which stand in order in front of the next position (all of them before the first call); the call records those it keeps. Of a sequence that
     shrinks the weights of entries keep to L - 1 (L: its length) become 0 and the positions from `keep` to the row's end -1; weights behind L stay as they were, and so does all of a
-    sequence of no more than `keep` tokens. Everything is done in place. Pages must not be
+    sequence of no more than `keep` tokens. Summaries of pages that entries move into are out of date then: `summarize_pages(kcache, block_table, new lengths, summaries, cu_q=None,
+    max_q_len=keep)` makes those of all full pages anew. Everything is done in place. Pages must not be
     shared with a sequence that is not to lose tokens, nor between sequences of the call."""
     stream = _place(kcache, vcache, block_table, kv_lens, weights, positions, next_positions)
     blocks, heads, bs, D, Dv = _check_cache(kcache, vcache)

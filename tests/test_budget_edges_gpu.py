@@ -114,6 +114,33 @@ def test_evictions_after_tokens_were_taken_back(cleared):
     assert same == [cleared, True, True, True]
 
 
+def test_pages_are_summarised_again_behind_an_eviction():
+    ops = _ops()
+    c = Cache([300, 90], [1, 1], seed=6, filler=0.0)
+    sums = ops.PageSummaries.empty(c.k)
+    ops.summarize_pages(c.k, c.table, c.kv_lens, sums, cu_q=None, max_q_len=300)
+    weights = torch.zeros(2, 2, c.per * 16, device=CUDA)
+    ops.tracked_attention(c.q, c.k, c.v, c.table, c.kv_lens, weights, scale=0.1, **c.step)
+    lens = ops.evict_tokens(c.k, c.v, c.table, c.kv_lens, weights, torch.full((2, 2, c.per * 16), -1, dtype=torch.int32, device=CUDA), c.kv_lens, keep=120, recent=8, first=2)
+    old = sums.codes.clone()
+    ops.summarize_pages(c.k, c.table, lens, sums, cu_q=None, max_q_len=120)
+    assert not torch.equal(old, sums.codes)
+    for b, n in enumerate(lens.tolist()):
+        for at in c.table[b, :n // 16].tolist():
+            for h in range(2):
+                code, scale = _summary(c.k[at, h].cpu())
+                assert torch.equal(sums.codes[at, h].cpu(), code) and float(sums.scales[at, h]) == scale
+    c.lens = lens.tolist()
+    some = ops.select_pages(c.q, sums, c.table, lens, block_size=16, top=2, first=1, last=1, **c.step)
+    for t, b, seen in c.tokens():
+        for h in range(2):
+            want = _select(c, sums, t, b, h, seen, 2, 1, 1)
+            assert some.pages[t, h].tolist() == want + [-1] * (4 - len(want))
+    host = some.pages.cpu()
+    _check_attention(c, ops.selected_attention(c.q, c.k, c.v, c.table, lens, some, scale=0.1, **c.step),
+                     lambda t, b, h, seen: [p * 16 + i for p in host[t, h].tolist() if p >= 0 for i in range(16) if p * 16 + i < seen], 0.1)
+
+
 # ---- in the engine ------------------------------------------------------------------------------------------------------------------------------------
 @pytest.fixture
 def read_by_pages(monkeypatch):
