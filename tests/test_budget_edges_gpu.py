@@ -310,3 +310,52 @@ def test_a_budget_beyond_the_table_takes_the_tables_room(read_by_pages):
         for x in read_by_pages:
             assert x[5].pages.shape[2] <= 64 + 64 + 1 and x[5].counts.eq(38).all()
     assert all(torch.equal(x, runs[0]) for x in runs)
+
+
+def test_summaries_of_forks_and_of_pages_that_are_taken_back():
+    """Two sequences share a prompt's pages. One goes back into a page that was full, which it then has to itself, and writes other tokens there: the other one still finds its own
+    page's summary, and both read what their summaries select."""
+    ops = _ops()
+    eng = _engine(ops.PageBudget(top=2, first=1, last=1), use_graphs=False)
+    from inference_b200.engine.backend import GpuBackend
+
+    backend = GpuBackend(eng.runner)
+    one = backend.new_sequence()
+    backend.forward([one], [_prompts()[0]])
+    two = backend.fork(one, 592)
+    assert two.blocks == one.blocks[:37]
+    two.truncate(580)                                  # within the last shared page
+    backend.forward([two], [[3 + i for i in range(40)]])
+    assert two.blocks[:36] == one.blocks[:36] and two.blocks[36] != one.blocks[36]
+    one.truncate(590)
+    for token in range(20):
+        backend.forward_greedy([one, two], [[token], [token + 5]])
+    three = backend.fork(two, 48)                      # whole pages, then tokens of its own
+    backend.forward([three], [_prompts()[2]])
+    seqs, seen = [one, two, three], []
+    real = ops.selected_attention
+
+    def spy(q, k, v, table, lens, sel, **kw):
+        out = real(q, k, v, table, lens, sel, **kw)
+        seen.append((q.clone(), k, v, table.clone(), sel, kw, out.clone()))
+        return out
+
+    ops.selected_attention = spy
+    try:
+        backend.forward_greedy(seqs, [[1], [2], [3]])
+    finally:
+        ops.selected_attention = real
+    assert len(seen) == 3
+    for layer, (q, k, v, table, sel, kw, out) in enumerate(seen):
+        for seq in seqs:
+            for at in seq.blocks[:seq.length // 16]:
+                for h in range(2):
+                    code, scale = _summary(eng.pool.data[layer, 0, at, h].cpu())
+                    assert torch.equal(eng.pool.summaries[layer].codes[at, h].cpu(), code) and float(eng.pool.summaries[layer].scales[at, h]) == scale
+        c = Cache([s.length for s in seqs], [1, 1, 1], heads=4, kv_heads=2)
+        c.k, c.v, c.table, c.q, c.blocks = k, v, table, q[:3], k.shape[0]
+        host = sel.pages.cpu()
+        for t, b, n in c.tokens():
+            for h in range(2):
+                assert host[t, h].tolist() == _select(c, eng.pool.summaries[layer], t, b, h, n, 2, 1, 1)
+        _check_attention(c, out[:3], lambda t, b, h, n: [p * 16 + i for p in host[t, h].tolist() for i in range(16) if p * 16 + i < n], kw["scale"])
