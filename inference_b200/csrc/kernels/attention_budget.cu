@@ -3,11 +3,11 @@
 //
 // A problem is up to 16 rows of queries with one key/value head: query heads that share it, of one token, or where tokens of a sequence read the same keys and the
 // heads are few, of several tokens. Its keys are dealt out to `num_splits` blocks. A block goes over its keys once with the running maximum and sum of the softmax in
-// 32 bits, and is left with an un-normalised sum of values and both. Up to 8 blocks of a problem are a cluster and join their parts from one another's
-// shared memory; more leave them in the workspace for a second launch. Weights need the maximum and sum over all keys, which are known at
-// the end only: the scores are kept (4 bytes a key and query head, beside the keys' and values' 2 (D + Dv) a key) and turned into weights there, by the
-// blocks themselves where every sequence has one token, else by the second launch, which adds up those of a key token by token and head by head. Every sum has
-// one order, and there are no atomics.
+// 32 bits, and is left with an un-normalised sum of values and both. Up to 8 blocks of a problem, where all problems' are 296 at most, are a cluster and join their parts from one
+// another's shared memory; otherwise they leave them in the workspace for a second launch. Weights need the maximum and sum over all keys, which are known at
+// the end only: the scores are kept (4 bytes a key and query head, beside the keys' and values' 2 (D + Dv) a key) and turned into weights there. With one token a sequence, up to 16
+// heads a group and one block or a cluster a problem, the blocks do so themselves; in every other case the second launch does, which adds up those of a key token by token
+// and head by head. Every sum has one order, and there are no atomics.
 //
 // Masked keys (behind what a token sees, on pages that are not there) take no part: their scores are -inf whatever the products were, and
 // their values are not multiplied at all, so that what the memory holds there does not matter.
@@ -40,7 +40,7 @@ struct BudgetParams {
   const int* kv_lens;
   int num_seqs, uniform_q, tokens, Hkv, G, head_tiles, D, Dv;
   float scale, softcap;
-  const int* pages;          // [tokens, Hkv, width]: the problem's pages by their place in the sequence; null: all pages
+  const int* pages;          // [tokens, Hkv, width]: the problem's pages by their place in the sequence; null: all pages, with weights
   const int* counts;         // [tokens, Hkv]
   int width;
   int num_splits;
@@ -48,7 +48,7 @@ struct BudgetParams {
   int cluster;               // the splits of a problem are a cluster
   int weigh_here;            // blocks add their weights themselves
   float* part_o;             // [tokens, Hq, num_splits, Dv], null where blocks or clusters finish the output
-  float* part_ml;            // [tokens, Hq, num_splits, 2]: maximum (log2 units) and sum, of a cluster's problem [tokens, Hq, 2]; null where nobody reads them
+  float* part_ml;            // [tokens, Hq, num_splits, 2]: maximum (log2 units) and sum; null where no second launch reads them
   float* scores;             // [tokens, Hq, capacity] in log2 units, where weights are kept
   long long capacity;
   float* weights;            // [num_seqs, Hkv, .], inner stride 1
@@ -603,7 +603,7 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
     *reinterpret_cast<float4*>(sWarps + tid * 4) = make_float4(m_of[0] * f, m_of[1] * f, m_of[2] * f, m_of[3] * f);
     sPart[tid * 2] = M, sPart[tid * 2 + 1] = L;
     sAll[tid * 2] = base, sAll[tid * 2 + 1] = inv;
-    if (p.part_ml && !p.cluster) *reinterpret_cast<float2*>(p.part_ml + part_at(p, token_at(tid), head_at(tid), split) * 2) = make_float2(M, L);
+    if (p.part_ml) *reinterpret_cast<float2*>(p.part_ml + part_at(p, token_at(tid), head_at(tid), split) * 2) = make_float2(M, L);
   }
   __syncthreads();
   const int d = lane * 4;                           // a row to a warp, four columns to a lane
@@ -649,7 +649,6 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
       for (int s = 0; s < MAX_CLUSTER; ++s) L = fmaf(m_of[s] = exp2f(m_of[s] - base), l_of[s], L);
       const float inv = L == 0.f ? 0.f : 1.f / L;
       sAll[tid * 2] = base, sAll[tid * 2 + 1] = inv;
-      if (p.part_ml && split == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)token_at(tid) * p.Hkv * p.G + head_at(tid)) * 2) = make_float2(M, L);
 #pragma unroll
       for (int s = 0; s < MAX_CLUSTER; ++s) sFactor[tid * MAX_CLUSTER + s] = m_of[s] * inv;
     }
@@ -932,7 +931,7 @@ extern "C" {
 
 // See BudgetParams. dims: host int[16] = tokens, num_seqs, tokens of each sequence (with cu_q: at most), table width, blocks, block_size, Hkv, G, D, Dv,
 // width of the page lists, splits, fp32, 0, 0, 0; strides: host long long[8] = q token and head, out token, table, weights sequence and head, 0, 0.
-// pages and counts, or weights, or neither. workspace (16-byte aligned), where results are joined by a second launch or weights are kept: 4 tokens Hq (splits (Dv + 2) +
+// pages and counts, or weights. workspace (16-byte aligned), where results are joined by a second launch or weights are kept: 4 tokens Hq (splits (Dv + 2) +
 // keys of the table, with weights) + 16 bytes.
 int swb_attn_budget(const int* dims, const long long* strides, const void* q, void* out, const void* k, const void* v, const int* table, const int* cu_q,
                     const int* kv_lens, const int* pages, const int* counts, float* weights, float scale, float softcap, void* workspace, long long workspace_bytes,
@@ -944,7 +943,7 @@ int swb_attn_budget(const int* dims, const long long* strides, const void* q, vo
   const int fp32 = dims[12];
   if (p.tokens <= 0 || p.num_seqs <= 0) return 0;
   if (p.num_seqs > 65535 || p.Hkv > 65535 || p.max_blocks < 1 || p.num_blocks < 1 || p.bs < 1 || p.Hkv < 1 || p.G < 1 || p.G > MAX_GROUP || p.D < 1 || p.D > 256 ||
-      p.Dv < 1 || p.Dv > 256 || p.num_splits < 1 || p.num_splits > MAX_SPLITS || p.uniform_q < 1 || (pages && (!counts || p.width < 1 || weights)) || !q || !out ||
+      p.Dv < 1 || p.Dv > 256 || p.num_splits < 1 || p.num_splits > MAX_SPLITS || p.uniform_q < 1 || !pages == !weights || (pages && (!counts || p.width < 1)) || !q || !out ||
       !k || !v || !table || !kv_lens)
     return -3;
   p.head_tiles = heads_in_tiles(p.G);
@@ -977,7 +976,6 @@ int swb_attn_budget(const int* dims, const long long* strides, const void* q, vo
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int rc = fast ? launch_fast(p, s) : fp32 ? launch_plain<float>(p, s) : launch_plain<bf16>(p, s);
   if (rc || !(join || weigh)) return rc;
-  if (p.cluster) p.num_splits = 1;               // the cluster left one pair a row
   return fp32 ? launch_finish<float>(p, join, weigh, s) : launch_finish<bf16>(p, join, weigh, s);
 }
 

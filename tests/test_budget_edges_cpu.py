@@ -79,3 +79,14 @@ def test_a_page_budget_that_no_step_could_keep_is_refused_with_its_runner(max_se
     with pytest.raises(Unsupported):
         ModelRunner(model, pool, max_batch=1, max_seq_len=max_seq_len, page_budget=PageBudget(top=1))
     assert pool.summaries is None
+
+
+@pytest.mark.parametrize("pages,weights", [(False, False), (True, True)])
+def test_the_library_takes_page_lists_or_weights(pages, weights):
+    from inference_b200._native import kernels
+    from inference_b200.ops.budget import _INTS, _LONGS
+
+    at = 1 << 20
+    dims, strides = _INTS[16](1, 1, 1, 8, 20, 16, 1, 1, 128, 128, 3, 1, 0, 0, 0, 0), _LONGS[8](128, 128, 128, 8, 128, 128, 0, 0)
+    assert kernels().swb_attn_budget(dims, strides, at, at, at, at, at, None, at, at if pages else None, at if pages else None, at if weights else None, 1.0, 0.0, at, 1 << 20,
+                                     None) == -3
