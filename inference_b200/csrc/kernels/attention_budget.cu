@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(FW * 32, FS == 2 && NT == 1 ? 3 : 2) attn_budg
         for (int k = 0; k < 4; ++k) x[k] = j0 + k * FW * 32 < end ? from[r * p.capacity + j0 + k * FW * 32] : -INFINITY;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (x[k] != -INFINITY) sum[k] = fmaf(exp2f(x[k] - sAll[r * 2]), sAll[r * 2 + 1], sum[k]);      // a key that is not there gets nothing of the row, whatever its sum is
+          if (x[k] != -INFINITY) sum[k] = fmaf(exp2_fast(x[k] - sAll[r * 2]), sAll[r * 2 + 1], sum[k]);      // a key that is not there gets nothing of the row, whatever its sum is
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k)

@@ -114,6 +114,20 @@ def test_evictions_after_tokens_were_taken_back(cleared):
     assert same == [cleared, True, True, True]
 
 
+@pytest.mark.parametrize("splits", [1, 3, 9])
+def test_weights_below_the_normal_range_are_zeros_however_splits_are_joined(splits):
+    """A key 90 below the largest has a weight of 2^-129.8, which 32 bits hold as a number below the normal range only."""
+    ops = _ops()
+    c = Cache([200], [1], filler=0.0)
+    c.q.zero_(), c.k.zero_()
+    c.q[..., 0] = 1
+    c.k[..., 0] = -90
+    c.k[c.table[0, 0].long(), :, 3, 0] = 0
+    weights = torch.zeros(1, 2, c.per * 16, device=CUDA)
+    ops.tracked_attention(c.q, c.k, c.v, c.table, c.kv_lens, weights, scale=1.0, num_splits=splits, **c.step)
+    assert weights[0, :, 3].eq(4).all() and weights.count_nonzero() == 2
+
+
 def test_pages_are_summarised_again_behind_an_eviction():
     ops = _ops()
     c = Cache([300, 90], [1, 1], seed=6, filler=0.0)
