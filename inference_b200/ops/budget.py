@@ -9,6 +9,9 @@ Two ways to spend less than the whole cache on a new token, both beside `paged_a
 
 Both go together as long as pages are summarised again behind an eviction.
 
+Scores, the softmax and all sums are 32-bit numbers (a page's sum of keys a 64-bit one). With bf16 caches each weight is rounded to bf16 in front of its product with the values, as in
+`paged_attention`; the softmax's sum and the weights that `tracked_attention` hands out are not. Weights below 2^-126 of a row's largest are zeros.
+
 Caches are one layer's pages [blocks, kv heads, block_size, width] with the block tables of `PagedSequence`. bf16, or fp32 in the 32-bit mode; widths up to 256.
 Calls run on the current stream, take no host reads and can be captured into graphs; buffers that a call fills (summaries, weights, positions, the cache) belong
 to the caller. Steps are described as in `paged_attention`: kv_lens int32 [num_seqs] counts a sequence's tokens with the new ones, cu_q int32 [num_seqs + 1]
