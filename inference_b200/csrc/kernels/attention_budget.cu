@@ -244,7 +244,9 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_budget_plain_kernel(const 
 // What a block costs before its first group and behind its last (some 4 us: look-ups that wait for one another, the joining of its warps) is hidden by the other
 // blocks of its SM. Rings of three groups leave room for two blocks, rings of two for three; the bytes on their way are the same. Two groups where blocks are many and
 // short (500 tokens with 4 key/value heads and 64 pages each: 90 us, 11.7 TB/s through the second-level cache; before the steps were shortened 126, and 165 with two
-// blocks), three where they are few (512 blocks of 128 pages: 87 us, 6.2 TB/s, 95 % of what a copy gets; with three blocks the last 68 of them run alone). 48 sequences of up
+// blocks), three where they are few (512 blocks of 128 pages: 87 us, 6.2 TB/s, 95 % of what a copy gets; with three blocks the last 68 of them run alone, 96 us). Many are
+// nine to an SM: 1600 blocks of 32, 64 and 128 pages take 73, 128 and 241 us with two groups, 77, 134 and 247 with three. Which is the better one in between hangs on how the last
+// round of blocks comes out: 512 of 64 pages take 54 and 50 us, 1120 take 93 and 98. 48 sequences of up
 // to 8191 keys, 8 key/value heads, in 8 splits: 192 us, 6.4 TB/s, and 17 for their weights. Warps that take equal runs of all problems' keys one behind the other, and fill
 // their rings across problems, took 112 us where these took 94: SMs differ in what they get of a busy memory, and nothing evens that out then.
 constexpr int FW = 4;                               // warps
@@ -712,7 +714,7 @@ int launch_fast(BudgetParams p, cudaStream_t s) {
   if (rc) return rc;
   const bool one = p.G * p.run <= 8, wide = p.D == 128 && p.Dv == 128;
   const int problems = (p.run > 1 ? p.num_seqs * ((p.uniform_q - 1) / p.run + 1) : p.tokens) * p.Hkv * p.head_tiles;
-  const bool many = one && (long long)problems * p.num_splits >= 9 * 148;
+  const bool many = one && (long long)problems * p.num_splits >= 9 * 148;      // measured at the kernel
   const int smem = fast_smem_bytes(many ? 2 : 3), which = (many ? 2 : one) + 3 * wide;
   using Kernel = decltype(&attn_budget_kernel<1, 2, true>);
   static constexpr Kernel kernels[6] = {attn_budget_kernel<2, 3, false>, attn_budget_kernel<1, 3, false>, attn_budget_kernel<1, 2, false>,

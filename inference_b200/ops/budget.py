@@ -181,7 +181,10 @@ def budget_splits(problems: int, keys: int, even: bool, tensor_cores: bool = Tru
     kernel on tensor cores, more of the plain one.
 
     Fewer problems than fit at once: as many splits as fit, up to 8, which join within the launch; more, joined by a second one, where 8 would leave SMs idle over
-    long caches. More problems: one block each, or where their lengths differ enough blocks of 512 keys and more to even out over seven rounds of the SMs."""
+    long caches (8 problems of 8192 keys: 21.0 us with 8 splits, 16.1 with 37; of 4096 keys 13.6 and 13.1; 16 of 16 384 keys: 39.4 with 8, 31.3 with 18). More problems: one block
+    each, or where their lengths differ enough blocks of 512 keys and more to even out over seven rounds of the SMs (384 problems of 4096 to 8191 keys: 280 us with one block each,
+    214 with 8, 218 with 16; 296 of 2048 to 4096, the border: 103 and 91; 512 of 512 to 1024: 48 with one, 53 with two). Cores without tensor instructions: eight blocks
+    to an SM, of 64 keys and more (64 problems of 2000 to 4000 32-bit keys: 713 us with one block each, 118 with 9, 101 with 18)."""
     slots, problems = 2 * sms, max(1, problems)
     if not tensor_cores:
         return max(1, min(MAX_SPLITS, (keys + 63) // 64, 8 * sms // problems))
