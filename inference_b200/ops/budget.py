@@ -256,7 +256,8 @@ def tracked_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tenso
     `weights.masked_fill_(torch.arange(N) >= kv_lens[:, None, None], 0)` does for all sequences.
 
     For decode steps, and for the last tokens of a prompt: keys are read once for every 16 rows (tokens * heads of a group) of a sequence, and scores are kept until the sums
-    are known, 4 bytes a token, query head and key of the table's width."""
+    are known, 4 bytes a token, query head and key of the table's width: give it the columns of a wide table that the longest
+    sequence needs (`block_table[:, :n]`; weights may stay wider)."""
     return _attention(q, kcache, vcache, block_table, kv_lens, cu_q, max_q_len, scale, softcap, num_splits, out, None, None, weights)
 
 

@@ -128,6 +128,28 @@ def test_weights_below_the_normal_range_are_zeros_however_splits_are_joined(spli
     assert weights[0, :, 3].eq(4).all() and weights.count_nonzero() == 2
 
 
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+def test_columns_of_a_wide_table(kind):
+    """What a caller with a table for long contexts gives for short ones: rows that lie apart, beside weights and positions of the whole width."""
+    ops = _ops()
+    got = []
+    for wide in (0, 500):
+        c = Cache([200, 90, 130], [1, 1, 1], kind=kind, seed=8, filler=0.0)
+        whole = torch.full((3, c.per + wide), -7, dtype=torch.int32, device=CUDA)
+        whole[:, :c.per] = c.table
+        table, n = whole[:, :c.per], (c.per + wide) * 16
+        weights, positions = torch.zeros(3, 2, n, device=CUDA), torch.full((3, 2, n), -1, dtype=torch.int32, device=CUDA)
+        sums = ops.PageSummaries.empty(c.k)
+        ops.summarize_pages(c.k, table, c.kv_lens, sums, cu_q=None, max_q_len=200)
+        some = ops.select_pages(c.q, sums, table, c.kv_lens, block_size=16, top=2, first=1, last=1, **c.step)
+        out = [ops.selected_attention(c.q, c.k, c.v, table, c.kv_lens, some, scale=0.1, **c.step), ops.tracked_attention(c.q, c.k, c.v, table, c.kv_lens, weights, scale=0.1, **c.step)]
+        lens = ops.evict_tokens(c.k, c.v, table, c.kv_lens, weights, positions, c.kv_lens, keep=100, recent=8)
+        m = c.per * 16
+        assert weights[..., m:].eq(0).all() and positions[..., m:].eq(-1).all()
+        got.append([*out, sums.codes, sums.scales, some.pages, some.counts, lens, weights[..., :m].clone(), positions[..., :m].clone(), c.k, c.v])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 def test_pages_are_summarised_again_behind_an_eviction():
     ops = _ops()
     c = Cache([300, 90], [1, 1], seed=6, filler=0.0)
