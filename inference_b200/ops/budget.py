@@ -284,7 +284,7 @@ def evict_tokens(kcache: torch.Tensor, vcache: torch.Tensor, block_table: torch.
     sequence's next token), and of the others those of largest weight (fp32 [num_seqs, kv heads, N], as `tracked_attention` adds them up; ties: the lowest index). Entries that stay
     and lie behind `keep` move in order into the holes in front of it: their rows of both caches, weight and position. positions int32 [num_seqs, kv heads, N]: -1 for
     entries without a record, which stand in order in front of the next position (all of them before the first call); the call records those it keeps. Of a sequence that
-    shrinks the weights of entries keep to L - 1 (L: its length) become 0 and the positions from `keep` to the row's end -1; weights behind L stay as they were, and so does all of a
+    shrinks the weights of entries keep to L - 1 (L: its length) become 0 and the positions from `keep` to the table's end -1; weights behind L stay as they were, and so does all of a
     sequence of no more than `keep` tokens. Summaries of pages that entries move into are out of date then: `summarize_pages(kcache, block_table, new lengths, summaries, cu_q=None,
     max_q_len=keep)` makes those of all full pages anew. Everything is done in place. Pages must not be
     shared with a sequence that is not to lose tokens, nor between sequences of the call."""
