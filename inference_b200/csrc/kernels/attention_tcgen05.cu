@@ -16,6 +16,7 @@
 // SDPA through cuBLAS matmuls + softmax, or FlashAttention-2 sm80 kernels).
 // Every wait is bounded; on expiry the CTA raises its abort flag, drains its own copies, frees TMEM and returns.
 #include "attention_common.cuh"
+#include "attention_tc.cuh"
 #include "common.cuh"
 
 #include <cuda.h>
@@ -34,7 +35,7 @@ namespace {
 constexpr int BM = 128;          // query rows per tile (two tiles per CTA)
 constexpr int BN = 128;          // keys per tile
 constexpr int MAX_STAGES = 2;
-constexpr uint32_t ATOM_BYTES = BM * 64 * 2;       // 16 KB: 128 rows of one 64-column swizzle atom
+constexpr uint32_t ATOM_BYTES = TC_ATOM_BYTES;    // 16 KB: 128 rows of one 64-column swizzle atom
 // Tile widths of q / k (QK) and of v (VD). 128 is two swizzle atoms per tile, 64 one atom (half the shared memory and half the
 // MMA work of the padded path); q and k of latent attention take up to three, which leaves room for one V stage.
 template <int QK, int VD>
@@ -103,87 +104,6 @@ struct FaParams {
   float2* part_ml;
 };
 
-__device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* tmap, uint64_t* bar, int c0, int c1, int c2,
-                                            int c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-      ::"r"(smem_u32(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
-      : "memory");
-}
-
-// D[tmem] (+)= A[tmem, packed bf16] * B[smem desc]
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                            uint32_t accumulate) {
-  asm volatile(
-      "{\n"
-      ".reg .pred p;\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
-      "}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// V tile as the B operand of O += P V: rows are keys (the MMA K dimension), 64 head-dim columns per 128-byte row
-// (MN-major), 8-key groups 1024 bytes apart, the second 64-column block one atom (16 KB) further.
-__device__ __forceinline__ uint64_t umma_desc_mnmajor_sw128(uint32_t smem_addr) {
-  uint64_t d = 0;
-  d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
-  d |= (uint64_t)(ATOM_BYTES >> 4) << 16;   // leading byte offset: next 64-element block along N
-  d |= (uint64_t)(1024 >> 4) << 32;         // stride byte offset: next 8-row group along K
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
-}
-
-// 32 consecutive 32-bit columns of this thread's TMEM lane (no wait inside).
-__device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
-      "%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,"
-      "%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const float* v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "f"(v[0]), "f"(v[1]),
-      "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]),
-      "f"(v[14]), "f"(v[15])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float rcp_approx(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
-  __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
-
 // tanh(x) / x on |x| <= 1 as a polynomial in x^2: a least-squares fit reweighted towards equal ripples; |error of tanh| < 2.4e-7.
 constexpr float TANH_0 = 0.99999685f, TANH_1 = -0.33324004f, TANH_2 = 0.13253525f, TANH_3 = -0.05097286f, TANH_4 = 0.01611418f,
                 TANH_5 = -0.00283947f;
@@ -208,47 +128,6 @@ struct Barriers {
 // 4608 tokens x 24 heads of 128: 274 us with a thread per row, 244 with two, 235 (1.11 PFLOP/s) with a quarter of the exponentials' pairs on
 // the multiply-add pipes (259 with half of them, 235 with an eighth), 229 with whole-warp MMA issue on another box; eight causal prompts of 1100 x 32 heads
 // 209 -> 164 us. Heads of 64: 4608 tokens x 24 heads 251 -> 198 us, 2 x 4250 x 38 718 -> 569 us, 8 x 197 x 12 10.4 -> 8.9 us.
-__device__ __forceinline__ unsigned long long pack2(float lo, float hi) {
-  unsigned long long r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpack2(unsigned long long v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
-  unsigned long long r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-// 2^x of two numbers at once on the multiply-add pipes: x = n + f, |f| <= 1/2, a polynomial in f fitted to 2^f with equal relative
-// ripples (8e-8, evaluated in fp32 within 2.2e-7: as exact as the special-function unit's) times 2^n. x is kept above -126, so what
-// should be zero comes out as 2^-126; what is not a number stays so.
-constexpr float EXP_0 = 1.00000012f, EXP_1 = 0.693146944f, EXP_2 = 0.240221202f, EXP_3 = 0.0555071309f, EXP_4 = 0.00967554096f, EXP_5 = 0.00132764713f;
-__device__ __forceinline__ unsigned long long ex2_fma2(unsigned long long x) {
-  float a, b;
-  unpack2(x, a, b);
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(a));
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(b));
-  x = pack2(a, b);
-  const unsigned long long magic = pack2(12582912.f, 12582912.f), minus = pack2(-12582912.f, -12582912.f), neg = pack2(-1.f, -1.f);
-  const unsigned long long t = add2(x, magic), f = fma2(add2(t, minus), neg, x);
-  unsigned long long r = fma2(pack2(EXP_5, EXP_5), f, pack2(EXP_4, EXP_4));
-  r = fma2(r, f, pack2(EXP_3, EXP_3));
-  r = fma2(r, f, pack2(EXP_2, EXP_2));
-  r = fma2(r, f, pack2(EXP_1, EXP_1));
-  r = fma2(r, f, pack2(EXP_0, EXP_0));
-  float t0, t1;
-  unpack2(t, t0, t1);
-  const unsigned long long power = pack2(__int_as_float((__float_as_int(t0) << 23) + 0x3f800000), __int_as_float((__float_as_int(t1) << 23) + 0x3f800000));
-  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(r) : "l"(power));
-  return r;
-}
-__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
-
 constexpr int FMA_EVERY = 8;   // one of the four pairs of exponentials of every FMA_EVERY keys leaves the special-function unit
 
 template <typename C, bool SPLIT>

@@ -8,6 +8,7 @@
 // Keys that no row of the tile sees (behind the cache's end, on pages that are not there) and those that single rows do not see take no part: their scores are -inf whatever
 // the products were, and their values are not multiplied, so that infinities and NaN there do not spread.
 #include "attention_common.cuh"
+#include "attention_tc.cuh"
 #include "gemm_tcgen05.cuh"
 
 #include <climits>
@@ -41,6 +42,7 @@ struct TreeParams {
   int tiles, num_splits;     // row tiles of a sequence, splits of a tile's keys
   float* part_o;             // [split][tokens][Hq][Dv]; null: one split
   float2* part_ml;           // [split][tokens][Hq]: maximum (log2 units) and sum
+  int q_vec, out_vec;        // rows of q and of out start on 16 bytes
 };
 
 // A sequence's part of the step.
@@ -222,6 +224,396 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_tree_plain_kernel(const Tr
   }
 }
 
+// ---- bf16, widths up to 128, pages of 16-key groups: products on the tensor memory's matrix instructions -----------------------------------------------------
+//
+// A block has 128 rows and walks its keys in tiles of 128.
+//   warp 8      producer: a box of 16 keys x 64 columns to a lane, so that a tile of K or V is one instruction of the warp; groups of keys that are not there are fetched
+//               from behind the cache, which fills zeros in
+//   warp 9      matrix instructions: S = Q K^T, then O += P V with P in tensor memory, where it takes the place of S, and V as it lies (its rows are the product's inner dimension)
+//   warps 0-7   softmax, two threads to a row with 64 of a tile's keys each; in tiles of the tree they apply the mask and see to it that V holds numbers
+// One tile of K and one of V fit beside Q where two blocks share an SM: the products of one run beside the softmax of the other.
+constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_THREADS = 320, TMA_WARP = 8, MMA_WARP = 9;
+constexpr uint32_t TC_COLS = 256, COL_S = 0, COL_O = 128;
+constexpr float TC_RESCALE = 8.f;          // O is rescaled when a maximum has grown by more than 2^8
+
+struct TcBars {
+  uint64_t q_full, k_full, k_empty, v_full, v_empty, s_full, p_full, o_final;
+  uint32_t tmem_base;
+  int abort;
+  int odd;                 // some new token's value is no number
+  unsigned dead[2];        // groups of a tile's keys that are not there
+};
+template <int DA, int VA>
+struct TcCfg {
+  static constexpr uint32_t Q = 0, K = DA * TC_ATOM_BYTES, V = 2 * DA * TC_ATOM_BYTES, BARS = V + VA * TC_ATOM_BYTES, EXCHANGE = BARS + 256;
+  static constexpr size_t BYTES = EXCHANGE + 2 * 2 * TC_ROWS * 4 + 1024;
+};
+
+// Which of the 64 keys from key0 on a row sees.
+__device__ __forceinline__ unsigned long long seen_keys(const unsigned* row, int words, int key0, int base, int len, unsigned dead) {
+  const int rel = key0 - base;
+  unsigned long long seen = ~0ull;
+  if (rel > -64) {
+    const int from = max(rel, 0), w = from >> 5, sh = from & 31;
+    const unsigned a = w < words ? row[w] : 0u, b = w + 1 < words ? row[w + 1] : 0u, c = w + 2 < words ? row[w + 2] : 0u;
+    seen = (unsigned long long)__funnelshift_r(b, c, sh) << 32 | __funnelshift_r(a, b, sh);
+    if (rel < 0) seen = seen << -rel | ((1ull << -rel) - 1);
+  }
+  const int left = len - key0;
+  if (left < 64) seen &= left > 0 ? (1ull << left) - 1 : 0ull;
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    if (dead >> g & 1u) seen &= ~(0xffffull << 16 * g);
+  return seen;
+}
+
+template <int DA, int VA, bool CAP>
+__device__ __forceinline__ void tree_softmax(const TreeParams& p, TcBars* bars, uint8_t* smem, uint32_t tmem, const Span& s, int seq, int h, int r0, int rows, int split, int t_lo, int n_tiles) {
+  using C = TcCfg<DA, VA>;
+  constexpr int OUT = VA * 32;                                              // output columns of a thread
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, half = warp >> 2, w4 = warp & 3, row = w4 * 32 + lane;
+  const uint32_t lane_base = (uint32_t)(w4 * 32) << 16, t_s = tmem + lane_base + COL_S, t_o = tmem + lane_base + COL_O + half * OUT;
+  float* exchange = reinterpret_cast<float*>(smem + C::EXCHANGE) + row;
+  const int t = s.q0 + (r0 + row) / p.G, head = h * p.G + (r0 + row) % p.G;
+  const bool mine = row < rows && (unsigned)t < (unsigned)p.tokens;
+  const unsigned* mask = p.mask + (mine ? t : 0) * p.mask_tok;
+  // Q: rows of 16-byte chunks in 128-byte swizzle atoms of 64 columns
+  for (int i = tid; i < TC_ROWS * DA * 8; i += 256) {
+    const int r = i / (DA * 8), c = i % (DA * 8), tr = s.q0 + (r0 + r) / p.G;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (r < rows && (unsigned)tr < (unsigned)p.tokens && c * 8 < p.D) {
+      const bf16* from = reinterpret_cast<const bf16*>(p.q) + tr * p.q_tok + (long long)(h * p.G + (r0 + r) % p.G) * p.q_head + c * 8;
+      if (p.q_vec) {
+        x = *reinterpret_cast<const uint4*>(from);
+      } else {
+        const uint16_t* w = reinterpret_cast<const uint16_t*>(from);
+        x = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+      }
+    }
+    *reinterpret_cast<uint4*>(smem + C::Q + (c >> 3) * TC_ATOM_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(&bars->q_full);
+
+  float scale_log2 = p.scale * 1.4426950408889634f, to_cap = 0.f;           // the capped score is cap (1 - 2 / (2^(to_cap s) + 1))
+  if constexpr (CAP) to_cap = 2.f * scale_log2 / p.softcap, scale_log2 = 1.4426950408889634f;
+  const float STOP = __int_as_float(0x7fffffff);                            // handed over instead of a maximum when a wait ran out
+  float m_used = -INFINITY, l = 0.f;
+  bool ok = true, values_ok = true;
+  for (int j = 0; j < n_tiles; ++j) {
+    ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full, j & 1, &bars->abort, 30));
+    const int tile0 = (t_lo + j) * TC_KEYS, key0 = tile0 + half * 64;
+    const bool tail = tile0 + TC_KEYS > s.base;
+    uint32_t x[64];
+    float mx = STOP;
+    if (ok) {
+      tc_fence_after_sync();
+      tmem_ld_x32(t_s + half * 64, x);
+      tmem_ld_x32(t_s + half * 64 + 32, x + 32);
+      tmem_ld_wait();
+      if constexpr (CAP) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) x[i] = __float_as_uint(fmaf(-2.f * p.softcap, rcp_approx(ex2(__uint_as_float(x[i]) * to_cap) + 1.f), p.softcap));
+      }
+      const unsigned dead = bars->dead[j & 1];
+      if (tail || dead) {
+        const unsigned long long seen = seen_keys(mask, p.words, key0, s.base, s.len, dead >> half * 4);
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+          if (!(seen >> i & 1ull)) x[i] = __float_as_uint(-INFINITY);
+      }
+      float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 64; i += 4) {
+        m0 = fmaxf(m0, __uint_as_float(x[i])), m1 = fmaxf(m1, __uint_as_float(x[i + 1]));
+        m2 = fmaxf(m2, __uint_as_float(x[i + 2])), m3 = fmaxf(m3, __uint_as_float(x[i + 3]));
+      }
+      mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+    }
+    float* slot = exchange + (j & 1) * (2 * TC_ROWS);
+    slot[half * TC_ROWS] = mx;
+    pair_sync(1 + w4);
+    const float other = slot[(half ^ 1) * TC_ROWS];
+    ok = ok && __all_sync(0xffffffffu, __float_as_int(other) != 0x7fffffff);
+    if (!ok) break;                                                         // both halves leave at the same tile
+    const float m_new = fmaxf(fmaxf(mx, other), m_used);
+    const bool grow = (m_new - m_used) * scale_log2 > TC_RESCALE;           // true on the first tile with a key that the row sees (m_used = -inf)
+    if (__any_sync(0xffffffffu, grow)) {
+      const float f = grow ? ex2((m_used - m_new) * scale_log2) : 1.f;
+      if (grow) l *= f, m_used = m_new;
+      if (j > 0) {
+#pragma unroll
+        for (int c = 0; c < OUT / 16; ++c) {
+          float o[16];
+          tmem_ld_32x32b_x16(t_o + c * 16, o);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] *= f;
+          tmem_st_x16(t_o + c * 16, o);
+        }
+      }
+    }
+    const float neg_m = m_used == -INFINITY ? 0.f : -m_used * scale_log2;
+    const unsigned long long sc2 = pack2(scale_log2, scale_log2), nm2 = pack2(neg_m, neg_m);
+    unsigned long long l0 = 0ull, l1 = 0ull;
+#pragma unroll
+    for (int i = 0; i < 64; i += 4) {       // packed P overwrites the row in place
+      float a, b, c, d;
+      unpack2(fma2(pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, nm2), a, b);
+      unpack2(fma2(pack2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), sc2, nm2), c, d);
+      a = ex2(a), b = ex2(b), c = ex2(c), d = ex2(d);
+      l0 = add2(l0, pack2(a, b)), l1 = add2(l1, pack2(c, d));
+      x[i >> 1] = pack_bf16x2(a, b), x[(i >> 1) + 1] = pack_bf16x2(c, d);
+    }
+    float x0, x1;
+    unpack2(add2(l0, l1), x0, x1);
+    l += x0 + x1;
+    tmem_st_x32(t_s + half * 32, x);
+    tmem_st_wait();
+    tc_fence_before_sync();
+    if (tail) {
+      // Values behind the sequence's end are anything, and those of new tokens are not for every row: what is no number becomes a zero in front of the product, and is added
+      // to the rows that see it at the end.
+      values_ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_full, j & 1, &bars->abort, 31));
+      if (!values_ok) continue;             // the next wait runs out too
+      for (int i = tid; i < TC_KEYS * VA * 8; i += 256) {
+        const int r = i / (VA * 8), c = i % (VA * 8);
+        if (tile0 + r < s.base) continue;
+        uint4* at = reinterpret_cast<uint4*>(smem + C::V + (c >> 3) * TC_ATOM_BYTES + r * 128 + ((c & 7) << 4));      // any chunk of the row
+        uint4 v = *at;
+        if (tile0 + r >= s.len) {
+          *at = make_uint4(0, 0, 0, 0);
+          continue;
+        }
+        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u, odd = true;
+          if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0xffffu, odd = true;
+        }
+        if (odd) *at = v, bars->odd = 1;
+      }
+      fence_proxy_async_smem();
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars->p_full);
+  }
+  if (!ok) return;
+  ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_final, 0, &bars->abort, 32)) && values_ok;
+  float* slot = exchange + (n_tiles & 1) * (2 * TC_ROWS);
+  slot[half * TC_ROWS] = ok ? l : STOP;
+  pair_sync(1 + w4);
+  const float other = slot[(half ^ 1) * TC_ROWS];
+  if (!ok) return;
+  tc_fence_after_sync();
+  const float sum = half ? other + l : l + other;
+  const bool odd = bars->odd != 0;
+  // values that are no numbers, of new tokens among this block's keys that the row sees: columns from d0 on
+  const auto add_odd = [&](uint32_t* o, int d0) {
+    const int* table = p.table + seq * p.table_stride;
+    for (int key = max(t_lo * TC_KEYS, max(s.base, 0)); key < min(s.len, (t_lo + n_tiles) * TC_KEYS); ++key) {
+      const int block = table[key / p.bs];
+      if (!mine || (unsigned)block >= (unsigned)p.num_blocks || !sees(mask, p.words, key - s.base)) continue;
+      const bf16* v = reinterpret_cast<const bf16*>(p.v) + (((long long)block * p.Hkv + h) * p.bs + key % p.bs) * p.Dv + d0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float y = d0 + i < p.Dv ? __bfloat162float(v[i]) : 0.f;
+        if (!isfinite(y)) o[i] = __float_as_uint(__uint_as_float(o[i]) + y);
+      }
+    }
+  };
+  if (p.part_o) {
+    const long long at = ((long long)split * p.tokens + t) * (p.Hkv * p.G) + head;
+#pragma unroll
+    for (int c = 0; c < OUT / 32; ++c) {
+      uint32_t o[32];
+      tmem_ld_x32(t_o + c * 32, o);
+      tmem_ld_wait();
+      const int d0 = half * OUT + c * 32;
+      if (odd) add_odd(o, d0);
+      if (mine) {
+        float* to = p.part_o + at * p.Dv + d0;
+#pragma unroll
+        for (int v = 0; v < 8; ++v)
+          if (d0 + v * 4 < p.Dv)
+            reinterpret_cast<float4*>(to)[v] = make_float4(__uint_as_float(o[v * 4]), __uint_as_float(o[v * 4 + 1]), __uint_as_float(o[v * 4 + 2]), __uint_as_float(o[v * 4 + 3]));
+      }
+    }
+    if (half == 0 && mine) p.part_ml[at] = make_float2(m_used == -INFINITY ? -INFINITY : m_used * scale_log2, sum);
+    return;
+  }
+  // through the idle Q and K tiles, so that rows are written in runs: 16-byte chunk c of row r lies at c ^ (r & (chunks - 1))
+  constexpr int BYTES = OUT * 2, CHUNKS = BYTES / 16;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint8_t* slab = smem + C::Q + warp * (32 * BYTES);
+#pragma unroll
+  for (int c = 0; c < OUT / 32; ++c) {
+    uint32_t o[32];
+    tmem_ld_x32(t_o + c * 32, o);
+    tmem_ld_wait();
+    if (odd) add_odd(o, half * OUT + c * 32);
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      uint4 u;
+      u.x = pack_bf16x2(__uint_as_float(o[v * 8]) * inv, __uint_as_float(o[v * 8 + 1]) * inv);
+      u.y = pack_bf16x2(__uint_as_float(o[v * 8 + 2]) * inv, __uint_as_float(o[v * 8 + 3]) * inv);
+      u.z = pack_bf16x2(__uint_as_float(o[v * 8 + 4]) * inv, __uint_as_float(o[v * 8 + 5]) * inv);
+      u.w = pack_bf16x2(__uint_as_float(o[v * 8 + 6]) * inv, __uint_as_float(o[v * 8 + 7]) * inv);
+      *reinterpret_cast<uint4*>(slab + lane * BYTES + (((c * 4 + v) ^ (lane & (CHUNKS - 1))) << 4)) = u;
+    }
+  }
+  __syncwarp();
+  bf16* out = reinterpret_cast<bf16*>(p.out);
+#pragma unroll
+  for (int it = 0; it < CHUNKS; ++it) {                                     // CHUNKS lanes write one row's part
+    const int r = (32 / CHUNKS) * it + lane / CHUNKS, ch = lane % CHUNKS, rr = r0 + w4 * 32 + r, to_t = s.q0 + rr / p.G, d = half * OUT + ch * 8;
+    if (w4 * 32 + r >= rows || (unsigned)to_t >= (unsigned)p.tokens || d >= p.Dv) continue;
+    const uint4 u = *reinterpret_cast<const uint4*>(slab + r * BYTES + ((ch ^ (r & (CHUNKS - 1))) << 4));
+    bf16* to = out + to_t * p.out_tok + (long long)(h * p.G + rr % p.G) * p.Dv + d;
+    if (p.out_vec) {
+      *reinterpret_cast<uint4*>(to) = u;
+    } else {
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) to[e] = __ushort_as_bfloat16((unsigned short)(w[e >> 1] >> (e & 1) * 16));
+    }
+  }
+}
+
+template <int DA, int VA, bool CAP>
+__global__ void __launch_bounds__(TC_THREADS, 2) attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const TreeParams p) {
+  using C = TcCfg<DA, VA>;
+  extern __shared__ uint8_t tc_smem[];
+  uint8_t* smem = tc_smem + ((1024u - (smem_u32(tc_smem) & 1023u)) & 1023u);
+  TcBars* bars = reinterpret_cast<TcBars*>(smem + C::BARS);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // row tiles of a problem are neighbours: they run together and find one another's keys in the second-level cache
+  const int tile = blockIdx.x % p.tiles, y = blockIdx.x / p.tiles, split = y % p.num_splits, z = y / p.num_splits, h = z % p.Hkv, seq = z / p.Hkv;
+  pdl_launch_dependents();
+  pdl_wait(TL_ATTN_DECODE);
+  const Span s = span_of(p, seq);
+  const int r0 = tile * TC_ROWS, rows = min(TC_ROWS, min(s.n, p.uniform_q) * p.G - r0);
+  if (rows <= 0) return;                                   // uniform, like the next one, in front of all barriers
+  const int all = (s.len + TC_KEYS - 1) / TC_KEYS, per = (all + p.num_splits - 1) / p.num_splits, t_lo = min(split * per, all), n_tiles = min(all, t_lo + per) - t_lo;
+  if (n_tiles <= 0) {                                      // fewer tiles than splits, or nothing in the cache
+    for (int r = threadIdx.x; r < rows; r += TC_THREADS) {
+      const int t = s.q0 + (r0 + r) / p.G, head = h * p.G + (r0 + r) % p.G;
+      if ((unsigned)t >= (unsigned)p.tokens) continue;
+      if (p.part_o) p.part_ml[((long long)split * p.tokens + t) * (p.Hkv * p.G) + head] = make_float2(-INFINITY, 0.f);
+      else
+        for (int d = 0; d < p.Dv; ++d) reinterpret_cast<bf16*>(p.out)[t * p.out_tok + (long long)head * p.Dv + d] = __float2bfloat16(0.f);
+    }
+    return;
+  }
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->q_full, 8);
+    mbar_init(&bars->k_full, 1);
+    mbar_init(&bars->k_empty, 1);
+    mbar_init(&bars->v_full, 1);
+    mbar_init(&bars->v_empty, 1);
+    mbar_init(&bars->s_full, 1);
+    mbar_init(&bars->p_full, 8);
+    mbar_init(&bars->o_final, 1);
+    bars->abort = 0, bars->odd = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  if (warp == MMA_WARP) {
+    tmem_alloc(&bars->tmem_base, TC_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = bars->tmem_base;
+  if (warp == TMA_WARP) {
+    // lane = group of 16 keys + 8 * swizzle atom
+    const int* table = p.table + seq * p.table_stride;
+    const int g = lane & 7, atom = lane >> 3, none = p.num_blocks * p.Hkv * p.bs;
+    bool ok = true;
+    int issued_k = 0, issued_v = 0;
+    for (int j = 0; j < n_tiles && ok; ++j) {
+      const int key = (t_lo + j) * TC_KEYS + g * 16;
+      int row = none;
+      if (key < s.len) {
+        const int block = table[key / p.bs];
+        if ((unsigned)block < (unsigned)p.num_blocks) row = (block * p.Hkv + h) * p.bs + key % p.bs;
+      }
+      const unsigned dead = __ballot_sync(0xffffffffu, row == none) & 0xffu;
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars->k_empty, (j & 1) ^ 1, &bars->abort, 10));
+      if (!ok) break;
+      if (lane == 0) {
+        bars->dead[j & 1] = dead;
+        mbar_arrive_expect_tx(&bars->k_full, DA * TC_ATOM_BYTES);
+      }
+      __syncwarp();
+      if (atom < DA) tma_load_2d(smem + C::K + atom * TC_ATOM_BYTES + g * 2048, &tmap_k, &bars->k_full, atom * 64, row);
+      issued_k = j + 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_empty, (j & 1) ^ 1, &bars->abort, 11));
+      if (!ok) break;
+      if (lane == 0) mbar_arrive_expect_tx(&bars->v_full, VA * TC_ATOM_BYTES);
+      __syncwarp();
+      if (atom < VA) tma_load_2d(smem + C::V + atom * TC_ATOM_BYTES + g * 2048, &tmap_v, &bars->v_full, atom * 64, row);
+      issued_v = j + 1;
+    }
+    if (!ok) {                                             // copies in flight land before the block's memory is released
+      volatile int never = 0;
+      if (issued_k) mbar_wait(&bars->k_full, (issued_k - 1) & 1, &never, 13);
+      if (issued_v) mbar_wait(&bars->v_full, (issued_v - 1) & 1, &never, 14);
+    }
+  } else if (warp == MMA_WARP) {
+    constexpr uint32_t IDESC_QK = umma_idesc_bf16_f32(TC_ROWS, TC_KEYS), IDESC_PV = umma_idesc_bf16_f32(TC_ROWS, VA * 64) | (1u << 16);      // V is MN-major
+    const uint64_t qd = umma_desc_kmajor_sw128(smem_u32(smem + C::Q)), kd = umma_desc_kmajor_sw128(smem_u32(smem + C::K)), vd = umma_desc_mnmajor_sw128(smem_u32(smem + C::V));
+    const auto wait = [&](uint64_t* bar, uint32_t parity, int where) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, &bars->abort, where)) != 0; };
+    bool ok = wait(&bars->q_full, 0, 20);
+    for (int j = 0; j <= n_tiles && ok; ++j) {
+      if (j > 0) {                                         // O += P V of the tile before
+        ok = wait(&bars->p_full, (j - 1) & 1, 22) && wait(&bars->v_full, (j - 1) & 1, 23);
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < TC_KEYS / 16; ++k) umma_f16_ts(tmem + COL_O, tmem + COL_S + k * 8, vd + k * (2048 >> 4), IDESC_PV, j > 1 || k > 0);
+          umma_commit(&bars->v_empty);
+        }
+        __syncwarp();
+      }
+      if (j < n_tiles) {
+        ok = wait(&bars->k_full, j & 1, 21);
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < DA * 4; ++k) {
+            const uint32_t off = ((k >> 2) * TC_ATOM_BYTES + (k & 3) * 32) >> 4;
+            umma_f16_ss(tmem + COL_S, qd + off, kd + off, IDESC_QK, k > 0);
+          }
+          umma_commit(&bars->s_full);
+          umma_commit(&bars->k_empty);
+        }
+        __syncwarp();
+      }
+    }
+    if (elect_one()) umma_commit(&bars->o_final);          // also where a wait ran out: it tracks what has been issued
+    __syncwarp();
+    if (!ok) {
+      volatile int never = 0;
+      mbar_wait(&bars->o_final, 0, &never, 27);
+      __syncwarp();
+    }
+  } else {
+    tree_softmax<DA, VA, CAP>(p, bars, smem, tmem, s, seq, h, r0, rows, split, t_lo, n_tiles);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == MMA_WARP) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, TC_COLS);
+  }
+}
+
 // ---- sum of the splits --------------------------------------------------------------------------------------------------------------------------------
 // A warp to a row and head, weighed by the distance of its splits' maxima to the common one.
 constexpr int JOIN_THREADS = 128;
@@ -251,7 +643,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_tree_join_kernel(const Tree
     float x = 0.f;
     for (int s = 0; s < S; ++s) {                            // all lanes: each has the factors of two splits
       const float f = __shfl_sync(0xffffffffu, s < 32 ? fa : fb, s & 31);
-      if (d < p.Dv) x = fmaf(f, p.part_o[(s * rows + i) * p.Dv + d], x);
+      if (d < p.Dv && f != 0.f) x = fmaf(f, p.part_o[(s * rows + i) * p.Dv + d], x);      // of a split without keys nothing was written
     }
     if (d < p.Dv) store_out(out + d, x * inv);
   }
@@ -278,6 +670,34 @@ int launch_plain(const TreeParams& p, cudaStream_t s) {
   return vec ? launch_plain<E, 4, true>(p, s) : launch_plain<E, 4, false>(p, s);
 }
 
+template <int DA, int VA, bool CAP>
+int launch_tc(const CUtensorMap& k, const CUtensorMap& v, const TreeParams& p, cudaStream_t s) {
+  auto kernel = attn_tree_tc_kernel<DA, VA, CAP>;
+  constexpr size_t smem = TcCfg<DA, VA>::BYTES;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return -(int)e;
+  return launch_kernel(kernel, dim3((unsigned)((long long)p.tiles * p.num_splits * p.Hkv * p.num_seqs)), dim3(TC_THREADS), smem, s, k, v, p);
+}
+
+template <bool CAP>
+int launch_tc(TreeParams p, cudaStream_t s) {
+  p.q_vec = (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 && p.q_tok % 8 == 0 && p.q_head % 8 == 0;
+  p.out_vec = (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.out_tok % 8 == 0;
+  CUtensorMap k, v;
+  const int rows = p.num_blocks * p.Hkv * p.bs;
+  int rc = make_tmap_bf16_2d(&k, p.k, rows, p.D, p.D, 16);
+  if (!rc) rc = make_tmap_bf16_2d(&v, p.v, rows, p.Dv, p.Dv, 16);
+  if (rc) return rc;
+  if (p.D <= 64) return p.Dv <= 64 ? launch_tc<1, 1, CAP>(k, v, p, s) : launch_tc<1, 2, CAP>(k, v, p, s);
+  return p.Dv <= 64 ? launch_tc<2, 1, CAP>(k, v, p, s) : launch_tc<2, 2, CAP>(k, v, p, s);
+}
+
+// The matrix instructions take widths of whole 16-byte chunks, the copies pages of whole groups of 16 keys; a maximum of products is one of scores where these grow with them.
+bool tc_fits(const TreeParams& p, int fp32) {
+  return !fp32 && p.D % 8 == 0 && p.Dv % 8 == 0 && p.D <= 128 && p.Dv <= 128 && p.bs % 16 == 0 && p.scale > 0.f && (long long)p.num_blocks * p.Hkv * p.bs < INT_MAX &&
+         ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) & 15) == 0;
+}
+
 }  // namespace
 }  // namespace swb
 
@@ -285,7 +705,7 @@ extern "C" {
 
 // See TreeParams. dims: host int[16] = tokens, num_seqs, tokens of each sequence (with cu_q: at most), table width, blocks, block_size, Hkv, G, D, Dv, words of a mask row, splits,
 // fp32, 0, 0, 0; strides: host long long[8] = q token and head, out token, table, mask token, 0, 0, 0. workspace (16-byte aligned), with more
-// than one split: 4 splits tokens Hq (Dv + 2) bytes.
+// than one split: 4 splits tokens Hq (Dv + 2) + 16 bytes.
 int swb_attn_tree(const int* dims, const long long* strides, const void* q, void* out, const void* k, const void* v, const int* table, const int* cu_q, const int* kv_lens,
                   const void* mask, float scale, float softcap, void* workspace, long long workspace_bytes, void* stream) {
   using namespace swb;
@@ -297,20 +717,22 @@ int swb_attn_tree(const int* dims, const long long* strides, const void* q, void
   if (p.num_seqs > 65535 || p.max_blocks < 1 || p.num_blocks < 1 || p.bs < 1 || p.Hkv < 1 || p.G < 1 || p.G > MAX_GROUP || p.D < 1 || p.D > 256 || p.Dv < 1 || p.Dv > 256 ||
       p.num_splits < 1 || p.num_splits > MAX_SPLITS || p.uniform_q < 1 || p.words < 1 || !q || !out || !k || !v || !table || !kv_lens || !mask)
     return -3;
-  if ((long long)p.max_blocks * p.bs > INT_MAX || (long long)p.uniform_q * p.G > INT_MAX - PR) return -3;
-  p.tiles = (p.uniform_q * p.G + PR - 1) / PR;
+  if ((long long)p.max_blocks * p.bs > INT_MAX || (long long)p.uniform_q * p.G > INT_MAX - TC_ROWS) return -3;
+  p.scale = scale, p.softcap = softcap, p.k = k, p.v = v;
+  const bool fast = tc_fits(p, fp32);
+  const int tile = fast ? TC_ROWS : PR;
+  p.tiles = (p.uniform_q * p.G + tile - 1) / tile;
   if ((long long)p.tiles * p.num_seqs * p.Hkv > INT_MAX / p.num_splits || (long long)p.tokens * p.Hkv * p.G > INT_MAX) return -3;
-  p.q = q, p.out = out, p.k = k, p.v = v, p.table = table, p.cu_q = cu_q, p.kv_lens = kv_lens, p.mask = reinterpret_cast<const unsigned*>(mask);
+  p.q = q, p.out = out, p.table = table, p.cu_q = cu_q, p.kv_lens = kv_lens, p.mask = reinterpret_cast<const unsigned*>(mask);
   p.q_tok = strides[0], p.q_head = strides[1], p.out_tok = strides[2], p.table_stride = strides[3], p.mask_tok = strides[4];
-  p.scale = scale, p.softcap = softcap;
   const long long rows = (long long)p.tokens * p.Hkv * p.G;
   if (p.num_splits > 1) {
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || 4 * rows * p.num_splits * (p.Dv + 2) > workspace_bytes) return -3;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || 4 * rows * p.num_splits * (p.Dv + 2) + 16 > workspace_bytes) return -3;
     p.part_ml = reinterpret_cast<float2*>(workspace);
-    p.part_o = reinterpret_cast<float*>(workspace) + rows * p.num_splits * 2;
+    p.part_o = reinterpret_cast<float*>(workspace) + (rows * p.num_splits * 2 + 3) / 4 * 4;      // on 16 bytes again
   }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int rc = fp32 ? launch_plain<float>(p, s) : launch_plain<bf16>(p, s);
+  const int rc = fast ? (softcap > 0.f ? launch_tc<true>(p, s) : launch_tc<false>(p, s)) : fp32 ? launch_plain<float>(p, s) : launch_plain<bf16>(p, s);
   if (rc || p.num_splits == 1) return rc;
   const dim3 grid((unsigned)((rows + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32)));
   return fp32 ? launch_kernel(attn_tree_join_kernel<float>, grid, dim3(JOIN_THREADS), 0, s, p) : launch_kernel(attn_tree_join_kernel<bf16>, grid, dim3(JOIN_THREADS), 0, s, p);

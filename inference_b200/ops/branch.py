@@ -60,9 +60,10 @@ def _check_ranges(cu_q: torch.Tensor | None, max_q_len: int, tokens: int) -> int
     return cu_q.shape[0] - 1
 
 
-def tree_splits(problems: int, keys: int, sms: int = 148) -> int:
-    """Blocks that share the keys of a tile of rows: as many as an SM holds of the kernel, of 64 keys and more."""
-    return max(1, min(MAX_SPLITS, (keys + 63) // 64, 4 * sms // max(1, problems)))
+def tree_splits(problems: int, keys: int, tensor_cores: bool = True, sms: int = 148) -> int:
+    """Blocks that share the keys of a tile of rows: as many as the SMs hold at once (two to an SM of the kernel on tensor memory, four of the plain one), of a tile of keys and more."""
+    slots, tile = (2 * sms, 128) if tensor_cores else (4 * sms, 64)
+    return max(1, min(MAX_SPLITS, (keys + tile - 1) // tile, slots // max(1, problems)))
 
 
 def tree_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, mask: torch.Tensor, *,
@@ -86,16 +87,18 @@ def tree_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, 
     else:
         _require(out.shape == (T, columns) and out.dtype == kind and out.stride(1) == 1, "out is [T, heads * value width] in the type of q, unit inner stride")
         _require(out.stride(0) >= columns or T <= 1, "rows of out share memory")
-    problems = n * heads * -(-max_q_len * G // 32)
-    splits = tree_splits(problems, per * bs) if num_splits is None else num_splits
+    k_ptr, v_ptr = kcache.data_ptr(), vcache.data_ptr()
+    fast = kind is torch.bfloat16 and (D | Dv) % 8 == 0 and D <= 128 and Dv <= 128 and bs % 16 == 0 and scale > 0 and (k_ptr | v_ptr) % 16 == 0 and blocks * heads * bs < 2 ** 31 - 1
+    problems = n * heads * -(-max_q_len * G // (128 if fast else 32))
+    splits = tree_splits(problems, per * bs, fast) if num_splits is None else num_splits
     _require(1 <= splits <= MAX_SPLITS, "1 to 64 splits")
     ws, nbytes = None, 0
     if splits > 1:
-        nbytes = 4 * splits * T * G * heads * (Dv + 2)
+        nbytes = 4 * splits * T * G * heads * (Dv + 2) + 16
         ws = q.new_empty(nbytes, dtype=torch.uint8)        # the call's own: two streams or graphs share none
     dims = _DIMS[16](T, n, max_q_len, per, blocks, bs, heads, G, D, Dv, mask.shape[1], splits, kind == torch.float32, 0, 0, 0)
     strides = _STRIDES(tok, head, out.stride(0), block_table.stride(0), mask.stride(0), 0, 0, 0)
-    check(kernels().swb_attn_tree(dims, strides, q.data_ptr(), out.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), block_table.data_ptr(), ptr(cu_q), kv_lens.data_ptr(),
+    check(kernels().swb_attn_tree(dims, strides, q.data_ptr(), out.data_ptr(), k_ptr, v_ptr, block_table.data_ptr(), ptr(cu_q), kv_lens.data_ptr(),
                                   mask.data_ptr(), scale, softcap, ptr(ws), nbytes, stream), "swb_attn_tree")
     return out
 
