@@ -226,27 +226,63 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_tree_plain_kernel(const Tr
 
 // ---- bf16, widths up to 128, pages of 16-key groups: products on the tensor memory's matrix instructions -----------------------------------------------------
 //
-// A block has 128 rows and walks its keys in tiles of 128.
-//   warp 8      producer: a box of 16 keys x 64 columns to a lane, so that a tile of K or V is one instruction of the warp; groups of keys that are not there are fetched
-//               from behind the cache, which fills zeros in
-//   warp 9      matrix instructions: S = Q K^T, then O += P V with P in tensor memory, where it takes the place of S, and V as it lies (its rows are the product's inner dimension)
-//   warps 0-7   softmax, two threads to a row with 64 of a tile's keys each; in tiles of the tree they apply the mask and see to it that V holds numbers
-// One tile of K and one of V fit beside Q where two blocks share an SM: the products of one run beside the softmax of the other.
-constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_THREADS = 320, TMA_WARP = 8, MMA_WARP = 9;
-constexpr uint32_t TC_COLS = 256, COL_S = 0, COL_O = 128;
+// A block has up to 256 rows of a problem and walks its keys in tiles of 128. It works on two things at once ("slots"), so that the products of one run beside the softmax of the other:
+// with more than 128 rows on their two halves, which share the tiles, else on the even and the odd tiles, whose results it joins at its end.
+//   warp 16      producer: a box of 16 keys x 64 columns to a lane, so that a tile of K or V is one instruction of the warp; groups of keys that are not there are fetched from
+//                behind the cache, which fills zeros in
+//   warps 17, 18 matrix instructions, one warp a slot: S = Q K^T, then O += P V with P in tensor memory, where it takes the place of S, and V as it lies (its rows are the product's
+//                inner dimension); the scores of the next tile follow the product that frees their place
+//   (warp 19 makes the last four a group that hands registers on)
+//   warps 0-15   softmax, eight to a slot, two threads to a row with 64 of a tile's keys each; in tiles of the tree they apply the mask and see to it that V holds numbers
+// Tensor memory of a slot: S (128 columns; P in the first half of each thread's own 64), O (128). Shared memory has seven buffers of a tile: Q, three of K, and two of V with Q's second half
+// or three of V.
+// 64 tokens x 32 heads (8 key/value heads) behind 100 000 keys, blocks of 256 rows and 44 tiles: 125 us with the sum of the splits, 0.84 PFLOP/s; 95 of them without any softmax. (One slot a block and
+// two blocks to an SM, each tile asked for when the one before it was used: 155.) What a slot waits for are its products, 2 x 8 of 64 cycles, beside those of the other, and its softmax, of which the
+// exponentials are 17 us. What did not help: tiles of 64 keys with two of scores a slot (their products take no less for being half as wide), references a tile old in place of a row's own
+// maximum (its steps cost more than the exchange), a quarter of the exponentials on the multiply-add pipes.
+constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_THREADS = 640, TMA_WARP = 16, MMA_WARP = 17, K_STAGES = 3, V_STAGES = 3, SOFT_REGS = 112, ROLE_REGS = 32;
+constexpr uint32_t TC_COLS = 512;
 constexpr float TC_RESCALE = 8.f;          // O is rescaled when a maximum has grown by more than 2^8
 
+// What a block works on. It lies in shared memory: the softmax has all of its registers full of scores, and reads what it needs of it where it needs it.
+struct Block {
+  Span s;
+  int seq, h, r0, rows, split, t_lo, n_tiles;
+  int tail;                // first tile that has keys of the tree, or behind it
+  int two;                 // the slots are halves of the rows
+};
+
 struct TcBars {
-  uint64_t q_full, k_full, k_empty, v_full, v_empty, s_full, p_full, o_final;
+  uint64_t q_full, k_full[K_STAGES], k_empty[K_STAGES], v_full[V_STAGES], v_empty[V_STAGES], v_clean[V_STAGES], s_full[2], p_full[2], o_final;
   uint32_t tmem_base;
   int abort;
   int odd;                 // some new token's value is no number
-  unsigned dead[2];        // groups of a tile's keys that are not there
+  unsigned dead[16];       // groups of a tile's keys that are not there
+  Block block;
 };
+static_assert(sizeof(TcBars) <= 512, "room in front of the exchange");
 template <int DA, int VA>
 struct TcCfg {
-  static constexpr uint32_t Q = 0, K = DA * TC_ATOM_BYTES, V = 2 * DA * TC_ATOM_BYTES, BARS = V + VA * TC_ATOM_BYTES, EXCHANGE = BARS + 256;
-  static constexpr size_t BYTES = EXCHANGE + 2 * 2 * TC_ROWS * 4 + 1024;
+  static constexpr uint32_t KT = DA * TC_ATOM_BYTES, VT = VA * TC_ATOM_BYTES, LAST = KT > VT ? KT : VT;      // the last buffer is Q's or V's
+  static constexpr uint32_t Q = 0, K = KT, V = K + K_STAGES * KT, X = V + 2 * VT, BARS = X + LAST, EXCHANGE = BARS + 512;
+  static constexpr size_t BYTES = EXCHANGE + 2 * 2 * TC_ROWS * 4;          // [slot][half][row]
+};
+
+__device__ __forceinline__ Block load_block(TcBars* bars) {
+  static_assert(sizeof(Block) % 4 == 0, "words");
+  Block b;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(Block) / 4); ++i) reinterpret_cast<int*>(&b)[i] = reinterpret_cast<volatile int*>(&bars->block)[i];
+  return b;
+}
+
+// A place in a ring of stages, and how often it has been gone round (its lowest bit).
+struct Ring {
+  int at, round;
+  __device__ __forceinline__ void advance(int by, int stages) {
+    at += by;
+    if (at >= stages) at -= stages, round ^= 1;
+  }
 };
 
 // Which of the 64 keys from key0 on a row sees.
@@ -267,164 +303,251 @@ __device__ __forceinline__ unsigned long long seen_keys(const unsigned* row, int
   return seen;
 }
 
-template <int DA, int VA, bool CAP>
-__device__ __forceinline__ void tree_softmax(const TreeParams& p, TcBars* bars, uint8_t* smem, uint32_t tmem, const Span& s, int seq, int h, int r0, int rows, int split, int t_lo, int n_tiles) {
+
+// A row's columns in tensor memory times f: whole warp.
+template <int COLS>
+__device__ __forceinline__ void scale_columns(uint32_t at, float f) {
+#pragma unroll
+  for (int c = 0; c < COLS / 16; ++c) {                                     // narrow pieces: scores stay in registers meanwhile
+    float o[16];
+    tmem_ld_32x32b_x16(at + c * 16, o);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] *= f;
+    tmem_st_x16(at + c * 16, o);
+  }
+}
+
+// Q of a slot: rows of 16-byte chunks in 128-byte swizzle atoms of 64 columns; the slots share the work where there is one half of the rows only.
+template <int DA, int VA>
+__device__ __forceinline__ void fetch_queries(const TreeParams& p, uint8_t* smem, const Block& b, int slot, int tid) {
   using C = TcCfg<DA, VA>;
-  constexpr int OUT = VA * 32;                                              // output columns of a thread
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, half = warp >> 2, w4 = warp & 3, row = w4 * 32 + lane;
-  const uint32_t lane_base = (uint32_t)(w4 * 32) << 16, t_s = tmem + lane_base + COL_S, t_o = tmem + lane_base + COL_O + half * OUT;
-  float* exchange = reinterpret_cast<float*>(smem + C::EXCHANGE) + row;
-  const int t = s.q0 + (r0 + row) / p.G, head = h * p.G + (r0 + row) % p.G;
-  const bool mine = row < rows && (unsigned)t < (unsigned)p.tokens;
-  const unsigned* mask = p.mask + (mine ? t : 0) * p.mask_tok;
-  // Q: rows of 16-byte chunks in 128-byte swizzle atoms of 64 columns
-  for (int i = tid; i < TC_ROWS * DA * 8; i += 256) {
-    const int r = i / (DA * 8), c = i % (DA * 8), tr = s.q0 + (r0 + r) / p.G;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (r < rows && (unsigned)tr < (unsigned)p.tokens && c * 8 < p.D) {
-      const bf16* from = reinterpret_cast<const bf16*>(p.q) + tr * p.q_tok + (long long)(h * p.G + (r0 + r) % p.G) * p.q_head + c * 8;
-      if (p.q_vec) {
-        x = *reinterpret_cast<const uint4*>(from);
-      } else {
-        const uint16_t* w = reinterpret_cast<const uint16_t*>(from);
-        x = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+  constexpr int CH = DA * 8, STEP = 256 / CH, N = TC_ROWS / STEP;           // a thread has chunk c of every STEP-th row
+  const Span s = b.s;
+  const int r0 = b.r0 + (b.two ? slot * TC_ROWS : 0), rows = b.rows - (b.two ? slot * TC_ROWS : 0), c = tid % CH, first = tid / CH;
+  uint8_t* to = smem + (b.two && slot ? C::X : C::Q) + (c >> 3) * TC_ATOM_BYTES;
+  uint4 x[N / 2];
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    if (!b.two && part != slot) continue;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const int r = first + (part * (N / 2) + i) * STEP, tr = s.q0 + (r0 + r) / p.G;
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (r < rows && (unsigned)tr < (unsigned)p.tokens && c * 8 < p.D) {
+        const bf16* from = reinterpret_cast<const bf16*>(p.q) + tr * p.q_tok + (long long)(b.h * p.G + (r0 + r) % p.G) * p.q_head + c * 8;
+        if (p.q_vec) {
+          x[i] = *reinterpret_cast<const uint4*>(from);
+        } else {
+          const uint16_t* w = reinterpret_cast<const uint16_t*>(from);
+          x[i] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+        }
       }
     }
-    *reinterpret_cast<uint4*>(smem + C::Q + (c >> 3) * TC_ATOM_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const int r = first + (part * (N / 2) + i) * STEP;
+      *reinterpret_cast<uint4*>(to + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x[i];
+    }
   }
+}
+
+template <int DA, int VA, bool CAP>
+__device__ __forceinline__ void tree_softmax(const TreeParams& p, TcBars* bars, uint8_t* smem, uint32_t tmem) {
+  using C = TcCfg<DA, VA>;
+  constexpr int OUT = VA * 32;                                              // output columns of a thread
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot = warp >> 3, half = (warp >> 2) & 1, w4 = warp & 3, tid = threadIdx.x & 255, row = w4 * 32 + lane;
+  const uint32_t t_s = tmem + ((uint32_t)(w4 * 32) << 16) + slot * 256 + half * 64, t_o = t_s - half * 64 + 128 + half * OUT;
+  float* word = reinterpret_cast<float*>(smem + C::EXCHANGE) + slot * (2 * TC_ROWS) + row;
+  int steps, by, j, tail;                                                   // tiles of this slot, from one to the next, the first one, the first of the tree
+  {
+    const Block b = load_block(bars);
+    fetch_queries<DA, VA>(p, smem, b, slot, tid);
+    steps = b.two ? b.n_tiles : (b.n_tiles - slot + 1) >> 1, by = b.two ? 1 : 2, j = b.two ? 0 : slot, tail = b.tail;
+  }
+  // token of this thread's row, and whether it is one of the step's
+  const auto token_of = [&](const Block& b, bool& mine) {
+    const int r = row + (b.two ? slot * TC_ROWS : 0), t = b.s.q0 + (b.r0 + r) / p.G;
+    mine = r < b.rows && (unsigned)t < (unsigned)p.tokens;
+    return t;
+  };
   fence_proxy_async_smem();
   __syncwarp();
   if (lane == 0) mbar_arrive(&bars->q_full);
 
   float scale_log2 = p.scale * 1.4426950408889634f, to_cap = 0.f;           // the capped score is cap (1 - 2 / (2^(to_cap s) + 1))
   if constexpr (CAP) to_cap = 2.f * scale_log2 / p.softcap, scale_log2 = 1.4426950408889634f;
-  const float STOP = __int_as_float(0x7fffffff);                            // handed over instead of a maximum when a wait ran out
-  float m_used = -INFINITY, l = 0.f;
-  bool ok = true, values_ok = true;
-  for (int j = 0; j < n_tiles; ++j) {
-    ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full, j & 1, &bars->abort, 30));
-    const int tile0 = (t_lo + j) * TC_KEYS, key0 = tile0 + half * 64;
-    const bool tail = tile0 + TC_KEYS > s.base;
+  const float STOP = __int_as_float(0x7fffffff);                            // handed over instead of a maximum, which is a number or infinite, when a wait ran out
+  float m = -INFINITY, l = 0.f;
+  bool ok = true, whole = true;                                             // whole: no wait inside a tile has run out
+  for (int i = 0; i < steps; ++i, j += by) {
+    ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[slot], i & 1, &bars->abort, 30 + slot));
     uint32_t x[64];
     float mx = STOP;
     if (ok) {
       tc_fence_after_sync();
-      tmem_ld_x32(t_s + half * 64, x);
-      tmem_ld_x32(t_s + half * 64 + 32, x + 32);
+      tmem_ld_x32(t_s, x);
+      tmem_ld_x32(t_s + 32, x + 32);
       tmem_ld_wait();
       if constexpr (CAP) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i) x[i] = __float_as_uint(fmaf(-2.f * p.softcap, rcp_approx(ex2(__uint_as_float(x[i]) * to_cap) + 1.f), p.softcap));
+        for (int e = 0; e < 64; ++e) x[e] = __float_as_uint(fmaf(-2.f * p.softcap, rcp_approx(ex2(__uint_as_float(x[e]) * to_cap) + 1.f), p.softcap));
       }
-      const unsigned dead = bars->dead[j & 1];
-      if (tail || dead) {
-        const unsigned long long seen = seen_keys(mask, p.words, key0, s.base, s.len, dead >> half * 4);
+      const unsigned dead = bars->dead[j & 15];
+      if (j >= tail || dead) {
+        const Block b = load_block(bars);
+        bool mine;
+        const int t = token_of(b, mine);
+        const unsigned long long seen = seen_keys(p.mask + (mine ? t : 0) * p.mask_tok, p.words, (b.t_lo + j) * TC_KEYS + half * 64, b.s.base, b.s.len, dead >> half * 4);
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
-          if (!(seen >> i & 1ull)) x[i] = __float_as_uint(-INFINITY);
+        for (int e = 0; e < 64; ++e)
+          if (!(seen >> e & 1ull)) x[e] = __float_as_uint(-INFINITY);
       }
       float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 64; i += 4) {
-        m0 = fmaxf(m0, __uint_as_float(x[i])), m1 = fmaxf(m1, __uint_as_float(x[i + 1]));
-        m2 = fmaxf(m2, __uint_as_float(x[i + 2])), m3 = fmaxf(m3, __uint_as_float(x[i + 3]));
+      for (int e = 0; e < 64; e += 4) {
+        m0 = fmaxf(m0, __uint_as_float(x[e])), m1 = fmaxf(m1, __uint_as_float(x[e + 1]));
+        m2 = fmaxf(m2, __uint_as_float(x[e + 2])), m3 = fmaxf(m3, __uint_as_float(x[e + 3]));
       }
       mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
     }
-    float* slot = exchange + (j & 1) * (2 * TC_ROWS);
-    slot[half * TC_ROWS] = mx;
-    pair_sync(1 + w4);
-    const float other = slot[(half ^ 1) * TC_ROWS];
-    ok = ok && __all_sync(0xffffffffu, __float_as_int(other) != 0x7fffffff);
+    // (Its word of the tile before is read by then: this tile's scores wait for that one's weights.)
+    word[half * TC_ROWS] = mx;
+    pair_sync(1 + slot * 4 + w4);
+    const float theirs = word[(half ^ 1) * TC_ROWS];
+    ok = ok && __all_sync(0xffffffffu, __float_as_int(theirs) != 0x7fffffff);
     if (!ok) break;                                                         // both halves leave at the same tile
-    const float m_new = fmaxf(fmaxf(mx, other), m_used);
-    const bool grow = (m_new - m_used) * scale_log2 > TC_RESCALE;           // true on the first tile with a key that the row sees (m_used = -inf)
+    const float m_new = fmaxf(fmaxf(mx, theirs), m);
+    const bool grow = (m_new - m) * scale_log2 > TC_RESCALE;                // true on the first tile with a key that the row sees (m = -inf)
     if (__any_sync(0xffffffffu, grow)) {
-      const float f = grow ? ex2((m_used - m_new) * scale_log2) : 1.f;
-      if (grow) l *= f, m_used = m_new;
-      if (j > 0) {
+      const float f = grow ? ex2((m - m_new) * scale_log2) : 1.f;
+      if (grow) l *= f, m = m_new;
+      if (i > 0) scale_columns<OUT>(t_o, f);                                // the product before this one is done: the scores came behind it
+    }
+    const float neg_m = m == -INFINITY ? 0.f : -m * scale_log2;
+    const unsigned long long sc2 = pack2(scale_log2, scale_log2), nm2 = pack2(neg_m, neg_m);
+    unsigned long long l0 = 0ull, l1 = 0ull;
+#pragma unroll
+    for (int e = 0; e < 64; e += 4) {       // packed P overwrites the row in place
+      float v0, v1, v2, v3;
+      unpack2(fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), sc2, nm2), v0, v1);
+      unpack2(fma2(pack2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])), sc2, nm2), v2, v3);
+      v0 = ex2(v0), v1 = ex2(v1), v2 = ex2(v2), v3 = ex2(v3);
+      l0 = add2(l0, pack2(v0, v1)), l1 = add2(l1, pack2(v2, v3));
+      x[e >> 1] = pack_bf16x2(v0, v1), x[(e >> 1) + 1] = pack_bf16x2(v2, v3);
+    }
+    float x0, x1;
+    unpack2(add2(l0, l1), x0, x1);
+    l += x0 + x1;
+    tmem_st_x32(t_s, x);
+    tmem_st_wait();
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars->p_full[slot]);
+    if (j >= tail && !(by == 1 && slot)) {
+      // Values behind the sequence's end are anything, and those of new tokens are not for every row: what is no number becomes a zero in front of the products, and is added
+      // to the rows that see it at the end.
+      const Block b = load_block(bars);
+      const int stages = b.two ? 2 : 3, at_stage = j % stages, tile0 = (b.t_lo + j) * TC_KEYS;
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars->v_full[at_stage], (j / stages) & 1, &bars->abort, 35))) {
+        whole = false;
+        continue;                                                           // the next tile's wait runs out too
+      }
+      for (int e = tid; e < TC_KEYS * VA * 8; e += 256) {
+        const int r = e / (VA * 8), c = e % (VA * 8);
+        if (tile0 + r < b.s.base) continue;
+        uint4* at = reinterpret_cast<uint4*>(smem + C::V + at_stage * C::VT + (c >> 3) * TC_ATOM_BYTES + r * 128 + ((c & 7) << 4));      // any chunk of the row
+        if (tile0 + r >= b.s.len) {
+          *at = make_uint4(0, 0, 0, 0);
+          continue;
+        }
+        uint4 v = *at;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+        bool odd = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if ((w[k] & 0x7f80u) == 0x7f80u) w[k] &= 0xffff0000u, odd = true;
+          if ((w[k] & 0x7f800000u) == 0x7f800000u) w[k] &= 0xffffu, odd = true;
+        }
+        if (odd) *at = v, bars->odd = 1;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->v_clean[at_stage]);
+    }
+  }
+  ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_final, 0, &bars->abort, 32 + slot)) && ok && whole;
+  word[half * TC_ROWS] = ok ? l : -1.f;                                     // a sum is not below zero, but may be no number
+  pair_sync(1 + slot * 4 + w4);
+  const float other = word[(half ^ 1) * TC_ROWS], m_used = m;
+  ok = ok && __all_sync(0xffffffffu, other != -1.f);
+  const Block b = load_block(bars);
+  const Span s = b.s;
+  bool mine;
+  const int t = token_of(b, mine), r0 = b.r0 + (b.two ? slot * TC_ROWS : 0), rows = b.rows - (b.two ? slot * TC_ROWS : 0), head = b.h * p.G + (r0 + row) % p.G;
+  tc_fence_after_sync();
+  float sum = half ? other + l : l + other, f = 1.f;
+  const bool both = !b.two && b.n_tiles > 1;                                // two parts of the same rows
+  float4* hand = reinterpret_cast<float4*>(smem + C::V) + tid;              // two idle V tiles: chunk c of a thread at 256 c
+  float* hand_ml = reinterpret_cast<float*>(smem + C::BARS - 1024) + row;   // and the end of the last one: of both threads of a row, which have the same
+  if (both) {
+    if (slot) {
+      if (ok) {
 #pragma unroll
         for (int c = 0; c < OUT / 16; ++c) {
           float o[16];
           tmem_ld_32x32b_x16(t_o + c * 16, o);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] *= f;
-          tmem_st_x16(t_o + c * 16, o);
+          for (int e = 0; e < 4; ++e) hand[(c * 4 + e) * 256] = make_float4(o[e * 4], o[e * 4 + 1], o[e * 4 + 2], o[e * 4 + 3]);
         }
       }
+      hand_ml[0] = ok ? m_used : STOP, hand_ml[TC_ROWS] = sum;
     }
-    const float neg_m = m_used == -INFINITY ? 0.f : -m_used * scale_log2;
-    const unsigned long long sc2 = pack2(scale_log2, scale_log2), nm2 = pack2(neg_m, neg_m);
-    unsigned long long l0 = 0ull, l1 = 0ull;
+    asm volatile("bar.sync 9, 512;" ::: "memory");
+    if (slot) return;
+    const float m1 = hand_ml[0], l1 = hand_ml[TC_ROWS];
+    ok = ok && __all_sync(0xffffffffu, __float_as_int(m1) != 0x7fffffff);
+    if (ok) {
+      const float top = fmaxf(m_used, m1), base = top == -INFINITY ? 0.f : top;
+      f = ex2((m_used - base) * scale_log2);
+      const float f1 = ex2((m1 - base) * scale_log2);
+      sum = fmaf(f, sum, f1 * l1);
+      m = top;
 #pragma unroll
-    for (int i = 0; i < 64; i += 4) {       // packed P overwrites the row in place
-      float a, b, c, d;
-      unpack2(fma2(pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, nm2), a, b);
-      unpack2(fma2(pack2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), sc2, nm2), c, d);
-      a = ex2(a), b = ex2(b), c = ex2(c), d = ex2(d);
-      l0 = add2(l0, pack2(a, b)), l1 = add2(l1, pack2(c, d));
-      x[i >> 1] = pack_bf16x2(a, b), x[(i >> 1) + 1] = pack_bf16x2(c, d);
-    }
-    float x0, x1;
-    unpack2(add2(l0, l1), x0, x1);
-    l += x0 + x1;
-    tmem_st_x32(t_s + half * 32, x);
-    tmem_st_wait();
-    tc_fence_before_sync();
-    if (tail) {
-      // Values behind the sequence's end are anything, and those of new tokens are not for every row: what is no number becomes a zero in front of the product, and is added
-      // to the rows that see it at the end.
-      values_ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_full, j & 1, &bars->abort, 31));
-      if (!values_ok) continue;             // the next wait runs out too
-      for (int i = tid; i < TC_KEYS * VA * 8; i += 256) {
-        const int r = i / (VA * 8), c = i % (VA * 8);
-        if (tile0 + r < s.base) continue;
-        uint4* at = reinterpret_cast<uint4*>(smem + C::V + (c >> 3) * TC_ATOM_BYTES + r * 128 + ((c & 7) << 4));      // any chunk of the row
-        uint4 v = *at;
-        if (tile0 + r >= s.len) {
-          *at = make_uint4(0, 0, 0, 0);
-          continue;
-        }
-        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-        bool odd = false;
+      for (int c = 0; c < OUT / 16; ++c) {
+        float o[16];
+        tmem_ld_32x32b_x16(t_o + c * 16, o);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u, odd = true;
-          if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0xffffu, odd = true;
+          const float4 y = hand[(c * 4 + e) * 256];
+          o[e * 4] = fmaf(f, o[e * 4], f1 * y.x), o[e * 4 + 1] = fmaf(f, o[e * 4 + 1], f1 * y.y);
+          o[e * 4 + 2] = fmaf(f, o[e * 4 + 2], f1 * y.z), o[e * 4 + 3] = fmaf(f, o[e * 4 + 3], f1 * y.w);
         }
-        if (odd) *at = v, bars->odd = 1;
+        tmem_st_x16(t_o + c * 16, o);
       }
-      fence_proxy_async_smem();
+      tmem_st_wait();
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&bars->p_full);
+  } else if (steps == 0) {
+    return;
   }
   if (!ok) return;
-  ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_final, 0, &bars->abort, 32)) && values_ok;
-  float* slot = exchange + (n_tiles & 1) * (2 * TC_ROWS);
-  slot[half * TC_ROWS] = ok ? l : STOP;
-  pair_sync(1 + w4);
-  const float other = slot[(half ^ 1) * TC_ROWS];
-  if (!ok) return;
-  tc_fence_after_sync();
-  const float sum = half ? other + l : l + other;
   const bool odd = bars->odd != 0;
   // values that are no numbers, of new tokens among this block's keys that the row sees: columns from d0 on
   const auto add_odd = [&](uint32_t* o, int d0) {
-    const int* table = p.table + seq * p.table_stride;
-    for (int key = max(t_lo * TC_KEYS, max(s.base, 0)); key < min(s.len, (t_lo + n_tiles) * TC_KEYS); ++key) {
+    const int* table = p.table + b.seq * p.table_stride;
+    for (int key = max(b.t_lo * TC_KEYS, max(s.base, 0)); key < min(s.len, (b.t_lo + b.n_tiles) * TC_KEYS); ++key) {
       const int block = table[key / p.bs];
-      if (!mine || (unsigned)block >= (unsigned)p.num_blocks || !sees(mask, p.words, key - s.base)) continue;
-      const bf16* v = reinterpret_cast<const bf16*>(p.v) + (((long long)block * p.Hkv + h) * p.bs + key % p.bs) * p.Dv + d0;
+      if (!mine || (unsigned)block >= (unsigned)p.num_blocks || !sees(p.mask + t * p.mask_tok, p.words, key - s.base)) continue;
+      const bf16* v = reinterpret_cast<const bf16*>(p.v) + (((long long)block * p.Hkv + b.h) * p.bs + key % p.bs) * p.Dv + d0;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const float y = d0 + i < p.Dv ? __bfloat162float(v[i]) : 0.f;
-        if (!isfinite(y)) o[i] = __float_as_uint(__uint_as_float(o[i]) + y);
+      for (int e = 0; e < 32; ++e) {
+        const float y = d0 + e < p.Dv ? __bfloat162float(v[e]) : 0.f;
+        if (!isfinite(y)) o[e] = __float_as_uint(__uint_as_float(o[e]) + y);
       }
     }
+    __syncwarp();
   };
   if (p.part_o) {
-    const long long at = ((long long)split * p.tokens + t) * (p.Hkv * p.G) + head;
+    const long long at = ((long long)b.split * p.tokens + t) * (p.Hkv * p.G) + head;
 #pragma unroll
     for (int c = 0; c < OUT / 32; ++c) {
       uint32_t o[32];
@@ -440,13 +563,14 @@ __device__ __forceinline__ void tree_softmax(const TreeParams& p, TcBars* bars, 
             reinterpret_cast<float4*>(to)[v] = make_float4(__uint_as_float(o[v * 4]), __uint_as_float(o[v * 4 + 1]), __uint_as_float(o[v * 4 + 2]), __uint_as_float(o[v * 4 + 3]));
       }
     }
-    if (half == 0 && mine) p.part_ml[at] = make_float2(m_used == -INFINITY ? -INFINITY : m_used * scale_log2, sum);
+    if (half == 0 && mine) p.part_ml[at] = make_float2(m == -INFINITY ? -INFINITY : m * scale_log2, sum);
     return;
   }
-  // through the idle Q and K tiles, so that rows are written in runs: 16-byte chunk c of row r lies at c ^ (r & (chunks - 1))
+  // through the idle Q tile (and K's behind it), so that rows are written in runs: 16-byte chunk c of row r lies at c ^ (r & (chunks - 1))
   constexpr int BYTES = OUT * 2, CHUNKS = BYTES / 16;
+  static_assert(8 * 32 * BYTES <= C::LAST && 8 * 32 * BYTES <= 4 * C::KT, "a slot's rows fit in front of what the other reads");
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint8_t* slab = smem + C::Q + warp * (32 * BYTES);
+  uint8_t* slab = smem + (slot ? C::X : C::Q) + (warp & 7) * (32 * BYTES);
 #pragma unroll
   for (int c = 0; c < OUT / 32; ++c) {
     uint32_t o[32];
@@ -470,7 +594,7 @@ __device__ __forceinline__ void tree_softmax(const TreeParams& p, TcBars* bars, 
     const int r = (32 / CHUNKS) * it + lane / CHUNKS, ch = lane % CHUNKS, rr = r0 + w4 * 32 + r, to_t = s.q0 + rr / p.G, d = half * OUT + ch * 8;
     if (w4 * 32 + r >= rows || (unsigned)to_t >= (unsigned)p.tokens || d >= p.Dv) continue;
     const uint4 u = *reinterpret_cast<const uint4*>(slab + r * BYTES + ((ch ^ (r & (CHUNKS - 1))) << 4));
-    bf16* to = out + to_t * p.out_tok + (long long)(h * p.G + rr % p.G) * p.Dv + d;
+    bf16* to = out + to_t * p.out_tok + (long long)(b.h * p.G + rr % p.G) * p.Dv + d;
     if (p.out_vec) {
       *reinterpret_cast<uint4*>(to) = u;
     } else {
@@ -482,43 +606,47 @@ __device__ __forceinline__ void tree_softmax(const TreeParams& p, TcBars* bars, 
 }
 
 template <int DA, int VA, bool CAP>
-__global__ void __launch_bounds__(TC_THREADS, 2) attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const TreeParams p) {
+__global__ void __launch_bounds__(TC_THREADS, 1) attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const TreeParams p) {
   using C = TcCfg<DA, VA>;
-  extern __shared__ uint8_t tc_smem[];
-  uint8_t* smem = tc_smem + ((1024u - (smem_u32(tc_smem) & 1023u)) & 1023u);
+  extern __shared__ __align__(1024) uint8_t smem[];
   TcBars* bars = reinterpret_cast<TcBars*>(smem + C::BARS);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // row tiles of a problem are neighbours: they run together and find one another's keys in the second-level cache
-  const int tile = blockIdx.x % p.tiles, y = blockIdx.x / p.tiles, split = y % p.num_splits, z = y / p.num_splits, h = z % p.Hkv, seq = z / p.Hkv;
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
   pdl_launch_dependents();
   pdl_wait(TL_ATTN_DECODE);
-  const Span s = span_of(p, seq);
-  const int r0 = tile * TC_ROWS, rows = min(TC_ROWS, min(s.n, p.uniform_q) * p.G - r0);
-  if (rows <= 0) return;                                   // uniform, like the next one, in front of all barriers
-  const int all = (s.len + TC_KEYS - 1) / TC_KEYS, per = (all + p.num_splits - 1) / p.num_splits, t_lo = min(split * per, all), n_tiles = min(all, t_lo + per) - t_lo;
-  if (n_tiles <= 0) {                                      // fewer tiles than splits, or nothing in the cache
-    for (int r = threadIdx.x; r < rows; r += TC_THREADS) {
-      const int t = s.q0 + (r0 + r) / p.G, head = h * p.G + (r0 + r) % p.G;
+  // row tiles of a problem are neighbours: they run together and find one another's keys in the second-level cache
+  Block b;
+  const int tile = blockIdx.x % p.tiles, y = blockIdx.x / p.tiles, z = y / p.num_splits;
+  b.split = y % p.num_splits, b.h = z % p.Hkv, b.seq = z / p.Hkv;
+  b.s = span_of(p, b.seq);
+  b.r0 = tile * 2 * TC_ROWS, b.rows = min(2 * TC_ROWS, min(b.s.n, p.uniform_q) * p.G - b.r0);
+  if (b.rows <= 0) return;                                 // uniform, like the next one, in front of all barriers
+  b.two = b.rows > TC_ROWS;
+  const int all = (b.s.len + TC_KEYS - 1) / TC_KEYS, per = (all + p.num_splits - 1) / p.num_splits;
+  b.t_lo = min(b.split * per, all), b.n_tiles = min(all, b.t_lo + per) - b.t_lo, b.tail = max(max(b.s.base, 0) / TC_KEYS - b.t_lo, 0);
+  if (b.n_tiles <= 0) {                                    // fewer tiles than splits, or nothing in the cache
+    for (int r = threadIdx.x; r < b.rows; r += TC_THREADS) {
+      const int t = b.s.q0 + (b.r0 + r) / p.G, head = b.h * p.G + (b.r0 + r) % p.G;
       if ((unsigned)t >= (unsigned)p.tokens) continue;
-      if (p.part_o) p.part_ml[((long long)split * p.tokens + t) * (p.Hkv * p.G) + head] = make_float2(-INFINITY, 0.f);
+      if (p.part_o) p.part_ml[((long long)b.split * p.tokens + t) * (p.Hkv * p.G) + head] = make_float2(-INFINITY, 0.f);
       else
         for (int d = 0; d < p.Dv; ++d) reinterpret_cast<bf16*>(p.out)[t * p.out_tok + (long long)head * p.Dv + d] = __float2bfloat16(0.f);
     }
     return;
   }
+  static_assert(16 * SOFT_REGS + 4 * ROLE_REGS <= 20 * 96, "registers that the block was launched with");
+  const int users = b.two ? 2 : 1, v_stages = b.two ? 2 : 3;
   if (threadIdx.x == 0) {
-    mbar_init(&bars->q_full, 8);
-    mbar_init(&bars->k_full, 1);
-    mbar_init(&bars->k_empty, 1);
-    mbar_init(&bars->v_full, 1);
-    mbar_init(&bars->v_empty, 1);
-    mbar_init(&bars->s_full, 1);
-    mbar_init(&bars->p_full, 8);
-    mbar_init(&bars->o_final, 1);
-    bars->abort = 0, bars->odd = 0;
+    mbar_init(&bars->q_full, 16);
+    for (int i = 0; i < K_STAGES; ++i) mbar_init(&bars->k_full[i], 1), mbar_init(&bars->k_empty[i], users);
+    for (int i = 0; i < V_STAGES; ++i) mbar_init(&bars->v_full[i], 1), mbar_init(&bars->v_empty[i], users), mbar_init(&bars->v_clean[i], 8);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars->s_full[i], 1), mbar_init(&bars->p_full[i], 8);
+    mbar_init(&bars->o_final, 2);
+    bars->abort = 0, bars->odd = 0, bars->block = b;
     mbar_fence_init();
-    tma_prefetch_desc(&tmap_k);
-    tma_prefetch_desc(&tmap_v);
   }
   if (warp == MMA_WARP) {
     tmem_alloc(&bars->tmem_base, TC_COLS);
@@ -528,83 +656,108 @@ __global__ void __launch_bounds__(TC_THREADS, 2) attn_tree_tc_kernel(const __gri
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = bars->tmem_base;
-  if (warp == TMA_WARP) {
-    // lane = group of 16 keys + 8 * swizzle atom
-    const int* table = p.table + seq * p.table_stride;
-    const int g = lane & 7, atom = lane >> 3, none = p.num_blocks * p.Hkv * p.bs;
-    bool ok = true;
-    int issued_k = 0, issued_v = 0;
-    for (int j = 0; j < n_tiles && ok; ++j) {
-      const int key = (t_lo + j) * TC_KEYS + g * 16;
-      int row = none;
-      if (key < s.len) {
-        const int block = table[key / p.bs];
-        if ((unsigned)block < (unsigned)p.num_blocks) row = (block * p.Hkv + h) * p.bs + key % p.bs;
+  if (warp >= TMA_WARP) {
+    // Scores and weights of a thread's 64 keys take more registers than a 640th of the SM's: what the other warps do not need goes to the softmax's, 20 * 96 = 16 * SOFT_REGS + 4 * ROLE_REGS at most.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(ROLE_REGS));
+    if (warp == TMA_WARP) {
+      // lane = group of 16 keys + 8 * swizzle atom of a copy; looked up 32 groups ahead of it, one to a lane
+      const int* table = p.table + b.seq * p.table_stride;
+      const int g = lane & 7, atom = lane >> 3, none = p.num_blocks * p.Hkv * p.bs;
+      const auto look_up = [&](int j) {
+        const int key = (b.t_lo + j) * TC_KEYS + lane * 16;
+        int row = none;
+        if (key < b.s.len) {
+          const int block = table[key / p.bs];
+          if ((unsigned)block < (unsigned)p.num_blocks) row = (block * p.Hkv + b.h) * p.bs + key % p.bs;
+        }
+        return row;
+      };
+      bool ok = true;
+      int issued_k = 0, issued_v = 0, rows = 0, ahead = look_up(0);
+      Ring k{0, 0}, v{0, 0};
+      for (int j = 0; j < b.n_tiles && ok; ++j) {
+        if ((j & 3) == 0) rows = ahead, ahead = look_up(j + 4);
+        const int row = __shfl_sync(0xffffffffu, rows, (j & 3) * 8 + g);
+        const unsigned dead = __ballot_sync(0xffffffffu, row == none) & 0xffu;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->k_empty[k.at], k.round ^ 1, &bars->abort, 10));
+        if (!ok) break;
+        if (lane == 0) {
+          bars->dead[j & 15] = dead;
+          mbar_arrive_expect_tx(&bars->k_full[k.at], C::KT);
+        }
+        __syncwarp();
+        if (atom < DA) tma_load_2d(smem + C::K + k.at * C::KT + atom * TC_ATOM_BYTES + g * 2048, &tmap_k, &bars->k_full[k.at], atom * 64, row);
+        issued_k = j + 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_empty[v.at], v.round ^ 1, &bars->abort, 11));
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&bars->v_full[v.at], C::VT);
+        __syncwarp();
+        if (atom < VA) tma_load_2d(smem + C::V + v.at * C::VT + atom * TC_ATOM_BYTES + g * 2048, &tmap_v, &bars->v_full[v.at], atom * 64, row);
+        issued_v = j + 1;
+        k.advance(1, K_STAGES);
+        v.advance(1, v_stages);
       }
-      const unsigned dead = __ballot_sync(0xffffffffu, row == none) & 0xffu;
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars->k_empty, (j & 1) ^ 1, &bars->abort, 10));
-      if (!ok) break;
-      if (lane == 0) {
-        bars->dead[j & 1] = dead;
-        mbar_arrive_expect_tx(&bars->k_full, DA * TC_ATOM_BYTES);
+      if (!ok) {                                             // copies in flight land before the block's memory is released
+        volatile int never = 0;
+        for (int j = max(0, issued_k - K_STAGES); j < issued_k; ++j) mbar_wait(&bars->k_full[j % K_STAGES], (j / K_STAGES) & 1, &never, 13);
+        for (int j = max(0, issued_v - v_stages); j < issued_v; ++j) mbar_wait(&bars->v_full[j % v_stages], (j / v_stages) & 1, &never, 14);
       }
-      __syncwarp();
-      if (atom < DA) tma_load_2d(smem + C::K + atom * TC_ATOM_BYTES + g * 2048, &tmap_k, &bars->k_full, atom * 64, row);
-      issued_k = j + 1;
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_empty, (j & 1) ^ 1, &bars->abort, 11));
-      if (!ok) break;
-      if (lane == 0) mbar_arrive_expect_tx(&bars->v_full, VA * TC_ATOM_BYTES);
-      __syncwarp();
-      if (atom < VA) tma_load_2d(smem + C::V + atom * TC_ATOM_BYTES + g * 2048, &tmap_v, &bars->v_full, atom * 64, row);
-      issued_v = j + 1;
-    }
-    if (!ok) {                                             // copies in flight land before the block's memory is released
-      volatile int never = 0;
-      if (issued_k) mbar_wait(&bars->k_full, (issued_k - 1) & 1, &never, 13);
-      if (issued_v) mbar_wait(&bars->v_full, (issued_v - 1) & 1, &never, 14);
-    }
-  } else if (warp == MMA_WARP) {
-    constexpr uint32_t IDESC_QK = umma_idesc_bf16_f32(TC_ROWS, TC_KEYS), IDESC_PV = umma_idesc_bf16_f32(TC_ROWS, VA * 64) | (1u << 16);      // V is MN-major
-    const uint64_t qd = umma_desc_kmajor_sw128(smem_u32(smem + C::Q)), kd = umma_desc_kmajor_sw128(smem_u32(smem + C::K)), vd = umma_desc_mnmajor_sw128(smem_u32(smem + C::V));
-    const auto wait = [&](uint64_t* bar, uint32_t parity, int where) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, &bars->abort, where)) != 0; };
-    bool ok = wait(&bars->q_full, 0, 20);
-    for (int j = 0; j <= n_tiles && ok; ++j) {
-      if (j > 0) {                                         // O += P V of the tile before
-        ok = wait(&bars->p_full, (j - 1) & 1, 22) && wait(&bars->v_full, (j - 1) & 1, 23);
+    } else if (warp <= MMA_WARP + 1) {
+      constexpr uint32_t IDESC_QK = umma_idesc_bf16_f32(TC_ROWS, TC_KEYS), IDESC_PV = umma_idesc_bf16_f32(TC_ROWS, VA * 64) | (1u << 16);      // V is MN-major
+      const int slot = warp - MMA_WARP, steps = b.two ? b.n_tiles : (b.n_tiles - slot + 1) >> 1, by = b.two ? 1 : 2, first = b.two ? 0 : slot;
+      const uint64_t qd = umma_desc_kmajor_sw128(smem_u32(smem + (b.two && slot ? C::X : C::Q))), kd = umma_desc_kmajor_sw128(smem_u32(smem + C::K)), vd = umma_desc_mnmajor_sw128(smem_u32(smem + C::V));
+      const uint32_t t_s = tmem + slot * 256, t_o = t_s + 128;
+      const auto wait = [&](uint64_t* bar, uint32_t parity, int where) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, &bars->abort, where)) != 0; };
+      Ring k{first, 0}, v{first, 0};
+      const auto scores = [&]() {                            // one lane
+#pragma unroll
+        for (int e = 0; e < DA * 4; ++e) {
+          const uint32_t off = ((e >> 2) * TC_ATOM_BYTES + (e & 3) * 32) >> 4;
+          umma_f16_ss(t_s, qd + off, kd + k.at * (C::KT >> 4) + off, IDESC_QK, e > 0);
+        }
+        umma_commit(&bars->s_full[slot]);
+        umma_commit(&bars->k_empty[k.at]);
+      };
+      bool ok = wait(&bars->q_full, 0, 20);
+      if (ok && steps > 0) {
+        ok = wait(&bars->k_full[k.at], k.round, 21);
+        if (ok) {
+          tc_fence_after_sync();
+          if (elect_one()) scores();
+          __syncwarp();
+          k.advance(by, K_STAGES);
+        }
+      }
+      for (int i = 0; i < steps && ok; ++i) {
+        const int j = first + i * by;
+        const bool more = i + 1 < steps;
+        ok = j < b.tail ? wait(&bars->v_full[v.at], v.round, 23) : wait(&bars->v_clean[v.at], (j - b.tail) / v_stages & 1, 23);
+        if (ok && more) ok = wait(&bars->k_full[k.at], k.round, 21);
+        if (ok) ok = wait(&bars->p_full[slot], i & 1, 24 + slot);
         if (!ok) break;
         tc_fence_after_sync();
         if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < TC_KEYS / 16; ++k) umma_f16_ts(tmem + COL_O, tmem + COL_S + k * 8, vd + k * (2048 >> 4), IDESC_PV, j > 1 || k > 0);
-          umma_commit(&bars->v_empty);
+          for (int e = 0; e < TC_KEYS / 16; ++e)
+            umma_f16_ts(t_o, t_s + (e >> 2) * 64 + (e & 3) * 8, vd + v.at * (C::VT >> 4) + e * (2048 >> 4), IDESC_PV, i > 0 || e > 0);
+          umma_commit(&bars->v_empty[v.at]);
+          if (more) scores();
         }
         __syncwarp();
+        v.advance(by, v_stages);
+        k.advance(by, K_STAGES);
       }
-      if (j < n_tiles) {
-        ok = wait(&bars->k_full, j & 1, 21);
-        if (!ok) break;
-        tc_fence_after_sync();
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < DA * 4; ++k) {
-            const uint32_t off = ((k >> 2) * TC_ATOM_BYTES + (k & 3) * 32) >> 4;
-            umma_f16_ss(tmem + COL_S, qd + off, kd + off, IDESC_QK, k > 0);
-          }
-          umma_commit(&bars->s_full);
-          umma_commit(&bars->k_empty);
-        }
-        __syncwarp();
-      }
-    }
-    if (elect_one()) umma_commit(&bars->o_final);          // also where a wait ran out: it tracks what has been issued
-    __syncwarp();
-    if (!ok) {
-      volatile int never = 0;
-      mbar_wait(&bars->o_final, 0, &never, 27);
+      if (elect_one()) umma_commit(&bars->o_final);          // also where a wait ran out: it tracks what has been issued
       __syncwarp();
+      if (!ok) {
+        volatile int never = 0;
+        mbar_wait(&bars->o_final, 0, &never, 27);
+        __syncwarp();
+      }
     }
   } else {
-    tree_softmax<DA, VA, CAP>(p, bars, smem, tmem, s, seq, h, r0, rows, split, t_lo, n_tiles);
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFT_REGS));
+    tree_softmax<DA, VA, CAP>(p, bars, smem, tmem);
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -615,15 +768,16 @@ __global__ void __launch_bounds__(TC_THREADS, 2) attn_tree_tc_kernel(const __gri
 }
 
 // ---- sum of the splits --------------------------------------------------------------------------------------------------------------------------------
-// A warp to a row and head, weighed by the distance of its splits' maxima to the common one.
-constexpr int JOIN_THREADS = 128;
+// A warp to a row and head, weighed by the distance of its splits' maxima to the common one; the parts of eight splits are on their way together. VEC: four columns to a lane.
+constexpr int JOIN_THREADS = 128, JOIN_AHEAD = 8;
 
-template <typename E>
+template <typename E, bool VEC>
 __global__ void __launch_bounds__(JOIN_THREADS) attn_tree_join_kernel(const TreeParams p) {
   pdl_launch_dependents();
+  constexpr int W = VEC ? 4 : 1;
   const int Hq = p.Hkv * p.G, lane = threadIdx.x & 31, S = p.num_splits;
   const long long i = (long long)blockIdx.x * (JOIN_THREADS / 32) + (threadIdx.x >> 5), rows = (long long)p.tokens * Hq;
-  pdl_wait();
+  pdl_wait(TL_ATTN_MERGE);
   if (i >= rows) return;
   const int t = (int)(i / Hq), head = (int)(i % Hq);
   if (p.cu_q) {
@@ -632,21 +786,55 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_tree_join_kernel(const Tree
     if (t - p.cu_q[seq] >= p.uniform_q) return;              // more tokens than the call was told of: not computed
   }
   float2 a = make_float2(-INFINITY, 0.f), b = a;
-  if (lane < S) a = p.part_ml[lane * rows + i];
-  if (lane + 32 < S) b = p.part_ml[(lane + 32) * rows + i];
+  if (lane < S) a = __ldcg(p.part_ml + lane * rows + i);
+  if (lane + 32 < S) b = __ldcg(p.part_ml + (lane + 32) * rows + i);
   const float top = warp_max(fmaxf(a.x, b.x)), base = top == -INFINITY ? 0.f : top;
-  const float fa = exp2f(a.x - base), fb = exp2f(b.x - base);
+  float fa = exp2f(a.x - base), fb = exp2f(b.x - base);
   const float sum = warp_sum(fmaf(fa, a.y, fb * b.y)), inv = sum == 0.f ? 0.f : 1.f / sum;
+  fa *= inv, fb *= inv;
   E* out = reinterpret_cast<E*>(p.out) + t * p.out_tok + (long long)head * p.Dv;
-  for (int d0 = 0; d0 < p.Dv; d0 += 32) {
-    const int d = d0 + lane;
-    float x = 0.f;
-    for (int s = 0; s < S; ++s) {                            // all lanes: each has the factors of two splits
-      const float f = __shfl_sync(0xffffffffu, s < 32 ? fa : fb, s & 31);
-      if (d < p.Dv && f != 0.f) x = fmaf(f, p.part_o[(s * rows + i) * p.Dv + d], x);      // of a split without keys nothing was written
+  for (int d0 = 0; d0 < p.Dv; d0 += 32 * W) {
+    const int d = d0 + lane * W;
+    const float* part = p.part_o + i * p.Dv + d;
+    float x[W];
+#pragma unroll
+    for (int k = 0; k < W; ++k) x[k] = 0.f;
+    for (int s0 = 0; s0 < S; s0 += JOIN_AHEAD) {
+      float y[JOIN_AHEAD][W], f[JOIN_AHEAD];
+#pragma unroll
+      for (int u = 0; u < JOIN_AHEAD; ++u) {                 // all lanes: each has the factors of two splits
+        const int s = s0 + u;
+        f[u] = __shfl_sync(0xffffffffu, s < 32 ? fa : fb, s & 31);
+        const bool take = s < S && d < p.Dv && f[u] != 0.f;  // of a split without keys nothing was written
+        if constexpr (VEC) {
+          const float4 v = take ? __ldcg(reinterpret_cast<const float4*>(part + s * rows * p.Dv)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          y[u][0] = v.x, y[u][W > 1] = v.y, y[u][W / 2] = v.z, y[u][W - 1] = v.w;
+        } else {
+          y[u][0] = take ? __ldcg(part + s * rows * p.Dv) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < JOIN_AHEAD; ++u)
+#pragma unroll
+        for (int k = 0; k < W; ++k)
+          if (f[u] != 0.f) x[k] = fmaf(f[u], y[u][k], x[k]);
     }
-    if (d < p.Dv) store_out(out + d, x * inv);
+    if (d >= p.Dv) continue;
+    if (VEC && p.out_vec) {
+      store_row4(out + d, make_float4(x[0], x[W > 1], x[W / 2], x[W - 1]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < W; ++k) store_out(out + d + k, x[k]);
+    }
   }
+}
+
+template <typename E>
+int launch_join(TreeParams p, cudaStream_t s) {
+  const long long rows = (long long)p.tokens * p.Hkv * p.G;
+  p.out_vec = (reinterpret_cast<uintptr_t>(p.out) & (4 * sizeof(E) - 1)) == 0 && p.out_tok % 4 == 0;
+  return launch_kernel(p.Dv % 4 == 0 ? attn_tree_join_kernel<E, true> : attn_tree_join_kernel<E, false>, dim3((unsigned)((rows + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32))),
+                       dim3(JOIN_THREADS), 0, s, p);
 }
 
 template <typename E, int COLS, bool VEC>
@@ -717,10 +905,10 @@ int swb_attn_tree(const int* dims, const long long* strides, const void* q, void
   if (p.num_seqs > 65535 || p.max_blocks < 1 || p.num_blocks < 1 || p.bs < 1 || p.Hkv < 1 || p.G < 1 || p.G > MAX_GROUP || p.D < 1 || p.D > 256 || p.Dv < 1 || p.Dv > 256 ||
       p.num_splits < 1 || p.num_splits > MAX_SPLITS || p.uniform_q < 1 || p.words < 1 || !q || !out || !k || !v || !table || !kv_lens || !mask)
     return -3;
-  if ((long long)p.max_blocks * p.bs > INT_MAX || (long long)p.uniform_q * p.G > INT_MAX - TC_ROWS) return -3;
+  if ((long long)p.max_blocks * p.bs > INT_MAX || (long long)p.uniform_q * p.G > INT_MAX - 2 * TC_ROWS) return -3;
   p.scale = scale, p.softcap = softcap, p.k = k, p.v = v;
   const bool fast = tc_fits(p, fp32);
-  const int tile = fast ? TC_ROWS : PR;
+  const int tile = fast ? 2 * TC_ROWS : PR;
   p.tiles = (p.uniform_q * p.G + tile - 1) / tile;
   if ((long long)p.tiles * p.num_seqs * p.Hkv > INT_MAX / p.num_splits || (long long)p.tokens * p.Hkv * p.G > INT_MAX) return -3;
   p.q = q, p.out = out, p.table = table, p.cu_q = cu_q, p.kv_lens = kv_lens, p.mask = reinterpret_cast<const unsigned*>(mask);
@@ -734,8 +922,7 @@ int swb_attn_tree(const int* dims, const long long* strides, const void* q, void
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int rc = fast ? (softcap > 0.f ? launch_tc<true>(p, s) : launch_tc<false>(p, s)) : fp32 ? launch_plain<float>(p, s) : launch_plain<bf16>(p, s);
   if (rc || p.num_splits == 1) return rc;
-  const dim3 grid((unsigned)((rows + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32)));
-  return fp32 ? launch_kernel(attn_tree_join_kernel<float>, grid, dim3(JOIN_THREADS), 0, s, p) : launch_kernel(attn_tree_join_kernel<bf16>, grid, dim3(JOIN_THREADS), 0, s, p);
+  return fp32 ? launch_join<float>(p, s) : launch_join<bf16>(p, s);
 }
 
 }  // extern "C"

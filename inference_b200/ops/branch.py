@@ -61,8 +61,8 @@ def _check_ranges(cu_q: torch.Tensor | None, max_q_len: int, tokens: int) -> int
 
 
 def tree_splits(problems: int, keys: int, tensor_cores: bool = True, sms: int = 148) -> int:
-    """Blocks that share the keys of a tile of rows: as many as the SMs hold at once (two to an SM of the kernel on tensor memory, four of the plain one), of a tile of keys and more."""
-    slots, tile = (2 * sms, 128) if tensor_cores else (4 * sms, 64)
+    """Blocks that share the keys of a tile of rows: as many as the SMs hold at once (one to an SM of the kernel on tensor memory, four of the plain one), of a tile of keys and more."""
+    slots, tile = (sms, 128) if tensor_cores else (4 * sms, 64)
     return max(1, min(MAX_SPLITS, (keys + tile - 1) // tile, slots // max(1, problems)))
 
 
@@ -89,7 +89,7 @@ def tree_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, 
         _require(out.stride(0) >= columns or T <= 1, "rows of out share memory")
     k_ptr, v_ptr = kcache.data_ptr(), vcache.data_ptr()
     fast = kind is torch.bfloat16 and (D | Dv) % 8 == 0 and D <= 128 and Dv <= 128 and bs % 16 == 0 and scale > 0 and (k_ptr | v_ptr) % 16 == 0 and blocks * heads * bs < 2 ** 31 - 1
-    problems = n * heads * -(-max_q_len * G // (128 if fast else 32))
+    problems = n * heads * -(-max_q_len * G // (256 if fast else 32))
     splits = tree_splits(problems, per * bs, fast) if num_splits is None else num_splits
     _require(1 <= splits <= MAX_SPLITS, "1 to 64 splits")
     ws, nbytes = None, 0
