@@ -137,7 +137,7 @@ def _declare_kernels(lib: ctypes.CDLL) -> None:
     sig("swb_plan_tree", [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p])
     sig("swb_accept_tree", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p])
     sig("swb_copy_pages", [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p])
-    sig("swb_beam_pieces", [c_int, c_int, c_void_p])
+    sig("swb_beam_workspace_bytes", [c_int, c_int, c_int, c_int], c_ll)
     sig("swb_beam_select", [c_void_p, c_ll, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_void_p])
     sig("swb_evict", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p])
     sig("swb_attn_simple", [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_int, c_int, c_void_p, c_void_p,

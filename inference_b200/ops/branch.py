@@ -12,7 +12,6 @@ Caches are bf16 or fp32, widths up to 256; the caches of all layers together are
 run on the current stream, take no host reads and can be captured into graphs. Scores, the softmax and all sums are 32-bit numbers, those of `beam_select` 64-bit ones."""
 from __future__ import annotations
 
-import ctypes
 import math
 import struct
 from dataclasses import dataclass
@@ -203,8 +202,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, count: int) -> Be
     _require(1 <= K <= MAX_BEAMS and B * K < 65536, "1 to 256 beams, fewer than 65536 of all prompts")
     _require(1 <= count <= MAX_COUNT and V < 2 ** 31 - 65536, "1 to 128 continuations, a vocabulary below 2^31 - 65536")
     got = BeamChoice(scores.new_empty((B, count)), scores.new_empty((B, count), dtype=torch.int32), scores.new_empty((B, count), dtype=torch.int64))
-    each = ctypes.c_longlong()
-    nbytes = kernels().swb_beam_pieces(V, count, ctypes.byref(each)) * each.value * B * K
+    nbytes = kernels().swb_beam_workspace_bytes(B, K, V, count)
     ws = scores.new_empty(nbytes, dtype=torch.uint8)
     check(kernels().swb_beam_select(logits.data_ptr(), logits.stride(0), logits.dtype == torch.float32, scores.data_ptr(), B, K, V, count, got.scores.data_ptr(), got.beams.data_ptr(),
                                     got.tokens.data_ptr(), ws.data_ptr(), nbytes, stream), "swb_beam_select")

@@ -450,7 +450,7 @@ def _check_beams(logits, scores, count):
         assert got.beams[b].tolist() == [w[1] for w in want], b
         assert got.tokens[b].tolist() == [w[2] for w in want], b
         for a, w in zip(got.scores[b].tolist(), want):
-            # rounded once to 32 bits; each exponential within 2^-30 of its value, and so the logarithm of their sum
+            # rounded once to 32 bits; each exponential within 2^-29 of its value, and so the logarithm of their sum
             assert a == w[0] or abs(a - w[0]) <= 2.0 ** -24 * abs(w[0]) + 2.0 ** -29, (a, w)
 
 
