@@ -13,7 +13,7 @@ import torch
 
 from ..contracts.errors import Unsupported
 from ..models.oracle import ContiguousKvCache, OracleLlama
-from .kv_pool import PagedSequence
+from .kv_pool import PagedSequence, unshare_tails
 from .runner import ModelRunner
 
 
@@ -34,6 +34,11 @@ class DecodeBackend(Protocol):
     def fork(self, seq: Any, n_tokens: int) -> Any:
         """A new sequence sharing the first n_tokens tokens of seq's cache (copy-on-write where supported)."""
     def release(self, seq: Any) -> None: ...
+    def reorder(self, seqs: list[Any], parents: list[int]) -> list[Any]:
+        """Sequences that continue seqs[parents[i]], as many as parents; a sequence with several children is copied (on write), one with none is released."""
+    def step_trees(self, seqs: list[Any], tokens: list[list[int]], parents: list[list[int]], choose) -> list[tuple[list[int], int]]:
+        """Appends to each sequence the path of its drafted tree (tokens, and the place of each one's parent, -1 of the root) that choose agrees with: the path's places and
+        the token behind it. choose(logits [all trees' tokens, vocab]) -> int64 tokens, one a row."""
 
 
 def set_embed_override(seq: Any, positions: list[int], values: torch.Tensor) -> None:
@@ -194,6 +199,47 @@ class GpuBackend:
     def release(self, seq):
         seq.release()
 
+    def reorder(self, seqs, parents):
+        keep = set(parents)
+        for i, s in enumerate(seqs):
+            if i not in keep:
+                s.release()                    # in front of the copies: their state slots and pages may be these
+        out, forks, used, src, dst = [], [], set(), [], []
+        try:
+            for p in parents:
+                if p not in used:
+                    used.add(p)
+                    out.append(seqs[p])
+                    continue
+                f = seqs[p].fork()
+                forks.append(f)
+                out.append(f)
+                if f.stateful and seqs[p].state_slot >= 0:
+                    f.state_slot = f.pool.slots.alloc()
+                    src.append(seqs[p].state_slot)
+                    dst.append(f.state_slot)
+            if src:
+                self.runner.pool.copy_states(src, dst)
+            unshare_tails(out)
+        except BaseException:                  # no page or slot is free: nothing is held that the caller does not know
+            for f in forks:
+                f.release()
+            raise
+        return out
+
+    def step_trees(self, seqs, tokens, parents, choose):
+        if any(getattr(s, "pending_embeds", None) is not None or getattr(s, "pending_mrope", None) is not None for s in seqs):
+            raise Unsupported("drafted trees behind a prompt whose embeddings have not been run")
+        lengths = [s.length for s in seqs]
+        try:
+            logits, step = self.runner.verify_trees(seqs, tokens, parents)
+            return self.runner.accept_trees(step, choose(logits))
+        except BaseException:                  # the trees' entries are not those of a text
+            for s, n in zip(seqs, lengths):
+                if s.length > n:
+                    s.truncate(n)
+            raise
+
 
 class _OracleSeq:
     def __init__(self, cache: ContiguousKvCache):
@@ -254,3 +300,38 @@ class OracleBackend:
 
     def release(self, seq):
         seq.cache.reset()
+
+    def reorder(self, seqs, parents):
+        out, used = [], set()
+        for p in parents:
+            out.append(self.fork(seqs[p], self.length(seqs[p])) if p in used else seqs[p])
+            used.add(p)
+        for i, s in enumerate(seqs):
+            if i not in used:
+                self.release(s)
+        return out
+
+    def step_trees(self, seqs, tokens, parents, choose):
+        """Each token of a tree by itself, behind its path."""
+        rows = []
+        for s, toks, ups in zip(seqs, tokens, parents):
+            for i in range(len(toks)):
+                path, j = [], i
+                while j >= 0:
+                    path.append(toks[j])
+                    j = ups[j]
+                f = self.fork(s, self.length(s))
+                rows.append(self.forward([f], [path[::-1]])[0])
+                self.release(f)
+        picks, out, at = choose(torch.stack(rows)).tolist(), [], 0
+        for s, toks, ups in zip(seqs, tokens, parents):
+            path = [0]
+            while True:
+                nxt = [i for i in range(path[-1] + 1, len(toks)) if ups[i] == path[-1] and toks[i] == picks[at + path[-1]]]
+                if not nxt:
+                    break
+                path.append(nxt[0])
+            self.forward([s], [[toks[i] for i in path]])
+            out.append((path, picks[at + path[-1]]))
+            at += len(toks)
+        return out

@@ -84,6 +84,14 @@ class BatchingBackend:
         with self._lock:
             return self.inner.release(seq)
 
+    def reorder(self, seqs, parents):
+        with self._lock:
+            return self.inner.reorder(seqs, parents)
+
+    def step_trees(self, seqs, tokens, parents, choose):
+        with self._lock:                         # a step of its own: trees are not merged with other callers' tokens
+            return self.inner.step_trees(seqs, tokens, parents, choose)
+
     # ---- model calls -------------------------------------------------------------------------------------------
     def _submit(self, call: _Call):
         with self._cv:

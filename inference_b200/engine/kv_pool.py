@@ -15,6 +15,25 @@ import torch
 from ..policy.paging import BlockAllocator
 
 
+def copy_entries(tensors, src: list[int], dst: list[int]) -> None:
+    """Entry dst[i] (a page, a state slot) of every tensor becomes a copy of its entry src[i]. tensors: a uniform pool's, or a list of [entries, ...] on one device. On the GPU one
+    launch for all of them."""
+    if not src:
+        return
+    whole = isinstance(tensors, torch.Tensor)
+    device = (tensors if whole else tensors[0]).device
+    if device.type == "cuda":
+        from ..ops import copy_pages
+
+        with torch.cuda.device(device):
+            copy_pages(tensors, src, dst)
+    elif whole:
+        tensors[:, :, dst] = tensors[:, :, src]
+    else:
+        for t in tensors:
+            t[dst] = t[src]
+
+
 class PagedKvPool:
     def __init__(self, num_layers: int, num_blocks: int, kv_heads: int, head_dim: int, block_size: int = 16,
                  device: torch.device | str = "cuda", dtype: torch.dtype = torch.bfloat16):
@@ -43,7 +62,11 @@ class PagedKvPool:
 
     def copy_block(self, src: int, dst: int) -> None:
         """Copy-on-write: duplicate one block across all layers (K and V)."""
-        self.data[:, :, dst].copy_(self.data[:, :, src])
+        self.copy_blocks([src], [dst])
+
+    def copy_blocks(self, src: list[int], dst: list[int]) -> None:
+        """Several blocks at once; the ones that are written are others than those that are copied."""
+        copy_entries(self.data, src, dst)
 
     @staticmethod
     def blocks_for_budget(bytes_budget: int, num_layers: int, kv_heads: int, head_dim: int, block_size: int = 16,
@@ -135,17 +158,23 @@ class LayeredKvPool:
     def bytes(self) -> int:
         return sum(t.numel() * t.element_size() for kv in self.data for t in kv)
 
+    def _tensors(self, per_sequence: bool) -> list[torch.Tensor]:
+        return [t for g, kv in zip(self.geometry, self.data) if isinstance(g, PER_SEQUENCE) == per_sequence for t in kv]
+
     def copy_block(self, src: int, dst: int) -> None:
-        for g, kv in zip(self.geometry, self.data):
-            if not isinstance(g, PER_SEQUENCE):
-                for t in kv:
-                    t[dst].copy_(t[src])
+        self.copy_blocks([src], [dst])
+
+    def copy_blocks(self, src: list[int], dst: list[int]) -> None:
+        tensors = self._tensors(False)
+        if tensors:
+            copy_entries(tensors, src, dst)
 
     def copy_state(self, src: int, dst: int) -> None:
-        for g, kv in zip(self.geometry, self.data):
-            if isinstance(g, PER_SEQUENCE):
-                for t in kv:
-                    t[dst].copy_(t[src])
+        if src != dst:
+            self.copy_states([src], [dst])
+
+    def copy_states(self, src: list[int], dst: list[int]) -> None:
+        copy_entries(self._tensors(True), src, dst)
 
     @staticmethod
     def block_bytes(geometry, block_size: int = 16, elem: int = 2) -> int:
@@ -177,6 +206,14 @@ class PagedSequence:
             pool.allocator.retain(b)
         s.blocks = list(blocks)
         s.length = length
+        return s
+
+    def fork(self) -> "PagedSequence":
+        """A sequence that shares all of this one's pages, the last one too, which whoever writes into it first takes a copy of (`unshare_tails`). A recurrent state is not copied here."""
+        s = PagedSequence.seeded(self.pool, self.blocks, self.length)
+        s.tokens = None if self.tokens is None else list(self.tokens)
+        if getattr(self, "rope_delta", 0):
+            s.rope_delta = self.rope_delta
         return s
 
     def reserve(self, n_tokens: int) -> list[int]:
@@ -245,3 +282,33 @@ class PagedSequence:
             self.pool.slots.release(self.state_slot)
             self.state_slot = -1
         self.tokens = []
+
+
+def unshare_tails(seqs: list[PagedSequence]) -> None:
+    """Gives every sequence whose next token goes into a page that it shares a copy of that page, all of them by one launch."""
+    if not seqs:
+        return
+    pool = seqs[0].pool
+    left = {}                                   # of each such page: the sequences that will still hold it
+    moves = []
+    for s in seqs:
+        at, inside = divmod(s.length, pool.block_size)
+        if inside:
+            page = s.blocks[at]
+            left[page] = left.get(page, pool.allocator.refcount(page)) - 1
+            if left[page] > 0:                  # the last one writes into the page itself
+                moves.append((s, at, page))
+    fresh = []
+    try:
+        for _ in moves:
+            fresh.append(pool.allocator.alloc())
+        if moves:
+            pool.copy_blocks([page for _, _, page in moves], fresh)
+    except BaseException:                       # no page is free: every sequence is as it was
+        for page in fresh:
+            pool.allocator.release(page)
+        raise
+    for (s, at, page), own in zip(moves, fresh):
+        s.blocks[at] = own
+        s.epoch += 1
+        pool.allocator.release(page)

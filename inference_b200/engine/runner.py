@@ -40,6 +40,15 @@ class _DecodeGraph:
     launches: int
 
 
+@dataclass
+class _TreeStep:
+    """A step over drafted trees between its forward and the acceptance."""
+    seqs: list[PagedSequence]
+    parents: list[list[int]]
+    inputs: StepInputs | None = None
+    device_parents: torch.Tensor | None = None
+
+
 class ModelRunner:
     MULTI_STEPS = 256
 
@@ -109,7 +118,7 @@ class ModelRunner:
     # ---- prefill (eager, ragged) ------------------------------------------------------------------
     def prefill(self, seqs: list[PagedSequence], new_tokens: list[list[int]], *, want_logits: bool = False,
                 all_positions: bool = False, embed_overrides: list[tuple[list[int], torch.Tensor] | None] | None = None,
-                mrope_overrides: list | None = None, want: list[list[int]] | None = None):
+                mrope_overrides: list | None = None, want: list[list[int]] | None = None, trees: "_TreeStep | None" = None):
         """Appends new_tokens[i] to seqs[i] (any mix of lengths, including chunked / prefix-seeded sequences)
         and returns greedy next tokens [num_seqs] (or fp32 logits when want_logits). embed_overrides[i] =
         (positions within new_tokens[i], vectors [len(positions), hidden]) replaces those tokens' embeddings (the
@@ -118,7 +127,7 @@ class ModelRunner:
         the residual stream at `rows` after decoder layer l; the sequence's later tokens continue at `next position`
         (kept on the sequence as `rope_delta`). all_positions: the fp32 logits of every token, as a step that verifies drafts asks for; with a page budget such a step reads what
         decode steps would. want[i] = places within new_tokens[i]: returns the fp32 logits of exactly
-        these places, sequence by sequence [sum of len(want[i]), vocab]."""
+        these places, sequence by sequence [sum of len(want[i]), vocab]. trees: see `verify_trees`, which this serves."""
         dev = self.model.device
         ids, pos, slots, cu, kvl, rows = [], [], [], [0], [], []
         fresh = all(s.length == 0 for s in seqs)     # no earlier context: attention can read K / V from the QKV buffer
@@ -127,7 +136,13 @@ class ModelRunner:
             sl = s.reserve(len(toks))
             ids += toks
             delta = getattr(s, "rope_delta", 0)
-            pos.extend(range(start + delta, start + delta + len(toks)))
+            if trees is None:
+                pos.extend(range(start + delta, start + delta + len(toks)))
+            else:
+                depths = []
+                for up in trees.parents[len(kvl)]:
+                    depths.append(depths[up] + 1 if up >= 0 else 0)
+                pos.extend(start + delta + d for d in depths)
             slots += sl
             cu.append(cu[-1] + len(toks))
             kvl.append(s.length)
@@ -137,10 +152,10 @@ class ModelRunner:
         maxb = max(len(s.blocks) for s in seqs)
         max_q = max(len(t) for t in new_tokens)
         G = self.model.cfg.groups
-        decode = max_q * G <= 16 and all(len(t) == max_q for t in new_tokens)
+        decode = trees is None and max_q * G <= 16 and all(len(t) == max_q for t in new_tokens)
         states = [s.state_slot for s in seqs] if self._stateful else []
-        d_ids, d_slots, d_rows, d_pos, d_cu, d_kvl, d_states, d_table = self._upload(
-            (ids, slots, [] if all_positions else rows), (pos, cu, kvl, states), [s.blocks for s in seqs], maxb)
+        d_ids, d_slots, d_rows, d_pos, d_cu, d_kvl, d_states, d_parents, d_table = self._upload(
+            (ids, slots, [] if all_positions else rows), (pos, cu, kvl, states, [] if trees is None else [up for p in trees.parents for up in p]), [s.blocks for s in seqs], maxb)
         inp = StepInputs(
             input_ids=d_ids, positions=d_pos, slot_mapping=d_slots, block_table=d_table, kv_lens=d_kvl,
             cu_q=None if decode else d_cu, max_q_len=max_q,
@@ -149,6 +164,11 @@ class ModelRunner:
             logits_rows=None if all_positions else d_rows,
             page_budget=self.page_budget if all_positions or max_q == 1 else None, summaries=self._summaries(),
             spans=[(len(t), n) for t, n in zip(new_tokens, kvl)])
+        if trees is not None:
+            from ..ops import plan_tree
+
+            inp.tree = plan_tree(d_parents, cu_q=d_cu, max_q_len=max_q).mask
+            trees.inputs, trees.device_parents = inp, d_parents
         if self._stateful:
             inp.state_slots = d_states
             for s, toks in zip(seqs, new_tokens):
@@ -170,6 +190,33 @@ class ModelRunner:
             if want_logits or all_positions or want is not None:
                 return self.model.logits(hidden)
             return self.model.greedy_tokens(hidden)
+
+    def verify_trees(self, seqs: list[PagedSequence], tokens: list[list[int]], parents: list[list[int]]) -> tuple[torch.Tensor, "_TreeStep"]:
+        """One step over drafted trees: fp32 logits of all their tokens [sum of len(tokens[i]), vocab], and what `accept_trees` takes. tokens[i][0] is the last token that is certain, the others hang on the
+        token of their sequence at place parents[i][j] < j (-1 for the first). `accept_trees` has to follow, which leaves the cache with the accepted tokens; without it the
+        sequences have to be truncated to what they were."""
+        if self._stateful or self.page_budget is not None or self._summaries() is not None or not (isinstance(self.model, LlamaGpu) and isinstance(self.pool, PagedKvPool)):
+            raise Unsupported("drafted trees need a decoder of the Llama family on a uniform pool without page summaries")
+        if any(len(t) != len(p) or not t or p[0] != -1 or any(not 0 <= up < j for j, up in enumerate(p) if j) for t, p in zip(tokens, parents)):
+            raise ValueError("a tree has a root and tokens that hang on tokens in front of them")
+        if not len(seqs) == len(tokens) == len(parents) or len({id(s) for s in seqs}) != len(seqs):
+            raise ValueError("a tree for each sequence, and each sequence once")
+        step = _TreeStep(list(seqs), parents)
+        return self.prefill(seqs, tokens, all_positions=True, trees=step), step
+
+    def accept_trees(self, step: "_TreeStep", picks: torch.Tensor) -> list[tuple[list[int], int]]:
+        """Ends the step of `verify_trees`: picks int64 [sum of len(tokens[i])] are the model's tokens behind each of the drafted ones. Per sequence the accepted places and the token
+        behind the last of them; the sequences end with the accepted tokens."""
+        from ..ops import accept_tree
+
+        inp = step.inputs
+        got = accept_tree(picks, inp.input_ids, step.device_parents, self.pool.data, inp.block_table, inp.kv_lens, cu_q=inp.cu_q, max_q_len=inp.max_q_len)
+        host = torch.cat([got.counts[:, None].long(), got.kv_lens[:, None].long(), got.next_tokens[:, None], got.path.long()], 1).tolist()
+        out = []
+        for s, (count, length, token, *path) in zip(step.seqs, host):
+            s.truncate(length)
+            out.append((path[:count], token))
+        return out
 
     def _upload(self, wide, narrow, tables, maxb: int):
         """Lists of int64 and of int32 and a ragged int32 table as device tensors, by one copy from pinned memory of the call's own: the host prepares the

@@ -47,6 +47,7 @@ class StepInputs:
     #                                           touch any: a padding row); None for models without recurrent layers
     page_budget: "ops.PageBudget | None" = None    # not None: the step reads the pages that it selects for each token ...
     summaries: list | None = None              # ... by these summaries, one `ops.PageSummaries` a layer, which every step keeps up
+    tree: torch.Tensor | None = None           # the new tokens are drafted trees: what each of them sees of its sequence's new tokens (`ops.TreePlan.mask`)
     spans: list[tuple[int, int]] | None = None # host copy of (new tokens, context length) per sequence; None in a decode
     #                                           step (one token each, lengths change under a captured graph)
 
@@ -402,7 +403,7 @@ class LlamaGpu:
         D = cfg.head_dim
         eps, woff = cfg.rms_norm_eps, cfg.norm_weight_offset
         T = inp.input_ids.numel()
-        if self._use_tp_prefill(T) and inp.page_budget is None and inp.embed_rows is None and inp.rope_table is None and inp.deepstack is None:
+        if self._use_tp_prefill(T) and inp.page_budget is None and inp.tree is None and inp.embed_rows is None and inp.rope_table is None and inp.deepstack is None:
             return self._forward_hidden_tp_prefill(inp, kv_pool)
         rope_pos, rope_cos, rope_sin = inp.positions, self.cos, self.sin
         if inp.rope_table is not None:
@@ -461,7 +462,10 @@ class LlamaGpu:
             if inp.summaries is not None:
                 ops.summarize_pages(kv_pool[li, 0], inp.block_table, inp.kv_lens, inp.summaries[li], cu_q=inp.cu_q, max_q_len=inp.max_q_len)
                 n += 1
-            if inp.page_budget is not None:
+            if inp.tree is not None:
+                attn = ops.tree_attention(q, kv_pool[li, 0], kv_pool[li, 1], inp.block_table, inp.kv_lens, inp.tree, cu_q=inp.cu_q, max_q_len=inp.max_q_len,
+                                          scale=cfg.attn_scale, softcap=cfg.attn_logit_softcap or 0.0)
+            elif inp.page_budget is not None:
                 budget, all_pages = inp.page_budget, inp.block_table.shape[1]      # what goes past the table's pages selects nothing more
                 chosen = ops.select_pages(q, inp.summaries[li], inp.block_table, inp.kv_lens, cu_q=inp.cu_q, max_q_len=inp.max_q_len, block_size=block_size,
                                           top=min(budget.top, all_pages), first=min(budget.first, all_pages), last=min(budget.last, all_pages))

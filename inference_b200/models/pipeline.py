@@ -12,6 +12,7 @@ from typing import Callable, Sequence
 import torch
 
 from ..contracts.errors import LoadError
+from ..engine.kv_pool import copy_entries
 from .config import ModelConfig
 from .llama import LlamaGpu, StepInputs
 
@@ -65,8 +66,11 @@ class ShardedKvPool:
         return sum(t.numel() * t.element_size() for t in self.data)
 
     def copy_block(self, src: int, dst: int) -> None:
+        self.copy_blocks([src], [dst])
+
+    def copy_blocks(self, src: list[int], dst: list[int]) -> None:
         for t in self.data:
-            t[:, :, dst].copy_(t[:, :, src])
+            copy_entries(t, src, dst)
 
 
 class PipelineLlama:

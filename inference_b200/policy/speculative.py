@@ -33,3 +33,30 @@ def accept_token(target: list[tuple[int, float]], draft: list[tuple[int, float]]
                                 i32_array([d[0] for d in draft]), f32_array([d[1] for d in draft]), len(draft),
                                 proposed, u_accept, u_resample, ctypes.byref(tok))
     return bool(ok), tok.value
+
+
+def ngram_tree(tokens: list[int], max_ngram: int, branches: int, depth: int) -> tuple[list[int], list[int]]:
+    """Prompt lookup with several answers: what followed the earlier occurrences of the longest repeated run that ends `tokens` (up to max_ngram long, shorter runs while there is room), the
+    latest first, up to `branches` different continuations of up to `depth` tokens, as one tree. Returns its tokens, the last of `tokens` first, and each one's parent (-1 of the root)."""
+    out, parents, children = [tokens[-1]], [-1], {}
+    found, seen = 0, set()
+    for n in range(min(max_ngram, len(tokens) - 1), 0, -1):
+        run = tokens[-n:]
+        for at in range(len(tokens) - n - 1, -1, -1):
+            if found >= branches or depth < 1:
+                return out, parents
+            if tokens[at:at + n] != run:
+                continue
+            follow = tuple(tokens[at + n:at + n + depth])
+            if follow in seen:
+                continue
+            seen.add(follow)
+            found += 1
+            node = 0
+            for t in follow:
+                if (node, t) not in children:
+                    children[node, t] = len(out)
+                    out.append(t)
+                    parents.append(node)
+                node = children[node, t]
+    return out, parents
