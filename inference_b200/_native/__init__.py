@@ -135,8 +135,8 @@ def _declare_kernels(lib: ctypes.CDLL) -> None:
                             c_float, c_float, c_void_p, c_ll, c_void_p])
     sig("swb_attn_tree", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_float, c_void_p, c_ll, c_void_p])
     sig("swb_plan_tree", [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p])
-    sig("swb_accept_tree", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p])
-    sig("swb_copy_pages", [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p])
+    sig("swb_accept_tree", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p])
+    sig("swb_copy_pages", [c_void_p, c_void_p, c_ll, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p])
     sig("swb_beam_workspace_bytes", [c_int, c_int, c_int, c_int], c_ll)
     sig("swb_beam_select", [c_void_p, c_ll, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_void_p])
     sig("swb_evict", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p])

@@ -4,6 +4,7 @@
 // Caches are tensors [blocks, ...], one or two a layer, whose pages have one number in all of them: a list of bases and row sizes goes to the kernels by value, so that a
 // launch takes every layer and nothing is uploaded in front of it.
 #include "common.cuh"
+#include "gemm_tcgen05.cuh"
 
 #include <climits>
 #include <cstring>
@@ -20,6 +21,7 @@ struct Tensors {
   char* base[MAX_TENSORS];
   long long page_bytes[MAX_TENSORS];
   int heads[MAX_TENSORS];                                  // a page is [heads, block_size, row]
+  int start[MAX_TENSORS], cols[MAX_TENSORS];               // of the acceptance: columns of the tensors in front of this one, and of one of its rows
   int n;
 };
 
@@ -69,37 +71,44 @@ struct AcceptParams {
   int* lens;
 };
 
-constexpr int ACCEPT_THREADS = 256, MOVES = 8;
+constexpr int ACCEPT_THREADS = 256, ACCEPT_BLOCKS = 4, MOVES = 8;         // ACCEPT_BLOCKS of them to an SM: 64 registers a thread
 
-// Block x of sequence y walks the tree (a warp; the other blocks' walks are the same), then each thread takes one column of one row of one tensor along the path: entry path[d]
-// goes to d. path[d] >= d and both ascend, so that an entry which is written has been read before, by the same thread, and none is read after it was written.
+struct Move {
+  int from_page, from_row, to_page, to_row;                // to_page < 0: nothing to move
+};
+
+// Block x of sequence y finds the sequence's path, then each of its threads takes columns of rows of all tensors along the path: entry path[d] goes to d. path[d] >= d and both
+// ascend, so that an entry which is written has been read before, by the same thread, and none is read after it was written.
+//
+// The path: each token asks whether it is its parent's pick, all at once, and a parent keeps the first child that is (a minimum of whole numbers: in any order the same); the walk
+// from the root is then one shared read a step. (A warp that looked for each step's child among the tokens waited for memory at every step: 12.2 us for one tree of 25 tokens, 41.7 us
+// for 64 trees of 48.) What is left of a small call is the latency of three dependent loads, the walk and one round of moves.
 template <typename V>
-__global__ void __launch_bounds__(ACCEPT_THREADS) accept_tree_kernel(const __grid_constant__ Tensors pages, const AcceptParams p) {
+__global__ void __launch_bounds__(ACCEPT_THREADS, ACCEPT_BLOCKS) accept_tree_kernel(const __grid_constant__ Tensors pages, const AcceptParams p) {
   pdl_launch_dependents();
   __shared__ int s_count;
-  extern __shared__ int s_path[];                          // [width]
-  const int seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  __shared__ Move s_move[ACCEPT_THREADS];
+  extern __shared__ int s_path[];                          // [width]: first each token's accepted child, then the path
+  const int seq = blockIdx.y, tid = threadIdx.x;
   pdl_wait();
   const int q0 = p.cu_q ? p.cu_q[seq] : seq * p.uniform_q, q1 = p.cu_q ? p.cu_q[seq + 1] : q0 + p.uniform_q;
-  const int n = q0 < 0 ? 0 : min(min(q1, p.total) - q0, p.uniform_q), len = max(min(p.kv_lens[seq], p.max_blocks * p.bs), 0), base = len - (q1 - q0);
-  if (tid < 32) {
-    int count = 0, node = 0;
-    while (count < p.width && node < n) {
-      if (lane == 0) s_path[count] = node;
-      ++count;
-      const long long pick = p.picks[q0 + node];
-      int found = n;
-      for (int i0 = node + 1; i0 < n; i0 += 32) {
-        const int i = i0 + lane;
-        const unsigned hit = __ballot_sync(0xffffffffu, i < n && p.parents[q0 + i] == node && p.tokens[q0 + i] == pick);
-        if (hit) {
-          found = i0 + __ffs(hit) - 1;
-          break;
-        }
-      }
-      node = found;
+  const int n = q0 < 0 ? 0 : min(min(min(q1, p.total) - q0, p.uniform_q), p.width), len = max(min(p.kv_lens[seq], p.max_blocks * p.bs), 0), base = len - (q1 - q0);
+  for (int i = tid; i < n; i += ACCEPT_THREADS) s_path[i] = n;
+  __syncthreads();
+  for (int i = 1 + tid; i < n; i += ACCEPT_THREADS) {
+    const int up = p.parents[q0 + i];
+    const long long token = p.tokens[q0 + i];
+    if (up >= 0 && up < i && p.picks[q0 + up] == token) atomicMin(s_path + up, i);
+  }
+  __syncthreads();
+  if (tid == 0) {
+    int count = 0;
+    for (int node = 0; node < n;) {                        // nodes ascend: count <= node, and what stands below node is not read again
+      const int next = s_path[node];
+      s_path[count++] = node;
+      node = next;
     }
-    if (lane == 0) s_count = count;
+    s_count = count;
   }
   __syncthreads();
   const int count = s_count;
@@ -111,34 +120,38 @@ __global__ void __launch_bounds__(ACCEPT_THREADS) accept_tree_kernel(const __gri
       p.lens[seq] = max(base + count, 0);
     }
   }
-  for (int u = blockIdx.x * ACCEPT_THREADS + tid; u < p.units; u += gridDim.x * ACCEPT_THREADS) {
-    int at = u, t = 0, cols = 0;
-    long long row_bytes = 0;
-    for (; t < pages.n; ++t) {
-      row_bytes = pages.page_bytes[t] / (pages.heads[t] * p.bs);
-      cols = (int)(row_bytes / sizeof(V));
-      if (at < cols * pages.heads[t]) break;
-      at -= cols * pages.heads[t];
+  const int* table = p.table + seq * p.table_stride;
+  for (int first = 1; first < count; first += ACCEPT_THREADS) {
+    const int d = first + tid;
+    Move mine = {0, 0, -1, 0};
+    if (d < count && s_path[d] != d && base + d >= 0) {
+      const int from = base + s_path[d], to = base + d, block = table[from / p.bs], there = table[to / p.bs];
+      if ((unsigned)block < (unsigned)p.num_blocks && (unsigned)there < (unsigned)p.num_blocks) mine = {block, from % p.bs, there, to % p.bs};
     }
-    const int head = at / cols, col = at % cols;
-    char* mine = pages.base[t] + (long long)head * p.bs * row_bytes + (long long)col * sizeof(V);
-    const int* table = p.table + seq * p.table_stride;
-    for (int d0 = 1; d0 < count; d0 += MOVES) {
-      V x[MOVES];
-      char* to[MOVES];
-#pragma unroll
-      for (int i = 0; i < MOVES; ++i) {
-        const int d = d0 + i;
-        to[i] = nullptr;
-        if (d >= count || s_path[d] == d || base + d < 0) continue;
-        const int from = base + s_path[d], block = table[from / p.bs], there = table[(base + d) / p.bs];
-        if ((unsigned)block >= (unsigned)p.num_blocks || (unsigned)there >= (unsigned)p.num_blocks) continue;
-        x[i] = *reinterpret_cast<const V*>(mine + block * pages.page_bytes[t] + from % p.bs * row_bytes);
-        to[i] = mine + there * pages.page_bytes[t] + (base + d) % p.bs * row_bytes;
+    __syncthreads();                                       // the moves before these have been read
+    s_move[tid] = mine;
+    __syncthreads();
+    const int moves = min(count - first, ACCEPT_THREADS);
+    for (int u = blockIdx.x * ACCEPT_THREADS + tid; u < p.units; u += gridDim.x * ACCEPT_THREADS) {
+      int lo = 0, hi = pages.n;                            // the tensor whose columns u is among
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pages.start[mid] <= u) lo = mid; else hi = mid;
       }
+      const int cols = pages.cols[lo], at = u - pages.start[lo], head = at / cols;
+      const long long row_bytes = (long long)cols * sizeof(V), page_bytes = pages.page_bytes[lo];
+      char* column = pages.base[lo] + head * p.bs * row_bytes + (at - head * cols) * (long long)sizeof(V);
+      for (int d0 = 0; d0 < moves; d0 += MOVES) {
+        V x[MOVES];
 #pragma unroll
-      for (int i = 0; i < MOVES; ++i)
-        if (to[i]) *reinterpret_cast<V*>(to[i]) = x[i];
+        for (int i = 0; i < MOVES; ++i)
+          if (d0 + i < moves && s_move[d0 + i].to_page >= 0)
+            x[i] = *reinterpret_cast<const V*>(column + s_move[d0 + i].from_page * page_bytes + s_move[d0 + i].from_row * row_bytes);
+#pragma unroll
+        for (int i = 0; i < MOVES; ++i)
+          if (d0 + i < moves && s_move[d0 + i].to_page >= 0)
+            *reinterpret_cast<V*>(column + s_move[d0 + i].to_page * page_bytes + s_move[d0 + i].to_row * row_bytes) = x[i];
+      }
     }
   }
 }
@@ -172,20 +185,22 @@ __global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const __grid_c
   }
 }
 
-// Tensors first .. first + MAX_TENSORS - 1 of the list; the widest access that all their rows start on.
+// Tensors first .. first + MAX_TENSORS - 1 of the list; the widest access that all their rows start on. step > 0: tensor i is like the first one and begins i * step behind it.
 struct TensorList {
   const long long* base;
   const long long* page_bytes;
   const int* heads;
   int n;
+  long long step;
 };
 Tensors part_of(const TensorList& list, int first) {
   Tensors t;
   t.n = list.n - first < MAX_TENSORS ? list.n - first : MAX_TENSORS;
   for (int i = 0; i < t.n; ++i) {
-    t.base[i] = reinterpret_cast<char*>(list.base[first + i]);
-    t.page_bytes[i] = list.page_bytes[first + i];
-    t.heads[i] = list.heads ? list.heads[first + i] : 1;
+    const int at = list.step > 0 ? 0 : first + i;
+    t.base[i] = reinterpret_cast<char*>(list.base[at]) + (list.step > 0 ? (first + i) * list.step : 0);
+    t.page_bytes[i] = list.page_bytes[at];
+    t.heads[i] = list.heads ? list.heads[at] : 1;
   }
   return t;
 }
@@ -196,13 +211,18 @@ int access_bytes(const Tensors& t, int rows_of_page) {
 }
 
 template <typename V>
-int launch_accept(const Tensors& t, AcceptParams p, cudaStream_t s) {
+int launch_accept(Tensors& t, AcceptParams p, cudaStream_t s) {
   long long units = 0;
-  for (int i = 0; i < t.n; ++i) units += t.page_bytes[i] / p.bs / (long long)sizeof(V);
-  if (units > INT_MAX) return -3;
+  for (int i = 0; i < t.n; ++i) {
+    const long long cols = t.page_bytes[i] / t.heads[i] / p.bs / (long long)sizeof(V);
+    if (units + cols * t.heads[i] > INT_MAX / 2) return -3;
+    t.start[i] = (int)units, t.cols[i] = (int)cols;
+    units += cols * t.heads[i];
+  }
   p.units = (int)units;
-  const long long want = (units + ACCEPT_THREADS - 1) / ACCEPT_THREADS;
-  const unsigned blocks = (unsigned)(want < 1 ? 1 : want > 65535 ? 65535 : want);
+  // as many columns to a thread as it takes for all blocks to be on the SMs at once: each of them finds the path by itself
+  const long long most = (units + ACCEPT_THREADS - 1) / ACCEPT_THREADS, each = (most * p.num_seqs + device_sm_count() * ACCEPT_BLOCKS - 1) / (device_sm_count() * ACCEPT_BLOCKS);
+  const unsigned blocks = (unsigned)(units ? (most + each - 1) / each : 1);
   return launch_kernel(accept_tree_kernel<V>, dim3(blocks, p.num_seqs), dim3(ACCEPT_THREADS), (size_t)p.width * 4, s, t, p);
 }
 
@@ -231,8 +251,8 @@ int swb_plan_tree(const int* parents, const int* cu_q, int num_seqs, int uniform
 }
 
 // dims: host int[8] = num_seqs, tokens of each sequence (with cu_q: at most), tokens, table width, blocks, block_size, width of path, tensors. base, page_bytes, heads: host lists
-// of the tensors [blocks, heads, block_size, row].
-int swb_accept_tree(const int* dims, const void* picks, const void* tokens, const int* parents, const long long* base, const long long* page_bytes, const int* heads, const int* table,
+// of the tensors [blocks, heads, block_size, row]; with step > 0 lists of one, all tensors are alike and begin step bytes apart.
+int swb_accept_tree(const int* dims, const void* picks, const void* tokens, const int* parents, const long long* base, const long long* page_bytes, const int* heads, long long step, const int* table,
                     long long table_stride, const int* cu_q, const int* kv_lens, int* path, int* counts, void* next, int* lens, void* stream) {
   using namespace swb;
   AcceptParams p = {};
@@ -244,12 +264,12 @@ int swb_accept_tree(const int* dims, const void* picks, const void* tokens, cons
     return -3;
   p.picks = reinterpret_cast<const long long*>(picks), p.tokens = reinterpret_cast<const long long*>(tokens), p.parents = parents, p.cu_q = cu_q, p.kv_lens = kv_lens, p.table = table;
   p.table_stride = table_stride, p.path = path, p.counts = counts, p.next = reinterpret_cast<long long*>(next), p.lens = lens;
-  for (int i = 0; i < n; ++i)
+  for (int i = 0; i < (step > 0 && n > 1 ? 1 : n); ++i)
     if (heads[i] < 1 || page_bytes[i] < 1 || page_bytes[i] % ((long long)heads[i] * p.bs)) return -3;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int first = 0;
   do {
-    const Tensors t = part_of({base, page_bytes, heads, n}, first);
+    Tensors t = part_of({base, page_bytes, heads, n, step}, first);
     int rc;
     switch (access_bytes(t, p.bs)) {
       case 16: rc = launch_accept<uint4>(t, p, s); break;
@@ -264,16 +284,16 @@ int swb_accept_tree(const int* dims, const void* picks, const void* tokens, cons
   return 0;
 }
 
-// src and dst: n pairs, on the device or (on_host) lists of the host. Pairs whose numbers are not pages of the tensors are passed over.
-int swb_copy_pages(const long long* base, const long long* page_bytes, int tensors, int num_blocks, const int* src, const int* dst, int n, int on_host, void* stream) {
+// base, page_bytes and step as above. src and dst: n pairs, on the device or (on_host) lists of the host. Pairs whose numbers are not pages of the tensors are passed over.
+int swb_copy_pages(const long long* base, const long long* page_bytes, long long step, int tensors, int num_blocks, const int* src, const int* dst, int n, int on_host, void* stream) {
   using namespace swb;
   if (n <= 0 || tensors <= 0) return 0;
   if (!base || !page_bytes || !src || !dst || num_blocks < 1 || n > INT_MAX / 64) return -3;
-  for (int i = 0; i < tensors; ++i)
+  for (int i = 0; i < (step > 0 ? 1 : tensors); ++i)
     if (page_bytes[i] < 1) return -3;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   for (int first = 0; first < tensors; first += MAX_TENSORS) {
-    const Tensors t = part_of({base, page_bytes, nullptr, tensors}, first);
+    const Tensors t = part_of({base, page_bytes, nullptr, tensors, step}, first);
     const int access = access_bytes(t, 1);
     for (int at = 0; at < n;) {
       Pairs pairs;

@@ -25,6 +25,7 @@ from .runtime import check, ptr
 MAX_SPLITS, MAX_PATH = 64, 8192
 MAX_BEAMS, MAX_COUNT = 256, 128
 
+_ONE = struct.Struct("q").pack
 _DIMS = {n: struct.Struct(f"{n}i").pack for n in (8, 16)}
 _STRIDES = struct.Struct("8q").pack
 
@@ -102,19 +103,24 @@ def tree_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, 
     return out
 
 
-def _tensors(pages) -> tuple[list[int], list[int], list[tuple], int, list]:
-    """Bases, bytes of a page, shapes of a page, number of pages, and the tensors themselves."""
+def _longs(numbers: list[int]) -> bytes:
+    return _ONE(numbers[0]) if len(numbers) == 1 else struct.pack(f"{len(numbers)}q", *numbers)
+
+
+def _tensors(pages) -> tuple[list[int], list[int], list[tuple], int, int, int, list]:
+    """Bases, bytes of a page and shapes of a page, the number of tensors and the bytes between them (0: the lists tell each; else they tell the first), the number of pages, and what
+    holds them."""
     if isinstance(pages, torch.Tensor):
         _require(pages.dim() == 6 and pages.is_contiguous(), "a pool's pages are one contiguous tensor [layers, 2, blocks, kv heads, block_size, width]")
         shape, n = pages.shape, pages.shape[0] * pages.shape[1]
         page = math.prod(shape[3:]) * pages.element_size()
         step = shape[2] * page
-        base = pages.data_ptr()
-        return list(range(base, base + n * step, step)) if step else [], [page] * n, [tuple(shape[3:])] * n, shape[2], [pages]
+        return [pages.data_ptr()], [page], [tuple(shape[3:])], n if step else 0, step, shape[2], [pages]
     pages = list(pages)
     _require(all(t.dim() >= 2 and t.is_contiguous() for t in pages) and len({t.shape[0] for t in pages}) <= 1, "pages are contiguous tensors [blocks, ...] of one number of blocks")
     live = [t for t in pages if t.numel()]
-    return ([t.data_ptr() for t in live], [t[0].numel() * t.element_size() for t in live], [tuple(t.shape[1:]) for t in live], pages[0].shape[0] if pages else 0, pages)
+    blocks = pages[0].shape[0] if pages else 0
+    return [t.data_ptr() for t in live], [t.numel() // blocks * t.element_size() for t in live], [tuple(t.shape[1:]) for t in live], len(live), 0, blocks, pages
 
 
 @dataclass
@@ -135,7 +141,7 @@ def accept_tree(picks: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
     tokens int64 [T] and parents int32 [T] as in `plan_tree`: the tree. The first new token is its root and always accepted (it was certain before); then, as long as there is one, the
     first child whose token is its parent's pick. Entries behind the path keep what they held; pages of a tree are its sequence's own. pages: a pool's tensor or a list of
     tensors [blocks, heads, block_size, width], [blocks, block_size, width] or [blocks, block_size]; an empty list moves nothing."""
-    bases, sizes, shapes, blocks, held = _tensors(pages)
+    bases, sizes, shapes, count, step, blocks, held = _tensors(pages)
     stream = _place(picks, tokens, parents, block_table, kv_lens, cu_q, *held)
     _require(picks.dim() == 1 and picks.dtype == tokens.dtype == torch.int64 and parents.dtype == torch.int32 and picks.shape == tokens.shape == parents.shape
              and picks.is_contiguous() and tokens.is_contiguous() and parents.is_contiguous(), "picks and tokens are int64 [T], parents int32 [T]")
@@ -144,14 +150,13 @@ def accept_tree(picks: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor
     _require(max_q_len <= MAX_PATH, f"trees of up to {MAX_PATH} tokens")
     heads = [s[0] if len(s) == 3 else 1 for s in shapes]
     rows = {s[-1] if len(s) == 1 else s[-2] for s in shapes}
-    _require(all(1 <= len(s) <= 3 for s in shapes) and len(rows) <= 1, "pages are [blocks, heads, block_size, width], [blocks, block_size, width] or [blocks, block_size], of one block_size")
-    _require(len({t.data_ptr() for t in held}) == len(held), "the same tensor twice")
+    _require(max(map(len, shapes), default=1) <= 3 and len(rows) <= 1, "pages are [blocks, heads, block_size, width], [blocks, block_size, width] or [blocks, block_size], of one block_size")
+    _require(len(set(bases)) == len(bases), "the same tensor twice")
     bs = rows.pop() if rows else 1
-    got = Acceptance(picks.new_empty((n, max_q_len), dtype=torch.int32), kv_lens.new_empty(n), picks.new_empty(n), kv_lens.new_empty(n))
-    count = len(bases)
+    got = Acceptance(kv_lens.new_empty((n, max_q_len)), torch.empty_like(kv_lens), picks.new_empty(n), torch.empty_like(kv_lens))
     dims = _DIMS[8](n, max_q_len, T, per, max(blocks, 1), bs, max_q_len, count)
-    check(kernels().swb_accept_tree(dims, picks.data_ptr(), tokens.data_ptr(), parents.data_ptr(), struct.pack(f"{count}q", *bases), struct.pack(f"{count}q", *sizes),
-                                    struct.pack(f"{count}i", *heads), block_table.data_ptr(), block_table.stride(0), ptr(cu_q), kv_lens.data_ptr(), got.path.data_ptr(),
+    check(kernels().swb_accept_tree(dims, picks.data_ptr(), tokens.data_ptr(), parents.data_ptr(), _longs(bases), _longs(sizes),
+                                    struct.pack(f"{len(bases)}i", *heads), step, block_table.data_ptr(), block_table.stride(0), ptr(cu_q), kv_lens.data_ptr(), got.path.data_ptr(),
                                     got.counts.data_ptr(), got.next_tokens.data_ptr(), got.kv_lens.data_ptr(), stream), "swb_accept_tree")
     return got
 
@@ -160,7 +165,7 @@ def copy_pages(pages, src, dst) -> None:
     """Page dst[i] of every tensor becomes a copy of its page src[i]. pages as in `accept_tree`, of any types and page shapes. src and dst: lists of whole numbers, or int32 tensors on the
     device, whose pairs are passed over where one of the two is no page. A page may be copied to several, but is written once and not copied from where it is: lists are
     checked for that, tensors are the caller's word."""
-    bases, sizes, _, blocks, held = _tensors(pages)
+    bases, sizes, _, count, step, blocks, held = _tensors(pages)
     on_device = isinstance(src, torch.Tensor)
     _require(on_device == isinstance(dst, torch.Tensor), "src and dst are both lists or both tensors")
     stream = _place(*held, *((src, dst) if on_device else ()))
@@ -174,10 +179,9 @@ def copy_pages(pages, src, dst) -> None:
         _require(min(min(src), min(dst)) >= 0 and max(max(src), max(dst)) < blocks, f"pages are 0 to {blocks - 1}")
         _require(len(to) == n and to.isdisjoint(src), "a page is written once, and none that is copied")
         a, b = struct.pack(f"{n}i", *src), struct.pack(f"{n}i", *dst)
-    if n == 0 or not bases:
+    if n == 0 or count == 0:
         return
-    count = len(bases)
-    check(kernels().swb_copy_pages(struct.pack(f"{count}q", *bases), struct.pack(f"{count}q", *sizes), count, blocks, a, b, n, 0 if on_device else 1, stream), "swb_copy_pages")
+    check(kernels().swb_copy_pages(_longs(bases), _longs(sizes), step, count, blocks, a, b, n, 0 if on_device else 1, stream), "swb_copy_pages")
 
 
 @dataclass

@@ -286,7 +286,7 @@ def test_a_whole_step_captured_into_one_graph():
 
     def run():
         plan = ops.plan_tree(parents, cu_q=cu, max_q_len=q_len)
-        a = ops.tree_attention(q, pool[0, 0], pool[0, 1], table, kv_lens, plan.mask, cu_q=cu, max_q_len=q_len)
+        a = ops.tree_attention(q, pool[0, 0], pool[0, 1], table, kv_lens, plan.mask, cu_q=cu, max_q_len=q_len, scale=0.125)
         logits = a.reshape(n * q_len, -1).float() @ head
         picks = ops.argmax(logits) % 3
         acc = ops.accept_tree(picks, tokens, parents, pool, table, kv_lens, cu_q=cu, max_q_len=q_len)
