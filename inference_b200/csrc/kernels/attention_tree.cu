@@ -67,18 +67,44 @@ __device__ __forceinline__ void store_out(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store_out(bf16* p, float x) { *p = __float2bfloat16(x); }
 
 // ---- any types and widths: 32-bit arithmetic on ordinary cores --------------------------------------------------------------------------------------
-constexpr int PR = 32, PK = 32, PLAIN_THREADS = 128;          // rows and keys of a tile
+// 32 x 32 tiles: two trees of 21 tokens x 16 heads behind 900 keys are 24 problems of 29 tiles.
+constexpr int PR = 32, PK = 32, PLAIN_THREADS = 128, ROUND = PLAIN_THREADS / PK;          // rows and keys of a tile; tiles whose keys are looked up at once
 
 __device__ __forceinline__ int padded4(int d) { return (d + 3) / 4 * 4; }
 
-// One row of `width` numbers as 32-bit numbers, zeros behind its end: a warp.
-template <typename E, bool VEC>
-__device__ __forceinline__ void fetch_row(float* to, const E* from, int width, int lane) {
-  if constexpr (VEC) {
-    for (int d = lane * 4; d < width; d += 128) *reinterpret_cast<float4*>(to + d) = load_row4(from + d);
-  } else {
-    for (int d = lane; d < padded4(width); d += 32) to[d] = d < width ? to_f(from[d]) : 0.f;
+// N rows of `width` numbers as 32-bit numbers, zeros behind their ends and for those without a place (from[i] null): a warp, with all of a round's loads in flight before the first of them
+// is kept (a row at a time each waited for memory: 24 of 53 us of two trees of 21 tokens x 16 heads behind 900 keys).
+template <typename E, bool VEC, int N>
+__device__ __forceinline__ void fetch_rows(float* to, int ld, const E* const (&from)[N], int width, int lane) {
+  constexpr int W = VEC ? 4 : 1;
+  const int end = VEC ? width : padded4(width);
+  for (int d = lane * W; d < end; d += 32 * W) {
+    float4 x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if constexpr (VEC) {
+        if (from[i]) x[i] = load_row4(from[i] + d);
+      } else {
+        if (from[i] && d < width) x[i].x = to_f(from[i][d]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (VEC) *reinterpret_cast<float4*>(to + i * ld + d) = x[i];
+      else to[i * ld + d] = x[i].x;
+    }
   }
+}
+
+// Word i of a token's row of the mask.
+__device__ __forceinline__ unsigned mask_word(const unsigned* row, int words, int i) { return i < words ? row[i] : 0u; }
+
+// Which of the 32 keys from `rel` places behind the cache's end on (in front of it: rel < 0) a token sees.
+__device__ __forceinline__ unsigned sees32(const unsigned* row, int words, int rel) {
+  if (rel <= -32) return 0xffffffffu;
+  if (rel < 0) return ((1u << -rel) - 1u) | (mask_word(row, words, 0) << -rel);
+  return __funnelshift_r(mask_word(row, words, rel >> 5), mask_word(row, words, (rel >> 5) + 1), rel & 31);
 }
 
 // COLS * 64 >= Dv. VEC: rows of the caches start on four numbers and are a multiple of four long.
@@ -91,9 +117,12 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_tree_plain_kernel(const Tr
   float* sk = sq + PR * ldk;                       // [PK][ldk]
   float* sv = sk + PK * ldk;                       // [PK][ldv]
   float* sp = sv + PK * ldv;                       // [PK][PR + 4]
-  constexpr int LDP = PR + 4;
-  __shared__ long long s_row[PK];                  // first row of the key's page + its place, -1: no such key
-  __shared__ float s_alpha[PR], s_m[PR], s_l[PR];
+  constexpr int LDP = PR + 4, MINE = PR / (PLAIN_THREADS / 32);        // rows, and keys of a tile, of a warp
+  static_assert(PR == 32 && PK == 32);
+  __shared__ long long s_row[ROUND * PK];          // of a round of tiles: first row of the key's page + its place, -1: no such key
+  __shared__ __align__(8) float s_alpha[PR];
+  __shared__ long long s_dst[PR], s_ml[PR];
+  __shared__ float s_m[PR], s_l[PR];               // at the end: a warp has its rows' in registers
   __shared__ unsigned s_seen[PR];                  // keys of the tile that a row sees
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int split = blockIdx.x % p.num_splits, y = blockIdx.x / p.num_splits, h = y % p.Hkv, z = y / p.Hkv, tile = z % p.tiles, seq = z / p.tiles;
@@ -102,25 +131,40 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_tree_plain_kernel(const Tr
   const int r0 = tile * PR, rows = min(PR, min(s.n, p.uniform_q) * p.G - r0);
   if (rows <= 0) return;
   const E* q = reinterpret_cast<const E*>(p.q);
-  for (int r = warp; r < PR; r += PLAIN_THREADS / 32) {
-    const int t = s.q0 + (r0 + r) / p.G, g = (r0 + r) % p.G;
-    const bool live = r < rows && (unsigned)t < (unsigned)p.tokens;
-    const E* from = q + (live ? t * p.q_tok + (long long)(h * p.G + g) * p.q_head : 0);
-    for (int d = lane; d < ldk - 4; d += 32) sq[r * ldk + d] = live && d < p.D ? to_f(from[d]) : 0.f;
+  // lane = row: its token, and where its results go (-1: there is no such row)
+  const int Hq = p.Hkv * p.G, token = s.q0 + (r0 + lane) / p.G, head = h * p.G + (r0 + lane) % p.G;
+  const bool live = lane < rows && (unsigned)token < (unsigned)p.tokens;
+  if (warp == 0) {
+    const long long at = ((long long)split * p.tokens + token) * Hq + head;
+    s_dst[lane] = !live ? -1 : p.part_o ? at * p.Dv : token * p.out_tok + (long long)head * p.Dv;
+    s_ml[lane] = at;
   }
-  if (tid < PR) s_m[tid] = -INFINITY, s_l[tid] = 0.f;
-  float o[COLS][16];                               // rows 16 (tid / 64) .. + 15 of columns tid % 64 + 64 c
+  {
+    const long long mine = live ? token * p.q_tok + head * p.q_head : -1;
+    const E* from[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      const long long at = __shfl_sync(0xffffffffu, mine, warp * MINE + i);
+      from[i] = at >= 0 ? q + at : nullptr;
+    }
+    if (VEC && p.q_vec) fetch_rows<E, VEC>(sq + warp * MINE * ldk, ldk, from, p.D, lane);
+    else fetch_rows<E, false>(sq + warp * MINE * ldk, ldk, from, p.D, lane);
+  }
+  float m[MINE], l[MINE];                          // of rows warp * MINE + i: maximum (log2 units) and sum, the same in all lanes
+#pragma unroll
+  for (int i = 0; i < MINE; ++i) m[i] = -INFINITY, l[i] = 0.f;
+  unsigned long long o[COLS][8];                   // rows 16 (tid / 64) .. + 15, two in a place, of columns tid % 64 + 64 c
 #pragma unroll
   for (int c = 0; c < COLS; ++c)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) o[c][r] = 0.f;
+    for (int r = 0; r < 8; ++r) o[c][r] = 0;
   const int col = tid % 64, half = tid / 64;
   const int kt = (s.len + PK - 1) / PK, per = (kt + p.num_splits - 1) / p.num_splits;
   const int lo = min(split * per, kt), hi = min(kt, lo + per);
   for (int it = lo; it < hi; ++it) {
-    const int j0 = it * PK;
+    const int j0 = it * PK, at = (it - lo) % ROUND * PK;
     __syncthreads();
-    if (tid < PK) {
+    if (at == 0) {                                 // where the keys of the next tiles lie: a thread to a key
       long long row = -1;
       const int j = j0 + tid;
       if (j < s.len) {
@@ -128,100 +172,147 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_tree_plain_kernel(const Tr
         if ((unsigned)block < (unsigned)p.num_blocks) row = ((long long)block * p.Hkv + h) * p.bs + j % p.bs;
       }
       s_row[tid] = row;
-      const unsigned there = __ballot_sync(0xffffffffu, row >= 0);
-      unsigned seen = 0;                           // lane = row
-      const int t = s.q0 + (r0 + tid) / p.G;
-      if (tid < rows && (unsigned)t < (unsigned)p.tokens) {
-        if (j0 + PK <= s.base) {
-          seen = 0xffffffffu;
-        } else {
-          for (int i = 0; i < PK; ++i) seen |= (unsigned)sees(p.mask + t * p.mask_tok, p.words, j0 + i - s.base) << i;
+      __syncthreads();
+    }
+    if (warp == 0) {
+      const unsigned there = __ballot_sync(0xffffffffu, s_row[at + lane] >= 0);
+      s_seen[lane] = live ? sees32(p.mask + token * p.mask_tok, p.words, j0 - s.base) & there : 0u;
+    }
+    {
+      const E *k[MINE], *v[MINE];
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        const long long row = s_row[at + warp * MINE + i];
+        k[i] = row >= 0 ? reinterpret_cast<const E*>(p.k) + row * p.D : nullptr;
+        v[i] = row >= 0 ? reinterpret_cast<const E*>(p.v) + row * p.Dv : nullptr;
+      }
+      fetch_rows<E, VEC>(sk + warp * MINE * ldk, ldk, k, p.D, lane);
+      fetch_rows<E, VEC>(sv + warp * MINE * ldv, ldv, v, p.Dv, lane);
+    }
+    __syncthreads();
+    // where rows differ in what they see: whether all values are numbers (else a product with a weight of zero would be none)
+    bool odd = false;
+    if (j0 + PK > s.base) {
+      for (int i = tid; i < PK * ldv; i += PLAIN_THREADS) odd |= !isfinite(sv[i]);
+      odd = __syncthreads_or(odd);
+    }
+    // scores: a thread has 8 rows of one key, sums of the even and the odd numbers
+    unsigned long long xx[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) xx[i] = 0;
+#pragma unroll 2
+    for (int d = 0; d < ldk - 4; d += 4) {
+      const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(sk + lane * ldk + d);
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(sq + (warp * MINE + i) * ldk + d);
+        xx[i] = fma2(a.y, k.y, fma2(a.x, k.x, xx[i]));
+      }
+    }
+    float x[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      float even, other;
+      unpack2(xx[i], even, other);
+      x[i] = even + other;
+    }
+    float top[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      x[i] = s_seen[warp * MINE + i] >> lane & 1u ? score_transform(x[i], p.scale, p.softcap) : -INFINITY;
+      top[i] = x[i];
+    }
+#pragma unroll
+    for (int step = 16; step; step >>= 1) {        // the rows' reductions side by side
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], step));
+    }
+    float sum[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      const int r = warp * MINE + i;
+      const float m1 = fmaxf(m[i], top[i]), base = m1 == -INFINITY ? 0.f : m1, alpha = exp2f(m[i] - base);
+      sum[i] = exp2f(x[i] - base);
+      sp[lane * LDP + r] = s_seen[r] >> lane & 1u ? sum[i] : 0.f;
+      if (lane == 0) s_alpha[r] = alpha;
+      l[i] *= alpha, m[i] = m1;
+    }
+#pragma unroll
+    for (int step = 16; step; step >>= 1) {
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], step);
+    }
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) l[i] += sum[i];
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const unsigned long long alpha = *reinterpret_cast<const unsigned long long*>(s_alpha + half * 16 + 2 * r);
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) o[c][r] = fma2(o[c][r], alpha, 0ull);
+    }
+    if (!odd) {
+#pragma unroll 4
+      for (int key = 0; key < PK; ++key) {
+        unsigned long long w[8];
+#pragma unroll
+        for (int r = 0; r < 8; r += 2) {
+          const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(sp + key * LDP + half * 16 + 2 * r);
+          w[r] = two.x, w[r + 1] = two.y;
+        }
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+          const int d = c * 64 + col;
+          const float val = d < p.Dv ? sv[key * ldv + d] : 0.f;
+          const unsigned long long both = pack2(val, val);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) o[c][r] = fma2(w[r], both, o[c][r]);
         }
       }
-      s_seen[tid] = seen & there;
-    }
-    __syncthreads();
-    for (int i = warp; i < PK; i += PLAIN_THREADS / 32) {
-      const long long row = s_row[i];
-      if (row >= 0) {
-        fetch_row<E, VEC>(sk + i * ldk, reinterpret_cast<const E*>(p.k) + row * p.D, p.D, lane);
-        fetch_row<E, VEC>(sv + i * ldv, reinterpret_cast<const E*>(p.v) + row * p.Dv, p.Dv, lane);
-      } else {
-        for (int d = lane; d < ldk; d += 32) sk[i * ldk + d] = 0.f;
-        for (int d = lane; d < ldv; d += 32) sv[i * ldv + d] = 0.f;
-      }
-    }
-    __syncthreads();
-    // scores: a thread has 8 rows of one key
-    float x[8];
+    } else {
+#pragma unroll 1
+      for (int key = 0; key < PK; ++key) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    for (int d = 0; d < ldk - 4; d += 4) {
-      const float4 k = *reinterpret_cast<const float4*>(sk + lane * ldk + d);
+        for (int c = 0; c < COLS; ++c) {
+          const int d = c * 64 + col;
+          const float val = d < p.Dv ? sv[key * ldv + d] : 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float4 a = *reinterpret_cast<const float4*>(sq + (warp * 8 + i) * ldk + d);
-        x[i] = fmaf(a.x, k.x, x[i]), x[i] = fmaf(a.y, k.y, x[i]), x[i] = fmaf(a.z, k.z, x[i]), x[i] = fmaf(a.w, k.w, x[i]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = warp * 8 + i;
-      const bool live = s_seen[r] >> lane & 1u;
-      const float sc = live ? score_transform(x[i], p.scale, p.softcap) : -INFINITY;
-      const float m0 = s_m[r], m1 = fmaxf(m0, warp_max(sc)), base = m1 == -INFINITY ? 0.f : m1;
-      const float e = exp2f(sc - base), sum = warp_sum(e);
-      sp[lane * LDP + r] = live ? e : 0.f;
-      __syncwarp();                                // s_m is read by all lanes before lane 0 writes it
-      if (lane == 0) {
-        const float alpha = exp2f(m0 - base);
-        s_alpha[r] = alpha, s_m[r] = m1, s_l[r] = s_l[r] * alpha + sum;
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float alpha = s_alpha[half * 16 + r];
-#pragma unroll
-      for (int c = 0; c < COLS; ++c) o[c][r] *= alpha;
-    }
-    const bool whole = j0 + PK <= s.base;          // all rows see all keys, or none does (then its value is a zero)
-    for (int key = 0; key < PK; ++key) {
-      float w[16];
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) *reinterpret_cast<float4*>(w + r) = *reinterpret_cast<const float4*>(sp + key * LDP + half * 16 + r);
-#pragma unroll
-      for (int c = 0; c < COLS; ++c) {
-        const int d = c * 64 + col;
-        const float val = d < p.Dv ? sv[key * ldv + d] : 0.f;
-        if (whole || isfinite(val)) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[c][r] = fmaf(w[r], val, o[c][r]);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (s_seen[half * 16 + r] >> key & 1u) o[c][r] = fmaf(w[r], val, o[c][r]);
+          for (int r = 0; r < 8; ++r) {
+            const int row = half * 16 + 2 * r;
+            float lower, upper;
+            unpack2(o[c][r], lower, upper);
+            if (s_seen[row] >> key & 1u) lower = fmaf(sp[key * LDP + row], val, lower);
+            if (s_seen[row + 1] >> key & 1u) upper = fmaf(sp[key * LDP + row + 1], val, upper);
+            o[c][r] = pack2(lower, upper);
+          }
         }
       }
     }
   }
+  // one row after another in little code: what a block runs once, it waits for from the instruction memory (all 16 rows unrolled, with their divisions: 10 us for a step without keys)
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) s_m[warp * MINE + i] = m[i], s_l[warp * MINE + i] = p.part_o ? l[i] : l[i] == 0.f ? 0.f : 1.f / l[i];
+  }
   __syncthreads();
-  const int Hq = p.Hkv * p.G;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const int row = half * 16 + r, t = s.q0 + (r0 + row) / p.G, head = h * p.G + (r0 + row) % p.G;
-    if (row >= rows || (unsigned)t >= (unsigned)p.tokens) continue;
-    const float l = s_l[row];
-    const long long at = ((long long)split * p.tokens + t) * Hq + head;
+    const int row = half * 16 + r;
+    const long long at = s_dst[row];
+    if (at < 0) continue;
+    const float factor = p.part_o ? 1.f : s_l[row];
 #pragma unroll
     for (int c = 0; c < COLS; ++c) {
       const int d = c * 64 + col;
+      float even, other;
+      unpack2(o[c][r / 2], even, other);
+      const float sum = (r % 2 ? other : even) * factor;
       if (d >= p.Dv) continue;
-      if (p.part_o) p.part_o[at * p.Dv + d] = o[c][r];
-      else store_out(reinterpret_cast<E*>(p.out) + t * p.out_tok + (long long)head * p.Dv + d, l == 0.f ? 0.f : o[c][r] / l);
+      if (p.part_o) p.part_o[at + d] = sum;
+      else store_out(reinterpret_cast<E*>(p.out) + at + d, sum);
     }
-    if (p.part_o && col == 0) p.part_ml[at] = make_float2(s_m[row], l);
   }
+  if (p.part_o && tid < PR && s_dst[tid] >= 0) p.part_ml[s_ml[tid]] = make_float2(s_m[tid], s_l[tid]);
 }
 
 // ---- bf16, widths up to 128, pages of 16-key groups: products on the tensor memory's matrix instructions -----------------------------------------------------
