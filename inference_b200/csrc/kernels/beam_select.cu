@@ -54,7 +54,7 @@ struct BeamParams {
 __device__ __forceinline__ bool alive(float score) { return isfinite(score); }
 
 __device__ __forceinline__ unsigned order_of(float x) {
-  const unsigned u = __float_as_uint(x);
+  const unsigned u = __float_as_uint(x + 0.f);             // zeros of both signs are one number
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 

@@ -564,3 +564,43 @@ def test_results_repeat():
     for _ in range(5):
         again = _ops().beam_select(logits, scores, count=30)
         assert torch.equal(again.scores, best.scores) and torch.equal(again.tokens, best.tokens)
+
+
+@pytest.mark.parametrize("n", [257, 700])
+def test_long_paths_shift_in_place(n):
+    """Every entry of the path moves one place to the front, onto what has been read before."""
+    cu = torch.tensor([0, n], dtype=torch.int32, device=CUDA)
+    parents = torch.tensor([-1, 0, 0] + list(range(2, n - 1)), dtype=torch.int32, device=CUDA)
+    tokens = torch.arange(n, device=CUDA)
+    picks = torch.tensor([2, -7] + list(range(3, n + 1)), device=CUDA)
+    base, bs = 13, 16
+    per = -(-(base + n) // bs)
+    table = torch.randperm(per + 3, generator=torch.Generator().manual_seed(n))[:per].to(torch.int32)[None].to(CUDA)
+    pool = torch.randn(60, 2, per + 3, 2, bs, 8, device=CUDA, generator=_gen(n))          # more tensors than a launch takes
+    before = pool.clone()
+    got = _ops().accept_tree(picks, tokens, parents, pool, table, torch.tensor([base + n], dtype=torch.int32, device=CUDA), cu_q=cu, max_q_len=n)
+    path = [0] + list(range(2, n))
+    assert got.path[0].tolist() == path + [-1] and int(got.next_tokens[0]) == n and int(got.kv_lens[0]) == base + n - 1
+    where = lambda j: (table[0, torch.tensor(j, device=CUDA) // bs].long(), torch.tensor(j, device=CUDA) % bs)
+    to, fro = where([base + d for d in range(n - 1)]), where([base + i for i in path])
+    want = before.clone()
+    want[:, :, to[0], :, to[1]] = before[:, :, fro[0], :, fro[1]]
+    assert torch.equal(pool, want)
+
+
+def test_copies_in_pools_of_many_layers():
+    pool = torch.randn(60, 2, 9, 3, 4, 5, device=CUDA, generator=_gen(5))
+    want = pool.clone()
+    want[:, :, [7, 2]] = pool[:, :, [1, 1]]
+    _ops().copy_pages(pool, [1, 1], [7, 2])
+    assert torch.equal(pool, want)
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+def test_zeros_of_both_signs_are_equal(kind):
+    """More ties at zero than a block takes notes of: the first tokens, whatever their signs."""
+    V, count = 9001, 11
+    logits = torch.zeros(2, V, dtype=kind, device=CUDA)
+    logits[torch.rand(2, V, device=CUDA, generator=_gen(3)) < 0.5] = -0.0
+    got = _ops().beam_select(logits, torch.zeros(1, 2, device=CUDA), count=count)
+    assert got.beams[0].tolist() == [0] * count and got.tokens[0].tolist() == list(range(count))

@@ -103,6 +103,23 @@ def test_logits_of_trees_and_steps_behind_them(kw):
     assert be.runner.pool.allocator.live_blocks() == 0
 
 
+def test_a_tree_is_a_sequences_first_step():
+    cfg = _cfg()
+    oracle, be = _build(cfg, seed=12)
+    seqs = [be.new_sequence(), be.new_sequence()]
+    be.forward([seqs[1]], [[9, 8]])
+    tokens, ups = [[5, 6, 7, 6], [4, 3]], [[-1, 0, 0, 2], [-1, 0]]
+
+    def choose(logits):
+        for at, front, path in ((0, [], [5]), (1, [], [5, 6]), (2, [], [5, 7]), (3, [], [5, 7, 6]), (4, [9, 8], [4]), (5, [9, 8], [4, 3])):
+            _near(logits[at], _logits(oracle, front + path))
+        return torch.tensor([7, 0, 6, 2, 1, 1], device="cuda")
+
+    assert be.step_trees(seqs, tokens, ups, choose) == [([0, 2, 3], 2), ([0], 1)]
+    for lg, text in zip(be.forward(seqs, [[2], [1]]), ([5, 7, 6, 2], [9, 8, 4, 1])):
+        _near(lg, _logits(oracle, text))
+
+
 def test_tree_lookup_is_greedy():
     from inference_b200.engine.branching import TreeConfig, generate_tree_lookup
     from inference_b200.engine.decode import GenerationConfig
