@@ -67,13 +67,15 @@ __device__ __forceinline__ void store_out(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store_out(bf16* p, float x) { *p = __float2bfloat16(x); }
 
 // ---- any types and widths: 32-bit arithmetic on ordinary cores --------------------------------------------------------------------------------------
-// 32 x 32 tiles: two trees of 21 tokens x 16 heads behind 900 keys are 24 problems of 29 tiles.
+// 32 x 32 tiles, as rows are few: two trees of 21 tokens x 16 heads behind 900 keys are 24 problems of 29 tiles, 34 us with the sum of the splits (53 with a row of keys fetched at a time, single
+// multiply-adds and a long epilogue). A block alone takes 5 to 6 us a tile, three on an SM 10: shared reads (9 for 16 paired multiply-adds of the scores, 6 for 16 of the values) and
+// multiply-adds wait for one another, at a quarter to a half of the issue slots.
 constexpr int PR = 32, PK = 32, PLAIN_THREADS = 128, ROUND = PLAIN_THREADS / PK;          // rows and keys of a tile; tiles whose keys are looked up at once
 
 __device__ __forceinline__ int padded4(int d) { return (d + 3) / 4 * 4; }
 
 // N rows of `width` numbers as 32-bit numbers, zeros behind their ends and for those without a place (from[i] null): a warp, with all of a round's loads in flight before the first of them
-// is kept (a row at a time each waited for memory: 24 of 53 us of two trees of 21 tokens x 16 heads behind 900 keys).
+// is kept (a row at a time each waited for memory: 11 of 53 us of two trees of 21 tokens x 16 heads behind 900 keys).
 template <typename E, bool VEC, int N>
 __device__ __forceinline__ void fetch_rows(float* to, int ld, const E* const (&from)[N], int width, int lane) {
   constexpr int W = VEC ? 4 : 1;
@@ -289,7 +291,7 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_tree_plain_kernel(const Tr
       }
     }
   }
-  // one row after another in little code: what a block runs once, it waits for from the instruction memory (all 16 rows unrolled, with their divisions: 10 us for a step without keys)
+  // one row after another in little code: what a block runs once, it waits for from the instruction memory (all 16 rows unrolled, with their divisions: 10 us for a step without keys, now 5)
   if (lane == 0) {
 #pragma unroll
     for (int i = 0; i < MINE; ++i) s_m[warp * MINE + i] = m[i], s_l[warp * MINE + i] = p.part_o ? l[i] : l[i] == 0.f ? 0.f : 1.f / l[i];
@@ -330,7 +332,8 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_tree_plain_kernel(const Tr
 // 64 tokens x 32 heads (8 key/value heads) behind 100 000 keys, blocks of 256 rows and 44 tiles: 125 us with the sum of the splits, 0.84 PFLOP/s; 95 of them without any softmax. (One slot a block and
 // two blocks to an SM, each tile asked for when the one before it was used: 155.) What a slot waits for are its products, 2 x 8 of 64 cycles, beside those of the other, and its softmax, of which the
 // exponentials are 17 us. What did not help: tiles of 64 keys with two of scores a slot (their products take no less for being half as wide), references a tile old in place of a row's own
-// maximum (its steps cost more than the exchange), a quarter of the exponentials on the multiply-add pipes.
+// maximum (its steps cost more than the exchange), a quarter of the exponentials on the multiply-add pipes, Q in tensor memory beside tiles of 64 keys, so that products read half as much
+// shared memory (152: the softmax's steps come twice as often), P handed over in two halves (147: one more wait for the stores and one more signal a tile).
 constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_THREADS = 640, TMA_WARP = 16, MMA_WARP = 17, K_STAGES = 3, V_STAGES = 3, SOFT_REGS = 112, ROLE_REGS = 32;
 constexpr uint32_t TC_COLS = 512;
 constexpr float TC_RESCALE = 8.f;          // O is rescaled when a maximum has grown by more than 2^8

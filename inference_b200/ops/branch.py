@@ -61,9 +61,16 @@ def _check_ranges(cu_q: torch.Tensor | None, max_q_len: int, tokens: int) -> int
 
 
 def tree_splits(problems: int, keys: int, tensor_cores: bool = True, sms: int = 148) -> int:
-    """Blocks that share the keys of a tile of rows: as many as the SMs hold at once (one to an SM of the kernel on tensor memory, four of the plain one), of a tile of keys and more."""
-    slots, tile = (sms, 128) if tensor_cores else (4 * sms, 64)
-    return max(1, min(MAX_SPLITS, (keys + tile - 1) // tile, slots // max(1, problems)))
+    """Blocks that share the keys of a tile of rows, of a tile of keys and more each.
+
+    On tensor memory no more than all SMs hold at once, one each: beyond that a block's start and the sum of the parts cost more than the last wave's idle SMs (30 tokens x 32 heads, 4100 keys, us:
+    4 sequences 33.0, 30.0 and 39.2 with 3, 4 and 6 splits, 8 sequences 58.2, 42.7 and 53.7 with 1, 2 and 3; 24 sequences of 48 tokens 109, 122 and 138). The plain kernel waits for its own
+    steps and wants several blocks an SM and waves that blend: eight blocks an SM in all (16 heads, us: 8 x 20 tokens, 900 keys 125, 78, 68 and 69 with 2, 4, 6 and 12; 16 x 30 tokens, 2000 keys 589,
+    360, 317 and 305 with 1, 2, 4 and 8; 40 x 30 tokens, 900 keys 441, 366 and 337 with 1, 2 and 4; 60 tokens, 20 000 keys 575, 739 and 637 with 12, 18 and 32)."""
+    problems = max(1, problems)
+    if tensor_cores:
+        return max(1, min(MAX_SPLITS, (keys + 127) // 128, sms // problems))
+    return max(1, min(MAX_SPLITS, (keys + 63) // 64, -(-8 * sms // problems)))
 
 
 def tree_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, mask: torch.Tensor, *,
