@@ -56,7 +56,7 @@ def generate_beam(backend: DecodeBackend, prompt: list[int], cfg: GenerationConf
     K, stops = beam.beams, set(cfg.stop_tokens)
     if not 1 <= K <= MAX_BEAMS:
         raise Unsupported(f"1 to {MAX_BEAMS} beams")
-    # as many as there may be texts that end, and K that do not
+    # as many as there may be texts that end, and K that do not (many beams with many stop tokens: as many as there is room for, so that fewer may go on)
     count = min(MAX_CONTINUATIONS, K * (1 + len(stops)))
     done: list[BeamResult] = []
     seqs, texts, scores, why = [backend.new_sequence()], [[]], [0.0], FinishReason.LENGTH
