@@ -329,11 +329,12 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_tree_plain_kernel(const Tr
 //   warps 0-15   softmax, eight to a slot, two threads to a row with 64 of a tile's keys each; in tiles of the tree they apply the mask and see to it that V holds numbers
 // Tensor memory of a slot: S (128 columns; P in the first half of each thread's own 64), O (128). Shared memory has seven buffers of a tile: Q, three of K, and two of V with Q's second half
 // or three of V.
-// 64 tokens x 32 heads (8 key/value heads) behind 100 000 keys, blocks of 256 rows and 44 tiles: 125 us with the sum of the splits, 0.84 PFLOP/s; 95 of them without any softmax. (One slot a block and
-// two blocks to an SM, each tile asked for when the one before it was used: 155.) What a slot waits for are its products, 2 x 8 of 64 cycles, beside those of the other, and its softmax, of which the
-// exponentials are 17 us. What did not help: tiles of 64 keys with two of scores a slot (their products take no less for being half as wide), references a tile old in place of a row's own
-// maximum (its steps cost more than the exchange), a quarter of the exponentials on the multiply-add pipes, Q in tensor memory beside tiles of 64 keys, so that products read half as much
-// shared memory (152: the softmax's steps come twice as often), P handed over in two halves (147: one more wait for the stores and one more signal a tile).
+// 64 tokens x 32 heads (8 key/value heads) behind 100 000 keys, blocks of 256 rows and 44 tiles: 121 us with the sum of the splits, 0.87 PFLOP/s; some 95 without any softmax. (One slot a block and
+// two blocks to an SM, each tile asked for when the one before it was used: 155.) A tile takes a slot some 3600 cycles: 2000 from its scores to its weights, of them 1190 for the exponentials, which
+// eight warps need 1024 for at least, and 1570 from there to the next scores, of them 1024 for the products; those of both slots together keep the tensor cores busy for 2048. Maxima
+// of three numbers and one vote in place of two were 3 % of it. What did not help: tiles of 64 keys with two of scores a slot, references a tile old in place of a row's own maximum (its steps cost more
+// than the exchange), a quarter of the exponentials on the multiply-add pipes, Q in tensor memory beside tiles of 64 keys (152: the softmax's steps come twice as often), P handed over in two
+// halves (147: one more wait for the stores and one more signal a tile), first tiles, Q and tensor memory asked for beside one another in front of the first barrier (no change).
 constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_THREADS = 640, TMA_WARP = 16, MMA_WARP = 17, K_STAGES = 3, V_STAGES = 3, SOFT_REGS = 112, ROLE_REGS = 32;
 constexpr uint32_t TC_COLS = 512;
 constexpr float TC_RESCALE = 8.f;          // O is rescaled when a maximum has grown by more than 2^8
@@ -397,6 +398,12 @@ __device__ __forceinline__ unsigned long long seen_keys(const unsigned* row, int
   return seen;
 }
 
+
+__device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+  return d;
+}
 
 // A row's columns in tensor memory times f: whole warp.
 template <int COLS>
@@ -496,23 +503,22 @@ __device__ __forceinline__ void tree_softmax(const TreeParams& p, TcBars* bars, 
         for (int e = 0; e < 64; ++e)
           if (!(seen >> e & 1ull)) x[e] = __float_as_uint(-INFINITY);
       }
-      float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+      float m0 = __uint_as_float(x[0]), m1 = __uint_as_float(x[1]), m2 = __uint_as_float(x[2]), m3 = __uint_as_float(x[3]);
 #pragma unroll
-      for (int e = 0; e < 64; e += 4) {
-        m0 = fmaxf(m0, __uint_as_float(x[e])), m1 = fmaxf(m1, __uint_as_float(x[e + 1]));
-        m2 = fmaxf(m2, __uint_as_float(x[e + 2])), m3 = fmaxf(m3, __uint_as_float(x[e + 3]));
-      }
+      for (int e = 4; e + 7 < 64; e += 8)
+        m0 = max3(m0, x[e], x[e + 1]), m1 = max3(m1, x[e + 2], x[e + 3]), m2 = max3(m2, x[e + 4], x[e + 5]), m3 = max3(m3, x[e + 6], x[e + 7]);
+      m0 = max3(m0, x[60], x[61]), m1 = max3(m1, x[62], x[63]);
       mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
     }
     // (Its word of the tile before is read by then: this tile's scores wait for that one's weights.)
     word[half * TC_ROWS] = mx;
     pair_sync(1 + slot * 4 + w4);
     const float theirs = word[(half ^ 1) * TC_ROWS];
-    ok = ok && __all_sync(0xffffffffu, __float_as_int(theirs) != 0x7fffffff);
-    if (!ok) break;                                                         // both halves leave at the same tile
     const float m_new = fmaxf(fmaxf(mx, theirs), m);
-    const bool grow = (m_new - m) * scale_log2 > TC_RESCALE;                // true on the first tile with a key that the row sees (m = -inf)
-    if (__any_sync(0xffffffffu, grow)) {
+    const bool grow = (m_new - m) * scale_log2 > TC_RESCALE, stop = !ok || __float_as_int(theirs) == 0x7fffffff;      // grow on the first tile with a key that the row sees (m = -inf)
+    if (__any_sync(0xffffffffu, grow || stop)) {
+      ok = !__any_sync(0xffffffffu, stop);
+      if (!ok) break;                                                       // both halves leave at the same tile
       const float f = grow ? ex2((m - m_new) * scale_log2) : 1.f;
       if (grow) l *= f, m = m_new;
       if (i > 0) scale_columns<OUT>(t_o, f);                                // the product before this one is done: the scores came behind it
