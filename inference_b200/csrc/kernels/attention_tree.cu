@@ -329,11 +329,11 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_tree_plain_kernel(const Tr
 //   warps 0-15   softmax, eight to a slot, two threads to a row with 64 of a tile's keys each; in tiles of the tree they apply the mask and see to it that V holds numbers
 // Tensor memory of a slot: S (128 columns; P in the first half of each thread's own 64), O (128). Shared memory has seven buffers of a tile: Q, three of K, and two of V with Q's second half
 // or three of V.
-// 64 tokens x 32 heads (8 key/value heads) behind 100 000 keys, blocks of 256 rows and 44 tiles: 121 us with the sum of the splits, 0.87 PFLOP/s; some 95 without any softmax. (One slot a block and
-// two blocks to an SM, each tile asked for when the one before it was used: 155.) A tile takes a slot some 3600 cycles: 2000 from its scores to its weights, of them 1190 for the exponentials, which
-// eight warps need 1024 for at least, and 1570 from there to the next scores, of them 1024 for the products; those of both slots together keep the tensor cores busy for 2048. Maxima
-// of three numbers and one vote in place of two were 3 % of it. What did not help: tiles of 64 keys with two of scores a slot, references a tile old in place of a row's own maximum (its steps cost more
-// than the exchange), a quarter of the exponentials on the multiply-add pipes, Q in tensor memory beside tiles of 64 keys (152: the softmax's steps come twice as often), P handed over in two
+// 64 tokens x 32 heads (8 key/value heads) behind 100 000 keys, blocks of 256 rows and 44 tiles: 116 us with the sum of the splits, 0.91 PFLOP/s; some 95 without any softmax. (One slot a block and
+// two blocks to an SM, each tile asked for when the one before it was used: 155.) A tile takes a slot some 3400 cycles: 1850 from its scores to its weights, of them 1000 for the exponentials, which
+// the special-function units alone would need 1024 for at least (1190 in fact), and 1570 from there to the next scores, of them 1024 for the products; those of both slots together keep the tensor
+// cores busy for 2048. Maxima of three numbers and one vote in place of two were 3 % of it. What did not help: tiles of 64 keys with two of scores a slot, references a tile old in place of a row's own maximum (its steps cost more
+// than the exchange), Q in tensor memory beside tiles of 64 keys (152: the softmax's steps come twice as often), P handed over in two
 // halves (147: one more wait for the stores and one more signal a tile), first tiles, Q and tensor memory asked for beside one another in front of the first barrier (no change).
 constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_THREADS = 640, TMA_WARP = 16, MMA_WARP = 17, K_STAGES = 3, V_STAGES = 3, SOFT_REGS = 112, ROLE_REGS = 32;
 constexpr uint32_t TC_COLS = 512;
@@ -403,6 +403,15 @@ __device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
   return d;
+}
+
+// 2^x on the multiply-add pipes, for x below 100: x = n + f, |f| <= 1/2, the polynomial of `ex2_fma2` in f times 2^n. Below -126.5 it is zero; what is not a number stays so.
+__device__ __forceinline__ float ex2_fma(float x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-127.f));
+  const float t = x + 12582912.f, f = x - (t - 12582912.f);
+  float r = fmaf(f, EXP_5, EXP_4);
+  r = fmaf(r, f, EXP_3), r = fmaf(r, f, EXP_2), r = fmaf(r, f, EXP_1), r = fmaf(r, f, EXP_0);
+  return r * __int_as_float((__float_as_int(t) << 23) + 0x3f800000);
 }
 
 // A row's columns in tensor memory times f: whole warp.
@@ -531,7 +540,7 @@ __device__ __forceinline__ void tree_softmax(const TreeParams& p, TcBars* bars, 
       float v0, v1, v2, v3;
       unpack2(fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), sc2, nm2), v0, v1);
       unpack2(fma2(pack2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])), sc2, nm2), v2, v3);
-      v0 = ex2(v0), v1 = ex2(v1), v2 = ex2(v2), v3 = ex2(v3);
+      v0 = ex2(v0), v1 = ex2(v1), v2 = ex2(v2), v3 = e % 8 == 4 ? ex2_fma(v3) : ex2(v3);        // one in eight beside the special-function unit: 122 us, 115 (one in four 122, in sixteen 117)
       l0 = add2(l0, pack2(v0, v1)), l1 = add2(l1, pack2(v2, v3));
       x[e >> 1] = pack_bf16x2(v0, v1), x[(e >> 1) + 1] = pack_bf16x2(v2, v3);
     }
