@@ -329,12 +329,13 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_tree_plain_kernel(const Tr
 //   warps 0-15   softmax, eight to a slot, two threads to a row with 64 of a tile's keys each; in tiles of the tree they apply the mask and see to it that V holds numbers
 // Tensor memory of a slot: S (128 columns; P in the first half of each thread's own 64), O (128). Shared memory has seven buffers of a tile: Q, three of K, and two of V with Q's second half
 // or three of V.
-// 64 tokens x 32 heads (8 key/value heads) behind 100 000 keys, blocks of 256 rows and 44 tiles: 116 us with the sum of the splits, 0.91 PFLOP/s; some 95 without any softmax. (One slot a block and
+// 64 tokens x 32 heads (8 key/value heads) behind 100 000 keys, blocks of 256 rows and 44 tiles: 119 us with the sum of the splits, 0.88 PFLOP/s; some 95 without any softmax. (One slot a block and
 // two blocks to an SM, each tile asked for when the one before it was used: 155.) A tile takes a slot some 3400 cycles: 1850 from its scores to its weights, of them 1000 for the exponentials, which
 // the special-function units alone would need 1024 for at least (1190 in fact), and 1570 from there to the next scores, of them 1024 for the products; those of both slots together keep the tensor
 // cores busy for 2048. Maxima of three numbers and one vote in place of two were 3 % of it. What did not help: tiles of 64 keys with two of scores a slot, references a tile old in place of a row's own maximum (its steps cost more
 // than the exchange), Q in tensor memory beside tiles of 64 keys (152: the softmax's steps come twice as often), P handed over in two
-// halves (147: one more wait for the stores and one more signal a tile), first tiles, Q and tensor memory asked for beside one another in front of the first barrier (no change).
+// halves (147: one more wait for the stores and one more signal a tile), copies of 16 keys x 128 columns, which take two thirds of the time of two of 64 columns (5 % more here, 3 % less for 48 trees
+// of up to 48 tokens behind 4100 keys), tiles asked for in the second-level cache four ahead (147), first tiles, Q and tensor memory asked for beside one another in front of the first barrier (no change).
 constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_THREADS = 640, TMA_WARP = 16, MMA_WARP = 17, K_STAGES = 3, V_STAGES = 3, SOFT_REGS = 112, ROLE_REGS = 32;
 constexpr uint32_t TC_COLS = 512;
 constexpr float TC_RESCALE = 8.f;          // O is rescaled when a maximum has grown by more than 2^8
