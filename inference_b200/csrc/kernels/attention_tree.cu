@@ -487,7 +487,8 @@ __device__ __forceinline__ void tree_softmax(const TreeParams& p, TcBars* bars, 
 
   float scale_log2 = p.scale * 1.4426950408889634f, to_cap = 0.f;           // the capped score is cap (1 - 2 / (2^(to_cap s) + 1))
   if constexpr (CAP) to_cap = 2.f * scale_log2 / p.softcap, scale_log2 = 1.4426950408889634f;
-  const float STOP = __int_as_float(0x7fffffff);                            // handed over instead of a maximum, which is a number or infinite, when a wait ran out
+  // Handed over instead of a maximum when a wait ran out. A maximum is a number or infinite also where all scores are NaN: -inf is among what it is taken of.
+  const float STOP = __int_as_float(0x7fffffff);
   float m = -INFINITY, l = 0.f;
   bool ok = true, whole = true;                                             // whole: no wait inside a tile has run out
   for (int i = 0; i < steps; ++i, j += by) {
@@ -518,17 +519,22 @@ __device__ __forceinline__ void tree_softmax(const TreeParams& p, TcBars* bars, 
       for (int e = 4; e + 7 < 64; e += 8)
         m0 = max3(m0, x[e], x[e + 1]), m1 = max3(m1, x[e + 2], x[e + 3]), m2 = max3(m2, x[e + 4], x[e + 5]), m3 = max3(m3, x[e + 6], x[e + 7]);
       m0 = max3(m0, x[60], x[61]), m1 = max3(m1, x[62], x[63]);
-      mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+      mx = fmaxf(fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)), -INFINITY);
     }
     // (Its word of the tile before is read by then: this tile's scores wait for that one's weights.)
     word[half * TC_ROWS] = mx;
     pair_sync(1 + slot * 4 + w4);
     const float theirs = word[(half ^ 1) * TC_ROWS];
     const float m_new = fmaxf(fmaxf(mx, theirs), m);
-    const bool grow = (m_new - m) * scale_log2 > TC_RESCALE, stop = !ok || __float_as_int(theirs) == 0x7fffffff;      // grow on the first tile with a key that the row sees (m = -inf)
+    // Both halves vote on the same two words, so that they leave at the same tile.
+    const bool stop = __float_as_int(mx) == 0x7fffffff || __float_as_int(theirs) == 0x7fffffff;
+    const bool grow = (m_new - m) * scale_log2 > TC_RESCALE;                // on the first tile with a key that the row sees (m = -inf)
     if (__any_sync(0xffffffffu, grow || stop)) {
       ok = !__any_sync(0xffffffffu, stop);
-      if (!ok) break;                                                       // both halves leave at the same tile
+      if (!ok) {
+        pair_sync(1 + slot * 4 + w4);                                       // both have read the words that are written next
+        break;
+      }
       const float f = grow ? ex2((m - m_new) * scale_log2) : 1.f;
       if (grow) l *= f, m = m_new;
       if (i > 0) scale_columns<OUT>(t_o, f);                                // the product before this one is done: the scores came behind it

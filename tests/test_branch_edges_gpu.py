@@ -1,0 +1,75 @@
+"""Drafted trees, accepted paths and beams at the edges of what their calls allow."""
+import math
+
+import pytest
+import torch
+
+from test_branch_gpu import CUDA, Step, _ops, _pack, _run, _trees, _visible
+
+pytestmark = pytest.mark.gpu
+
+KINDS = pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+
+
+# ---- scores that are not numbers ------------------------------------------------------------------------------------------------------------------------
+# Tokens x 4 heads of a group: 28 rows are one half of a block, whose tiles of 128 keys are dealt out by turns; 240 rows are both halves, which share the tiles.
+@KINDS
+@pytest.mark.parametrize("q_lens", [[7, 5], [60, 33]], ids=["half", "two"])
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("base", [[300, 140], [100, 0], [131, 513]], ids=str)
+@pytest.mark.parametrize("what", ["nan", "inf", "cancel", "nan, capped"])
+def test_a_query_that_is_no_number_is_its_own_rows_matter(kind, q_lens, splits, base, what):
+    """One head of one token has NaN, or infinities whose products are, or add up to, none: its result is NaN, all others are those of the clean run, bit by bit."""
+    c = Step(base, q_lens, kind=kind, seed=71)
+    sees, _ = _visible(_trees(q_lens, 72), c.max_q)
+    mask, cap = _pack(sees), 20.0 if "capped" in what else 0.0
+    clean = _run(c, mask, 0.1, softcap=cap, num_splits=splits)
+    t, head = q_lens[0] - 1, 5          # sees more than one key
+    if "nan" in what:
+        c.q[t, head, 3] = math.nan
+    elif what == "inf":
+        c.q[t, head, 3] = math.inf      # products of both signs: of the larger ones none is a number
+    else:
+        c.q[t, head, 3], c.q[t, head, 4] = math.inf, -math.inf
+    out = _run(c, mask, 0.1, softcap=cap, num_splits=splits)
+    _ops().check_status()
+    out, clean = (x.view(c.T, c.heads, -1) for x in (out, clean))
+    assert out[t, head].isnan().all()
+    rest = torch.ones(c.T, c.heads, dtype=torch.bool, device=CUDA)
+    rest[t, head] = False
+    assert torch.equal(out[rest], clean[rest])
+
+
+@KINDS
+@pytest.mark.parametrize("q_lens", [[7, 5], [64, 33]], ids=["half", "two"])
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("base,first,n", [(b, f, min(n, b - f)) for b in (100, 130, 300, 520) for f, n in ((0, 64), (64, 64), (0, 100), (128, 64), (192, 64), (128, 128), (256, 40)) if f < b])
+@pytest.mark.parametrize("lone", [False, True], ids=["", "and a query"])
+def test_keys_that_are_no_numbers_fill_half_a_tile(kind, q_lens, splits, base, first, n, lone):
+    """64 cached keys and more of one key/value head are NaN, which all of its sequence's tokens see; with a query that is NaN too. Everything else is that of the clean run."""
+    c = Step([base, 200], q_lens, kind=kind, seed=73)
+    sees, _ = _visible(_trees(q_lens, 74), c.max_q)
+    clean = _run(c, _pack(sees), 0.1, num_splits=splits)
+    for key in range(first, first + n):
+        page, at = c.place(0, key)
+        c.k[page, 1, at] = math.nan
+    bad = torch.zeros(c.T, c.heads, dtype=torch.bool, device=CUDA)
+    bad[:q_lens[0], 4:] = True
+    if lone:
+        c.q[2, 1, 0] = math.nan
+        bad[2, 1] = True
+    out = _run(c, _pack(sees), 0.1, num_splits=splits)
+    _ops().check_status()
+    out, clean = (x.view(c.T, c.heads, -1) for x in (out, clean))
+    assert out[bad].isnan().all() and torch.equal(out[~bad], clean[~bad])
+
+
+@KINDS
+@pytest.mark.parametrize("splits", [1, 2])
+def test_everything_is_no_number(kind, splits):
+    c = Step([700, 3], [70, 2], kind=kind, seed=75)
+    sees, _ = _visible(_trees(c.q_lens, 76), c.max_q)
+    c.q.fill_(math.nan)
+    out = _run(c, _pack(sees), 0.1, num_splits=splits)
+    _ops().check_status()
+    assert out.isnan().all()
