@@ -14,6 +14,8 @@ import time
 from dataclasses import dataclass, field
 from typing import Any
 
+import torch
+
 
 @dataclass
 class _Call:
@@ -151,6 +153,9 @@ class BatchingBackend:
             with self._lock:
                 out = (self.inner.forward_greedy(seqs, toks) if kind == "greedy"
                        else self.inner.forward(seqs, toks, all_positions))
+                if kind == "logits" and not all_positions and out:
+                    # rows of a decode step lie in a buffer that the next step writes, which may run before a caller has read them
+                    out = list(torch.stack(out).unbind(0))
             i = 0
             for c in group:
                 n = len(c.seqs)
