@@ -16,11 +16,13 @@ from ..policy.paging import BlockAllocator
 
 
 def copy_entries(tensors, src: list[int], dst: list[int]) -> None:
-    """Entry dst[i] (a page, a state slot) of every tensor becomes a copy of its entry src[i]. tensors: a uniform pool's, or a list of [entries, ...] on one device. On the GPU one
-    launch for all of them."""
-    if not src:
-        return
+    """Entry dst[i] (a page, a state slot) of every tensor becomes a copy of its entry src[i]; one that is its own copy stays. tensors: a uniform pool's, or a list of [entries, ...] on
+    one device. On the GPU one launch for all of them."""
     whole = isinstance(tensors, torch.Tensor)
+    moves = [(a, b) for a, b in zip(src, dst, strict=True) if a != b]
+    if not moves or not (whole or tensors):
+        return
+    src, dst = [a for a, _ in moves], [b for _, b in moves]
     device = (tensors if whole else tensors[0]).device
     if device.type == "cuda":
         from ..ops import copy_pages
@@ -165,13 +167,10 @@ class LayeredKvPool:
         self.copy_blocks([src], [dst])
 
     def copy_blocks(self, src: list[int], dst: list[int]) -> None:
-        tensors = self._tensors(False)
-        if tensors:
-            copy_entries(tensors, src, dst)
+        copy_entries(self._tensors(False), src, dst)
 
     def copy_state(self, src: int, dst: int) -> None:
-        if src != dst:
-            self.copy_states([src], [dst])
+        self.copy_states([src], [dst])
 
     def copy_states(self, src: list[int], dst: list[int]) -> None:
         copy_entries(self._tensors(True), src, dst)

@@ -1,9 +1,12 @@
 """Loops that carry several continuations, and the pools and proxies below them, where their calls are easily missed."""
+import contextlib
 import threading
 
+import pytest
 import torch
 
 from inference_b200.engine.batching import BatchingBackend
+from inference_b200.engine.kv_pool import KvGeometry, LayeredKvPool, PagedKvPool, StateGeometry, copy_entries
 
 
 class _OneBuffer:
@@ -36,3 +39,50 @@ def test_a_clients_logits_outlive_the_steps_of_others():
         batch.close()
     for name, tokens in (("a", [3, 4]), ("b", [5, 6, 7]), ("c", [8])):
         assert [row.tolist() for row in got[name]] == [[float(t)] * 6 for t in tokens]
+
+
+# ---- copies in pools ----------------------------------------------------------------------------------------------------------------------------------------
+@pytest.fixture
+def on_a_device(monkeypatch):
+    """Copies as they are on the GPU: `ops.copy_pages` with its checks, its launch put in by elementary operations."""
+    from inference_b200 import ops
+    from inference_b200.ops import branch
+
+    class Device:
+        type = "cuda"
+
+    class OnDevice(torch.Tensor):
+        device = Device()
+
+    def launch(pages, src, dst):
+        _, _, _, _, _, blocks, held = branch._tensors(pages)
+        assert min(*src, *dst) >= 0 and max(*src, *dst) < blocks and len(set(dst)) == len(dst) and not set(dst) & set(src)
+        for t in held:
+            t = t.flatten(0, 1) if isinstance(pages, torch.Tensor) else t[None]
+            for a, b in zip(src, dst):
+                t[:, b] = t[:, a].clone()
+
+    monkeypatch.setattr(ops, "copy_pages", launch)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    return lambda t: t.as_subclass(OnDevice)
+
+
+def test_a_page_that_is_copied_to_itself_stays(on_a_device):
+    pool = PagedKvPool(2, 5, 1, 4, 2, device="cpu", dtype=torch.float32)
+    pool.data.copy_(torch.randn(pool.data.shape))
+    want = pool.data.clone()
+    pool.data = on_a_device(pool.data)
+    pool.copy_block(3, 3)
+    assert (torch.Tensor(pool.data) == want).all()
+    pool.copy_blocks([1, 2, 1], [1, 4, 0])
+    want[:, :, 4], want[:, :, 0] = want[:, :, 2].clone(), want[:, :, 1].clone()
+    assert (torch.Tensor(pool.data) == want).all()
+
+
+def test_pools_that_keep_no_states_or_no_pages():
+    pages = LayeredKvPool([KvGeometry(1, 4, 4)], 3, 2, device="cpu", dtype=torch.float32)
+    pages.copy_state(0, 1)
+    states = LayeredKvPool([StateGeometry((2,), (3,))], 3, 2, device="cpu", dtype=torch.float32, state_slots=2)
+    states.copy_block(0, 1)
+    with pytest.raises(ValueError):
+        copy_entries(pages.data[0], [0, 1], [2])
