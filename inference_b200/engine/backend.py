@@ -41,6 +41,12 @@ class DecodeBackend(Protocol):
         the token behind it. choose(logits [all trees' tokens, vocab]) -> int64 tokens, one a row."""
 
 
+def _check_parents(seqs: list[Any], parents: list[int]) -> None:
+    """In front of what a reordering releases: a parent is the number of a sequence, counted from the front."""
+    if not all(0 <= p < len(seqs) for p in parents):
+        raise ValueError(f"parents are places among {len(seqs)} sequences")
+
+
 def set_embed_override(seq: Any, positions: list[int], values: torch.Tensor) -> None:
     """Vision-language prompts: the next forward that appends tokens to `seq` replaces the embeddings of the new
     tokens at `positions` (indices within that call's token list) by `values` [len(positions), hidden]."""
@@ -200,6 +206,7 @@ class GpuBackend:
         seq.release()
 
     def reorder(self, seqs, parents):
+        _check_parents(seqs, parents)
         keep = set(parents)
         for i, s in enumerate(seqs):
             if i not in keep:
@@ -302,6 +309,7 @@ class OracleBackend:
         seq.cache.reset()
 
     def reorder(self, seqs, parents):
+        _check_parents(seqs, parents)
         out, used = [], set()
         for p in parents:
             out.append(self.fork(seqs[p], self.length(seqs[p])) if p in used else seqs[p])

@@ -5,8 +5,16 @@ import threading
 import pytest
 import torch
 
+from inference_b200.engine.backend import GpuBackend, OracleBackend
 from inference_b200.engine.batching import BatchingBackend
-from inference_b200.engine.kv_pool import KvGeometry, LayeredKvPool, PagedKvPool, StateGeometry, copy_entries
+from inference_b200.engine.kv_pool import KvGeometry, LayeredKvPool, PagedKvPool, PagedSequence, StateGeometry, copy_entries
+from inference_b200.models import ModelConfig
+from inference_b200.models.oracle import OracleLlama, random_llama_weights
+
+
+def _oracle(seed=0, vocab=96, std=0.3):
+    cfg = ModelConfig(hidden_size=32, intermediate_size=64, num_layers=2, num_heads=4, num_kv_heads=2, head_dim=8, vocab_size=vocab, rope_theta=10000.0, tie_word_embeddings=True)
+    return OracleBackend(OracleLlama(cfg, random_llama_weights(cfg, seed=seed, std=std)))
 
 
 class _OneBuffer:
@@ -86,3 +94,25 @@ def test_pools_that_keep_no_states_or_no_pages():
     states.copy_block(0, 1)
     with pytest.raises(ValueError):
         copy_entries(pages.data[0], [0, 1], [2])
+
+
+# ---- reorderings --------------------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("parents", [[-1], [0, -2], [2], [1, 0, 7]], ids=str)
+def test_reorderings_by_numbers_of_no_sequence_touch_nothing(parents):
+    oracle = _oracle()
+    seqs = [oracle.new_sequence(), oracle.new_sequence()]
+    oracle.forward(seqs, [[1, 2, 3], [4]])
+    with pytest.raises(ValueError):
+        oracle.reorder(seqs, parents)
+    assert [oracle.length(s) for s in seqs] == [3, 1]
+    pool = PagedKvPool(1, 9, 1, 4, 4, device="cpu", dtype=torch.float32)
+    paged = GpuBackend.__new__(GpuBackend)
+    paged.runner = type("Runner", (), {"pool": pool})()
+    seqs = [PagedSequence(pool), PagedSequence(pool)]
+    seqs[0].reserve(6)
+    seqs[1].reserve(3)
+    with pytest.raises(ValueError):
+        paged.reorder(seqs, parents)
+    assert [s.length for s in seqs] == [6, 3] and pool.allocator.live_blocks() == 3
+    a, b, c = paged.reorder(seqs, [0, 0, 0])
+    assert a is seqs[0] and (a.length, b.length, c.length) == (6, 6, 6) and seqs[1].length == 0 and pool.allocator.live_blocks() == 4
