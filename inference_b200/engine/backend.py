@@ -13,6 +13,7 @@ import torch
 
 from ..contracts.errors import Unsupported
 from ..models.oracle import ContiguousKvCache, OracleLlama
+from ..policy.speculative import check_trees
 from .kv_pool import PagedSequence, unshare_tails
 from .runner import ModelRunner
 
@@ -321,6 +322,7 @@ class OracleBackend:
 
     def step_trees(self, seqs, tokens, parents, choose):
         """Each token of a tree by itself, behind its path."""
+        check_trees(seqs, tokens, parents)
         rows = []
         for s, toks, ups in zip(seqs, tokens, parents):
             for i in range(len(toks)):

@@ -17,6 +17,7 @@ import torch
 from ..contracts.errors import Unsupported
 from ..models.llama import LlamaGpu, StepInputs, splits_for as _splits_for
 from ..ops import budget
+from ..policy.speculative import check_trees
 from ..utils import tracing
 from ..utils.graphs import recording
 from .kv_pool import PagedKvPool, PagedSequence
@@ -197,10 +198,7 @@ class ModelRunner:
         sequences have to be truncated to what they were."""
         if self._stateful or self.page_budget is not None or self._summaries() is not None or not (isinstance(self.model, LlamaGpu) and isinstance(self.pool, PagedKvPool)):
             raise Unsupported("drafted trees need a decoder of the Llama family on a uniform pool without page summaries")
-        if any(len(t) != len(p) or not t or p[0] != -1 or any(not 0 <= up < j for j, up in enumerate(p) if j) for t, p in zip(tokens, parents)):
-            raise ValueError("a tree has a root and tokens that hang on tokens in front of them")
-        if not len(seqs) == len(tokens) == len(parents) or len({id(s) for s in seqs}) != len(seqs):
-            raise ValueError("a tree for each sequence, and each sequence once")
+        check_trees(seqs, tokens, parents)
         step = _TreeStep(list(seqs), parents)
         return self.prefill(seqs, tokens, all_positions=True, trees=step), step
 

@@ -35,6 +35,14 @@ def accept_token(target: list[tuple[int, float]], draft: list[tuple[int, float]]
     return bool(ok), tok.value
 
 
+def check_trees(seqs: list, tokens: list[list[int]], parents: list[list[int]]) -> None:
+    """A tree for each sequence, each sequence once: its first token the root (parent -1), the others behind their parents."""
+    if not len(seqs) == len(tokens) == len(parents) or len({id(s) for s in seqs}) != len(seqs):
+        raise ValueError("a tree for each sequence, and each sequence once")
+    if any(len(t) != len(p) or not t or p[0] != -1 or any(not 0 <= up < j for j, up in enumerate(p) if j) for t, p in zip(tokens, parents)):
+        raise ValueError("a tree has a root and tokens that hang on tokens in front of them")
+
+
 def ngram_tree(tokens: list[int], max_ngram: int, branches: int, depth: int) -> tuple[list[int], list[int]]:
     """Prompt lookup with several answers: what followed the earlier occurrences of the longest repeated run that ends `tokens` (up to max_ngram long, shorter runs while there is room), the
     latest first, up to `branches` different continuations of up to `depth` tokens, as one tree. Returns its tokens, the last of `tokens` first, and each one's parent (-1 of the root)."""

@@ -116,3 +116,16 @@ def test_reorderings_by_numbers_of_no_sequence_touch_nothing(parents):
     assert [s.length for s in seqs] == [6, 3] and pool.allocator.live_blocks() == 3
     a, b, c = paged.reorder(seqs, [0, 0, 0])
     assert a is seqs[0] and (a.length, b.length, c.length) == (6, 6, 6) and seqs[1].length == 0 and pool.allocator.live_blocks() == 4
+
+
+# ---- trees --------------------------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("tokens,parents", [([[1, 2]], [[0, 0]]), ([[1, 2]], [[-1, 1]]), ([[1, 2, 3]], [[-1, 2, 0]]), ([[1, 2]], [[-1]]), ([[]], [[]]), ([[1], [2]], [[-1], [-1]]), ([], [])], ids=str)
+def test_trees_that_are_none_are_refused_on_the_oracle_too(tokens, parents):
+    be = _oracle()
+    seq = be.new_sequence()
+    be.forward([seq], [[1, 2, 3]])
+    with pytest.raises(ValueError):
+        be.step_trees([seq], tokens, parents, lambda logits: torch.argmax(logits, -1))
+    assert be.length(seq) == 3
+    with pytest.raises(ValueError):
+        be.step_trees([seq, seq], [[1], [1]], [[-1], [-1]], lambda logits: torch.argmax(logits, -1))
