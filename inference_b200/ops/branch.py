@@ -44,9 +44,10 @@ def plan_tree(parents: torch.Tensor, *, cu_q: torch.Tensor | None, max_q_len: in
     _require(parents.dim() == 1 and parents.dtype == torch.int32 and parents.is_contiguous(), "parents are int32 [T]")
     T = parents.shape[0]
     n = _check_ranges(cu_q, max_q_len, T)
-    words = (max_q_len + 31) // 32
+    most = max(1, min(max_q_len, T))               # no sequence has more tokens than the step, however loose the bound is
+    words = (most + 31) // 32
     mask, depths = parents.new_zeros((T, words)), parents.new_zeros(T)
-    check(kernels().swb_plan_tree(parents.data_ptr(), ptr(cu_q), n, max_q_len, T, words, mask.data_ptr(), depths.data_ptr(), stream), "swb_plan_tree")
+    check(kernels().swb_plan_tree(parents.data_ptr(), ptr(cu_q), n, most, T, words, mask.data_ptr(), depths.data_ptr(), stream), "swb_plan_tree")
     return TreePlan(mask, depths)
 
 
@@ -86,6 +87,7 @@ def tree_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, 
     blocks, heads, bs, D, Dv = _check_cache(kcache, vcache)
     T, G, tok, head = _check_rows(q, heads, D)
     n, per = _check_step(block_table, kv_lens, cu_q, max_q_len, T)
+    most = max(1, min(max_q_len, T))
     kind, columns = q.dtype, G * heads * Dv
     _require(kind == kcache.dtype, "queries and cache have one type")
     _require(mask.dim() == 2 and mask.dtype == torch.int32 and mask.shape[0] == T and mask.shape[1] >= 1 and mask.stride(1) == 1, "mask is int32 [T, words], unit inner stride")
@@ -96,14 +98,14 @@ def tree_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, 
         _require(out.stride(0) >= columns or T <= 1, "rows of out share memory")
     k_ptr, v_ptr = kcache.data_ptr(), vcache.data_ptr()
     fast = kind is torch.bfloat16 and (D | Dv) % 8 == 0 and D <= 128 and Dv <= 128 and bs % 16 == 0 and scale > 0 and (k_ptr | v_ptr) % 16 == 0 and blocks * heads * bs < 2 ** 31 - 1
-    problems = n * heads * -(-max_q_len * G // (256 if fast else 32))
+    problems = n * heads * -(-most * G // (256 if fast else 32))
     splits = tree_splits(problems, per * bs, fast) if num_splits is None else num_splits
     _require(1 <= splits <= MAX_SPLITS, "1 to 64 splits")
     ws, nbytes = None, 0
     if splits > 1:
         nbytes = 4 * splits * T * G * heads * (Dv + 2) + 16
         ws = q.new_empty(nbytes, dtype=torch.uint8)        # the call's own: two streams or graphs share none
-    dims = _DIMS[16](T, n, max_q_len, per, blocks, bs, heads, G, D, Dv, mask.shape[1], splits, kind == torch.float32, 0, 0, 0)
+    dims = _DIMS[16](T, n, most, per, blocks, bs, heads, G, D, Dv, mask.shape[1], splits, kind == torch.float32, 0, 0, 0)
     strides = _STRIDES(tok, head, out.stride(0), block_table.stride(0), mask.stride(0), 0, 0, 0)
     check(kernels().swb_attn_tree(dims, strides, q.data_ptr(), out.data_ptr(), k_ptr, v_ptr, block_table.data_ptr(), ptr(cu_q), kv_lens.data_ptr(),
                                   mask.data_ptr(), scale, softcap, ptr(ws), nbytes, stream), "swb_attn_tree")

@@ -73,3 +73,17 @@ def test_everything_is_no_number(kind, splits):
     out = _run(c, _pack(sees), 0.1, num_splits=splits)
     _ops().check_status()
     assert out.isnan().all()
+
+
+# ---- bounds of a step ---------------------------------------------------------------------------------------------------------------------------------------
+@KINDS
+def test_a_steps_bound_may_be_the_largest_number(kind):
+    ops, c = _ops(), Step([70, 9], [9, 20], kind=kind, seed=81)
+    parents = torch.tensor(sum(_trees(c.q_lens, 82), []), dtype=torch.int32, device=CUDA)
+    near, far = ops.plan_tree(parents, cu_q=c.cu, max_q_len=20), ops.plan_tree(parents, cu_q=c.cu, max_q_len=2 ** 31 - 1)
+    assert torch.equal(near.mask, far.mask) and torch.equal(near.depths, far.depths)
+    out = _run(c, near.mask, 0.1, num_splits=2)
+    c.max_q = 2 ** 31 - 1
+    assert torch.equal(_run(c, far.mask, 0.1, num_splits=2), out)
+    empty = ops.plan_tree(parents[:0], cu_q=torch.zeros(3, dtype=torch.int32, device=CUDA), max_q_len=5)
+    assert empty.mask.shape == (0, 1) and empty.depths.shape == (0,)
