@@ -1021,7 +1021,8 @@ int swb_attn_tree(const int* dims, const long long* strides, const void* q, void
   if (p.num_seqs > 65535 || p.max_blocks < 1 || p.num_blocks < 1 || p.bs < 1 || p.Hkv < 1 || p.G < 1 || p.G > MAX_GROUP || p.D < 1 || p.D > 256 || p.Dv < 1 || p.Dv > 256 ||
       p.num_splits < 1 || p.num_splits > MAX_SPLITS || p.uniform_q < 1 || p.words < 1 || !q || !out || !k || !v || !table || !kv_lens || !mask)
     return -3;
-  if ((long long)p.max_blocks * p.bs > INT_MAX || (long long)p.uniform_q * p.G > INT_MAX - 2 * TC_ROWS) return -3;
+  // tiles and the pages that are looked up ahead of them reach up to 1007 keys behind a sequence's end
+  if ((long long)p.max_blocks * p.bs > INT_MAX - 1024 || (long long)p.uniform_q * p.G > INT_MAX - 2 * TC_ROWS) return -3;
   p.scale = scale, p.softcap = softcap, p.k = k, p.v = v;
   const bool fast = tc_fits(p, fp32);
   const int tile = fast ? 2 * TC_ROWS : PR;

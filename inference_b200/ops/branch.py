@@ -23,6 +23,7 @@ from .budget import _check_cache, _check_rows, _check_step, _place, _require
 from .runtime import check, ptr
 
 MAX_SPLITS, MAX_PATH = 64, 8192
+MAX_TOKENS = 2 ** 31 - 1025       # of a sequence in a table: places behind its end, up to 1024 of them, are whole numbers of 32 bits too
 MAX_BEAMS, MAX_COUNT = 256, 128
 
 _ONE = struct.Struct("q").pack
@@ -87,6 +88,7 @@ def tree_attention(q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, 
     blocks, heads, bs, D, Dv = _check_cache(kcache, vcache)
     T, G, tok, head = _check_rows(q, heads, D)
     n, per = _check_step(block_table, kv_lens, cu_q, max_q_len, T)
+    _require(per * bs <= MAX_TOKENS, f"block_table has room for {MAX_TOKENS} tokens at most")
     most = max(1, min(max_q_len, T))
     kind, columns = q.dtype, G * heads * Dv
     _require(kind == kcache.dtype, "queries and cache have one type")
