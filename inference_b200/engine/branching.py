@@ -164,7 +164,8 @@ def generate_tree_lookup(target: DecodeBackend, prompt: list[int], cfg: Generati
             if cfg.cancel is not None and cfg.cancel.is_cancelled():
                 why = FinishReason.CANCELLED
                 break
-            tokens, parents = ngram_tree(list(prompt) + out, spec.max_ngram, spec.branches, min(spec.depth, cfg.max_new_tokens - len(out) - 1))
+            room = cfg.max_new_tokens - len(out)        # a tree takes no more of the cache than the text may
+            tokens, parents = (x[:room] for x in ngram_tree(list(prompt) + out, spec.max_ngram, spec.branches, min(spec.depth, room - 1)))
             (path, last), = target.step_trees([seq], [tokens], [parents], choose(tokens, parents))
             stats.forwards += 1
             stats.proposed += len(tokens) - 1

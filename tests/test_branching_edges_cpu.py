@@ -7,6 +7,8 @@ import torch
 
 from inference_b200.engine.backend import GpuBackend, OracleBackend
 from inference_b200.engine.batching import BatchingBackend
+from inference_b200.engine.branching import TreeConfig, generate_tree_lookup
+from inference_b200.engine.decode import GenerationConfig, generate
 from inference_b200.engine.kv_pool import KvGeometry, LayeredKvPool, PagedKvPool, PagedSequence, StateGeometry, copy_entries
 from inference_b200.models import ModelConfig
 from inference_b200.models.oracle import OracleLlama, random_llama_weights
@@ -129,3 +131,25 @@ def test_trees_that_are_none_are_refused_on_the_oracle_too(tokens, parents):
     assert be.length(seq) == 3
     with pytest.raises(ValueError):
         be.step_trees([seq, seq], [[1], [1]], [[-1], [-1]], lambda logits: torch.argmax(logits, -1))
+
+
+class _Full(OracleBackend):
+    """A cache with room for so many tokens."""
+    room = 0
+
+    def forward(self, seqs, new_tokens, all_positions=False):
+        assert all(self.length(s) + len(t) <= self.room for s, t in zip(seqs, new_tokens)), "no room"
+        return super().forward(seqs, new_tokens, all_positions)
+
+    def step_trees(self, seqs, tokens, parents, choose):
+        assert all(self.length(s) + len(t) <= self.room for s, t in zip(seqs, tokens)), "no room"
+        return super().step_trees(seqs, tokens, parents, choose)
+
+
+@pytest.mark.parametrize("prompt", [[4, 4, 8, 4, 4, 8, 4, 4], [2, 3, 2, 4, 2, 3, 2, 4, 2]])
+@pytest.mark.parametrize("new", [1, 2, 5, 13])
+def test_trees_need_no_more_room_than_plain_decoding(prompt, new):
+    be = _Full(_oracle().model)
+    be.room = len(prompt) + new - 1
+    cfg = GenerationConfig(max_new_tokens=new)
+    assert generate_tree_lookup(be, prompt, cfg, TreeConfig(max_ngram=2, branches=8, depth=6))[0].tokens == generate(be, prompt, cfg).tokens
