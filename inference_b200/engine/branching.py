@@ -45,7 +45,7 @@ def best_continuations(logits: torch.Tensor, scores: torch.Tensor, count: int) -
         rows = torch.stack([got.scores[0].double(), got.beams[0].double(), got.tokens[0].double()]).tolist()
         return [(s, int(b), int(t)) for s, b, t in zip(*rows) if b >= 0]
     s = scores.double()[:, None] + torch.log_softmax(logits.double(), -1)
-    s = torch.where(s > -math.inf, s, -math.inf).flatten()
+    s = torch.where(s.isfinite(), s, -math.inf).flatten()      # of a beam that is not alive, or whose logits are no distribution: nothing
     order = torch.sort(s, descending=True, stable=True).indices[:count].tolist()
     return [(float(s[i]), i // logits.shape[1], i % logits.shape[1]) for i in order if s[i] > -math.inf]
 

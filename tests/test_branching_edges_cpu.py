@@ -1,5 +1,6 @@
 """Loops that carry several continuations, and the pools and proxies below them, where their calls are easily missed."""
 import contextlib
+import math
 import threading
 
 import pytest
@@ -7,7 +8,7 @@ import torch
 
 from inference_b200.engine.backend import GpuBackend, OracleBackend
 from inference_b200.engine.batching import BatchingBackend
-from inference_b200.engine.branching import TreeConfig, generate_tree_lookup
+from inference_b200.engine.branching import TreeConfig, best_continuations, generate_tree_lookup
 from inference_b200.engine.decode import GenerationConfig, generate
 from inference_b200.engine.kv_pool import KvGeometry, LayeredKvPool, PagedKvPool, PagedSequence, StateGeometry, copy_entries
 from inference_b200.models import ModelConfig
@@ -153,3 +154,12 @@ def test_trees_need_no_more_room_than_plain_decoding(prompt, new):
     be.room = len(prompt) + new - 1
     cfg = GenerationConfig(max_new_tokens=new)
     assert generate_tree_lookup(be, prompt, cfg, TreeConfig(max_ngram=2, branches=8, depth=6))[0].tokens == generate(be, prompt, cfg).tokens
+
+
+# ---- continuations --------------------------------------------------------------------------------------------------------------------------------------------
+def test_beams_that_offer_nothing_on_the_host():
+    """As `ops.beam_select` has it: scores that are not finite, logits with NaN or +inf, tokens that are not allowed."""
+    logits = torch.zeros(6, 3)
+    logits[3, 1], logits[4, 0], logits[5, :2] = math.nan, math.inf, -math.inf
+    got = best_continuations(logits, torch.tensor([math.inf, -math.inf, math.nan, 0.0, 0.0, -1.0]), 20)
+    assert got == [(-1.0, 5, 2)]
