@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_branch_gpu import CUDA, Step, _ops, _pack, _run, _trees, _visible
+from test_branch_gpu import CUDA, Step, _check_beams, _gen, _ops, _pack, _run, _trees, _visible
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +87,49 @@ def test_a_steps_bound_may_be_the_largest_number(kind):
     assert torch.equal(_run(c, far.mask, 0.1, num_splits=2), out)
     empty = ops.plan_tree(parents[:0], cu_q=torch.zeros(3, dtype=torch.int32, device=CUDA), max_q_len=5)
     assert empty.mask.shape == (0, 1) and empty.depths.shape == (0,)
+
+
+# ---- logits far from zero -----------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("shift", [300, 2000, 20000, 29900, 31000, -20000, -31000])
+def test_logits_far_from_zero_lose_nothing(shift):
+    """Two beams with the same logits, one of them moved by a whole number, whose scores differ by 2e-8: the better one is first at every token. (Logits are multiples of 1 / 64, so that
+    the move is exact; a logarithm is off by 2^-29 of a sum at most, 2e-9.)"""
+    V = 6000
+    row = (torch.randn(V, device=CUDA, generator=_gen(91)) * 3 * 64).round() / 64
+    logits = torch.stack([row + shift, row])
+    assert torch.equal(logits[0] - shift, row)
+    for scores in ([2e-8, 0.0], [0.0, 2e-8]):
+        _check_beams(logits, torch.tensor([scores], device=CUDA), 60)
+
+
+@KINDS
+@pytest.mark.parametrize("V", [90, 9001, 70001])
+def test_tokens_forbidden_by_a_finite_number(kind, V):
+    """What is filled in for them is a logit like others: it ties, and comes behind what is allowed."""
+    for fill in (-1e4, -1e9, float(torch.finfo(kind).min)):
+        logits = torch.full((3, V), fill, device=CUDA, dtype=kind)
+        allowed = torch.randperm(V, device=CUDA, generator=_gen(V))[:7]
+        logits[0, allowed] = torch.randn(7, device=CUDA, generator=_gen(92)).to(kind)
+        logits[1, 3 * V // 4:] = torch.randn(V - 3 * V // 4, device=CUDA, generator=_gen(93)).to(kind)
+        _check_beams(logits, torch.tensor([[-1.0, -2.0, -0.5]], device=CUDA), 12)
+
+
+@KINDS
+def test_logits_that_pass_the_rounding_s_reach(kind):
+    """Rows above and below it, and rows that cross it on the way, up and down."""
+    V = 40000
+    ramp = torch.linspace(-1, 1, V, device=CUDA) * 40000
+    step = torch.where(torch.arange(V, device=CUDA) < V // 2, 29000.0, 31000.0) + torch.randn(V, device=CUDA, generator=_gen(94)) * 3
+    near = torch.randn(V, device=CUDA, generator=_gen(95)) * 3
+    rows = torch.stack([ramp, ramp.flip(0), step, step.flip(0), near + 40000, near - 40000, -step, near]).to(kind)
+    _check_beams(rows, -10 * torch.rand(2, 4, device=CUDA, generator=_gen(96)), 20)
+    _check_beams(rows, -10 * torch.rand(8, 1, device=CUDA, generator=_gen(97)), 100)
+
+
+@KINDS
+@pytest.mark.parametrize("count", [1, 9, 128])
+def test_logits_that_rise_with_the_tokens_number(kind, count):
+    """Every step's are above the bound that the ones before it gave: more candidates than a block takes notes of."""
+    V = 128256
+    rise = torch.arange(V, device=CUDA, dtype=torch.float32) / 4096
+    _check_beams(torch.stack([rise, rise * 2, rise.flip(0)]).to(kind), torch.tensor([[-1.0, -1.5, -2.0]], device=CUDA), count)
