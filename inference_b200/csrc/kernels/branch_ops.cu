@@ -15,7 +15,8 @@ SWB_REGISTER_STATUS_UNIT(branch_ops);
 
 namespace {
 
-constexpr int MAX_TENSORS = 96, MAX_PAIRS = 256;          // of a launch: kernel arguments are 4 KB
+constexpr int MAX_TENSORS = 96, MAX_PAIRS = 256;          // of a launch
+constexpr size_t MAX_ARGUMENTS = 32764;                    // bytes that a kernel's arguments may take (CUDA 12.1 and later, from compute capability 7.0 on)
 
 struct Tensors {
   char* base[MAX_TENSORS];
@@ -160,6 +161,7 @@ __global__ void __launch_bounds__(ACCEPT_THREADS, ACCEPT_BLOCKS) accept_tree_ker
 struct Pairs {
   int src[MAX_PAIRS], dst[MAX_PAIRS];
 };
+static_assert(sizeof(Tensors) + sizeof(Pairs) + 64 <= MAX_ARGUMENTS && sizeof(Tensors) + sizeof(AcceptParams) <= MAX_ARGUMENTS, "arguments of a launch");
 constexpr int COPY_THREADS = 256, COPY_UNROLL = 8;
 
 // Block (pair, piece of the page, tensor). from / to: the pairs on the device, where they are not among the arguments.
