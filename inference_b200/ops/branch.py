@@ -5,8 +5,9 @@
   beams              `beam_select` picks the best continuations, `copy_pages` gives beams that part pages of their own
 
 Steps are described as in `paged_attention`: kv_lens int32 [num_seqs] counts a sequence's tokens with the new ones, cu_q int32 [num_seqs + 1] are the new tokens' ranges within the rows of the
-step and max_q_len bounds a sequence's number (None: every sequence has max_q_len of them). Rows in front of the first range and behind the last are left as they were, and so are those
-of a sequence that has more than max_q_len of them. Lengths beyond a table's pages count as the table's end; pages whose number is not in the cache are passed over.
+step and max_q_len bounds a sequence's number (None: every sequence has max_q_len of them). Rows in front of the first range and behind the last are left as they were. Of a sequence that
+has more than max_q_len of them the first max_q_len are computed, and may be accepted, where they lie among all of them; the rows behind these are left too. Lengths beyond a table's pages
+count as the table's end, which lies in front of 2^31 - 1024 tokens; pages whose number is not in the cache are passed over.
 
 Caches are bf16 or fp32, widths up to 256; the caches of all layers together are a pool's tensor [layers, 2, blocks, kv heads, block_size, width] or a list of tensors [blocks, ...]. Calls
 run on the current stream, take no host reads and can be captured into graphs. Scores, the softmax and all sums are 32-bit numbers, those of `beam_select` 64-bit ones."""

@@ -133,3 +133,35 @@ def test_logits_that_rise_with_the_tokens_number(kind, count):
     V = 128256
     rise = torch.arange(V, device=CUDA, dtype=torch.float32) / 4096
     _check_beams(torch.stack([rise, rise * 2, rise.flip(0)]).to(kind), torch.tensor([[-1.0, -1.5, -2.0]], device=CUDA), count)
+
+
+# ---- more tokens than the step was told of ------------------------------------------------------------------------------------------------------------------
+@KINDS
+@pytest.mark.parametrize("splits", [1, 3])
+def test_of_more_tokens_than_the_bound_the_first_are_computed(kind, splits):
+    c = Step([90, 40], [12, 5], kind=kind, seed=83)
+    sees, _ = _visible(_trees(c.q_lens, 84), c.max_q)
+    whole = _run(c, _pack(sees), 0.1, num_splits=splits)
+    c.max_q = 7
+    out = torch.full_like(whole, 7.0)
+    _run(c, _pack(sees), 0.1, num_splits=splits, out=out)
+    left = torch.zeros(c.T, dtype=torch.bool, device=CUDA)
+    left[7:12] = True
+    assert (out[left] == 7).all()
+    c.q_lens[0] = 7         # the definition for the first seven, which lie behind 90 keys as in the whole step
+    c.check(out, sees, 0.1)
+
+
+def test_of_more_tokens_than_the_bound_the_first_may_be_accepted():
+    ops = _ops()
+    tokens = torch.arange(8, device=CUDA)
+    picks = torch.tensor([1, 3, 9, 4, 5, 6, 7, 2], device=CUDA)           # 0 -> 1 -> 3 -> 4 -> 5 ..
+    parents = torch.tensor([-1, 0, 0, 1, 3, 4, 5, 6], dtype=torch.int32, device=CUDA)
+    pool = torch.arange(2 * 4 * 4 * 8, device=CUDA, dtype=torch.float32).view(1, 2, 4, 1, 4, 8)
+    table, lens = torch.tensor([[2, 0, 3]], dtype=torch.int32, device=CUDA), torch.tensor([11], dtype=torch.int32, device=CUDA)      # tokens at 3 to 10
+    want = pool.clone()
+    for to, fro in ((5, 6), (6, 7)):                                        # 3 and 4 close up behind 0 and 1
+        want[:, :, table[0, to // 4], :, to % 4] = pool[:, :, table[0, fro // 4], :, fro % 4]
+    got = ops.accept_tree(picks, tokens, parents, pool, table, lens, cu_q=torch.tensor([0, 8], dtype=torch.int32, device=CUDA), max_q_len=5)
+    assert got.path.tolist() == [[0, 1, 3, 4, -1]] and got.counts.tolist() == [4] and got.next_tokens.tolist() == [5] and got.kv_lens.tolist() == [7]
+    assert torch.equal(pool, want)
