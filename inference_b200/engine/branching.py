@@ -13,7 +13,7 @@ import torch
 from ..contracts.core_llm.output import FinishReason
 from ..contracts.errors import Unsupported
 from ..policy import sampler as hs
-from ..policy.speculative import ngram_tree
+from ..policy.speculative import NgramIndex
 from .backend import DecodeBackend
 from .decode import GenerationConfig, GenerationResult, SpeculativeStats, TokenSink, _pick
 
@@ -118,6 +118,7 @@ def generate_tree_lookup(target: DecodeBackend, prompt: list[int], cfg: Generati
     spec = spec or TreeConfig()
     stats, rng, sp = SpeculativeStats(), hs.SplitMix64(cfg.seed), cfg.sampling
     seq, out, why = target.new_sequence(), [], FinishReason.LENGTH
+    index = NgramIndex(prompt, spec.max_ngram)
 
     def choose(tokens: list[int], parents: list[int]):
         def run(logits: torch.Tensor) -> torch.Tensor:
@@ -149,6 +150,7 @@ def generate_tree_lookup(target: DecodeBackend, prompt: list[int], cfg: Generati
             why = FinishReason.STOP
             return False
         out.append(token)
+        index.append(token)
         if sink is not None and sink(token) is False:
             why = FinishReason.STOP
             return False
@@ -165,7 +167,7 @@ def generate_tree_lookup(target: DecodeBackend, prompt: list[int], cfg: Generati
                 why = FinishReason.CANCELLED
                 break
             room = cfg.max_new_tokens - len(out)        # a tree takes no more of the cache than the text may
-            tokens, parents = (x[:room] for x in ngram_tree(list(prompt) + out, spec.max_ngram, spec.branches, min(spec.depth, room - 1)))
+            tokens, parents = (x[:room] for x in index.tree(spec.branches, min(spec.depth, room - 1)))
             (path, last), = target.step_trees([seq], [tokens], [parents], choose(tokens, parents))
             stats.forwards += 1
             stats.proposed += len(tokens) - 1

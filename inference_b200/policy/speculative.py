@@ -43,28 +43,45 @@ def check_trees(seqs: list, tokens: list[list[int]], parents: list[list[int]]) -
         raise ValueError("a tree has a root and tokens that hang on tokens in front of them")
 
 
+class NgramIndex:
+    """What followed each run of up to max_ngram tokens of a text, kept up as the text grows: a draft takes as long as there are matches, however long the text is."""
+
+    def __init__(self, tokens: list[int], max_ngram: int):
+        self.tokens: list[int] = []
+        self._behind: list[dict[tuple[int, ...], list[int]]] = [{} for _ in range(max(max_ngram, 0))]      # of n + 1 tokens: places behind the run, ascending
+        for t in tokens:
+            self.append(t)
+
+    def append(self, token: int) -> None:
+        at = len(self.tokens)
+        for n, behind in enumerate(self._behind[:at], 1):
+            behind.setdefault(tuple(self.tokens[at - n:]), []).append(at)
+        self.tokens.append(token)
+
+    def tree(self, branches: int, depth: int) -> tuple[list[int], list[int]]:
+        """Prompt lookup with several answers: what followed the earlier occurrences of the longest repeated run that ends the text (shorter runs while there is room), the latest first, up
+        to `branches` different continuations of up to `depth` tokens, as one tree. Returns its tokens, the text's last one first, and each one's parent (-1 of the root)."""
+        out, parents, children = [self.tokens[-1]], [-1], {}
+        found, seen = 0, set()
+        for n in range(min(len(self._behind), len(self.tokens) - 1), 0, -1):
+            for at in reversed(self._behind[n - 1].get(tuple(self.tokens[-n:]), ())):
+                if found >= branches or depth < 1:
+                    return out, parents
+                follow = tuple(self.tokens[at:at + depth])
+                if follow in seen:
+                    continue
+                seen.add(follow)
+                found += 1
+                node = 0
+                for t in follow:
+                    if (node, t) not in children:
+                        children[node, t] = len(out)
+                        out.append(t)
+                        parents.append(node)
+                    node = children[node, t]
+        return out, parents
+
+
 def ngram_tree(tokens: list[int], max_ngram: int, branches: int, depth: int) -> tuple[list[int], list[int]]:
-    """Prompt lookup with several answers: what followed the earlier occurrences of the longest repeated run that ends `tokens` (up to max_ngram long, shorter runs while there is room), the
-    latest first, up to `branches` different continuations of up to `depth` tokens, as one tree. Returns its tokens, the last of `tokens` first, and each one's parent (-1 of the root)."""
-    out, parents, children = [tokens[-1]], [-1], {}
-    found, seen = 0, set()
-    for n in range(min(max_ngram, len(tokens) - 1), 0, -1):
-        run = tokens[-n:]
-        for at in range(len(tokens) - n - 1, -1, -1):
-            if found >= branches or depth < 1:
-                return out, parents
-            if tokens[at:at + n] != run:
-                continue
-            follow = tuple(tokens[at + n:at + n + depth])
-            if follow in seen:
-                continue
-            seen.add(follow)
-            found += 1
-            node = 0
-            for t in follow:
-                if (node, t) not in children:
-                    children[node, t] = len(out)
-                    out.append(t)
-                    parents.append(node)
-                node = children[node, t]
-    return out, parents
+    """The tree of one text; see `NgramIndex.tree`. (A text that grows is better kept in an index: this one is made anew.)"""
+    return NgramIndex(tokens, max_ngram).tree(branches, depth)

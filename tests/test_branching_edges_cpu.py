@@ -1,6 +1,7 @@
 """Loops that carry several continuations, and the pools and proxies below them, where their calls are easily missed."""
 import contextlib
 import math
+import random
 import threading
 
 import pytest
@@ -13,6 +14,7 @@ from inference_b200.engine.decode import GenerationConfig, generate
 from inference_b200.engine.kv_pool import KvGeometry, LayeredKvPool, PagedKvPool, PagedSequence, StateGeometry, copy_entries
 from inference_b200.models import ModelConfig
 from inference_b200.models.oracle import OracleLlama, random_llama_weights
+from inference_b200.policy.speculative import NgramIndex, ngram_tree
 
 
 def _oracle(seed=0, vocab=96, std=0.3):
@@ -163,3 +165,46 @@ def test_beams_that_offer_nothing_on_the_host():
     logits[3, 1], logits[4, 0], logits[5, :2] = math.nan, math.inf, -math.inf
     got = best_continuations(logits, torch.tensor([math.inf, -math.inf, math.nan, 0.0, 0.0, -1.0]), 20)
     assert got == [(-1.0, 5, 2)]
+
+
+# ---- drafts -------------------------------------------------------------------------------------------------------------------------------------------------
+def _scanned(tokens, max_ngram, branches, depth):
+    """The definition, by going through the text: the continuations of the longest repeated runs that end it, the latest first, as one tree."""
+    paths = []
+    for n in range(min(max_ngram, len(tokens) - 1), 0, -1):
+        for at in range(len(tokens) - n - 1, -1, -1):
+            if len(paths) < branches and depth > 0 and tokens[at:at + n] == tokens[-n:] and tokens[at + n:at + n + depth] not in paths:
+                paths.append(tokens[at + n:at + n + depth])
+    nodes = [()]
+    for p in paths:
+        nodes += [tuple(p[:i]) for i in range(1, len(p) + 1) if tuple(p[:i]) not in nodes]
+    return [n[-1] if n else tokens[-1] for n in nodes], [nodes.index(n[:-1]) if n else -1 for n in nodes]
+
+
+@pytest.mark.parametrize("vocab", [1, 3, 40])
+@pytest.mark.parametrize("max_ngram,branches,depth", [(3, 4, 8), (1, 8, 3), (2, 1, 1), (5, 3, 2), (0, 4, 4), (3, 0, 4)])
+def test_an_index_that_grows_drafts_what_the_whole_text_offers(vocab, max_ngram, branches, depth):
+    rng = random.Random(vocab)
+    text = [rng.randrange(vocab) for _ in range(5)]
+    index = NgramIndex(text, max_ngram)
+    for _ in range(60):
+        text.append(rng.randrange(vocab))
+        index.append(text[-1])
+        assert index.tree(branches, depth) == _scanned(text, max_ngram, branches, depth) == ngram_tree(text, max_ngram, branches, depth)
+
+
+def test_a_draft_does_not_go_through_the_text():
+    """Of a long text only the matches are looked at: 200 000 tokens in which the last one stood before once."""
+    class Watched(list):
+        read = 0
+
+        def __getitem__(self, i):
+            Watched.read += 1 if isinstance(i, int) else len(range(*i.indices(len(self))))
+            return super().__getitem__(i)
+
+    index = NgramIndex(list(range(200000)), 3)
+    index.tokens = Watched(index.tokens)
+    index.append(77)
+    Watched.read = 0
+    assert index.tree(4, 5) == ([77, 78, 79, 80, 81, 82], [-1, 0, 1, 2, 3, 4])
+    assert Watched.read < 20
