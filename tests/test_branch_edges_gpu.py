@@ -165,3 +165,23 @@ def test_of_more_tokens_than_the_bound_the_first_may_be_accepted():
     got = ops.accept_tree(picks, tokens, parents, pool, table, lens, cu_q=torch.tensor([0, 8], dtype=torch.int32, device=CUDA), max_q_len=5)
     assert got.path.tolist() == [[0, 1, 3, 4, -1]] and got.counts.tolist() == [4] and got.next_tokens.tolist() == [5] and got.kv_lens.tolist() == [7]
     assert torch.equal(pool, want)
+
+
+# ---- alignment ----------------------------------------------------------------------------------------------------------------------------------------------
+@KINDS
+@pytest.mark.parametrize("D,Dv,bs", [(128, 128, 16), (256, 64, 16), (36, 20, 5), (33, 20, 16)])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_queries_and_results_lie_anywhere(kind, D, Dv, bs, splits):
+    """Rows that start on 16 bytes or on any number, far apart or side by side: the same results, bit by bit."""
+    c = Step([70, 9], [9, 30], D=D, Dv=Dv, bs=bs, kind=kind, seed=85)
+    sees, _ = _visible(_trees(c.q_lens, 86), c.max_q)
+    whole = _run(c, _pack(sees), 0.1, num_splits=splits)
+    c.check(whole, sees, 0.1)
+    T, H, q = c.T, c.heads, c.q
+    for shift, gap in ((0, 0), (1, 0), (2, 1), (4, 4), (8, 3)):
+        room = torch.zeros(shift + T * H * (D + gap) + 8, dtype=kind, device=CUDA)
+        c.q = room[shift:shift + T * H * (D + gap)].view(T, H, D + gap)[..., :D]
+        c.q.copy_(q)
+        to = torch.full((T, H * Dv + gap + 3), 7.0, dtype=kind, device=CUDA)
+        got = _run(c, _pack(sees), 0.1, num_splits=splits, out=to[:, gap:gap + H * Dv])
+        assert torch.equal(got, whole) and (to[:, :gap] == 7).all() and (to[:, gap + H * Dv:] == 7).all()
