@@ -19,3 +19,53 @@ def test_a_page_that_is_copied_to_itself_stays():
     layered = LayeredKvPool([KvGeometry(1, 8, 8)], 3, 16)
     layered.copy_block(1, 1)
     layered.copy_state(0, 1)        # it keeps none
+
+
+def test_two_beam_searches_whose_steps_run_back_to_back():
+    """Two clients of a batching proxy with as many beams each, one group behind the other: each has the texts and scores that it has by itself."""
+    import threading
+
+    from test_branching_gpu import _build, _cfg
+
+    from inference_b200.engine.batching import BatchingBackend
+    from inference_b200.engine.branching import BeamConfig, generate_beam
+    from inference_b200.engine.decode import GenerationConfig
+
+    _, be = _build(_cfg(), seed=21)
+    draw = lambda seed: torch.randint(0, 2048, (19,), generator=torch.Generator().manual_seed(seed)).tolist()
+    run = lambda backend, seed: [(r.tokens, r.score) for r in generate_beam(backend, draw(seed), GenerationConfig(max_new_tokens=24), BeamConfig(beams=4))]
+    alone = [run(be, seed) for seed in (1, 2)]
+    for _ in range(3):
+        batch, got, errors, start = BatchingBackend(be, max_batch=1), {}, [], threading.Barrier(2)
+
+        def client(seed):
+            try:
+                with batch:
+                    start.wait(60)
+                    got[seed] = run(batch, seed)
+            except BaseException as e:
+                errors.append(e)
+
+        jobs = [threading.Thread(target=client, args=(seed,)) for seed in (1, 2)]
+        for j in jobs:
+            j.start()
+        for j in jobs:
+            j.join(120)
+        batch.close()
+        assert not errors and [got.get(1), got.get(2)] == alone
+    assert be.runner.pool.allocator.live_blocks() == 0
+
+
+def test_trees_on_a_pool_that_is_sized_for_the_text():
+    from test_branching_gpu import _build, _cfg
+
+    from inference_b200.engine.branching import TreeConfig, generate_tree_lookup
+    from inference_b200.engine.decode import GenerationConfig, generate
+
+    prompt = [3, 4, 5, 3, 4, 6, 3, 4, 7, 3, 4]
+    _, be = _build(_cfg(vocab_size=64), seed=22, blocks=3)       # 11 tokens and 37 new ones, of which the last is not kept
+    cfg = GenerationConfig(max_new_tokens=38)
+    assert len(generate(be, prompt, cfg).tokens) == 38
+    got, stats = generate_tree_lookup(be, prompt, cfg, TreeConfig(branches=8, depth=8))
+    assert len(got.tokens) == 38 and stats.proposed > 0
+    assert be.runner.pool.allocator.live_blocks() == 0
