@@ -16,7 +16,8 @@ _collect_after = False
 def recording(graph: "torch.cuda.CUDAGraph"):
     """`torch.cuda.graph(graph)` during which no cycles are collected. Engines and pipelines hold their graphs in cycles, and destroying a graph of one that
     nobody holds any more is an error in any recording of the process. Recordings of several threads may overlap: the collector
-    is on again, if it was, when the last of them has ended."""
+    is on again, if it was, when the last of them has ended. Other threads may take memory and wait for their own results meanwhile,
+    as the clients of a batching proxy do while its worker records."""
     global _recordings, _collect_after
     with _lock:
         if _recordings == 0:
@@ -24,7 +25,7 @@ def recording(graph: "torch.cuda.CUDAGraph"):
             gc.disable()
         _recordings += 1
     try:
-        with torch.cuda.graph(graph):
+        with torch.cuda.graph(graph, capture_error_mode="thread_local"):
             yield
     finally:
         with _lock:

@@ -69,3 +69,41 @@ def test_trees_on_a_pool_that_is_sized_for_the_text():
     got, stats = generate_tree_lookup(be, prompt, cfg, TreeConfig(branches=8, depth=8))
     assert len(got.tokens) == 38 and stats.proposed > 0
     assert be.runner.pool.allocator.live_blocks() == 0
+
+
+def test_a_client_chooses_while_another_ones_step_is_recorded():
+    """Steps of a new size are recorded by the proxy's worker; clients of others choose their beams meanwhile, take memory and wait for their results."""
+    import threading
+
+    from inference_b200.engine.branching import best_continuations
+    from inference_b200.utils.graphs import recording
+
+    begun, chosen, x, errors = threading.Event(), threading.Event(), torch.ones(64, device="cuda"), []
+    logits = torch.randn(5, 70001, device="cuda")
+    want = best_continuations(logits, torch.zeros(5, device="cuda"), 10)
+    graph = torch.cuda.CUDAGraph()
+
+    def record():
+        try:
+            with recording(graph):
+                y = x + 1
+                begun.set()
+                chosen.wait(60)
+                y += x
+            graph.replay()
+            torch.cuda.synchronize()
+            assert (y == 3).all()
+        except BaseException as e:
+            errors.append(e)
+            begun.set()
+
+    job = threading.Thread(target=record)
+    job.start()
+    begun.wait(60)
+    try:
+        room = torch.empty(1 << 29, dtype=torch.uint8, device="cuda")       # more than the allocator has at hand
+        got = best_continuations(logits.clone(), torch.zeros(5, device="cuda"), 10)
+    finally:
+        chosen.set()
+        job.join(60)
+    assert not errors and got == want and room.numel() == 1 << 29
