@@ -490,7 +490,7 @@ class ModelRunner:
         fused = self.model.comm.fused
         if fused is not None:
             fused.begin_capture()
-        with recording(graph):
+        with recording(graph, shared=True):
             toks, logits = self._decode_body(B, splits, want_logits, feedback)
         if fused is not None:
             fused.end_capture()

@@ -71,39 +71,46 @@ def test_trees_on_a_pool_that_is_sized_for_the_text():
     assert be.runner.pool.allocator.live_blocks() == 0
 
 
-def test_a_client_chooses_while_another_ones_step_is_recorded():
+def test_a_client_chooses_while_another_ones_step_is_recorded(monkeypatch):
     """Steps of a new size are recorded by the proxy's worker; clients of others choose their beams meanwhile, take memory and wait for their results."""
     import threading
 
-    from inference_b200.engine.branching import best_continuations
-    from inference_b200.utils.graphs import recording
+    from test_branching_gpu import _build, _cfg
 
-    begun, chosen, x, errors = threading.Event(), threading.Event(), torch.ones(64, device="cuda"), []
+    from inference_b200.engine.branching import best_continuations
+
+    _, be = _build(_cfg(), seed=23)
+    begun, chosen, errors, rows, plain = threading.Event(), threading.Event(), [], {}, be.runner.model.logits
     logits = torch.randn(5, 70001, device="cuda")
     want = best_continuations(logits, torch.zeros(5, device="cuda"), 10)
-    graph = torch.cuda.CUDAGraph()
+
+    def waits(hidden):
+        got = plain(hidden)
+        if torch.cuda.is_current_stream_capturing():
+            begun.set()
+            chosen.wait(60)
+        return got
+
+    monkeypatch.setattr(be.runner.model, "logits", waits)
+    first, again = be.new_sequence(), be.new_sequence()
+    be.forward([first, again], [[1, 2, 3], [1, 2, 3]])
 
     def record():
         try:
-            with recording(graph):
-                y = x + 1
-                begun.set()
-                chosen.wait(60)
-                y += x
-            graph.replay()
+            rows["recorded"] = be.forward([first], [[7]])[0].clone()
             torch.cuda.synchronize()
-            assert (y == 3).all()
         except BaseException as e:
             errors.append(e)
             begun.set()
 
     job = threading.Thread(target=record)
     job.start()
-    begun.wait(60)
     try:
+        assert begun.wait(60)
         room = torch.empty(1 << 29, dtype=torch.uint8, device="cuda")       # more than the allocator has at hand
         got = best_continuations(logits.clone(), torch.zeros(5, device="cuda"), 10)
     finally:
         chosen.set()
         job.join(60)
     assert not errors and got == want and room.numel() == 1 << 29
+    assert torch.equal(rows["recorded"], be.forward([again], [[7]])[0])
