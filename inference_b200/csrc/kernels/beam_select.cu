@@ -2,7 +2,7 @@
 // beam and token.
 //
 // Two scores may differ in the last bits of 32-bit numbers only, and which of them is the better one decides which beam lives. So logarithms and scores are 64-bit numbers, rounded once when
-// they are handed out, and an exponential is within 2^-29 of its value. Within a beam the order is that of the logits, which takes none of them.
+// they are handed out, and an exponential, and a sum of however many, is within 2^-28.5 of its value. Within a beam the order is that of the logits, which takes none of them.
 //
 // The first launch reads every logit once: a block walks over a piece of a row, 16 logits a thread at a time with the next ones on their way, adds up their exponentials and keeps a note of the
 // sixteens whose largest may be among its `count` largest; their logits are looked at in the end, when the bound for these is tight. It comes from the threads' own maxima so far: each of
@@ -14,8 +14,9 @@
 // candidates looked up as they came and ranked one by one 75, 22 and 150.
 //
 // Exponentials run on the multiply-add pipes, two at a time, by the table method of Tang (1989): x = k ln2 / 32 + r, where k times the first part of ln2 / 32 leaves x without a rounding, and e^x = 2^(k / 32) (1 +
-// e^r - 1) with 2^(k mod 32 / 32) from a table of two numbers each; the top's whole power of two leaves the exponent, so that nothing is larger than two. The larger part, the
-// table's first number times a power of two, is added up together with what each sum rounds off: it starts at two, and no part is larger, so that three additions give that exactly.
+// e^r - 1) with 2^(k mod 32 / 32) from a table of two numbers each; the top's whole power of two leaves the exponent, so that nothing is larger than two. What a sum rounds off is added up beside it:
+// the sum starts at two, and no part is larger, so that one subtraction gives what was really added, and the rest of a part is a small number. (Adding up e^r - 1 beside the table's numbers took an operation
+// less; with hundreds of equal logits a thread its roundings all went one way, 6e-8 of the sum.)
 #include "attention_tc.cuh"
 
 #include <cfloat>
@@ -91,7 +92,7 @@ constexpr float MAGIC = 12582912.f;                        // x + MAGIC has x ro
 constexpr float LEAST = 80.f;                              // what lies further below the top counts as that far: 2^-115 of it
 constexpr float FAR = 30000.f;                             // |x| 32 / ln 2 is below 2^22
 
-// large += the table's part of e^x for two logits, at least e^least, over the power of two 2^((MAGIC - magic) / 32); small += the rest of it and what large rounds off
+// large += e^x for two logits, at least e^least, over the power of two 2^((MAGIC - magic) / 32); small += what large rounds off
 __device__ __forceinline__ void add_exponentials(float x0, float x1, float least, float magic, const float2* powers, unsigned long long& large, unsigned long long& small) {
   const unsigned long long x = pack2(fmaxf(x0, least), fmaxf(x1, least)), neg = pack2(-1.f, -1.f);
   const unsigned long long t = fma2(x, pack2(PER_STEP, PER_STEP), pack2(magic, magic)), k = add2(t, pack2(-magic, -magic));
@@ -102,9 +103,9 @@ __device__ __forceinline__ void add_exponentials(float x0, float x1, float least
   const float2 w0 = powers[n0 & 31], w1 = powers[n1 & 31];
   const unsigned long long q = fma2(fma2(fma2(r, pack2(1.f / 6.f, 1.f / 6.f), pack2(0.5f, 0.5f)), r, pack2(1.f, 1.f)), r, pack2(w0.y, w1.y));      // e^r - 1 and the table's share
   const unsigned long long v = pack2(__int_as_float((n0 & ~31) * (1 << 18) + __float_as_int(w0.x)), __int_as_float((n1 & ~31) * (1 << 18) + __float_as_int(w1.x)));
-  const unsigned long long sum = add2(large, v), lost = fma2(fma2(large, neg, sum), neg, v);
+  const unsigned long long sum = add2(large, fma2(v, q, v)), less = fma2(sum, neg, large);      // less: what was added, exactly, with the other sign
+  small = add2(small, fma2(v, q, add2(v, less)));                                                // and what of v + v q was not
   large = sum;
-  small = add2(fma2(v, q, small), lost);
 }
 
 // A warp's numbers in descending order.
@@ -284,8 +285,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 4) beam_chunk_kernel(const Beam
       const int i = atomicAdd(&s_notes, 1);
       if (i < ROOM) s_note[i] = Entry{mine, step * CHUNK_THREADS + tid};
     }
-    if (__any_sync(0xffffffffu, mine > limit)) {           // the warp's top has a new power of two
-      const float top = warp_max(mine);
+    if (__any_sync(0xffffffffu, mine > limit) || step % 64 == 63) {      // the warp's top has a new power of two, or small has grown
+      const float top = fmaxf(warp_max(mine), warp_top);
       flush();
       if (fabsf(top) <= FAR) {
         const int next = (__float_as_int(fmaf(top, PER_STEP, MAGIC)) & ~31) - 0x4b400000;

@@ -93,7 +93,7 @@ def test_a_steps_bound_may_be_the_largest_number(kind):
 @pytest.mark.parametrize("shift", [300, 2000, 20000, 29900, 31000, -20000, -31000])
 def test_logits_far_from_zero_lose_nothing(shift):
     """Two beams with the same logits, one of them moved by a whole number, whose scores differ by 2e-8: the better one is first at every token. (Logits are multiples of 1 / 64, so that
-    the move is exact; a logarithm is off by 2^-29 of a sum at most, 2e-9.)"""
+    the move is exact; a logarithm is off by 2^-28.5 at most, 3e-9.)"""
     V = 6000
     row = (torch.randn(V, device=CUDA, generator=_gen(91)) * 3 * 64).round() / 64
     logits = torch.stack([row + shift, row])
@@ -185,3 +185,23 @@ def test_queries_and_results_lie_anywhere(kind, D, Dv, bs, splits):
         to = torch.full((T, H * Dv + gap + 3), 7.0, dtype=kind, device=CUDA)
         got = _run(c, _pack(sees), 0.1, num_splits=splits, out=to[:, gap:gap + H * Dv])
         assert torch.equal(got, whole) and (to[:, :gap] == 7).all() and (to[:, gap + H * Dv:] == 7).all()
+
+
+# ---- sums of many alike -------------------------------------------------------------------------------------------------------------------------------------
+@KINDS
+@pytest.mark.parametrize("apart", [1e-8, -1e-8])
+def test_sums_of_many_logits_that_are_alike(kind, apart):
+    """Two beams a prompt: all logits of one are c, all of the other 0, so that every continuation has -log V. Of as many rows as fill the SMs a thread adds up hundreds of
+    equal exponentials, whose roundings all go one way: the better beam is first nevertheless. (A sum is off by 2^-28.5 of itself at most, 3e-9, however many it is of.)"""
+    B, V, count = 300, 128256, 7
+    c = (torch.randn(B, device=CUDA, generator=_gen(98)) * 3).to(kind)
+    logits = torch.zeros(B, 2, V, device=CUDA, dtype=kind)
+    logits[:, 0] = c[:, None]
+    scores = torch.tensor([[apart, 0.0]], device=CUDA).expand(B, 2).contiguous()
+    got = _ops().beam_select(logits.view(2 * B, V), scores, count=count)
+    better = 0 if apart > 0 else 1
+    wrong = (got.beams != better).any(1).nonzero()[:, 0].tolist()
+    assert not wrong, (len(wrong), c[wrong[0]].item())
+    assert (got.tokens == torch.arange(count, device=CUDA)).all()
+    assert ((got.scores.double() - (float(scores[0, better]) - math.log(V))).abs() <= 2.0 ** -24 * 12 + 2.0 ** -28.5).all()
+
