@@ -114,3 +114,50 @@ def test_a_client_chooses_while_another_ones_step_is_recorded(monkeypatch):
         job.join(60)
     assert not errors and got == want and room.numel() == 1 << 29
     assert torch.equal(rows["recorded"], be.forward([again], [[7]])[0])
+
+
+MOE = dict(model_type="qwen2_moe", num_experts=8, num_experts_per_tok=2, moe_intermediate_size=256, shared_expert_intermediate_size=256)
+
+
+@pytest.mark.parametrize("sizes", [[1], [5, 9, 1], [70, 33, 130]], ids=str)
+@pytest.mark.parametrize("kw,fmt", [({}, None), ({}, "Q8_0"), (MOE, None)], ids=["dense", "packed", "experts"])
+def test_chains_as_trees_have_the_logits_of_chains(kw, fmt, sizes):
+    """Steps of up to 64 tokens and of more, dense, packed and routed weights: the tree of a chain against the step that verifies it, on one model. A second one, whose tokens part behind the
+    third, against chains of its paths. (Not of many tokens on routed experts: of those one or two go to another expert in another batch, chains too.)"""
+    from test_branching_gpu import _build, _cfg, _near
+
+    if kw and max(sizes) > 64:
+        sizes = sizes[1:2]
+    _, be = _build(_cfg(vocab_size=1024, **kw), seed=24)
+    if fmt:
+        be.runner.model.quantize_(fmt)
+    g = torch.Generator().manual_seed(len(sizes))
+    draw = lambda n: torch.randint(0, 1024, (n,), generator=g).tolist()
+    prompts, drafts = [draw(11 + 9 * i) for i in range(len(sizes))], [draw(n) for n in sizes]
+    seqs, chains = [be.new_sequence() for _ in sizes], [be.new_sequence() for _ in sizes]
+    be.forward(seqs + chains, prompts + prompts)
+    want, got = torch.cat(be.forward(chains, drafts, all_positions=True)), {}
+
+    def choose(logits):
+        got["rows"] = logits.clone()
+        return torch.full((logits.shape[0],), -1, device="cuda")
+
+    assert be.step_trees(seqs, drafts, [list(range(-1, n - 1)) for n in sizes], choose) == [([0], -1)] * len(sizes)
+    _near(got["rows"], want)
+    for s, prompt in zip(seqs, prompts):
+        be.truncate(s, len(prompt))
+    parents = [[-1] + [i - 1 if i < 3 else max(2, i - 2) for i in range(1, n)] for n in sizes]       # two chains, token by token by turns
+    be.step_trees(seqs, drafts, parents, choose)
+    for side in (3, 4):
+        at = 0
+        for prompt, toks, ups, n in zip(prompts, drafts, parents, sizes):
+            path = list(range(min(n, 3))) + list(range(side, n, 2))
+            assert all(ups[b] == a for a, b in zip(path, path[1:]))
+            seq = be.new_sequence()
+            be.forward([seq], [prompt])
+            _near(got["rows"][[at + i for i in path]], be.forward([seq], [[toks[i] for i in path]], all_positions=True)[0])
+            be.release(seq)
+            at += n
+    for s in seqs + chains:
+        be.release(s)
+    assert be.runner.pool.allocator.live_blocks() == 0
