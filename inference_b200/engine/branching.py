@@ -146,6 +146,9 @@ def generate_tree_lookup(target: DecodeBackend, prompt: list[int], cfg: Generati
     def emit(token: int) -> bool:
         """Whether the text goes on behind this token."""
         nonlocal why
+        if cfg.cancel is not None and cfg.cancel.is_cancelled():
+            why = FinishReason.CANCELLED
+            return False
         if token in cfg.stop_tokens:
             why = FinishReason.STOP
             return False
@@ -159,13 +162,12 @@ def generate_tree_lookup(target: DecodeBackend, prompt: list[int], cfg: Generati
     try:
         if cfg.max_new_tokens <= 0:
             return GenerationResult([], FinishReason.LENGTH, len(prompt)), stats
+        if cfg.cancel is not None and cfg.cancel.is_cancelled():
+            return GenerationResult([], FinishReason.CANCELLED, len(prompt)), stats
         logits = target.forward([seq], [list(prompt)])[0]
         stats.forwards += 1
         last = _pick(target, logits, list(prompt), cfg, rng, None)
         while emit(last):
-            if cfg.cancel is not None and cfg.cancel.is_cancelled():
-                why = FinishReason.CANCELLED
-                break
             room = cfg.max_new_tokens - len(out)        # a tree takes no more of the cache than the text may
             tokens, parents = (x[:room] for x in index.tree(spec.branches, min(spec.depth, room - 1)))
             (path, last), = target.step_trees([seq], [tokens], [parents], choose(tokens, parents))

@@ -7,6 +7,7 @@ import threading
 import pytest
 import torch
 
+from inference_b200.contracts.core_llm import CancelFlag, FinishReason
 from inference_b200.engine.backend import GpuBackend, OracleBackend
 from inference_b200.engine.batching import BatchingBackend
 from inference_b200.engine.branching import TreeConfig, best_continuations, generate_tree_lookup
@@ -208,3 +209,26 @@ def test_a_draft_does_not_go_through_the_text():
     Watched.read = 0
     assert index.tree(4, 5) == ([77, 78, 79, 80, 81, 82], [-1, 0, 1, 2, 3, 4])
     assert Watched.read < 20
+
+
+@pytest.mark.parametrize("after", [0, 1, 3, 6])
+@pytest.mark.parametrize("prompt", [[4, 4, 8, 4, 4, 8, 4, 4], [2, 3, 2, 4, 2, 3, 2, 4, 2]])
+def test_a_cancelled_text_ends_where_plain_decoding_ends_it(prompt, after):
+    """No token behind the one at which it was cancelled, drafted and accepted ones neither."""
+    def run(loop):
+        flag, seen = CancelFlag(), []
+        if after == 0:
+            flag.cancel()
+
+        def sink(token):
+            seen.append(token)
+            if len(seen) == after:
+                flag.cancel()
+            return True
+
+        got = loop(_oracle(vocab=12), prompt, GenerationConfig(max_new_tokens=12, cancel=flag), sink=sink)
+        got = got[0] if isinstance(got, tuple) else got
+        assert got.tokens == seen and got.finish_reason is FinishReason.CANCELLED
+        return seen
+
+    assert run(generate_tree_lookup) == run(generate) and len(run(generate_tree_lookup)) == after
