@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(PLAIN_THREADS) attn_tree_plain_kernel(const Tr
 //   warps 0-15   softmax, eight to a slot, two threads to a row with 64 of a tile's keys each; in tiles of the tree they apply the mask and see to it that V holds numbers
 // Tensor memory of a slot: S (128 columns; P in the first half of each thread's own 64), O (128). Shared memory has seven buffers of a tile: Q, three of K, and two of V with Q's second half
 // or three of V.
-// 64 tokens x 32 heads (8 key/value heads) behind 100 000 keys, blocks of 256 rows and 44 tiles: 119 us with the sum of the splits, 0.88 PFLOP/s; some 95 without any softmax. (One slot a block and
+// 64 tokens x 32 heads (8 key/value heads) behind 100 000 keys, blocks of 256 rows and 44 tiles: 121 us with the sum of the splits, 0.87 PFLOP/s; some 95 without any softmax. (One slot a block and
 // two blocks to an SM, each tile asked for when the one before it was used: 155.) A tile takes a slot some 3400 cycles: 1850 from its scores to its weights, of them 1000 for the exponentials, which
 // the special-function units alone would need 1024 for at least (1190 in fact), and 1570 from there to the next scores, of them 1024 for the products; those of both slots together keep the tensor
 // cores busy for 2048. Maxima of three numbers and one vote in place of two were 3 % of it. What did not help: tiles of 64 keys with two of scores a slot, references a tile old in place of a row's own maximum (its steps cost more
@@ -545,7 +545,9 @@ __device__ __forceinline__ void tree_softmax(const TreeParams& p, TcBars* bars, 
     const unsigned long long sc2 = pack2(scale_log2, scale_log2), nm2 = pack2(neg_m, neg_m);
     unsigned long long l0 = 0ull, l1 = 0ull;
 #pragma unroll
-    for (int e = 0; e < 64; e += 4) {       // packed P overwrites the row in place
+    // Packed P overwrites the row in place. Weights are rounded to bf16, half a step each, as the product with bf16 values takes both operands in one type: results are off by 0.0023 of their size in place of
+    // the 0.0017 that their own rounding to bf16 costs. Two parts of each weight would double that product. Their sum l is of the 32-bit numbers.
+    for (int e = 0; e < 64; e += 4) {
       float v0, v1, v2, v3;
       unpack2(fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), sc2, nm2), v0, v1);
       unpack2(fma2(pack2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])), sc2, nm2), v2, v3);

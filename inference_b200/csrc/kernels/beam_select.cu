@@ -9,9 +9,13 @@
 // the eight warps gives its (count / 8)-th largest, and the smallest of these has `count` logits at least as large as itself, of different threads, and not many more; it is raised behind 1, 2, 4, 8..
 // steps. The second launch joins the pieces, one block a prompt, with a bound from their ordered lists. Rows of beams that are not alive (scores that are not finite) are not read.
 //
-// Measured on the device: 32 prompts of 8 beams over 128 256 tokens (131 MB) 56 us, of them 45 the pieces (2.9 TB/s; 27 without exponentials, which take 18 instructions a logit and whose sums wait for one
-// another); 4 beams of one prompt 16 us, of them 7 the pieces; 50 beams of 3 prompts, 100 continuations, 62 us. With exponentials and sums in 64 bits throughout it took 178, 22 and 135 us, with the
-// candidates looked up as they came and ranked one by one 75, 22 and 150.
+// Measured on the device: 32 prompts of 8 beams over 128 256 tokens (131 MB) 59 us (bf16, half the bytes: 55), of them some 12 the join; the pieces alone would take 27 without exponentials, at 18 to 19
+// instructions a logit. A warp there waits 12 cycles between two instructions: 2.6 for logits, 2.1 for results of the multiply-adds, 1.5 each for the table's numbers and for its turn, 1.2 each for barriers and
+// for a pipe that is busy; 41 % of the issue slots are used, with 3.5 blocks to an SM of the four that it holds. 4 beams of one prompt 16 us, of them 7 the pieces; 50 beams of 3 prompts, 100 continuations, 60 to
+// 65 us. With exponentials and sums in 64 bits throughout it took 178, 22 and 135 us, with the candidates looked up as they came and ranked one by one 75, 22 and 150.
+//
+// Where more than 1024 sixteens, or logits, of a piece are as large as its bound (ties of a finite number in place of tokens that are not allowed, logits that rise with the token's number), the piece is gone
+// through some 65 times: 4 beams over 128 256 tokens 90 us where logits rise, 122 where all are alike, 96 with five tokens allowed and -1e9 for the others, 14 with -inf for them.
 //
 // Exponentials run on the multiply-add pipes, two at a time, by the table method of Tang (1989): x = k ln2 / 32 + r, where k times the first part of ln2 / 32 leaves x without a rounding, and e^x = 2^(k / 32) (1 +
 // e^r - 1) with 2^(k mod 32 / 32) from a table of two numbers each; the top's whole power of two leaves the exponent, so that nothing is larger than two. What a sum rounds off is added up beside it:

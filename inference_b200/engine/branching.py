@@ -1,8 +1,11 @@
 """Generation loops that carry several continuations of a sequence: beam search, and speculation over trees of drafts.
 
 Both run on any `DecodeBackend` with `reorder` and `step_trees`. On the GPU a beam step picks its continuations with `ops.beam_select` and parts pages with one `ops.copy_pages`; a tree is verified in one forward
-with `ops.tree_attention`, and `ops.accept_tree` closes the accepted entries up. Law kept: greedy tree speculation gives the tokens of plain greedy decoding, sampled one draws each token from the model's own
-distribution whatever was drafted."""
+with `ops.tree_attention`, and `ops.accept_tree` closes the accepted entries up. Law kept: greedy tree speculation gives the model's own largest logit at each place, sampled one draws each token from the
+model's own distribution, whatever was drafted. On the oracle these are the tokens of plain decoding; in bf16 a tree's step and a decode step are different kernels, so that logits within its
+rounding of one another may change places, as they may between a chain's verification and decoding. Routed experts, which such a change may switch, widen that.
+
+Each loop serves one prompt: a beam step is a `beam_select` of one prompt, a tree step one tree. Trees of several sequences in one step are `step_trees`, several prompts' beams `ops.beam_select`."""
 from __future__ import annotations
 
 import math

@@ -208,7 +208,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, count: int) -> Be
     """The `count` best of all continuations of each prompt's beams by one token: scores[b, k] + log softmax(logits[b K + k])[v], equal ones in the order of beam and token.
 
     logits [B * K, V] bf16 or fp32 (row stride free), scores fp32 [B, K]: what the beams have added up so far. A beam whose score is not finite, or with a logit that is NaN or +inf,
-    offers nothing, nor does a logit of -inf (a token that is not allowed). A search that keeps K beams asks for 2 K: so many are left when each of K may end."""
+    offers nothing, nor does a logit of -inf (a token that is not allowed; a finite number in its place ties with others like it, which takes up to eight times as long). A sum of
+    exponentials is within 2^-28.5 of its value. A search that keeps K beams asks for 2 K: so many are left when each of K may end."""
     stream = _place(logits, scores)
     _require(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32) and logits.shape[1] >= 1 and (logits.stride(1) == 1 or logits.shape[1] == 1),
              "logits are bf16 or fp32 [B * K, V], unit inner stride")
